@@ -244,6 +244,104 @@ JITNN_HIP_API int jitnn_hip_gguf_tensor_read(const jitnn_hip_gguf *f, const char
  * JITNN_HIP_EUNSUPPORTED. */
 JITNN_HIP_API int jitnn_hip_gguf_tensor_upload(const jitnn_hip_gguf *f, const char *name, jitnn_hip_weight **out);
 
+/* ---- rotary positions -------------------------------------------------------------------------- */
+
+/* Rotary embedding beyond the reference's (core/ops/Rope.java:86-150, which a plain jitnn_hip_rope repeats): part of a head, and contexts longer
+ * than the trained one.  Pair i < rot_dim / 2 of a head turns by position * f_i, f_i = theta^(-2 i / rot_dim) before scaling; pairs are
+ * (i, i + rot_dim / 2), or (2 i, 2 i + 1) when interleaved; the values of a head behind rot_dim stay as they are.
+ *   JITNN_HIP_ROPE_LINEAR   f_i / factor
+ *   JITNN_HIP_ROPE_YARN     f_i for pairs that turn more than beta_fast times in original_context positions, f_i / factor below beta_slow times, in
+ *                           between a mixture linear in i; cosine and sine times attention_factor (0: 0.1 ln(factor) + 1)
+ *                           (Peng, Quesnelle, Fan, Shippole, "YaRN: Efficient Context Window Extension of Large Language Models", 2023)
+ * freq_factors (or NULL): [rot_dim / 2] in host memory, f_i / freq_factors[i] before any scaling - the rope_freqs.weight of GGUF files.
+ * attention_factor other than 0 counts with every kind. */
+typedef struct jitnn_hip_rope jitnn_hip_rope;
+#define JITNN_HIP_ROPE_PLAIN 0
+#define JITNN_HIP_ROPE_LINEAR 1
+#define JITNN_HIP_ROPE_YARN 2
+typedef struct jitnn_hip_rope_scaling {
+    int kind; /* JITNN_HIP_ROPE_* */
+    int original_context;
+    double factor, beta_fast, beta_slow, attention_factor;
+} jitnn_hip_rope_scaling;
+/* scaling NULL: plain.  rot_dim even, 2 .. 1024; theta > 0; immutable afterwards and usable by any number of threads. */
+JITNN_HIP_API int jitnn_hip_rope_create(int rot_dim, int interleaved, double theta, const jitnn_hip_rope_scaling *scaling, const float *freq_factors,
+                                        jitnn_hip_rope **out);
+JITNN_HIP_API int jitnn_hip_rope_free(jitnn_hip_rope *r);
+/* y [tokens, heads, head_dim] = x rotated, token t by positions[t] (any int: -p undoes p but for the attention factor).  Tokens start x_stride and
+ * y_stride floats apart (at least heads * head_dim); y may be x with the same stride, and may not overlap it otherwise.  Angles are exact to
+ * FP32 at any position.  tokens 0: nothing is done.  Any alignment; fastest with 16-byte aligned rows and multiples of 8 for rot_dim and head_dim. */
+JITNN_HIP_API int jitnn_hip_rope_dev(const jitnn_hip_rope *r, const float *x_dev, long long x_stride, const int *positions_dev, int tokens, int heads,
+                                     int head_dim, float *y_dev, long long y_stride, void *stream);
+
+/* ---- a batch over a paged cache ----------------------------------------------------------------- */
+
+/* Keys and values of many sequences in pages of page_tokens positions (16, 32, 64, 128 or 256): keys and values are each
+ * [layers][pages][kv_heads][page_tokens][head_dim], head_dim 64, 128, 192 or 256, in ggml type F32 (0) or F16 (1).  Which page holds which positions of
+ * which sequence is the caller's bookkeeping (jitnn_hip_batch.tables).  The reference has no KV-cache operator. */
+typedef struct jitnn_hip_paged_cache jitnn_hip_paged_cache;
+/* Bytes of the keys (and as many of the values) of such a cache, or JITNN_HIP_EINVAL. */
+JITNN_HIP_API long long jitnn_hip_paged_cache_nbytes(int layers, int kv_heads, int head_dim, int pages, int page_tokens, int ggml_type);
+JITNN_HIP_API int jitnn_hip_paged_cache_create(int layers, int kv_heads, int head_dim, int pages, int page_tokens, int ggml_type, jitnn_hip_paged_cache **out);
+/* The same in the caller's device memory (not owned, kept alive by the caller; 16-byte aligned). */
+JITNN_HIP_API int jitnn_hip_paged_cache_wrap_dev(void *k_dev, void *v_dev, int layers, int kv_heads, int head_dim, int pages, int page_tokens, int ggml_type,
+                                                 jitnn_hip_paged_cache **out);
+JITNN_HIP_API int jitnn_hip_paged_cache_free(jitnn_hip_paged_cache *c);
+/* Page `from` of every layer to page `to`: a sequence that goes on alone from a page it shared. */
+JITNN_HIP_API int jitnn_hip_paged_cache_copy_page_dev(const jitnn_hip_paged_cache *c, int from, int to, void *stream);
+
+/* The tokens of one pass: `tokens` rows, those of sequence s being rows starts[s] .. starts[s + 1] - 1 (ascending; a sequence may have none), its last
+ * `starts[s + 1] - starts[s]` positions of the lens[s] it then has.  Position p of sequence s lies on page tables[s * table_stride + p / page_tokens].
+ * The arrays are device memory and read when the work runs, so that a recorded graph can be replayed with others; the numbers are host values:
+ * max_tokens and max_len bound a sequence's rows and its lens, shared_pages counts the leading pages that all rows of tables have in common (0:
+ * none; attention reads them once for the whole batch, by the first row of tables).
+ * What the arrays hold is checked where it is used: rows of x, q, y in front of starts[0] or behind starts[sequences] are left as they were.  A position
+ * below 0 (a lens smaller than its rows) is appended nowhere and attends to nothing: a zero row.  A page id outside the cache is neither read nor
+ * written, and a sequence whose lens is above max_len is not attended: the rows that would have seen them are NaN.  Rows of a sequence beyond
+ * max_tokens may stay as they were. */
+typedef struct jitnn_hip_batch {
+    int sequences, tokens, max_tokens, max_len;
+    int shared_pages, table_stride;
+    const int *tables; /* [sequences, table_stride] */
+    const int *starts; /* [sequences + 1] */
+    const int *lens;   /* [sequences] */
+} jitnn_hip_batch;
+
+/* Keys k and values v [tokens, kv_heads, head_dim] of the batch into their pages of `layer`, keys rotated by r (NULL: as they are), and the queries
+ * q [tokens, heads, head_dim] rotated to q_out, in one launch (heads 0: no queries).  Rows start *_stride floats apart, pointers 16-byte aligned,
+ * strides multiples of 4; q_out may be q with the same stride.  rot_dim a multiple of 8, at most head_dim (JITNN_HIP_EUNSUPPORTED).  FP16 pages: rounded to nearest, finite
+ * values beyond its range as its largest.  Two rows of one pass on the same place of a page leave either. */
+JITNN_HIP_API int jitnn_hip_paged_append_dev(const jitnn_hip_paged_cache *c, int layer, const jitnn_hip_batch *batch, const jitnn_hip_rope *r, const float *q_dev,
+                                             long long q_stride, int heads, float *q_out_dev, long long q_out_stride, const float *k_dev, long long k_stride,
+                                             const float *v_dev, long long v_stride, void *stream);
+
+/* y [tokens, heads, head_dim] = softmax(scale q K^T) V over the positions up to the row's own, query head h reading key/value head h / (heads / kv_heads)
+ * (F.scaledDotProductAttentionBTHD with F.repeatHeads, core/F.java:588-624).  FP32-grade with both cache types.  Keys and values that a row sees must be
+ * finite (a row that sees others is not); what it does not see - later tokens, the rest of a page - may hold anything.  A row whose scores are all
+ * -inf is zero.  The workspace is device memory of at least jitnn_hip_paged_attention_workspace bytes (0 where it returns 0; 16-byte aligned), used until the work has run: calls that may
+ * overlap in time, recorded graphs among them, need one each.  Allocates nothing; may be recorded. */
+JITNN_HIP_API long long jitnn_hip_paged_attention_workspace(const jitnn_hip_paged_cache *c, const jitnn_hip_batch *batch, int heads);
+JITNN_HIP_API int jitnn_hip_paged_attention_dev(const jitnn_hip_paged_cache *c, int layer, const jitnn_hip_batch *batch, int heads, const float *q_dev,
+                                                long long q_stride, float scale, float *y_dev, long long y_stride, void *workspace_dev, long long workspace_bytes,
+                                                void *stream);
+
+/* ---- drafted tokens ------------------------------------------------------------------------------ */
+
+/* Which of the drafted tokens a target model keeps, and the token after them, from given random numbers (Leviathan, Kalman, Matias, "Fast Inference from
+ * Transformers via Speculative Decoding", 2023): the tokens follow the target's own distribution.  Sequence s has the rows starts[s] .. starts[s + 1] - 1:
+ * its last known token and the drafted ones after it, tokens [rows]; logits [rows, vocab], rows logits_stride floats apart, are what the target says comes
+ * after each.  With p = softmax(logits / temperatures[s]) - temperature 0 or below: everything on the largest, the lowest index among equals -
+ * the draft x after row r is kept while uniforms[r][0] * q(x) < p(x), q = draft_probs row r (or NULL: drafted with certainty, q(x) = 1).  At the first that is not kept a token is
+ * drawn from max(p - q, 0), with all kept from p of the last row: the first index whose cumulative sum exceeds uniforms[r][1] times the total, r being
+ * that row.  Sums in FP64.  uniforms [rows, 2] in [0, 1).
+ * accepted[s]: drafts kept.  out [rows]: per sequence the kept drafts, the drawn token, then -1.  A draft outside [0, vocab) is not kept.  NaN logits
+ * have no weight; a row of nothing but NaN and -inf gives its lowest index that is not NaN.  A sequence without rows: accepted 0.  Rows in front of starts[0] and behind
+ * starts[sequences] are left as they were.  starts, tokens, draft_probs, temperatures, uniforms, out, accepted: device memory.  Workspace as above. */
+JITNN_HIP_API long long jitnn_hip_verify_workspace(int rows, int sequences, int vocab);
+JITNN_HIP_API int jitnn_hip_verify_drafts_dev(const float *logits_dev, long long logits_stride, int rows, int vocab, const int *starts_dev, int sequences,
+                                              const int *tokens_dev, const float *draft_probs_dev, long long draft_stride, const float *temperatures_dev,
+                                              const float *uniforms_dev, int *out_dev, int *accepted_dev, void *workspace_dev, long long workspace_bytes, void *stream);
+
 /* ---- Llama-style decode step on quantised weights --------------------------------------------- */
 
 /* The reference has no quantised Llama and no KV-cache operator; the step is the composition of its operators as
@@ -317,6 +415,19 @@ JITNN_HIP_API int jitnn_hip_prompt_attention(int heads, int kv_heads, int head_d
 JITNN_HIP_API int jitnn_hip_llama_set_packing(jitnn_hip_llama *m, int allow);
 /* What the model's last prompt pass took; JITNN_HIP_EINVAL before the first. */
 JITNN_HIP_API int jitnn_hip_llama_last_attention(const jitnn_hip_llama *m);
+
+/* The model's rotary positions: those of r (copied; its rot_dim must be head_dim, or any smaller one when interleaved), pairing included, from the next call on.  Not while work of this
+ * model is under way, nor between a recording and its replays. */
+JITNN_HIP_API int jitnn_hip_llama_set_rope(jitnn_hip_llama *m, const jitnn_hip_rope *r);
+
+/* One pass of a batch of sequences over a paged cache (layers, kv_heads and head_dim of the model): x [batch->tokens, d_model] are the embeddings of
+ * the batch's rows; every row's keys and values are appended, turned by the model's rotary positions, and logits [logit_count, vocab] are those of the
+ * rows logit_rows [logit_count] (device memory; a row outside the batch gives NaN): a decode step names every row, a prompt's pass its last.
+ * logit_count 0: none.  The rows go through the linears together, as in jitnn_hip_llama_prefill; the model's own cache is not touched.
+ * The model's many-token buffers and the attention's workspace belong to it and grow with the largest pass (which waits for the device; such a
+ * call cannot be recorded: JITNN_HIP_EINVAL). */
+JITNN_HIP_API int jitnn_hip_llama_step_dev(jitnn_hip_llama *m, const jitnn_hip_paged_cache *c, const jitnn_hip_batch *batch, const float *x_dev,
+                                           const int *logit_rows_dev, int logit_count, float *logits_dev, void *stream);
 
 /* ---- generation loop ------------------------------------------------------------------------------------------------ */
 

@@ -22,11 +22,30 @@ class JitnnError(RuntimeError):
     """A native call failed (the reference's JitnnException, core/JitnnException.java:18-25)."""
 
 
+class RopeScaling(C.Structure):
+    """jitnn_hip_rope_scaling."""
+
+    _fields_ = [("kind", C.c_int), ("original_context", C.c_int), ("factor", C.c_double), ("beta_fast", C.c_double), ("beta_slow", C.c_double),
+                ("attention_factor", C.c_double)]
+
+
+class Batch(C.Structure):
+    """jitnn_hip_batch: the tokens of one pass over a paged cache (include/jitnn_hip.h).  The arrays - tables [sequences, table_stride], starts
+    [sequences + 1], lens [sequences], 32-bit whole numbers - are addresses in device memory."""
+
+    _fields_ = [("sequences", C.c_int), ("tokens", C.c_int), ("max_tokens", C.c_int), ("max_len", C.c_int), ("shared_pages", C.c_int), ("table_stride", C.c_int),
+                ("tables", C.c_void_p), ("starts", C.c_void_p), ("lens", C.c_void_p)]
+
+    def __init__(self, sequences, tokens, max_tokens, max_len, tables_ptr, table_stride, starts_ptr, lens_ptr, shared_pages=0):
+        super().__init__(sequences, tokens, max_tokens, max_len, shared_pages, table_stride, tables_ptr or None, starts_ptr or None, lens_ptr or None)
+
+
 def _bind() -> C.CDLL:
     if not LIB_PATH.exists():
         raise JitnnError(f"{LIB_PATH} is not built: run `make -C jitnn_amd/csrc` (or __graft_entry__.build())")
     lib = C.CDLL(str(LIB_PATH))
     vp, i, ll, fp = C.c_void_p, C.c_int, C.c_longlong, C.POINTER(C.c_float)
+    batch = C.POINTER(Batch)
     sig = {
         "jitnn_hip_init": (i, [i]),
         "jitnn_hip_device_info": (i, [C.c_char_p, i, C.POINTER(i), C.POINTER(ll)]),
@@ -85,6 +104,21 @@ def _bind() -> C.CDLL:
         "jitnn_hip_llama_argmax_dev": (i, [vp, vp, vp, vp]),
         "jitnn_hip_llama_generate": (i, [vp, vp, i, i, i, i, vp, vp, vp]),
         "jitnn_hip_llama_prefill_dev": (i, [vp, vp, i, i, vp, vp]),
+        "jitnn_hip_rope_create": (i, [i, i, C.c_double, C.POINTER(RopeScaling), fp, C.POINTER(vp)]),
+        "jitnn_hip_rope_free": (i, [vp]),
+        "jitnn_hip_rope_dev": (i, [vp, vp, ll, vp, i, i, i, vp, ll, vp]),
+        "jitnn_hip_paged_cache_nbytes": (ll, [i, i, i, i, i, i]),
+        "jitnn_hip_paged_cache_create": (i, [i, i, i, i, i, i, C.POINTER(vp)]),
+        "jitnn_hip_paged_cache_wrap_dev": (i, [vp, vp, i, i, i, i, i, i, C.POINTER(vp)]),
+        "jitnn_hip_paged_cache_free": (i, [vp]),
+        "jitnn_hip_paged_cache_copy_page_dev": (i, [vp, i, i, vp]),
+        "jitnn_hip_paged_append_dev": (i, [vp, i, batch, vp, vp, ll, i, vp, ll, vp, ll, vp, ll, vp]),
+        "jitnn_hip_paged_attention_workspace": (ll, [vp, batch, i]),
+        "jitnn_hip_paged_attention_dev": (i, [vp, i, batch, i, vp, ll, C.c_float, vp, ll, vp, ll, vp]),
+        "jitnn_hip_verify_workspace": (ll, [i, i, i]),
+        "jitnn_hip_verify_drafts_dev": (i, [vp, ll, i, i, vp, i, vp, vp, ll, vp, vp, vp, vp, vp, ll, vp]),
+        "jitnn_hip_llama_set_rope": (i, [vp, vp]),
+        "jitnn_hip_llama_step_dev": (i, [vp, vp, batch, vp, vp, i, vp, vp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)  # AttributeError if the library lacks a declared symbol

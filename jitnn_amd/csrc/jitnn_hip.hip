@@ -31,6 +31,7 @@
 #include "glue.h"
 #include "prefill.h"
 #include "scratch.h"
+#include "serving.h"
 #include "tu.h"
 
 using namespace jitnn;
@@ -1906,6 +1907,413 @@ int jitnn_hip_gguf_tensor_upload(const jitnn_hip_gguf *h, const char *name, jitn
 
 }  // extern "C"
 
+// ================================================================================================ rotary positions
+
+struct jitnn_hip_rope {
+    int rot = 0;
+    bool interleaved = false;
+    double magnitude = 1.0;
+    std::vector<double> frequency;         // [rot / 2], after scaling
+    unsigned long long *turns = nullptr;  // [rot / 2] on the device: 2^64 of a frequency as a fraction of a turn
+};
+
+namespace {
+
+void rope_drop(jitnn_hip_rope *r) {
+    if (r && r->turns) (void)hipFree(r->turns);
+    delete r;
+}
+
+// Frequencies, magnitude and the device's copy; the arguments have been checked.
+int rope_build(int rot, bool interleaved, double theta, const jitnn_hip_rope_scaling *sc, const float *factors, jitnn_hip_rope **out) {
+    jitnn_hip_rope *r = nullptr;
+    std::vector<unsigned long long> turns;
+    try {
+        r = new jitnn_hip_rope;
+        r->frequency.resize((size_t)rot / 2);
+        turns.resize((size_t)rot / 2);
+    } catch (const std::bad_alloc &) {
+        delete r;
+        return fail(JITNN_HIP_ENOMEM, "out of host memory");
+    }
+    r->rot = rot;
+    r->interleaved = interleaved;
+    const int kind = sc ? sc->kind : JITNN_HIP_ROPE_PLAIN;
+    constexpr double two_pi = 6.283185307179586476925;
+    double lo = 0, hi = 0;
+    if (kind == JITNN_HIP_ROPE_YARN) {
+        // the pair that turns beta times in the original context
+        auto pair_of = [&](double beta) { return rot * log(sc->original_context / (two_pi * beta)) / (2.0 * log(theta)); };
+        lo = std::max(0.0, floor(pair_of(sc->beta_fast)));
+        hi = std::min((double)rot - 1, ceil(pair_of(sc->beta_slow)));
+        r->magnitude = 0.1 * log(sc->factor) + 1.0;
+    }
+    if (sc && sc->attention_factor != 0.0) r->magnitude = sc->attention_factor;
+    for (int i = 0; i < rot / 2; ++i) {
+        double f = pow(theta, -2.0 * i / rot);
+        if (factors) f /= (double)factors[i];
+        if (kind == JITNN_HIP_ROPE_LINEAR) f /= sc->factor;
+        if (kind == JITNN_HIP_ROPE_YARN) {
+            const double ramp = std::min(1.0, std::max(0.0, (i - lo) / std::max(hi - lo, 0.001)));
+            f = f * (1.0 - ramp) + f / sc->factor * ramp;
+        }
+        r->frequency[i] = f;
+        const double turn = f / two_pi, part = turn - floor(turn);  // (positions are whole: whole turns of a frequency are none)
+        turns[i] = (unsigned long long)std::min(ldexp(part, 64), 18446744073709549568.0);
+    }
+    const size_t bytes = turns.size() * sizeof(turns[0]);
+    if (hipMalloc(&r->turns, bytes) != hipSuccess) {
+        (void)hipGetLastError();
+        r->turns = nullptr;
+        rope_drop(r);
+        return fail(JITNN_HIP_ENOMEM, "no %zu bytes of device memory for the rotary frequencies", bytes);
+    }
+    const hipError_t e = hipMemcpy(r->turns, turns.data(), bytes, hipMemcpyHostToDevice);
+    if (e != hipSuccess) {
+        rope_drop(r);
+        return fail(JITNN_HIP_EDEVICE, "copying the rotary frequencies: %s", hipGetErrorString(e));
+    }
+    *out = r;
+    return JITNN_HIP_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int jitnn_hip_rope_create(int rot_dim, int interleaved, double theta, const jitnn_hip_rope_scaling *scaling, const float *freq_factors, jitnn_hip_rope **out) {
+    if (!out) return fail(JITNN_HIP_EINVAL, "out is NULL");
+    *out = nullptr;
+    if (rot_dim < 2 || rot_dim > 1024 || rot_dim % 2 != 0) return fail(JITNN_HIP_EINVAL, "rot_dim %d (even, 2 to 1024)", rot_dim);
+    if (!(theta > 0) || !std::isfinite(theta)) return fail(JITNN_HIP_EINVAL, "theta %g", theta);
+    if (scaling) {
+        if (scaling->kind < JITNN_HIP_ROPE_PLAIN || scaling->kind > JITNN_HIP_ROPE_YARN) return fail(JITNN_HIP_EINVAL, "rotary scaling %d", scaling->kind);
+        if (scaling->kind != JITNN_HIP_ROPE_PLAIN && (!(scaling->factor > 0) || !std::isfinite(scaling->factor)))
+            return fail(JITNN_HIP_EINVAL, "rotary scaling factor %g", scaling->factor);
+        if (scaling->kind == JITNN_HIP_ROPE_YARN &&
+            (scaling->original_context < 1 || !(scaling->beta_slow > 0) || !(scaling->beta_fast >= scaling->beta_slow) || !std::isfinite(scaling->beta_fast) || theta == 1.0))
+            return fail(JITNN_HIP_EINVAL, "original context %d, beta_fast %g, beta_slow %g, theta %g", scaling->original_context, scaling->beta_fast, scaling->beta_slow, theta);
+        if (!std::isfinite(scaling->attention_factor) || scaling->attention_factor < 0) return fail(JITNN_HIP_EINVAL, "attention factor %g", scaling->attention_factor);
+    }
+    for (int i = 0; freq_factors && i < rot_dim / 2; ++i)
+        if (!(freq_factors[i] > 0) || !std::isfinite(freq_factors[i])) return fail(JITNN_HIP_EINVAL, "frequency factor %g of pair %d", (double)freq_factors[i], i);
+    if (int rc = check_ready()) return rc;
+    return rope_build(rot_dim, interleaved != 0, theta, scaling, freq_factors, out);
+}
+
+int jitnn_hip_rope_free(jitnn_hip_rope *r) {
+    rope_drop(r);
+    return JITNN_HIP_OK;
+}
+
+int jitnn_hip_rope_dev(const jitnn_hip_rope *r, const float *x_dev, long long x_stride, const int *positions_dev, int tokens, int heads, int head_dim, float *y_dev,
+                       long long y_stride, void *stream) {
+    if (!r) return fail(JITNN_HIP_EINVAL, "rope is NULL");
+    if (tokens < 0 || heads < 1 || head_dim < r->rot || head_dim > 65536 || heads > 65536)
+        return fail(JITNN_HIP_EINVAL, "%d tokens, %d heads of %d values (rot_dim %d)", tokens, heads, head_dim, r->rot);
+    if (tokens == 0) return JITNN_HIP_OK;
+    if (!x_dev || !positions_dev || !y_dev) return fail(JITNN_HIP_EINVAL, "NULL argument");
+    const long long row = (long long)heads * head_dim;
+    if (x_stride < row || y_stride < row) return fail(JITNN_HIP_EINVAL, "strides %lld and %lld of rows of %lld values", x_stride, y_stride, row);
+    if (x_dev == y_dev && x_stride != y_stride) return fail(JITNN_HIP_EINVAL, "in place with strides %lld and %lld", x_stride, y_stride);
+    RopeArgs a;
+    a.x = x_dev;
+    a.y = y_dev;
+    a.positions = positions_dev;
+    a.turns = r->turns;
+    a.x_stride = x_stride;
+    a.y_stride = y_stride;
+    a.magnitude = (float)r->magnitude;
+    a.tokens = tokens;
+    a.heads = heads;
+    a.D = head_dim;
+    a.rot = r->rot;
+    a.interleaved = r->interleaved;
+    rope_launch(a, g.cus, (hipStream_t)stream);
+    HIP_TRY(hipGetLastError());
+    return JITNN_HIP_OK;
+}
+
+}  // extern "C"
+
+// ================================================================================================ a batch over a paged cache
+
+struct jitnn_hip_paged_cache {
+    int layers, kv, hd, pages, page_tokens, type;
+    uint8_t *k, *v;
+    bool owned;
+    size_t page_bytes() const { return (size_t)kv * page_tokens * hd * (type == 0 ? 4 : 2); }
+    size_t layer_bytes() const { return page_bytes() * pages; }
+    int page_shift() const { return __builtin_ctz((unsigned)page_tokens); }
+};
+
+namespace {
+
+int check_cache(const jitnn_hip_paged_cache *c, int layer) {
+    if (!c) return fail(JITNN_HIP_EINVAL, "cache is NULL");
+    if (layer < 0 || layer >= c->layers) return fail(JITNN_HIP_EINVAL, "layer %d of %d", layer, c->layers);
+    return JITNN_HIP_OK;
+}
+
+// The numbers of a batch; what its arrays hold is the kernels' to check.
+int check_batch(const jitnn_hip_paged_cache *c, const jitnn_hip_batch *b) {
+    if (!b) return fail(JITNN_HIP_EINVAL, "batch is NULL");
+    if (b->sequences < 0 || b->tokens < 0 || b->max_tokens < 0 || b->max_len < 0 || b->shared_pages < 0 || b->table_stride < 0 || b->sequences > 65535)
+        return fail(JITNN_HIP_EINVAL, "%d sequences, %d tokens (at most %d each), lengths to %d, %d shared of %d pages", b->sequences, b->tokens, b->max_tokens, b->max_len,
+                    b->shared_pages, b->table_stride);
+    if (b->shared_pages > b->table_stride || (long long)b->max_len > (long long)b->table_stride * c->page_tokens)
+        return fail(JITNN_HIP_EINVAL, "lengths to %d and %d shared pages in tables of %d pages of %d", b->max_len, b->shared_pages, b->table_stride, c->page_tokens);
+    if (b->tokens > 0 && b->sequences > 0 && (!b->starts || !b->lens || (!b->tables && b->table_stride > 0))) return fail(JITNN_HIP_EINVAL, "NULL array of the batch");
+    return JITNN_HIP_OK;
+}
+
+// the positions that all sequences share (none behind the longest)
+int batch_shared(const jitnn_hip_paged_cache *c, const jitnn_hip_batch *b) {
+    return (int)(std::min<long long>(b->shared_pages, ((long long)b->max_len + c->page_tokens - 1) / c->page_tokens) * c->page_tokens);
+}
+
+int check_heads(const jitnn_hip_paged_cache *c, int heads) {
+    if (heads < 1 || heads > 65535 || heads % c->kv != 0) return fail(JITNN_HIP_EINVAL, "%d query heads over %d key/value heads", heads, c->kv);
+    return JITNN_HIP_OK;
+}
+
+AttnPlan attention_plan(const jitnn_hip_paged_cache *c, const jitnn_hip_batch *b, int heads) {
+    return paged_attn_plan(c->type == 1, c->hd, heads, c->kv, b->sequences, b->tokens, std::min(std::max(b->max_tokens, 1), b->tokens), b->max_len, batch_shared(c, b), g.cus);
+}
+
+// the size of a cache, or what is wrong with it
+long long cache_nbytes(int layers, int kv_heads, int head_dim, int pages, int page_tokens, int type) {
+    if (layers < 1 || kv_heads < 1 || kv_heads > 65535 || pages < 1) return fail(JITNN_HIP_EINVAL, "%d layers, %d key/value heads, %d pages", layers, kv_heads, pages);
+    if (head_dim != 64 && head_dim != 128 && head_dim != 192 && head_dim != 256) return fail(JITNN_HIP_EINVAL, "head_dim %d (64, 128, 192 and 256 are built)", head_dim);
+    if (page_tokens < 16 || page_tokens > 256 || (page_tokens & (page_tokens - 1)) != 0)
+        return fail(JITNN_HIP_EINVAL, "pages of %d positions (16, 32, 64, 128 or 256)", page_tokens);
+    if (type != 0 && type != 1) return fail(JITNN_HIP_EINVAL, "a cache of ggml type %d (F32 = 0 and F16 = 1 are built)", type);
+    const __int128 n = (__int128)layers * kv_heads * head_dim * pages * page_tokens * (type == 0 ? 4 : 2);
+    if (n > ((__int128)1 << 46)) return fail(JITNN_HIP_EINVAL, "%d layers of %d pages do not fit any memory", layers, pages);
+    return (long long)n;
+}
+
+int append_rows(const jitnn_hip_paged_cache *c, int layer, const jitnn_hip_batch *b, const jitnn_hip_rope *r, bool interleaved, const float *q_dev, long long q_stride,
+                int heads, float *q_out_dev, long long q_out_stride, const float *k_dev, long long k_stride, const float *v_dev, long long v_stride, hipStream_t stream) {
+    if (int rc = check_cache(c, layer)) return rc;
+    if (int rc = check_batch(c, b)) return rc;
+    if (heads < 0 || heads > 65535) return fail(JITNN_HIP_EINVAL, "%d query heads", heads);
+    if (b->tokens == 0 || b->sequences == 0) return JITNN_HIP_OK;
+    if (!k_dev || !v_dev || (heads > 0 && (!q_dev || !q_out_dev))) return fail(JITNN_HIP_EINVAL, "NULL argument");
+    const long long row = (long long)c->kv * c->hd, qrow = (long long)heads * c->hd;
+    if (k_stride < row || v_stride < row || (heads > 0 && (q_stride < qrow || q_out_stride < qrow)))
+        return fail(JITNN_HIP_EINVAL, "strides %lld, %lld, %lld, %lld of rows of %lld queries and %lld keys and values", q_stride, q_out_stride, k_stride, v_stride, qrow, row);
+    if (heads > 0 && q_dev == q_out_dev && q_stride != q_out_stride) return fail(JITNN_HIP_EINVAL, "in place with strides %lld and %lld", q_stride, q_out_stride);
+    if (r && r->rot > c->hd) return fail(JITNN_HIP_EINVAL, "rot_dim %d of heads of %d values", r->rot, c->hd);
+    if (r && r->rot % 8 != 0) return fail(JITNN_HIP_EUNSUPPORTED, "rot_dim %d is not a multiple of 8", r->rot);
+    const uintptr_t all = (uintptr_t)k_dev | (uintptr_t)v_dev | (heads > 0 ? (uintptr_t)q_dev | (uintptr_t)q_out_dev : 0);
+    if ((all & 15) != 0 || ((k_stride | v_stride | (heads > 0 ? q_stride | q_out_stride : 0)) & 3) != 0)
+        return fail(JITNN_HIP_EUNSUPPORTED, "rows that are not aligned to 16 bytes");
+    if (int rc = check_ready()) return rc;
+    AppendArgs a;
+    a.q = q_dev;
+    a.k = k_dev;
+    a.v = v_dev;
+    a.q_out = q_out_dev;
+    a.k_pages = c->k + (size_t)layer * c->layer_bytes();
+    a.v_pages = c->v + (size_t)layer * c->layer_bytes();
+    a.tables = b->tables;
+    a.starts = b->starts;
+    a.lens = b->lens;
+    a.turns = r ? r->turns : nullptr;
+    a.q_stride = q_stride;
+    a.q_out_stride = q_out_stride;
+    a.k_stride = k_stride;
+    a.v_stride = v_stride;
+    a.magnitude = r ? (float)r->magnitude : 1.f;
+    a.tokens = b->tokens;
+    a.sequences = b->sequences;
+    a.table_stride = b->table_stride;
+    a.pages = c->pages;
+    a.page_shift = c->page_shift();
+    a.heads = heads;
+    a.kv = c->kv;
+    a.D = c->hd;
+    a.rot = r ? r->rot : 0;
+    a.interleaved = interleaved;
+    paged_append_launch(c->type == 1, a, g.cus, stream);
+    HIP_TRY(hipGetLastError());
+    return JITNN_HIP_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+long long jitnn_hip_paged_cache_nbytes(int layers, int kv_heads, int head_dim, int pages, int page_tokens, int ggml_type) {
+    return cache_nbytes(layers, kv_heads, head_dim, pages, page_tokens, ggml_type);
+}
+
+int jitnn_hip_paged_cache_wrap_dev(void *k_dev, void *v_dev, int layers, int kv_heads, int head_dim, int pages, int page_tokens, int ggml_type,
+                                   jitnn_hip_paged_cache **out) {
+    if (!out) return fail(JITNN_HIP_EINVAL, "out is NULL");
+    *out = nullptr;
+    const long long n = cache_nbytes(layers, kv_heads, head_dim, pages, page_tokens, ggml_type);
+    if (n < 0) return (int)n;
+    if (!k_dev || !v_dev || ((uintptr_t)k_dev & 15) != 0 || ((uintptr_t)v_dev & 15) != 0) return fail(JITNN_HIP_EINVAL, "cache memory is NULL or not aligned to 16 bytes");
+    jitnn_hip_paged_cache *c = new (std::nothrow) jitnn_hip_paged_cache{layers, kv_heads, head_dim, pages, page_tokens, ggml_type, (uint8_t *)k_dev, (uint8_t *)v_dev, false};
+    if (!c) return fail(JITNN_HIP_ENOMEM, "out of host memory");
+    *out = c;
+    return JITNN_HIP_OK;
+}
+
+int jitnn_hip_paged_cache_create(int layers, int kv_heads, int head_dim, int pages, int page_tokens, int ggml_type, jitnn_hip_paged_cache **out) {
+    if (!out) return fail(JITNN_HIP_EINVAL, "out is NULL");
+    *out = nullptr;
+    const long long n = cache_nbytes(layers, kv_heads, head_dim, pages, page_tokens, ggml_type);
+    if (n < 0) return (int)n;
+    if (int rc = check_ready()) return rc;
+    void *k = nullptr, *v = nullptr;
+    if (hipMalloc(&k, (size_t)n) != hipSuccess || hipMalloc(&v, (size_t)n) != hipSuccess) {
+        (void)hipGetLastError();
+        if (k) (void)hipFree(k);
+        return fail(JITNN_HIP_ENOMEM, "no 2 x %lld bytes of device memory for the cache", n);
+    }
+    const int rc = jitnn_hip_paged_cache_wrap_dev(k, v, layers, kv_heads, head_dim, pages, page_tokens, ggml_type, out);
+    if (rc) {
+        (void)hipFree(k);
+        (void)hipFree(v);
+        return rc;
+    }
+    (*out)->owned = true;
+    return JITNN_HIP_OK;
+}
+
+int jitnn_hip_paged_cache_free(jitnn_hip_paged_cache *c) {
+    if (!c) return JITNN_HIP_OK;
+    if (c->owned) {
+        (void)hipFree(c->k);
+        (void)hipFree(c->v);
+    }
+    delete c;
+    return JITNN_HIP_OK;
+}
+
+int jitnn_hip_paged_cache_copy_page_dev(const jitnn_hip_paged_cache *c, int from, int to, void *stream) {
+    if (!c) return fail(JITNN_HIP_EINVAL, "cache is NULL");
+    if (from < 0 || from >= c->pages || to < 0 || to >= c->pages) return fail(JITNN_HIP_EINVAL, "page %d to %d of %d", from, to, c->pages);
+    if (from == to) return JITNN_HIP_OK;
+    if (int rc = check_ready()) return rc;
+    paged_copy_launch(c->k, c->v, (long long)c->page_bytes(), (long long)c->layer_bytes(), c->layers, from, to, (hipStream_t)stream);
+    HIP_TRY(hipGetLastError());
+    return JITNN_HIP_OK;
+}
+
+int jitnn_hip_paged_append_dev(const jitnn_hip_paged_cache *c, int layer, const jitnn_hip_batch *b, const jitnn_hip_rope *r, const float *q_dev, long long q_stride,
+                               int heads, float *q_out_dev, long long q_out_stride, const float *k_dev, long long k_stride, const float *v_dev, long long v_stride,
+                               void *stream) {
+    return append_rows(c, layer, b, r, r && r->interleaved, q_dev, q_stride, heads, q_out_dev, q_out_stride, k_dev, k_stride, v_dev, v_stride, (hipStream_t)stream);
+}
+
+long long jitnn_hip_paged_attention_workspace(const jitnn_hip_paged_cache *c, const jitnn_hip_batch *b, int heads) {
+    if (int rc = check_cache(c, 0)) return rc;
+    if (int rc = check_batch(c, b)) return rc;
+    if (int rc = check_heads(c, heads)) return rc;
+    if (b->tokens == 0 || b->sequences == 0) return 0;
+    if (int rc = check_ready()) return rc;
+    return (long long)attention_plan(c, b, heads).workspace(b->tokens, heads, c->hd);
+}
+
+int jitnn_hip_paged_attention_dev(const jitnn_hip_paged_cache *c, int layer, const jitnn_hip_batch *b, int heads, const float *q_dev, long long q_stride, float scale,
+                                  float *y_dev, long long y_stride, void *workspace_dev, long long workspace_bytes, void *stream) {
+    if (int rc = check_cache(c, layer)) return rc;
+    if (int rc = check_batch(c, b)) return rc;
+    if (int rc = check_heads(c, heads)) return rc;
+    if (!std::isfinite(scale)) return fail(JITNN_HIP_EINVAL, "scale %g", (double)scale);
+    if (b->tokens == 0 || b->sequences == 0) return JITNN_HIP_OK;
+    if (!q_dev || !y_dev) return fail(JITNN_HIP_EINVAL, "NULL argument");
+    const long long row = (long long)heads * c->hd;
+    if (q_stride < row || y_stride < row) return fail(JITNN_HIP_EINVAL, "strides %lld and %lld of rows of %lld values", q_stride, y_stride, row);
+    if (int rc = check_ready()) return rc;
+    const AttnPlan p = attention_plan(c, b, heads);
+    const size_t need = p.workspace(b->tokens, heads, c->hd);
+    if (need > 0 && (!workspace_dev || workspace_bytes < (long long)need || ((uintptr_t)workspace_dev & 15) != 0))
+        return fail(JITNN_HIP_EINVAL, "a workspace of %lld bytes, %zu are needed (aligned to 16)", workspace_dev ? workspace_bytes : 0ll, need);
+    const long long units = (long long)p.own.spans * c->kv * b->sequences * p.own.blocks + (long long)p.ahead.spans * c->kv * p.ahead.blocks,
+                    merges = ((long long)b->tokens * heads + 3) / 4;
+    if (units > (1 << 28) || merges > (1 << 28)) return fail(JITNN_HIP_EINVAL, "%d sequences of up to %d tokens are too many for one pass", b->sequences, b->max_tokens);
+    AttnArgs a;
+    a.k = c->k + (size_t)layer * c->layer_bytes();
+    a.v = c->v + (size_t)layer * c->layer_bytes();
+    a.q = q_dev;
+    a.y = y_dev;
+    a.part = need ? (float *)workspace_dev : nullptr;
+    a.stat = need ? a.part + (size_t)b->tokens * heads * p.spans() * c->hd : nullptr;
+    a.tables = b->tables;
+    a.starts = b->starts;
+    a.lens = b->lens;
+    a.q_stride = q_stride;
+    a.y_stride = y_stride;
+    a.scale = (float)((double)scale * 1.44269504088896340736);
+    a.tokens = b->tokens;
+    a.sequences = b->sequences;
+    a.heads = heads;
+    a.kv = c->kv;
+    a.pages = c->pages;
+    a.page_shift = c->page_shift();
+    a.table_stride = b->table_stride;
+    a.max_len = b->max_len;
+    a.shared = batch_shared(c, b);
+    a.ahead = p.ahead;
+    a.own = p.own;
+    paged_attn_launch(c->type == 1, c->hd, (hipStream_t)stream, a);
+    HIP_TRY(hipGetLastError());
+    return JITNN_HIP_OK;
+}
+
+// ---- drafted tokens
+
+static int check_drafts(int rows, int sequences, int vocab) {
+    if (rows < 0 || sequences < 0 || vocab < 1 || rows > 65535 || sequences > 65535)
+        return fail(JITNN_HIP_EINVAL, "%d rows of %d sequences (at most 65535) over a vocabulary of %d", rows, sequences, vocab);
+    return JITNN_HIP_OK;
+}
+
+long long jitnn_hip_verify_workspace(int rows, int sequences, int vocab) {
+    if (int rc = check_drafts(rows, sequences, vocab)) return rc;
+    return (long long)verify_workspace(rows, sequences, vocab);
+}
+
+int jitnn_hip_verify_drafts_dev(const float *logits_dev, long long logits_stride, int rows, int vocab, const int *starts_dev, int sequences, const int *tokens_dev,
+                                const float *draft_probs_dev, long long draft_stride, const float *temperatures_dev, const float *uniforms_dev, int *out_dev,
+                                int *accepted_dev, void *workspace_dev, long long workspace_bytes, void *stream) {
+    if (int rc = check_drafts(rows, sequences, vocab)) return rc;
+    if (sequences == 0) return JITNN_HIP_OK;
+    if (!starts_dev || !temperatures_dev || !accepted_dev || (rows > 0 && (!logits_dev || !tokens_dev || !uniforms_dev || !out_dev)))
+        return fail(JITNN_HIP_EINVAL, "NULL argument");
+    if (logits_stride < vocab || (draft_probs_dev && draft_stride < vocab)) return fail(JITNN_HIP_EINVAL, "strides %lld and %lld of rows of %d values", logits_stride, draft_stride, vocab);
+    const size_t need = verify_workspace(rows, sequences, vocab);
+    if (!workspace_dev || workspace_bytes < (long long)need || ((uintptr_t)workspace_dev & 15) != 0)
+        return fail(JITNN_HIP_EINVAL, "a workspace of %lld bytes, %zu are needed (aligned to 16)", workspace_dev ? workspace_bytes : 0ll, need);
+    if (int rc = check_ready()) return rc;
+    VerifyArgs a;
+    a.logits = logits_dev;
+    a.draft_probs = draft_probs_dev;
+    a.temperatures = temperatures_dev;
+    a.uniforms = uniforms_dev;
+    a.starts = starts_dev;
+    a.tokens = tokens_dev;
+    a.out = out_dev;
+    a.accepted = accepted_dev;
+    a.part = workspace_dev;
+    a.logits_stride = logits_stride;
+    a.draft_stride = draft_stride;
+    a.rows = rows;
+    a.vocab = vocab;
+    a.sequences = sequences;
+    a.chunks = 0;
+    verify_launch(a, (hipStream_t)stream);
+    HIP_TRY(hipGetLastError());
+    return JITNN_HIP_OK;
+}
+
+}  // extern "C"
+
 // ================================================================================================ decode step
 
 struct jitnn_hip_llama {
@@ -1925,6 +2333,9 @@ struct jitnn_hip_llama {
     bool no_packing;    // the caller's wish: packed stays as it is and unused
     int attention;      // the PromptAttention of the last prompt pass, -1: there was none
     int rope_interleaved;  // 0: rotate-half pairs (i, i + D/2); 1: pairs (2i, 2i + 1)
+    jitnn_hip_rope *rope;  // what cosv and sinv hold, for positions of a paged cache (the pairing is rope_interleaved)
+    void *paged_ws;        // workspace of the attention over a paged cache, grown by jitnn_hip_llama_step_dev
+    size_t paged_ws_bytes;
     // token embedding table [vocab, d] in ggml type embd_fmt (F32 = 0, F16 = 1 or a block format), owned
     uint8_t *embd;
     int embd_fmt;
@@ -2257,6 +2668,76 @@ int launch_attention_rows(const jitnn_hip_llama *m, int layer, int pos0, int tok
     return JITNN_HIP_OK;
 }
 
+// The layers of a pass over T rows x [T, d]: attend(layer, q, k, v, att, pending) turns the queries, appends keys and values and writes the
+// attention's output.  defer: q, k and v may reach it in K slices (pending.part).  *out: the rows behind the last layer, in a buffer of the model.
+template <class Attend>
+int run_layers(jitnn_hip_llama *m, const float *x_dev, int T, bool defer, hipStream_t st, const float **out, Attend &&attend) {
+    const int d = m->d;
+    float *xn = m->pf[0], *q = m->pf[1], *k = m->pf[2], *v = m->pf[3], *att = m->pf[4], *xa = m->pf[5], *xb = m->pf[6], *gate = m->pf[7],
+          *up = m->pf[8], *h = m->pf[9];
+    const float *x = x_dev;
+    PfPending pend;  // the K slices of the linear that wrote x, when their join is still to come
+    PfGroupPending gp;  // the K slices of q, k and v between their launch and the rotation
+    for (int l = 0; l < m->layers; ++l) {
+        const jitnn_hip_weight *const *w = m->w + (size_t)l * 7;
+        const float *nw = m->norms + (size_t)l * 2 * d;
+        {
+            const jitnn_hip_weight *ws[3] = {w[JITNN_HIP_W_ATTN_Q], w[JITNN_HIP_W_ATTN_K], w[JITNN_HIP_W_ATTN_V]};
+            float *ys[3] = {q, k, v};
+            if (int rc = normed_linears_rows(m, ws, ys, 3, x, T, nw, xn, st, &pend, defer ? &gp : nullptr)) return rc;
+        }
+        if (int rc = attend(l, q, k, v, att, gp)) return rc;
+        // xa = x + Wo att, xb = xa + W2 (silu(W1 n) * (W3 n)), n = RMSNorm(xa)
+        if (int rc = residual_linear_rows(w[JITNN_HIP_W_ATTN_O], att, T, x, xn, xa, st, nullptr, nullptr, m->pf[10], &pend)) return rc;
+        if (T > g.gemv_max_rows && prefill_dual_ok(w[JITNN_HIP_W_FFN_GATE], w[JITNN_HIP_W_FFN_UP])) {
+            // gate and up as one product with the SwiGLU in its epilogue: h = silu(W1 n) * (W3 n) directly
+            const bool fused = pend.part && pend.out == xa && pend.n == d;
+            if (!fused) flush_pending(pend, T, st);
+            const int rc = launch_prefill_dual(w[JITNN_HIP_W_FFN_GATE], w[JITNN_HIP_W_FFN_UP], h, xa, T, nw + d, m->eps, st, fused ? &pend : nullptr);
+            if (fused) pend = PfPending{};
+            if (rc) return rc;
+            if (int rc2 = residual_linear_rows(w[JITNN_HIP_W_FFN_DOWN], h, T, xa, xn, xb, st, nullptr, nullptr, m->pf[10], &pend)) return rc2;
+        } else {
+            const jitnn_hip_weight *ws[2] = {w[JITNN_HIP_W_FFN_GATE], w[JITNN_HIP_W_FFN_UP]};
+            float *ys[2] = {gate, up};
+            RowsFfn ffn;
+            if (T <= g.gemv_max_rows && rows_ffn_pays(ws[0], ws[1], w[JITNN_HIP_W_FFN_DOWN], T, st, &ffn)) {
+                norm_rows(m, xa, T, nw + d, xn, st, &pend);
+                if (int rc = launch_rows_ffn(ffn, ws[0], ws[1], w[JITNN_HIP_W_FFN_DOWN], xn, T, xa, xb, st, m->pf[10], &pend)) return rc;
+            } else {
+                if (int rc = normed_linears_rows(m, ws, ys, 2, xa, T, nw + d, xn, st, &pend)) return rc;
+                if (int rc = residual_linear_rows(w[JITNN_HIP_W_FFN_DOWN], gate, T, xa, xn, xb, st, up, h, m->pf[10], &pend)) return rc;
+            }
+        }
+        x = xb;
+    }
+    flush_pending(pend, T, st);  // the last layer's output exists whole
+    *out = x;
+    return JITNN_HIP_OK;
+}
+
+// cos/sin of t * base^(-2i/D) in double, stored FP32: Rope.tables (core/ops/Rope.java:86-102); other frequencies and a magnitude where the model has
+// been given some.  Pairs behind the rotated part do not turn.
+bool rope_tables(jitnn_hip_llama *m, const jitnn_hip_rope *r) {
+    const int half = m->hd / 2;
+    float *c = new (std::nothrow) float[(size_t)m->max_ctx * half], *s = new (std::nothrow) float[(size_t)m->max_ctx * half];
+    bool ok = c && s;
+    if (ok) {
+        for (int t = 0; t < m->max_ctx; ++t)
+            for (int i = 0; i < half; ++i) {
+                const bool turns = i < r->rot / 2;
+                const double angle = turns ? t * r->frequency[i] : 0.0, magnitude = turns ? r->magnitude : 1.0;
+                c[(size_t)t * half + i] = (float)(magnitude * cos(angle));
+                s[(size_t)t * half + i] = (float)(magnitude * sin(angle));
+            }
+        ok = hipMemcpy(m->cosv, c, (size_t)m->max_ctx * half * 4, hipMemcpyHostToDevice) == hipSuccess &&
+             hipMemcpy(m->sinv, s, (size_t)m->max_ctx * half * 4, hipMemcpyHostToDevice) == hipSuccess;
+    }
+    delete[] c;
+    delete[] s;
+    return ok;
+}
+
 }  // namespace
 
 extern "C" {
@@ -2297,24 +2778,7 @@ int jitnn_hip_llama_create(int layers, int d_model, int heads, int kv_heads, int
         m->k = m->q + qd;
         m->v = m->k + kd;
     }
-    if (ok) {
-        // cos/sin of t * base^(-2i/D) in double, stored FP32: Rope.tables (core/ops/Rope.java:86-102)
-        float *c = new (std::nothrow) float[(size_t)max_ctx * half], *s = new (std::nothrow) float[(size_t)max_ctx * half];
-        ok = c && s;
-        if (ok) {
-            for (int t = 0; t < max_ctx; ++t)
-                for (int i = 0; i < half; ++i) {
-                    const double frequency = pow((double)rope_theta, -2.0 * i / head_dim);
-                    const double angle = t * frequency;
-                    c[(size_t)t * half + i] = (float)cos(angle);
-                    s[(size_t)t * half + i] = (float)sin(angle);
-                }
-            ok = hipMemcpy(m->cosv, c, (size_t)max_ctx * half * 4, hipMemcpyHostToDevice) == hipSuccess &&
-                 hipMemcpy(m->sinv, s, (size_t)max_ctx * half * 4, hipMemcpyHostToDevice) == hipSuccess;
-        }
-        delete[] c;
-        delete[] s;
-    }
+    ok = ok && rope_build(head_dim, false, (double)rope_theta, nullptr, nullptr, &m->rope) == JITNN_HIP_OK && rope_tables(m, m->rope);
     if (!ok) {
         jitnn_hip_llama_free(m);
         return fail(JITNN_HIP_ENOMEM, "allocating the model buffers (%zu bytes of KV cache) failed", 2 * cache * sizeof(float));
@@ -2331,6 +2795,8 @@ int jitnn_hip_llama_free(jitnn_hip_llama *m) {
     for (float *b : m->pf)
         if (b) (void)hipFree(b);
     if (m->packed) (void)hipFree(m->packed);
+    if (m->paged_ws) (void)hipFree(m->paged_ws);
+    rope_drop(m->rope);
     if (m->embd) (void)hipFree(m->embd);
     if (m->tok_dev) (void)hipFree(m->tok_dev);
     if (m->tok_pin) (void)hipHostFree(m->tok_pin);
@@ -2457,25 +2923,14 @@ int jitnn_hip_llama_prefill_dev(jitnn_hip_llama *m, const float *x_dev, int pos0
     hipStream_t st = (hipStream_t)stream;
     count_op(ST_PREFILL, model_weight_bytes(m) + 4ll * m->layers * 2 * (pos0 + tokens) * m->kv * m->hd + 4ll * ((long long)tokens * m->d + (logits_dev ? m->vocab : 0)));
     StatNest nest;
-    const int d = m->d, T = tokens, qd = m->heads * m->hd;
+    const int d = m->d, T = tokens;
     prefill_reserve(m, T, st);
     PromptAttention how = prompt_attention(m->hd, m->heads, m->kv, pos0, T, !m->no_packing, g.cus);
     if (how == ATTN_PACKED && !packed_room(m, st)) how = prompt_attention(m->hd, m->heads, m->kv, pos0, T, false, g.cus);
     m->attention = how;
-    float *xn = m->pf[0], *q = m->pf[1], *k = m->pf[2], *v = m->pf[3], *att = m->pf[4], *xa = m->pf[5], *xb = m->pf[6], *gate = m->pf[7],
-          *up = m->pf[8], *h = m->pf[9];
-    const float *x = x_dev;
-    PfPending pend;  // the K slices of the linear that wrote x, when their join is still to come
-    PfGroupPending gp;  // the K slices of q, k and v between their launch and the rotation
-    for (int l = 0; l < m->layers; ++l) {
-        const jitnn_hip_weight *const *w = m->w + (size_t)l * 7;
-        const float *nw = m->norms + (size_t)l * 2 * d;
+    const float *x = nullptr;
+    const int rc = run_layers(m, x_dev, T, true, st, &x, [&](int l, float *q, const float *k, const float *v, float *att, PfGroupPending &gp) {
         const size_t lo = (size_t)l * m->max_ctx * m->kv * m->hd;
-        {
-            const jitnn_hip_weight *ws[3] = {w[JITNN_HIP_W_ATTN_Q], w[JITNN_HIP_W_ATTN_K], w[JITNN_HIP_W_ATTN_V]};
-            float *ys[3] = {q, k, v};
-            if (int rc = normed_linears_rows(m, ws, ys, 3, x, T, nw, xn, st, &pend, &gp)) return rc;
-        }
         if (gp.part) {  // q, k and v still lie in K slices: the rotation adds them up as it reads them
             hipLaunchKernelGGL(rope_append_rows_join_kernel, dim3(T, T < 256 ? 4 : 1), dim3(256), 0, st, gp.part, gp.sg.splits[0], gp.sg.splits[1], gp.sg.splits[2], T, q,
                                m->kc + lo, m->vc + lo, m->cosv, m->sinv, m->heads, m->kv, m->hd, pos0, m->rope_interleaved);
@@ -2484,44 +2939,103 @@ int jitnn_hip_llama_prefill_dev(jitnn_hip_llama *m, const float *x_dev, int pos0
             hipLaunchKernelGGL(rope_append_rows_kernel, dim3(T, T < 256 ? 4 : 1), dim3(256), 0, st, q, k, v, m->kc + lo, m->vc + lo, m->cosv, m->sinv, m->heads, m->kv,
                                m->hd, pos0, m->rope_interleaved);
         }
-        int arc;
         switch (m->hd) {
-        case 64: arc = launch_attention_rows<64>(m, l, pos0, T, how, q, att, st); break;
-        case 128: arc = launch_attention_rows<128>(m, l, pos0, T, how, q, att, st); break;
-        case 192: arc = launch_attention_rows<192>(m, l, pos0, T, how, q, att, st); break;
-        default: arc = launch_attention_rows<256>(m, l, pos0, T, how, q, att, st); break;
+        case 64: return launch_attention_rows<64>(m, l, pos0, T, how, q, att, st);
+        case 128: return launch_attention_rows<128>(m, l, pos0, T, how, q, att, st);
+        case 192: return launch_attention_rows<192>(m, l, pos0, T, how, q, att, st);
+        default: return launch_attention_rows<256>(m, l, pos0, T, how, q, att, st);
         }
-        if (arc) return arc;
-        // xa = x + Wo att, xb = xa + W2 (silu(W1 n) * (W3 n)), n = RMSNorm(xa)
-        if (int rc = residual_linear_rows(w[JITNN_HIP_W_ATTN_O], att, T, x, xn, xa, st, nullptr, nullptr, m->pf[10], &pend)) return rc;
-        if (T > g.gemv_max_rows && prefill_dual_ok(w[JITNN_HIP_W_FFN_GATE], w[JITNN_HIP_W_FFN_UP])) {
-            // gate and up as one product with the SwiGLU in its epilogue: h = silu(W1 n) * (W3 n) directly
-            const bool fused = pend.part && pend.out == xa && pend.n == d;
-            if (!fused) flush_pending(pend, T, st);
-            const int rc = launch_prefill_dual(w[JITNN_HIP_W_FFN_GATE], w[JITNN_HIP_W_FFN_UP], h, xa, T, nw + d, m->eps, st, fused ? &pend : nullptr);
-            if (fused) pend = PfPending{};
-            if (rc) return rc;
-            if (int rc2 = residual_linear_rows(w[JITNN_HIP_W_FFN_DOWN], h, T, xa, xn, xb, st, nullptr, nullptr, m->pf[10], &pend)) return rc2;
-        } else {
-            const jitnn_hip_weight *ws[2] = {w[JITNN_HIP_W_FFN_GATE], w[JITNN_HIP_W_FFN_UP]};
-            float *ys[2] = {gate, up};
-            RowsFfn ffn;
-            if (T <= g.gemv_max_rows && rows_ffn_pays(ws[0], ws[1], w[JITNN_HIP_W_FFN_DOWN], T, st, &ffn)) {
-                norm_rows(m, xa, T, nw + d, xn, st, &pend);
-                if (int rc = launch_rows_ffn(ffn, ws[0], ws[1], w[JITNN_HIP_W_FFN_DOWN], xn, T, xa, xb, st, m->pf[10], &pend)) return rc;
-            } else {
-                if (int rc = normed_linears_rows(m, ws, ys, 2, xa, T, nw + d, xn, st, &pend)) return rc;
-                if (int rc = residual_linear_rows(w[JITNN_HIP_W_FFN_DOWN], gate, T, xa, xn, xb, st, up, h, m->pf[10], &pend)) return rc;
-            }
-        }
-        x = xb;
-    }
-    (void)qd;
-    flush_pending(pend, T, st);  // the last layer's output exists whole
+    });
+    if (rc) return rc;
     if (logits_dev) {  // the last token's logits
         const jitnn_hip_weight *ws[1] = {m->w_out};
         float *ys[1] = {logits_dev};
-        if (int rc = normed_linears(m, ws, ys, 1, x + (size_t)(T - 1) * d, m->norms + (size_t)m->layers * 2 * d, st)) return rc;
+        if (int rc2 = normed_linears(m, ws, ys, 1, x + (size_t)(T - 1) * d, m->norms + (size_t)m->layers * 2 * d, st)) return rc2;
+    }
+    HIP_TRY(hipGetLastError());
+    return JITNN_HIP_OK;
+}
+
+int jitnn_hip_llama_set_rope(jitnn_hip_llama *m, const jitnn_hip_rope *r) {
+    if (!m || !r) return fail(JITNN_HIP_EINVAL, "model or rope is NULL");
+    if (r->rot > m->hd || (r->rot < m->hd && !r->interleaved))
+        return fail(JITNN_HIP_EINVAL, "rot_dim %d of heads of %d values (a part of a head: interleaved pairs only)", r->rot, m->hd);
+    if (int rc = check_ready()) return rc;
+    jitnn_hip_rope *copy = nullptr;
+    const size_t bytes = (size_t)r->rot / 2 * sizeof(unsigned long long);
+    try {
+        copy = new jitnn_hip_rope(*r);
+    } catch (const std::bad_alloc &) {
+        return fail(JITNN_HIP_ENOMEM, "out of host memory");
+    }
+    copy->turns = nullptr;
+    if (hipMalloc(&copy->turns, bytes) != hipSuccess) {
+        (void)hipGetLastError();
+        copy->turns = nullptr;
+        rope_drop(copy);
+        return fail(JITNN_HIP_ENOMEM, "no %zu bytes of device memory for the rotary frequencies", bytes);
+    }
+    const hipError_t e = hipMemcpy(copy->turns, r->turns, bytes, hipMemcpyDeviceToDevice);
+    if (e != hipSuccess || !rope_tables(m, copy)) {
+        rope_drop(copy);
+        return fail(JITNN_HIP_EDEVICE, "copying the rotary tables: %s", hipGetErrorString(e));
+    }
+    rope_drop(m->rope);
+    m->rope = copy;
+    m->rope_interleaved = copy->interleaved;
+    return JITNN_HIP_OK;
+}
+
+int jitnn_hip_llama_step_dev(jitnn_hip_llama *m, const jitnn_hip_paged_cache *c, const jitnn_hip_batch *b, const float *x_dev, const int *logit_rows_dev, int logit_count,
+                             float *logits_dev, void *stream) {
+    if (int rc = check_model(m)) return rc;
+    if (int rc = check_cache(c, 0)) return rc;
+    if (int rc = check_batch(c, b)) return rc;
+    if (c->layers != m->layers || c->kv != m->kv || c->hd != m->hd)
+        return fail(JITNN_HIP_EINVAL, "a cache of %d layers of %d heads of %d values for a model of %d layers of %d of %d", c->layers, c->kv, c->hd, m->layers, m->kv, m->hd);
+    if (logit_count < 0 || logit_count > b->tokens || (logit_count > 0 && (!logit_rows_dev || !logits_dev)))
+        return fail(JITNN_HIP_EINVAL, "logits of %d rows of %d", logit_count, b->tokens);
+    if (m->d % 4 != 0) return fail(JITNN_HIP_EUNSUPPORTED, "d_model %d is not a multiple of 4", m->d);
+    if (m->rope->rot % 8 != 0) return fail(JITNN_HIP_EUNSUPPORTED, "rot_dim %d is not a multiple of 8", m->rope->rot);
+    if (b->tokens == 0 || b->sequences == 0) return JITNN_HIP_OK;
+    if (!x_dev) return fail(JITNN_HIP_EINVAL, "input is NULL");
+    hipStream_t st = (hipStream_t)stream;
+    const int d = m->d, T = b->tokens;
+    const long long need = jitnn_hip_paged_attention_workspace(c, b, m->heads);
+    if (need < 0) return (int)need;
+    if ((T > m->pf_cap || (size_t)need > m->paged_ws_bytes) && stream_recording(st))
+        return fail(JITNN_HIP_EINVAL, "a pass of %d tokens needs larger buffers than the model has, which a recording cannot allocate", T);
+    if (int rc = ensure_prefill(m, T)) return rc;
+    if ((size_t)need > m->paged_ws_bytes) {
+        HIP_TRY(hipDeviceSynchronize());  // earlier passes may still use the old one
+        if (m->paged_ws) (void)hipFree(m->paged_ws);
+        m->paged_ws = nullptr;
+        m->paged_ws_bytes = 0;
+        if (hipMalloc(&m->paged_ws, (size_t)need) != hipSuccess) {
+            (void)hipGetLastError();
+            m->paged_ws = nullptr;
+            return fail(JITNN_HIP_ENOMEM, "no %lld bytes of device memory for the attention's workspace", need);
+        }
+        m->paged_ws_bytes = (size_t)need;
+    }
+    count_op(ST_PREFILL, model_weight_bytes(m) + 4ll * ((long long)T * d + (long long)logit_count * m->vocab));
+    StatNest nest;
+    prefill_reserve(m, T, st);
+    const long long qd = (long long)m->heads * m->hd, kd = (long long)m->kv * m->hd;
+    const float scale = 1.0f / sqrtf((float)m->hd);
+    const float *x = nullptr;
+    const int rc = run_layers(m, x_dev, T, false, st, &x, [&](int l, float *q, const float *k, const float *v, float *att, PfGroupPending &) {
+        if (int arc = append_rows(c, l, b, m->rope, m->rope_interleaved != 0, q, qd, m->heads, q, qd, k, kd, v, kd, st)) return arc;
+        return jitnn_hip_paged_attention_dev(c, l, b, m->heads, q, qd, scale, att, qd, m->paged_ws, (long long)m->paged_ws_bytes, stream);
+    });
+    if (rc) return rc;
+    if (logit_count > 0) {
+        float *rows = m->pf[5], *xn = m->pf[0];  // (free behind the last layer)
+        hipLaunchKernelGGL(embed_plain_rows_kernel, dim3((unsigned)logit_count), dim3(256), 0, st, (const void *)x, 0, logit_rows_dev, rows, d, T);
+        const jitnn_hip_weight *ws[1] = {m->w_out};
+        float *ys[1] = {logits_dev};
+        const float *nw = m->norms + (size_t)m->layers * 2 * d;
+        if (int rc2 = logit_count == 1 ? normed_linears(m, ws, ys, 1, rows, nw, st) : normed_linears_rows(m, ws, ys, 1, rows, logit_count, nw, xn, st)) return rc2;
     }
     HIP_TRY(hipGetLastError());
     return JITNN_HIP_OK;
@@ -2553,6 +3067,7 @@ int jitnn_hip_llama_last_attention(const jitnn_hip_llama *m) {
 
 int jitnn_hip_llama_set_rope_interleaved(jitnn_hip_llama *m, int interleaved) {
     if (!m) return fail(JITNN_HIP_EINVAL, "model is NULL");
+    if (!interleaved && m->rope->rot < m->hd) return fail(JITNN_HIP_EINVAL, "%d of %d values of a head turn: interleaved pairs only", m->rope->rot, m->hd);
     m->rope_interleaved = interleaved != 0;
     return JITNN_HIP_OK;
 }

@@ -1,0 +1,102 @@
+// Launches of the operators of a served batch: rotary positions, the paged cache's append, the plan and the merge of its attention (whose kernels
+// are in paged_f16.hip and paged_f32.hip), the verification of drafted tokens.
+#include "serving.h"
+
+#include <algorithm>
+#include <cmath>
+
+#include "paged_attn.h"
+#include "rope.h"
+#include "verify.h"
+
+namespace jitnn {
+
+static bool aligned16(const void *p, long long stride) { return ((uintptr_t)p & 15) == 0 && stride % 4 == 0; }
+
+void rope_launch(const RopeArgs &a, int cus, hipStream_t s) {
+    const bool items = a.rot % 8 == 0 && a.D % 8 == 0 && aligned16(a.x, a.x_stride) && aligned16(a.y, a.y_stride);
+    const long long count = (long long)a.tokens * a.heads * (items ? a.D / 8 : (a.D + 1) / 2);
+    const unsigned blocks = (unsigned)std::min<long long>((count + ROPE_THREADS - 1) / ROPE_THREADS, (long long)cus * 64);
+    if (items) hipLaunchKernelGGL(rope_kernel, dim3(blocks), dim3(ROPE_THREADS), 0, s, a);
+    else hipLaunchKernelGGL(rope_pairs_kernel, dim3(blocks), dim3(ROPE_THREADS), 0, s, a);
+}
+
+void paged_append_launch(bool half, AppendArgs a, int cus, hipStream_t s) {
+    const long long n = (long long)(a.heads + 2 * a.kv) * (a.D / 8);  // items of a token
+    a.per_block = (int)std::min<long long>(std::max<long long>(1, ROPE_THREADS / n), APPEND_TOKENS);
+    const unsigned blocks = (unsigned)((a.tokens + a.per_block - 1) / a.per_block);
+    // few tokens: several workgroups to a token's heads
+    const unsigned shares = (unsigned)std::max<long long>(1, std::min<long long>((n * a.per_block + ROPE_THREADS - 1) / ROPE_THREADS, 4ll * cus / blocks));
+    if (half) hipLaunchKernelGGL(paged_append_kernel<_Float16>, dim3(blocks, shares), dim3(ROPE_THREADS), 0, s, a);
+    else hipLaunchKernelGGL(paged_append_kernel<float>, dim3(blocks, shares), dim3(ROPE_THREADS), 0, s, a);
+}
+
+void paged_copy_launch(void *k, void *v, long long page_bytes, long long layer_bytes, int layers, int from, int to, hipStream_t s) {
+    const long long page16 = page_bytes / 16;
+    hipLaunchKernelGGL(paged_copy_kernel, dim3((unsigned)std::min<long long>((page16 + 255) / 256, 64), layers, 2), dim3(256), 0, s, (uint4 *)k, (uint4 *)v, page16,
+                       layer_bytes / 16, from, to);
+}
+
+// ---- attention
+
+// How the rows of a part go to workgroups: few rows, all four waves on keys of their own; many, two tiles of rows to a wave (heads of
+// up to 128 values: their queries and outputs leave the registers for it) and all waves on the same keys.
+static AttnPart rows_shape(long long rows, int D) {
+    AttnPart p;
+    p.tiles = D <= 128 && rows > 16 ? 2 : 1;
+    p.key_waves = rows <= 16 * p.tiles ? 4 : rows <= 32 * p.tiles ? 2 : 1;
+    const int per = 16 * p.tiles * (PA_WAVES / p.key_waves);
+    p.blocks = (int)std::min<long long>((rows + per - 1) / per, 1 << 24);
+    return p;
+}
+
+AttnPlan paged_attn_plan(bool half, int D, int heads, int kv, int sequences, long long tokens, int max_tokens, int max_len, int shared, int cus) {
+    const int group = heads / kv, keys = half ? 32 : 16;
+    AttnPlan p;
+    if (shared > 0) p.ahead = rows_shape(tokens * group, D);
+    p.own = rows_shape((long long)max_tokens * group, D);
+    // spans of about equal time, for four workgroups to a CU
+    auto step = [](const AttnPart &q) { return q.tiles == 2 ? 1.6 : 1.0; };  // of a wave, in units of one tile's
+    const double own_len = std::max(max_len - shared, 1);
+    auto work = [&](const AttnPart &q, double n, double len) { return n * q.blocks * kv * len / q.key_waves * step(q); };
+    const double all = (shared > 0 ? work(p.ahead, 1, shared) : 0) + work(p.own, sequences, own_len), each = all / (4. * cus);
+    auto cut = [&](AttnPart &q, double len) {
+        const int least = keys * q.key_waves;  // one step of every wave
+        const double want = std::max(each * q.key_waves / step(q), len / 128);
+        q.span = (int)std::min<double>(std::ceil(want / least) * least, std::ceil(len / least) * least);
+        q.spans = (int)((len + q.span - 1) / q.span);
+    };
+    if (shared > 0) cut(p.ahead, shared);
+    cut(p.own, own_len);
+    return p;
+}
+
+void paged_attn_launch(bool half, int D, hipStream_t s, const AttnArgs &a) {
+    const unsigned units_ahead = (unsigned)(a.ahead.spans * a.kv), units_own = (unsigned)(a.own.spans * a.kv * a.sequences);
+    const unsigned blocks = (units_ahead + 7) / 8 * 8 * (unsigned)a.ahead.blocks + (units_own + 7) / 8 * 8 * (unsigned)a.own.blocks;
+    if (half) paged_attn_launch_f16(D, blocks, s, a);
+    else paged_attn_launch_f32(D, blocks, s, a);
+    if (a.ahead.spans + a.own.spans == 1) return;
+    const unsigned merge = (unsigned)(((long long)a.tokens * a.heads + 3) / 4);
+    switch (D) {
+    case 64: hipLaunchKernelGGL(paged_merge_kernel<64>, dim3(merge), dim3(256), 0, s, a); break;
+    case 128: hipLaunchKernelGGL(paged_merge_kernel<128>, dim3(merge), dim3(256), 0, s, a); break;
+    case 192: hipLaunchKernelGGL(paged_merge_kernel<192>, dim3(merge), dim3(256), 0, s, a); break;
+    default: hipLaunchKernelGGL(paged_merge_kernel<256>, dim3(merge), dim3(256), 0, s, a); break;
+    }
+}
+
+// ---- verification
+
+static int verify_chunks(int vocab) { return (vocab + VERIFY_CHUNK - 1) / VERIFY_CHUNK; }
+size_t verify_workspace(int rows, int sequences, int vocab) {
+    return (size_t)verify_chunks(vocab) * ((size_t)rows * sizeof(VerifyStat) + (size_t)sequences * sizeof(double));
+}
+void verify_launch(VerifyArgs a, hipStream_t s) {
+    a.chunks = verify_chunks(a.vocab);
+    hipLaunchKernelGGL(verify_stats_kernel, dim3(a.chunks, a.rows), dim3(VERIFY_THREADS), 0, s, a);
+    if (a.draft_probs) hipLaunchKernelGGL(verify_rest_kernel, dim3(a.chunks, a.sequences), dim3(VERIFY_THREADS), 0, s, a);
+    hipLaunchKernelGGL(verify_draw_kernel, dim3(a.sequences), dim3(VERIFY_DRAW_THREADS), 0, s, a);
+}
+
+}  // namespace jitnn

@@ -1,0 +1,126 @@
+"""Operators of a served batch (jitnn_hip_rope_*, jitnn_hip_paged_*, jitnn_hip_verify_*): rotary positions, a paged cache of keys and values with its
+append and its attention, and the verification of drafted tokens.  `*_ptr` arguments are addresses in device memory, `stream_ptr` a hipStream_t (0:
+the null stream); the calls only enqueue.  What each does, checks and leaves alone is said in include/jitnn_hip.h.
+
+The reference has the plain rotary embedding (core/ops/Rope.java:86-150) and attention without a cache (core/F.java:588-624); batches over a cache
+are its third-party engine's."""
+from __future__ import annotations
+
+import ctypes as C
+import weakref
+
+import numpy as np
+
+from . import _lib
+from ._lib import Batch  # noqa: F401
+
+ROPE_KINDS = {None: 0, "none": 0, "linear": 1, "yarn": 2}
+
+
+class Rope:
+    """The frequencies of rotary positions: `rot_dim` values of a head in pairs (i, i + rot_dim / 2), or (2 i, 2 i + 1) when interleaved.
+    scaling None, "linear" or "yarn" by `factor`; freq_factors [rot_dim / 2] divide the frequencies (rope_freqs.weight of GGUF files)."""
+
+    def __init__(self, rot_dim, theta=10000.0, interleaved=False, scaling=None, factor=1.0, original_context=0, beta_fast=32.0, beta_slow=1.0,
+                 attention_factor=0.0, freq_factors=None):
+        if scaling not in ROPE_KINDS:
+            raise ValueError(f"rotary scaling {scaling!r} (None, 'linear' and 'yarn' are built)")
+        factors = None if freq_factors is None else np.ascontiguousarray(freq_factors, dtype=np.float32).reshape(-1)
+        if factors is not None and factors.size != rot_dim // 2:
+            raise ValueError(f"{factors.size} frequency factors for {rot_dim // 2} pairs")
+        _lib.init()
+        sc = _lib.RopeScaling(ROPE_KINDS[scaling], original_context, factor, beta_fast, beta_slow, attention_factor)
+        h = C.c_void_p()
+        _lib.check(_lib.lib.jitnn_hip_rope_create(rot_dim, bool(interleaved), theta, C.byref(sc),
+                                                  None if factors is None else factors.ctypes.data_as(C.POINTER(C.c_float)), C.byref(h)), "jitnn_hip_rope_create")
+        self.rot_dim, self.interleaved, self._h = rot_dim, bool(interleaved), h
+        weakref.finalize(self, _lib.lib.jitnn_hip_rope_free, h)
+
+    @property
+    def handle(self):
+        return self._h
+
+    def apply_dev(self, x_ptr: int, positions_ptr: int, tokens: int, heads: int, head_dim: int, y_ptr: int, x_stride: int = 0, y_stride: int = 0,
+                  stream_ptr: int = 0) -> None:
+        """y [tokens, heads, head_dim] = x, token t turned by positions[t]; y may be x.  Strides in floats from token to token (0: dense)."""
+        dense = heads * head_dim
+        rc = _lib.lib.jitnn_hip_rope_dev(self._h, x_ptr, x_stride or dense, positions_ptr, tokens, heads, head_dim, y_ptr, y_stride or dense, stream_ptr)
+        if rc:
+            _lib.check(rc, "jitnn_hip_rope_dev")
+
+
+class PagedCache:
+    """Keys and values of many sequences in `pages` pages of `page_tokens` positions, ggml type F32 (0) or F16 (1)."""
+
+    def __init__(self, layers, kv_heads, head_dim, pages, page_tokens=64, ggml_type=1):
+        _lib.init()
+        h = C.c_void_p()
+        _lib.check(_lib.lib.jitnn_hip_paged_cache_create(layers, kv_heads, head_dim, pages, page_tokens, ggml_type, C.byref(h)), "jitnn_hip_paged_cache_create")
+        self._own(h, layers, kv_heads, head_dim, pages, page_tokens, ggml_type)
+
+    @classmethod
+    def wrap_dev(cls, k_ptr: int, v_ptr: int, layers, kv_heads, head_dim, pages, page_tokens=64, ggml_type=1) -> "PagedCache":
+        """The same in memory of the caller, who keeps it alive: keys and values [layers][pages][kv_heads][page_tokens][head_dim]."""
+        _lib.init()
+        h = C.c_void_p()
+        _lib.check(_lib.lib.jitnn_hip_paged_cache_wrap_dev(k_ptr, v_ptr, layers, kv_heads, head_dim, pages, page_tokens, ggml_type, C.byref(h)),
+                   "jitnn_hip_paged_cache_wrap_dev")
+        self = cls.__new__(cls)
+        self._own(h, layers, kv_heads, head_dim, pages, page_tokens, ggml_type)
+        return self
+
+    def _own(self, h, layers, kv_heads, head_dim, pages, page_tokens, ggml_type):
+        self.layers, self.kv_heads, self.head_dim, self.pages, self.page_tokens, self.ggml_type = layers, kv_heads, head_dim, pages, page_tokens, ggml_type
+        self._h = h
+        weakref.finalize(self, _lib.lib.jitnn_hip_paged_cache_free, h)
+
+    @property
+    def handle(self):
+        return self._h
+
+    def copy_page_dev(self, source: int, target: int, stream_ptr: int = 0) -> None:
+        """Page `source` of every layer to page `target`."""
+        _lib.check(_lib.lib.jitnn_hip_paged_cache_copy_page_dev(self._h, source, target, stream_ptr), "jitnn_hip_paged_cache_copy_page_dev")
+
+    def append_dev(self, layer: int, batch: Batch, rope: Rope | None, heads: int, q_ptr: int, q_out_ptr: int, k_ptr: int, v_ptr: int, q_stride: int = 0,
+                   q_out_stride: int = 0, k_stride: int = 0, v_stride: int = 0, stream_ptr: int = 0) -> None:
+        """Keys (turned by rope) and values of the batch's rows into their pages, queries turned to q_out (which may be q; heads 0: none)."""
+        q, kv = heads * self.head_dim, self.kv_heads * self.head_dim
+        rc = _lib.lib.jitnn_hip_paged_append_dev(self._h, layer, batch, None if rope is None else rope.handle, q_ptr, q_stride or q, heads, q_out_ptr,
+                                                 q_out_stride or q, k_ptr, k_stride or kv, v_ptr, v_stride or kv, stream_ptr)
+        if rc:
+            _lib.check(rc, "jitnn_hip_paged_append_dev")
+
+    def attention_workspace(self, batch: Batch, heads: int) -> int:
+        """Bytes of device memory that attention_dev needs for such a batch."""
+        n = _lib.lib.jitnn_hip_paged_attention_workspace(self._h, batch, heads)
+        if n < 0:
+            _lib.check(n, "jitnn_hip_paged_attention_workspace")
+        return n
+
+    def attention_dev(self, layer: int, batch: Batch, heads: int, q_ptr: int, scale: float, y_ptr: int, workspace_ptr: int, workspace_bytes: int, q_stride: int = 0,
+                      y_stride: int = 0, stream_ptr: int = 0) -> None:
+        """y = softmax(scale q K^T) V of every row over its sequence's positions up to its own."""
+        dense = heads * self.head_dim
+        rc = _lib.lib.jitnn_hip_paged_attention_dev(self._h, layer, batch, heads, q_ptr, q_stride or dense, scale, y_ptr, y_stride or dense, workspace_ptr,
+                                                    workspace_bytes, stream_ptr)
+        if rc:
+            _lib.check(rc, "jitnn_hip_paged_attention_dev")
+
+
+def verify_workspace(rows: int, sequences: int, vocab: int) -> int:
+    """Bytes of device memory that verify_drafts_dev needs."""
+    n = _lib.lib.jitnn_hip_verify_workspace(rows, sequences, vocab)
+    if n < 0:
+        _lib.check(n, "jitnn_hip_verify_workspace")
+    return n
+
+
+def verify_drafts_dev(logits_ptr: int, rows: int, vocab: int, starts_ptr: int, sequences: int, tokens_ptr: int, temperatures_ptr: int, uniforms_ptr: int, out_ptr: int,
+                      accepted_ptr: int, workspace_ptr: int, workspace_bytes: int, draft_probs_ptr: int = 0, logits_stride: int = 0, draft_stride: int = 0,
+                      stream_ptr: int = 0) -> None:
+    """Which drafted tokens each sequence keeps, and the token drawn behind them, from given random numbers."""
+    rc = _lib.lib.jitnn_hip_verify_drafts_dev(logits_ptr, logits_stride or vocab, rows, vocab, starts_ptr, sequences, tokens_ptr, draft_probs_ptr or None,
+                                              draft_stride or vocab, temperatures_ptr, uniforms_ptr, out_ptr, accepted_ptr, workspace_ptr, workspace_bytes, stream_ptr)
+    if rc:
+        _lib.check(rc, "jitnn_hip_verify_drafts_dev")
