@@ -13,4 +13,4 @@ from .gguf_file import GgufFile, GgufTensorInfo  # noqa: F401
 from ._lib import UnsupportedTypeError  # noqa: F401
 from .tokenizer import Tokenizer  # noqa: F401
 from .llm import GenerationRequest, GenerationResult, Llm, ModelInfo  # noqa: F401
-from .serving import Batch, PagedCache, Rope, verify_drafts_dev, verify_workspace  # noqa: F401
+from .serving import Batch, PagedCache, Rope, SharedPrompt, verify_drafts_dev, verify_workspace  # noqa: F401

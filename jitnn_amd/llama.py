@@ -87,6 +87,16 @@ class LlamaDecoder:
         """Rotary pairs (2i, 2i + 1) instead of the default (i, i + head_dim / 2): the two forms of Rope (core/ops/Rope.java:126-150)."""
         _lib.check(_lib.lib.jitnn_hip_llama_set_rope_interleaved(self._h, 1 if on else 0), "jitnn_hip_llama_set_rope_interleaved")
 
+    def set_rope(self, rope) -> None:
+        """Rotary positions (serving.Rope) in place of the plain ones: scaled for long contexts, or a part of each head (interleaved pairs)."""
+        _lib.check(_lib.lib.jitnn_hip_llama_set_rope(self._h, rope.handle), "jitnn_hip_llama_set_rope")
+
+    def step_dev(self, cache, batch, x_ptr: int, logit_rows_ptr: int = 0, logit_count: int = 0, logits_ptr: int = 0, stream_ptr: int = 0) -> None:
+        """One pass of a batch of sequences over a paged cache (serving.PagedCache, serving.Batch): x [batch.tokens, d_model] are the embeddings of its rows,
+        logits [logit_count, vocab] those of the rows named by logit_rows."""
+        _lib.check(_lib.lib.jitnn_hip_llama_step_dev(self._h, cache.handle, batch, x_ptr, logit_rows_ptr or None, logit_count, logits_ptr or None, stream_ptr),
+                   "jitnn_hip_llama_step_dev")
+
     def set_packing(self, allow: bool) -> None:
         """Whether prompt passes may keep a layer's keys and values packed as FP16 operands (the default), in a buffer of the model."""
         _lib.check(_lib.lib.jitnn_hip_llama_set_packing(self._h, 1 if allow else 0), "jitnn_hip_llama_set_packing")

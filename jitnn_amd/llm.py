@@ -20,6 +20,7 @@ import numpy as np
 from . import _lib
 from .gguf_file import GgufFile
 from .llama import LlamaDecoder, W_OUTPUT
+from .serving import Rope, SharedPrompt
 from .tokenizer import StreamDecoder, Tokenizer
 
 # GGUF tensor names of a Llama-style layer in the order of the decoder's weight slots
@@ -32,12 +33,17 @@ _TOKEN_CB = C.CFUNCTYPE(None, C.c_int, C.c_void_p)
 class GenerationRequest:
     """What Llm.generate(request) hands to the engine (Llm.java:84-93 passes a jitllm GenerationRequest through): the prompt,
     the length limit, sampling and stop sequences.  temperature 0 is the greedy choice; top_k 0 and top_p 1 put no limit
-    on the candidates; seed None draws from a fresh generator.  Chat messages and tools are jitllm's and are not built."""
+    on the candidates; seed None draws from a fresh generator.  Chat messages and tools are jitllm's and are not built.
+    draft_tokens: up to so many tokens per pass are drafted by looking up what followed the text's last tokens before, and verified in that pass; the
+    text follows the model's distribution all the same.  With a temperature it takes top_k 0 and top_p 1."""
 
     def __init__(self, prompt: str, max_new_tokens: int = 128, temperature: float = 0.0, top_k: int = 0, top_p: float = 1.0, seed=None,
-                 stop=(), on_token=None):
+                 stop=(), on_token=None, draft_tokens: int = 0):
         if max_new_tokens < 0 or temperature < 0 or top_k < 0 or not 0.0 < top_p <= 1.0:
             raise ValueError(f"max_new_tokens {max_new_tokens}, temperature {temperature}, top_k {top_k}, top_p {top_p}")
+        if draft_tokens < 0 or (draft_tokens and temperature > 0 and (top_k not in (0, 1) or top_p < 1.0)):
+            raise ValueError(f"draft_tokens {draft_tokens} with temperature {temperature}, top_k {top_k}, top_p {top_p}")
+        self.draft_tokens = int(draft_tokens)
         self.prompt, self.max_new_tokens, self.temperature, self.top_k, self.top_p = prompt, max_new_tokens, float(temperature), int(top_k), float(top_p)
         self.seed, self.stop, self.on_token = seed, tuple(s for s in ([stop] if isinstance(stop, str) else stop) if s), on_token
 
@@ -74,6 +80,18 @@ def sample_token(logits, temperature: float, top_k: int, top_p: float, rng) -> i
     return int(order[min(int(np.searchsorted(np.cumsum(p), rng.random(), side="right")), len(order) - 1)])
 
 
+def look_up_draft(tokens, count: int) -> list:
+    """Up to `count` tokens that followed the last two tokens, or else the last one, where these stood last before."""
+    for n in (2, 1):
+        if len(tokens) <= n:
+            continue
+        tail = tokens[-n:]
+        for at in range(len(tokens) - n - 1, -1, -1):
+            if tokens[at:at + n] == tail:
+                return tokens[at + n:at + n + count]
+    return []
+
+
 class StopFilter:
     """Text pieces in, text pieces out, holding back whatever could still turn into a stop sequence: push returns
     (text to emit, stopped); after a stop nothing more comes out and the stop sequence itself is never emitted."""
@@ -101,6 +119,41 @@ class StopFilter:
     def flush(self) -> str:
         out, self._held = ("" if self.stopped else self._held), ""
         return out
+
+
+class _Text:
+    """One sequence of Llm.continuations: its tokens, their text, and why it ended (None: it has not)."""
+
+    def __init__(self, tokenizer, rq: "GenerationRequest", prompt_ids, seed, emit):
+        self.known, self.out, self.pieces, self.reason = list(prompt_ids), [], [], None
+        self.rng = np.random.default_rng(seed)
+        self._eos, self._rq, self._emit = tokenizer.eos if tokenizer.eos is not None else -1, rq, emit
+        self._stream, self._stops = StreamDecoder(tokenizer), StopFilter(rq.stop)
+
+    def _push(self, s, stopped):
+        if s:
+            self.pieces.append(s)
+            if self._emit is not None:
+                self._emit(s)
+        return stopped
+
+    def take(self, token: int) -> None:
+        if token == self._eos:
+            self.reason = "eos"
+        else:
+            self.out.append(token)
+            self.known.append(token)
+            if self._push(*self._stops.push(self._stream.push(token))):
+                self.reason = "stop"
+            elif len(self.out) == self._rq.max_new_tokens:
+                self.reason = "length"
+
+    def result(self, prompt_tokens: int) -> "GenerationResult":
+        if self.reason != "stop":
+            if self._push(*self._stops.push(self._stream.flush())):
+                self.reason = "stop"
+            self._push(self._stops.flush(), False)
+        return GenerationResult("".join(self.pieces), self.out, prompt_tokens, self.reason or "length")
 
 
 class ModelInfo:
@@ -154,6 +207,9 @@ class Llm:
             dec.set_weight(0, W_OUTPUT, f.tensor("output.weight" if f.has_tensor("output.weight") else "token_embd.weight"))
             dec.set_embedding(emb.type_id, f.raw("token_embd.weight"))
             dec.set_rope_interleaved(arch in INTERLEAVED_ROPE_ARCHS)
+            rope = Llm._rope(f, arch, hd, theta)
+            if rope is not None:
+                dec.set_rope(rope)
             tok = Tokenizer.from_gguf(f)
             if len(tok.tokens) != vocab:
                 raise ValueError(f"{path}: {len(tok.tokens)} tokens for an embedding table of {vocab} rows")
@@ -163,6 +219,21 @@ class Llm:
         except Exception:
             f.close()
             raise
+
+    @staticmethod
+    def _rope(f: GgufFile, arch: str, head_dim: int, theta: float):
+        """The rotary positions that the file asks for, None where they are the plain ones: a part of the head (rope.dimension_count), linear or YaRN scaling
+        (rope.scaling.*), factors of the frequencies (rope_freqs.weight)."""
+        rot = f.integer(f"{arch}.rope.dimension_count", head_dim)
+        kind = f.get(f"{arch}.rope.scaling.type") if f.has(f"{arch}.rope.scaling.type") else "none"
+        factors = f.raw("rope_freqs.weight").view(np.float32) if f.has_tensor("rope_freqs.weight") else None
+        if rot == head_dim and kind == "none" and factors is None:
+            return None
+        if kind not in ("none", "linear", "yarn"):
+            raise ValueError(f"rotary scaling {kind!r} (linear and yarn are built)")
+        context = f.integer(f"{arch}.rope.scaling.original_context_length", f.integer(f"{arch}.context_length", 2048))
+        return Rope(rot, theta, arch in INTERLEAVED_ROPE_ARCHS, None if kind == "none" else kind, f.float_value(f"{arch}.rope.scaling.factor", 1.0), context,
+                    attention_factor=f.float_value(f"{arch}.rope.scaling.attn_factor", 0.0), freq_factors=factors)
 
     def generate(self, prompt, max_new_tokens: int | None = None, on_text=None):
         """generate(prompt, max_new_tokens[, on_text]): the greedy (temperature 0) continuation of `prompt` as a string, at most
@@ -193,9 +264,53 @@ class Llm:
                 on_text(tail)
         return "".join(pieces)
 
+    def continuations(self, request: GenerationRequest, count: int, page_tokens: int = 64, cache_type: int = 1) -> list:
+        """`count` GenerationResults for one request, decoded together: the prompt runs through the model once, its pages of the cache (ggml type F16 1 or F32 0)
+        are shared and read once a pass, and every sequence draws with a generator of its own (seed, seed + 1, ...).  The request's on_token is for
+        generate and has to be None."""
+        if request.on_token is not None:
+            raise ValueError("on_token is for one sequence: Llm.generate")
+        return self._continue(request, count, page_tokens, cache_type, None)
+
+    def _continue(self, rq: GenerationRequest, count: int, page_tokens: int, cache_type: int, emit) -> list:
+        ids = self._tok.encode(rq.prompt)
+        if not ids:
+            raise ValueError("the prompt has no tokens")
+        if count < 1:
+            raise ValueError(f"{count} continuations")
+        if len(ids) + rq.max_new_tokens > self._info.context:
+            raise ValueError(f"{len(ids)} prompt tokens + {rq.max_new_tokens} new ones in a context of {self._info.context}")
+        texts = [_Text(self._tok, rq, ids, None if rq.seed is None else rq.seed + i, emit) for i in range(count)]
+        if rq.max_new_tokens > 0:
+            drafts = min(rq.draft_tokens, rq.max_new_tokens - 1)
+            # (a sequence's last pass may hold drafts behind its last position)
+            run = SharedPrompt(self._dec, ids, count, len(ids) + rq.max_new_tokens + drafts, 1 + drafts, page_tokens, cache_type)
+            greedy = rq.temperature <= 0.0 or rq.top_k == 1
+            for t in texts:
+                t.take(sample_token(run.prompt_logits, rq.temperature, rq.top_k, rq.top_p, t.rng))
+            while True:
+                live = [i for i, t in enumerate(texts) if t.reason is None]
+                if not live:
+                    break
+                if not drafts:
+                    logits = run.step(live, [[texts[i].known[-1]] for i in live])
+                    for i, row in zip(live, logits):
+                        texts[i].take(sample_token(row, rq.temperature, rq.top_k, rq.top_p, texts[i].rng))
+                    continue
+                tokens = [[texts[i].known[-1]] + look_up_draft(texts[i].known, drafts) for i in live]
+                numbers = np.concatenate([texts[i].rng.random((len(ts), 2)) for i, ts in zip(live, tokens)])
+                got = run.verify(live, tokens, [0.0 if greedy else rq.temperature] * len(live), np.minimum(numbers.astype(np.float32), np.float32(1 - 2.0 ** -24)))
+                for i, ts, (kept, token) in zip(live, tokens, got):
+                    for t in ts[1:1 + kept] + [token]:
+                        if texts[i].reason is None:
+                            texts[i].take(t)
+        return [t.result(len(ids)) for t in texts]
+
     def _generate_request(self, rq: GenerationRequest) -> GenerationResult:
         """The token loop on the host, for requests the library's greedy loop does not cover: the prompt in one pass
-        (jitnn_hip_llama_prefill), then logits -> sample_token -> embedding row -> one decode step per token."""
+        (jitnn_hip_llama_prefill), then logits -> sample_token -> embedding row -> one decode step per token.  Drafted tokens go through a paged cache."""
+        if rq.draft_tokens:
+            return self._continue(rq, 1, 64, 0, rq.on_token)[0]
         ids = self._tok.encode(rq.prompt)
         if not ids:
             raise ValueError("the prompt has no tokens")

@@ -124,3 +124,118 @@ def verify_drafts_dev(logits_ptr: int, rows: int, vocab: int, starts_ptr: int, s
                                               draft_stride or vocab, temperatures_ptr, uniforms_ptr, out_ptr, accepted_ptr, workspace_ptr, workspace_bytes, stream_ptr)
     if rc:
         _lib.check(rc, "jitnn_hip_verify_drafts_dev")
+
+
+class DeviceArray:
+    """Device memory of the library's for `count` values of a numpy type."""
+
+    def __init__(self, count: int, dtype):
+        self.dtype, self.count = np.dtype(dtype), int(count)
+        h = C.c_void_p()
+        _lib.check(_lib.lib.jitnn_hip_malloc(max(16, self.count * self.dtype.itemsize), C.byref(h)), "jitnn_hip_malloc")
+        self.ptr = h.value
+        weakref.finalize(self, _lib.lib.jitnn_hip_free, h)
+
+    def put(self, values) -> "DeviceArray":
+        a = np.ascontiguousarray(values, dtype=self.dtype).reshape(-1)
+        if a.size > self.count:
+            raise ValueError(f"{a.size} values for {self.count}")
+        if a.size:
+            _lib.check(_lib.lib.jitnn_hip_memcpy_h2d(self.ptr, a.ctypes.data_as(C.c_void_p), a.nbytes), "jitnn_hip_memcpy_h2d")
+        return self
+
+    def get(self, count: int) -> np.ndarray:
+        a = np.empty(min(count, self.count), dtype=self.dtype)
+        if a.size:
+            _lib.check(_lib.lib.jitnn_hip_memcpy_d2h(a.ctypes.data_as(C.c_void_p), self.ptr, a.nbytes), "jitnn_hip_memcpy_d2h")
+        return a
+
+
+class SharedPrompt:
+    """`count` sequences that go on from one prompt, over a paged cache of their own: the prompt runs through the model once, its whole pages belong to all of
+    them and are read once a pass for all of them, and each gets a copy of the page it ends in.  decoder: llama.LlamaDecoder with its embedding table;
+    each sequence may grow to max_len positions, with at most `rows` tokens of a sequence in one pass."""
+
+    PROMPT_ROWS = 512  # of a pass over the prompt
+
+    def __init__(self, decoder, prompt_ids, count: int, max_len: int, rows: int = 1, page_tokens: int = 64, ggml_type: int = 1):
+        cfg = decoder.cfg
+        prompt = [int(t) for t in prompt_ids]
+        if not prompt or count < 1 or rows < 1 or max_len < len(prompt):
+            raise ValueError(f"{len(prompt)} prompt tokens, {count} sequences of up to {max_len} positions, {rows} rows a pass")
+        if min(prompt) < 0 or max(prompt) >= cfg["vocab"]:
+            raise ValueError(f"token id outside [0, {cfg['vocab']})")
+        self._dec, self._vocab, self._rows, self.max_len = decoder, cfg["vocab"], rows, max_len
+        self.shared = len(prompt) // page_tokens
+        self._width = -(-max_len // page_tokens)
+        own = self._width - self.shared
+        self._cache = PagedCache(cfg["layers"], cfg["kv_heads"], cfg["head_dim"], max(1, self.shared + count * own), page_tokens, ggml_type)
+        self._tables = np.empty((count, self._width), dtype=np.int32)
+        self._tables[:, : self.shared] = np.arange(self.shared)
+        self._tables[:, self.shared:] = self.shared + np.arange(count * own).reshape(count, own)
+        self.lens = [len(prompt)] * count  # positions whose tokens are known
+        most = max(min(len(prompt), self.PROMPT_ROWS), count * rows)
+        self._tok, self._x, self._logits = DeviceArray(most, np.int32), DeviceArray(most * cfg["d_model"], np.float32), DeviceArray(count * rows * self._vocab, np.float32)
+        self._ints = [DeviceArray(n, np.int32) for n in (self._tables.size, count + 1, count, most)]  # tables, starts, lens, rows of the logits
+        self._verify = None
+        for at in range(0, len(prompt), self.PROMPT_ROWS):
+            chunk = prompt[at:at + self.PROMPT_ROWS]
+            last = at + len(chunk) == len(prompt)
+            self._pass([0], [chunk], [at + len(chunk)], 0, [len(chunk) - 1] if last else [])
+        self.prompt_logits = self._logits.get(self._vocab)  # of the token after the prompt
+        if len(prompt) % page_tokens:
+            for i in range(1, count):
+                self._cache.copy_page_dev(int(self._tables[0, self.shared]), int(self._tables[i, self.shared]))
+
+    def _pass(self, which, tokens, lens, shared, logit_rows):
+        counts = [len(t) for t in tokens]
+        flat = [t for ts in tokens for t in ts]
+        tables, starts, ends, rows = self._ints
+        tables.put(self._tables[list(which)])
+        starts.put(np.concatenate([[0], np.cumsum(counts)]))
+        ends.put(lens)
+        rows.put(logit_rows)
+        self._tok.put(flat)
+        batch = Batch(len(counts), len(flat), max(counts), max(lens), tables.ptr, self._width, starts.ptr, ends.ptr, shared)
+        _lib.check(_lib.lib.jitnn_hip_llama_embed_dev(self._dec.handle, self._tok.ptr, len(flat), self._x.ptr, None), "jitnn_hip_llama_embed_dev")
+        self._dec.step_dev(self._cache, batch, self._x.ptr, rows.ptr, len(logit_rows), self._logits.ptr)
+
+    def _step(self, which, tokens):
+        which = list(which)
+        if not which or len(set(which)) != len(which) or len(tokens) != len(which) or any(not 0 < len(t) <= self._rows for t in tokens):
+            raise ValueError(f"sequences {which} with {[len(t) for t in tokens]} tokens (1 to {self._rows} each)")
+        if any(not 0 <= t < self._vocab for ts in tokens for t in ts):
+            raise ValueError(f"token id outside [0, {self._vocab})")
+        lens = [self.lens[i] + len(t) for i, t in zip(which, tokens)]
+        if max(lens) > self.max_len:
+            raise ValueError(f"position {max(lens) - 1} of {self.max_len}")
+        self._pass(which, tokens, lens, self.shared, range(sum(len(t) for t in tokens)))
+        return lens
+
+    def step(self, which, tokens) -> np.ndarray:
+        """The next tokens of the sequences `which` (a list per sequence): appended, and the logits [rows, vocab] after each of them."""
+        lens = self._step(which, tokens)
+        for i, n in zip(which, lens):
+            self.lens[i] = n
+        n = sum(len(t) for t in tokens)
+        return self._logits.get(n * self._vocab).reshape(n, self._vocab)
+
+    def verify(self, which, tokens, temperatures, uniforms):
+        """The same for sequences whose tokens after the first are drafted: [(drafts kept, the token drawn after them)].  Of each sequence the first token and the kept
+        drafts are appended.  uniforms [rows, 2]: two random numbers in [0, 1) for each token."""
+        self._step(which, tokens)
+        count, rows = len(self._tables), len(self._tables) * self._rows
+        if self._verify is None:
+            n = verify_workspace(rows, count, self._vocab)
+            self._verify = [DeviceArray(count, np.float32), DeviceArray(2 * rows, np.float32), DeviceArray(rows, np.int32), DeviceArray(count, np.int32), DeviceArray(n, np.uint8)]
+        temps, nums, out, accepted, space = self._verify
+        n = sum(len(t) for t in tokens)
+        temps.put(temperatures)
+        nums.put(uniforms)
+        verify_drafts_dev(self._logits.ptr, n, self._vocab, self._ints[1].ptr, len(tokens), self._tok.ptr, temps.ptr, nums.ptr, out.ptr, accepted.ptr, space.ptr, space.count)
+        got, kept, at, result = out.get(n), accepted.get(len(tokens)), 0, []
+        for i, ts, k in zip(which, tokens, kept):
+            result.append((int(k), int(got[at + k])))
+            self.lens[i] += 1 + int(k)
+            at += len(ts)
+        return result
