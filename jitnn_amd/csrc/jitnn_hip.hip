@@ -2235,7 +2235,7 @@ int jitnn_hip_paged_attention_dev(const jitnn_hip_paged_cache *c, int layer, con
     if (need > 0 && (!workspace_dev || workspace_bytes < (long long)need || ((uintptr_t)workspace_dev & 15) != 0))
         return fail(JITNN_HIP_EINVAL, "a workspace of %lld bytes, %zu are needed (aligned to 16)", workspace_dev ? workspace_bytes : 0ll, need);
     const long long units = (long long)p.own.spans * c->kv * b->sequences * p.own.blocks + (long long)p.ahead.spans * c->kv * p.ahead.blocks,
-                    merges = ((long long)b->tokens * heads + 3) / 4;
+                    merges = (long long)b->tokens * heads;
     if (units > (1 << 28) || merges > (1 << 28)) return fail(JITNN_HIP_EINVAL, "%d sequences of up to %d tokens are too many for one pass", b->sequences, b->max_tokens);
     AttnArgs a;
     a.k = c->k + (size_t)layer * c->layer_bytes();
@@ -2261,7 +2261,7 @@ int jitnn_hip_paged_attention_dev(const jitnn_hip_paged_cache *c, int layer, con
     a.shared = batch_shared(c, b);
     a.ahead = p.ahead;
     a.own = p.own;
-    paged_attn_launch(c->type == 1, c->hd, (hipStream_t)stream, a);
+    paged_attn_launch(c->type == 1, c->hd, g.cus, (hipStream_t)stream, a);
     HIP_TRY(hipGetLastError());
     return JITNN_HIP_OK;
 }

@@ -58,6 +58,7 @@ struct AttnArgs {
     int tokens, sequences, heads, kv, pages, page_shift, table_stride, max_len;
     int shared;          // positions
     AttnPart ahead, own;
+    int chunk, chunks_ahead, chunks_own, pairs;  // the order of the workgroups: see paged_attn_kernel
 };
 struct AttnPlan {
     AttnPart ahead, own;
@@ -69,7 +70,7 @@ struct AttnPlan {
 AttnPlan paged_attn_plan(bool half, int D, int heads, int kv, int sequences, long long tokens, int max_tokens, int max_len, int shared, int cus);
 void paged_attn_launch_f16(int D, unsigned blocks, hipStream_t s, const AttnArgs &a);
 void paged_attn_launch_f32(int D, unsigned blocks, hipStream_t s, const AttnArgs &a);
-void paged_attn_launch(bool half, int D, hipStream_t s, const AttnArgs &a);  // and the merge of its spans
+void paged_attn_launch(bool half, int D, int cus, hipStream_t s, AttnArgs a);  // and the merge of its spans
 
 // ---- verify.h
 struct VerifyArgs {

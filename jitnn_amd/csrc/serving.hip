@@ -55,14 +55,16 @@ AttnPlan paged_attn_plan(bool half, int D, int heads, int kv, int sequences, lon
     AttnPlan p;
     if (shared > 0) p.ahead = rows_shape(tokens * group, D);
     p.own = rows_shape((long long)max_tokens * group, D);
-    // spans of about equal time, for four workgroups to a CU
+    // Spans of about equal time: for two workgroups to a CU, as many as run at once, where some share their keys (each leaves its rows' sums in memory, so that
+    // more of them cost more than their balance gains: 64 sequences behind 16384 shared positions 70 us with two, 96 with three, 93 with four); for
+    // four where all stream (8 sequences of up to 2000 positions 38.1 us, with two 38.7).
     auto step = [](const AttnPart &q) { return q.tiles == 2 ? 1.6 : 1.0; };  // of a wave, in units of one tile's
     const double own_len = std::max(max_len - shared, 1);
     auto work = [&](const AttnPart &q, double n, double len) { return n * q.blocks * kv * len / q.key_waves * step(q); };
-    const double all = (shared > 0 ? work(p.ahead, 1, shared) : 0) + work(p.own, sequences, own_len), each = all / (4. * cus);
+    const double all = (shared > 0 ? work(p.ahead, 1, shared) : 0) + work(p.own, sequences, own_len), each = all / ((p.own.key_waves == 1 || (shared > 0 && p.ahead.key_waves == 1) ? 2. : 4.) * cus);
     auto cut = [&](AttnPart &q, double len) {
         const int least = keys * q.key_waves;  // one step of every wave
-        const double want = std::max(each * q.key_waves / step(q), len / 128);
+        const double want = std::max(each * q.key_waves / step(q), len / 120);  // (at most 128 spans of each part: PA_MERGE)
         q.span = (int)std::min<double>(std::ceil(want / least) * least, std::ceil(len / least) * least);
         q.spans = (int)((len + q.span - 1) / q.span);
     };
@@ -71,18 +73,23 @@ AttnPlan paged_attn_plan(bool half, int D, int heads, int kv, int sequences, lon
     return p;
 }
 
-void paged_attn_launch(bool half, int D, hipStream_t s, const AttnArgs &a) {
+void paged_attn_launch(bool half, int D, int cus, hipStream_t s, AttnArgs a) {
     const unsigned units_ahead = (unsigned)(a.ahead.spans * a.kv), units_own = (unsigned)(a.own.spans * a.kv * a.sequences);
-    const unsigned blocks = (units_ahead + 7) / 8 * 8 * (unsigned)a.ahead.blocks + (units_own + 7) / 8 * 8 * (unsigned)a.own.blocks;
+    const unsigned ahead = (units_ahead + 7) / 8 * 8 * (unsigned)a.ahead.blocks, own = (units_own + 7) / 8 * 8 * (unsigned)a.own.blocks;
+    a.chunk = std::max(8, cus / 8 * 8);  // one to a CU
+    a.chunks_ahead = (int)((ahead + a.chunk - 1) / a.chunk);
+    a.chunks_own = (int)((own + a.chunk - 1) / a.chunk);
+    a.pairs = std::min(a.chunks_ahead, a.chunks_own);
+    const unsigned blocks = (unsigned)(a.chunks_ahead + a.chunks_own) * (unsigned)a.chunk;
     if (half) paged_attn_launch_f16(D, blocks, s, a);
     else paged_attn_launch_f32(D, blocks, s, a);
     if (a.ahead.spans + a.own.spans == 1) return;
-    const unsigned merge = (unsigned)(((long long)a.tokens * a.heads + 3) / 4);
+    const unsigned merge = (unsigned)((long long)a.tokens * a.heads);
     switch (D) {
-    case 64: hipLaunchKernelGGL(paged_merge_kernel<64>, dim3(merge), dim3(256), 0, s, a); break;
-    case 128: hipLaunchKernelGGL(paged_merge_kernel<128>, dim3(merge), dim3(256), 0, s, a); break;
-    case 192: hipLaunchKernelGGL(paged_merge_kernel<192>, dim3(merge), dim3(256), 0, s, a); break;
-    default: hipLaunchKernelGGL(paged_merge_kernel<256>, dim3(merge), dim3(256), 0, s, a); break;
+    case 64: hipLaunchKernelGGL(paged_merge_kernel<64>, dim3(merge), dim3(PA_MERGE), 0, s, a); break;
+    case 128: hipLaunchKernelGGL(paged_merge_kernel<128>, dim3(merge), dim3(PA_MERGE), 0, s, a); break;
+    case 192: hipLaunchKernelGGL(paged_merge_kernel<192>, dim3(merge), dim3(PA_MERGE), 0, s, a); break;
+    default: hipLaunchKernelGGL(paged_merge_kernel<256>, dim3(merge), dim3(PA_MERGE), 0, s, a); break;
     }
 }
 
