@@ -15,7 +15,7 @@
 
 namespace jitnn {
 
-constexpr int VERIFY_THREADS = 256, VERIFY_VALUES = 32, VERIFY_CHUNK = VERIFY_THREADS * VERIFY_VALUES;
+constexpr int VERIFY_THREADS = 256, VERIFY_VALUES = 16, VERIFY_CHUNK = VERIFY_THREADS * VERIFY_VALUES;
 
 struct VerifyStat {
     double sum;  // of exp((l - largest) / T); T <= 0: unused
@@ -25,31 +25,52 @@ struct VerifyStat {
 
 typedef float f32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));  // (rows of an odd vocabulary start anywhere)
 
-// 2^y for y <= 0: the Taylor series of exp(f ln 2), |f| <= 1/2, to the twelfth power (the next term is 2e-16)
-__device__ __forceinline__ double verify_exp2(double y) {
-    y = fmax(y, -1100.);  // (-inf too)
-    const double n = rint(y), x = (y - n) * 0.69314718055994530942;
-    double p = 1. / 479001600.;
-    p = fma(p, x, 1. / 39916800.);
-    p = fma(p, x, 1. / 3628800.);
-    p = fma(p, x, 1. / 362880.);
-    p = fma(p, x, 1. / 40320.);
-    p = fma(p, x, 1. / 5040.);
-    p = fma(p, x, 1. / 720.);
-    p = fma(p, x, 1. / 120.);
-    p = fma(p, x, 1. / 24.);
-    p = fma(p, x, 1. / 6.);
-    p = fma(p, x, .5);
-    p = fma(p, x, 1.);
-    p = fma(p, x, 1.);
-    return ldexp(p, (int)n);
-}
-// exp((l - largest) / T), rate = log2(e) / T; NaN has no weight, equal infinities have 1
-__device__ __forceinline__ double verify_weight(float l, float largest, double rate) {
-    return l == largest ? 1. : l < largest ? verify_exp2(((double)l - (double)largest) * rate) : 0.;
-}
+__constant__ const double VERIFY_ROOTS[32] = {  // 2^(i / 32)
+    1, 1.0218971486541166, 1.0442737824274138, 1.0671404006768237,
+    1.0905077326652577, 1.1143867425958924, 1.1387886347566916, 1.1637248587775775,
+    1.189207115002721, 1.215247359980469, 1.241857812073484, 1.2690509571917332,
+    1.2968395546510096, 1.3252366431597413, 1.3542555469368927, 1.383909881963832,
+    1.4142135623730951, 1.4451808069770467, 1.4768261459394993, 1.5091644275934228,
+    1.5422108254079407, 1.5759808451078865, 1.6104903319492543, 1.6457554781539649,
+    1.681792830507429, 1.7186192981224779, 1.7562521603732995, 1.7947090750031072,
+    1.8340080864093424, 1.8741676341103, 1.9152065613971474, 1.9571441241754002,
+};
+
+// exp((l - largest) / T) in FP64 as 2^(n / 32) 2^(f / 32), n whole and |f| <= 1/2: a table and the Taylor series to the fifth power (the next term is 2e-15).
+// With the series alone, to the twelfth power over |f| <= 1/2 of a whole octave, the weights of 160 rows of 128256 took 17 us on top of the 17 that
+// reading them takes.
+struct VerifyWeight {
+    const double *table;  // [32]: 2^(i / 32), in LDS
+    double rate;  // 32 log2(e) / T
+    float largest;
+    // (a barrier behind it)
+    static __device__ __forceinline__ void fill(double *table) {
+        if (threadIdx.x < 32) table[threadIdx.x] = VERIFY_ROOTS[threadIdx.x];
+    }
+    __device__ __forceinline__ VerifyWeight(const double *table, float temperature, float largest)
+        : table(table), rate(temperature > 0.f ? 32. * 1.44269504088896340736 / (double)temperature : 0.), largest(largest) {}
+    // of a logit at or below the largest, which is finite; NaN and -inf have none
+    __device__ __forceinline__ double operator()(float l) const {
+        constexpr double whole = 6755399441055744.;  // 1.5 2^52: whole numbers end in the last bit
+        constexpr double c1 = 0.02166084939249829, c2 = 0.00023459619820224677, c3 = 1.6938509724371819e-06, c4 = 9.172562701824643e-09, c5 = 3.9737099845494154e-11;  // (ln 2 / 32)^k / k!
+        const double y = fmax(((double)l - (double)largest) * rate, -40000.), t = y + whole, f = y - (t - whole);
+        const int n = (int)(unsigned)__double2loint(t);
+        const double p = fma(f, fma(f, fma(f, fma(f, fma(f, c5, c4), c3), c2), c1), 1.);
+        return ldexp(p * table[n & 31], n >> 5);
+    }
+    // the same where the largest may be infinite: equal infinities share all the weight
+    __device__ __forceinline__ double any(float l) const { return fabsf(largest) < INFINITY ? (*this)(l) : l == largest ? 1. : 0.; }
+};
 __device__ __forceinline__ double verify_wave_sum(double v) {
     for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off);
+    return v;
+}
+__device__ __forceinline__ double verify_wave_scan(double v) {  // the sum up to this lane
+    const int lane = threadIdx.x & 63;
+    for (int off = 1; off < 64; off <<= 1) {
+        const double o = __shfl_up(v, off);
+        if (lane >= off) v += o;
+    }
     return v;
 }
 __device__ __forceinline__ void verify_take(float v, int i, float &best, int &index) {
@@ -65,28 +86,31 @@ __device__ __forceinline__ void verify_wave_best(float &best, int &index) {
         verify_take(v, i, best, index);
     }
 }
-__device__ __forceinline__ double verify_rate(float temperature) { return temperature > 0.f ? 1.44269504088896340736 / (double)temperature : 0.; }
-
-// grid (chunks, rows)
-__global__ void __launch_bounds__(VERIFY_THREADS) verify_stats_kernel(const VerifyArgs a) {
-    __shared__ float best_of[VERIFY_THREADS / 64];
-    __shared__ int index_of[VERIFY_THREADS / 64];
-    __shared__ double sum_of[VERIFY_THREADS / 64];
-    const int r = blockIdx.y, c0 = blockIdx.x * VERIFY_CHUNK, tid = threadIdx.x, wave = tid >> 6;
-    const float *row = a.logits + (size_t)r * a.logits_stride;
-    float v[VERIFY_VALUES];
+// VERIFY_VALUES values of a chunk per thread, four neighbours at a time; behind the row's end -inf
+__device__ __forceinline__ void verify_load(const float *__restrict__ row, int c0, int vocab, float (&v)[VERIFY_VALUES]) {
 #pragma unroll
     for (int u = 0; u < VERIFY_VALUES / 4; ++u) {
-        const int i = c0 + 4 * (u * VERIFY_THREADS + tid);
-        if (i + 4 <= a.vocab) {
+        const int i = c0 + 4 * (u * VERIFY_THREADS + (int)threadIdx.x);
+        if (i + 4 <= vocab) {
             const f32x4_a4 x = *reinterpret_cast<const f32x4_a4 *>(row + i);
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[4 * u + e] = x[e];
         } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[4 * u + e] = i + e < a.vocab ? row[i + e] : -INFINITY;
+            for (int e = 0; e < 4; ++e) v[4 * u + e] = i + e < vocab ? row[i + e] : -INFINITY;
         }
     }
+}
+
+// grid (chunks, rows)
+__global__ void __launch_bounds__(VERIFY_THREADS) verify_stats_kernel(const VerifyArgs a) {
+    __shared__ float best_of[VERIFY_THREADS / 64];
+    __shared__ int index_of[VERIFY_THREADS / 64];
+    __shared__ double sum_of[VERIFY_THREADS / 64], table[32];
+    const int r = blockIdx.y, c0 = blockIdx.x * VERIFY_CHUNK, tid = threadIdx.x, wave = tid >> 6;
+    float v[VERIFY_VALUES];
+    verify_load(a.logits + (size_t)r * a.logits_stride, c0, a.vocab, v);
+    VerifyWeight::fill(table);
     const int s = batch_sequence(a.starts, a.sequences, r);
     if (s >= a.sequences || r < a.starts[0]) return;  // a row of no sequence
     const float temperature = a.temperatures[s];
@@ -109,9 +133,14 @@ __global__ void __launch_bounds__(VERIFY_THREADS) verify_stats_kernel(const Veri
     for (int w = 1; w < VERIFY_THREADS / 64; ++w) verify_take(best_of[w], index_of[w], best, index);
     double sum = 0.;
     if (temperature > 0.f && best > -INFINITY) {
-        const double rate = verify_rate(temperature);
-#pragma unroll 4
-        for (int u = 0; u < VERIFY_VALUES; ++u) sum += verify_weight(v[u], best, rate);
+        const VerifyWeight weight(table, temperature, best);
+        if (best < INFINITY) {
+#pragma unroll
+            for (int u = 0; u < VERIFY_VALUES; ++u) sum += weight(v[u]);
+        } else {
+#pragma unroll
+            for (int u = 0; u < VERIFY_VALUES; ++u) sum += weight.any(v[u]);
+        }
     }
     sum = verify_wave_sum(sum);
     if ((tid & 63) == 0) sum_of[wave] = sum;
@@ -125,84 +154,94 @@ __global__ void __launch_bounds__(VERIFY_THREADS) verify_stats_kernel(const Veri
 }
 
 // A row's largest logit, its index and the sum of its weights, from the chunks'; one wave, every lane receives them.
-__device__ __forceinline__ VerifyStat verify_row(const VerifyStat *__restrict__ st, int chunks, double rate) {
+__device__ __forceinline__ VerifyStat verify_row(const VerifyStat *__restrict__ st, int chunks, const double *table, float temperature) {
     const int lane = threadIdx.x & 63;
-    VerifyStat t{0., -INFINITY, 0x7fffffff};
-    for (int c = lane; c < chunks; c += 64) verify_take(st[c].largest, st[c].index, t.largest, t.index);
+    VerifyStat t{0., -INFINITY, 0x7fffffff}, mine{0., -INFINITY, 0x7fffffff};
+    if (lane < chunks) mine = st[lane];
+    verify_take(mine.largest, mine.index, t.largest, t.index);
+    for (int c = lane + 64; c < chunks; c += 64) verify_take(st[c].largest, st[c].index, t.largest, t.index);
     verify_wave_best(t.largest, t.index);
-    for (int c = lane; c < chunks; c += 64)
-        if (st[c].largest > -INFINITY) t.sum += st[c].sum * verify_weight(st[c].largest, t.largest, rate);
+    const VerifyWeight weight(table, temperature, t.largest);
+    if (mine.largest > -INFINITY) t.sum = mine.sum * weight.any(mine.largest);
+    for (int c = lane + 64; c < chunks; c += 64)
+        if (st[c].largest > -INFINITY) t.sum += st[c].sum * weight.any(st[c].largest);
     t.sum = verify_wave_sum(t.sum);
-    if (t.index == 0x7fffffff) t.index = 0;  // (nothing but -inf and NaN)
+    if (t.index == 0x7fffffff) t.index = 0;  // (nothing but NaN)
     return t;
 }
 
-// Where a sequence's drafts end.  A workgroup of WAVES waves, a row to each of them at a time.
+// Where a sequence's drafts end.  A wave to each of its rows at a time; the last one has no draft to judge but may be the one that draws.
 struct VerifyEnd {
-    int first, kept, row;  // the sequence's first row, the drafts kept, the row that draws
-    bool refused;          // ... from what its draft left, and not behind the last draft
+    int first, end, kept, row;  // the sequence's first row, the one behind its last, the drafts kept, the row that draws (-1: the sequence has none)
+    bool refused;               // it draws from what its draft left, and is not behind the last draft
     float temperature;
-    VerifyStat stat;       // of that row
+    VerifyStat stat;            // of that row
+};
+constexpr int VERIFY_ROWS = 32;  // rows whose sums are kept
+struct VerifyShared {
+    int first_refused;
+    VerifyStat row[VERIFY_ROWS + 1];
+    double table[32];
 };
 template <int WAVES>
-__device__ __forceinline__ VerifyEnd verify_end(const VerifyArgs &a, int s, int *first_refused, VerifyStat *stat) {
-    const int begin = min(max(a.starts[s], 0), a.rows), end = min(max(a.starts[s + 1], begin), a.rows), tid = threadIdx.x, wave = tid >> 6;
-    const float temperature = a.temperatures[s];
-    const double rate = verify_rate(temperature);
-    if (tid == 0) *first_refused = end - begin - 1;
-    __syncthreads();
-    for (int j = wave; j < end - begin - 1; j += WAVES) {
-        const int r = begin + j, x = a.tokens[r + 1];
-        const bool known = x >= 0 && x < a.vocab;  // (a draft that is no token is never kept)
-        const float lx = known ? a.logits[(size_t)r * a.logits_stride + x] : 0.f, qx = known && a.draft_probs ? a.draft_probs[(size_t)r * a.draft_stride + x] : 1.f,
-                    u = a.uniforms[2 * (size_t)r];
-        const VerifyStat t = verify_row((const VerifyStat *)a.part + (size_t)r * a.chunks, a.chunks, rate);
-        const bool keep = known && (temperature > 0.f ? t.largest > -INFINITY && (double)u * (double)qx < verify_weight(lx, t.largest, rate) / t.sum : x == t.index);
-        if (!keep && (tid & 63) == 0) atomicMin(first_refused, j);
-    }
-    __syncthreads();
+__device__ __forceinline__ VerifyEnd verify_end(const VerifyArgs &a, int s, VerifyShared &sh) {
     VerifyEnd e;
-    e.first = begin;
-    e.kept = max(*first_refused, 0);
-    e.row = begin + e.kept;
-    e.refused = e.kept < end - begin - 1;
-    e.temperature = temperature;
-    if (wave == 0 && end > begin) {
-        const VerifyStat t = verify_row((const VerifyStat *)a.part + (size_t)e.row * a.chunks, a.chunks, rate);
-        if (tid == 0) *stat = t;
+    e.first = min(max(a.starts[s], 0), a.rows);
+    e.end = min(max(a.starts[s + 1], e.first), a.rows);
+    e.temperature = a.temperatures[s];
+    const int count = e.end - e.first, tid = threadIdx.x, wave = tid >> 6;
+    if (tid == 0) sh.first_refused = count - 1;
+    VerifyWeight::fill(sh.table);
+    __syncthreads();
+    for (int j = wave; j < count; j += WAVES) {
+        const int r = e.first + j;
+        const bool drafted = j + 1 < count;
+        const int x = drafted ? a.tokens[r + 1] : -1;
+        const bool known = x >= 0 && x < a.vocab;  // (a draft that is no token is never kept)
+        const float u = a.uniforms[2 * (size_t)r], lx = known ? a.logits[(size_t)r * a.logits_stride + x] : 0.f,
+                    qx = known && a.draft_probs ? a.draft_probs[(size_t)r * a.draft_stride + x] : 1.f;
+        const VerifyStat t = verify_row((const VerifyStat *)a.part + (size_t)r * a.chunks, a.chunks, sh.table, e.temperature);
+        const VerifyWeight weight(sh.table, e.temperature, t.largest);
+        const bool keep = known && (e.temperature > 0.f ? t.largest > -INFINITY && (double)u * (double)qx < weight.any(lx) / t.sum : x == t.index);
+        if ((tid & 63) == 0) {
+            if (j < VERIFY_ROWS) sh.row[j] = t;
+            if (drafted && !keep) atomicMin(&sh.first_refused, j);
+        }
     }
     __syncthreads();
-    if (end == begin) e.row = -1;
-    else e.stat = *stat;
+    e.kept = max(sh.first_refused, 0);
+    e.row = count > 0 ? e.first + e.kept : -1;
+    e.refused = e.kept < count - 1;
+    if (count <= 0) return e;
+    if (e.kept >= VERIFY_ROWS) {
+        if (wave == 0) {
+            const VerifyStat t = verify_row((const VerifyStat *)a.part + (size_t)e.row * a.chunks, a.chunks, sh.table, e.temperature);
+            if (tid == 0) sh.row[VERIFY_ROWS] = t;
+        }
+        __syncthreads();
+    }
+    e.stat = sh.row[min(e.kept, VERIFY_ROWS)];
     return e;
-}
-
-// The weight of index i in the row that draws, over the row's sum.
-__device__ __forceinline__ double verify_share(float l, float q, const VerifyEnd &e, double rate) {
-    return fmax(verify_weight(l, e.stat.largest, rate) / e.stat.sum - (double)q, 0.);
 }
 
 // grid (chunks, sequences)
 __global__ void __launch_bounds__(VERIFY_THREADS) verify_rest_kernel(const VerifyArgs a) {
-    __shared__ int first_refused;
-    __shared__ VerifyStat stat;
+    __shared__ VerifyShared sh;
     __shared__ double sum_of[VERIFY_THREADS / 64];
     const int s = blockIdx.y, c0 = blockIdx.x * VERIFY_CHUNK, tid = threadIdx.x;
-    const VerifyEnd e = verify_end<VERIFY_THREADS / 64>(a, s, &first_refused, &stat);
+    const VerifyEnd e = verify_end<VERIFY_THREADS / 64>(a, s, sh);
     if (e.row < 0 || !e.refused || !(e.temperature > 0.f)) return;
-    const double rate = verify_rate(e.temperature);
-    const float *row = a.logits + (size_t)e.row * a.logits_stride, *q = a.draft_probs + (size_t)e.row * a.draft_stride;
-    float l[VERIFY_VALUES], d[VERIFY_VALUES];
+    float l[VERIFY_VALUES], q[VERIFY_VALUES];
+    verify_load(a.logits + (size_t)e.row * a.logits_stride, c0, a.vocab, l);
+    verify_load(a.draft_probs + (size_t)e.row * a.draft_stride, c0, a.vocab, q);
+    const VerifyWeight weight(sh.table, e.temperature, e.stat.largest);
+    const double share = 1. / e.stat.sum;
+    double sum = 0.;
 #pragma unroll
     for (int u = 0; u < VERIFY_VALUES; ++u) {
-        const int i = min(c0 + u * VERIFY_THREADS + tid, a.vocab - 1);
-        l[u] = row[i];
-        d[u] = q[i];
+        const double rest = fma(weight.any(l[u]), share, -(double)q[u]);
+        sum += rest > 0. && q[u] > -INFINITY ? rest : 0.;  // (behind the row's end q is -inf)
     }
-    double sum = 0.;
-#pragma unroll 4
-    for (int u = 0; u < VERIFY_VALUES; ++u)
-        if (c0 + u * VERIFY_THREADS + tid < a.vocab) sum += verify_share(l[u], d[u], e, rate);
     sum = verify_wave_sum(sum);
     if ((tid & 63) == 0) sum_of[tid >> 6] = sum;
     __syncthreads();
@@ -210,50 +249,48 @@ __global__ void __launch_bounds__(VERIFY_THREADS) verify_rest_kernel(const Verif
 }
 
 // grid (sequences)
-constexpr int VERIFY_DRAW_THREADS = 1024, VERIFY_DRAW_VALUES = VERIFY_CHUNK / VERIFY_DRAW_THREADS;
+constexpr int VERIFY_DRAW_THREADS = 512, VERIFY_DRAW_VALUES = VERIFY_CHUNK / VERIFY_DRAW_THREADS;
+static_assert(VERIFY_DRAW_VALUES % 4 == 0, "whole loads");
 __global__ void __launch_bounds__(VERIFY_DRAW_THREADS) verify_draw_kernel(const VerifyArgs a) {
     constexpr int WAVES = VERIFY_DRAW_THREADS / 64;
-    __shared__ int first_refused, chosen_chunk;
-    __shared__ VerifyStat stat;
+    __shared__ VerifyShared sh;
+    __shared__ int chosen_chunk, first_at[WAVES], last_at[WAVES];
     __shared__ double left, sum_of[WAVES];
     const int s = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const VerifyEnd e = verify_end<WAVES>(a, s, &first_refused, &stat);
+    const VerifyEnd e = verify_end<WAVES>(a, s, sh);
     if (tid == 0) a.accepted[s] = e.row < 0 ? 0 : e.kept;
     if (e.row < 0) return;
-    const int end = min(max(a.starts[s + 1], e.first), a.rows);
-    for (int r = e.first + tid; r < end; r += VERIFY_DRAW_THREADS)
+    for (int r = e.first + tid; r < e.end; r += VERIFY_DRAW_THREADS)
         if (r != e.row) a.out[r] = r < e.row ? a.tokens[r + 1] : -1;
-    const double rate = verify_rate(e.temperature);
     if (!(e.temperature > 0.f) || !(e.stat.largest > -INFINITY)) {
         if (tid == 0) a.out[e.row] = e.stat.index;
         return;
     }
-    const bool certain = e.refused && !a.draft_probs;  // drafted with probability 1: the rest is p without it
-    const int x = certain ? a.tokens[e.row + 1] : -1;
+    const VerifyWeight weight(sh.table, e.temperature, e.stat.largest);
+    const double share = 1. / e.stat.sum;
+    const int x = e.refused && !a.draft_probs ? a.tokens[e.row + 1] : -1;  // drafted with probability 1: the rest is p without it
     const float *row = a.logits + (size_t)e.row * a.logits_stride, *q = e.refused && a.draft_probs ? a.draft_probs + (size_t)e.row * a.draft_stride : nullptr;
     // ---- the chunk: one wave, 64 chunks at a time
     if (wave == 0) {
         const VerifyStat *st = (const VerifyStat *)a.part + (size_t)e.row * a.chunks;
         const double *rest = (const double *)((const VerifyStat *)a.part + (size_t)a.rows * a.chunks) + (size_t)s * a.chunks;
+        const float lx = x >= 0 && x < a.vocab ? row[x] : -INFINITY;
+        const float number = a.uniforms[2 * (size_t)e.row + 1];
         auto weight_of = [&](int c) {
             if (c >= a.chunks) return 0.;
             if (q) return rest[c];
-            double w = st[c].largest > -INFINITY ? st[c].sum * verify_weight(st[c].largest, e.stat.largest, rate) : 0.;
-            if (x >= 0 && x < a.vocab && x / VERIFY_CHUNK == c) w = fmax(w - verify_weight(row[x], e.stat.largest, rate), 0.);
-            return w / e.stat.sum;
+            double w = st[c].largest > -INFINITY ? st[c].sum * weight.any(st[c].largest) : 0.;
+            if (x >= 0 && x / VERIFY_CHUNK == c) w = fmax(w - weight.any(lx), 0.);
+            return w * share;
         };
-        double total = 0.;
-        for (int c0 = 0; c0 < a.chunks; c0 += 64) total += verify_wave_sum(weight_of(c0 + lane));
-        const double target = (double)a.uniforms[2 * (size_t)e.row + 1] * total;
+        const double first = weight_of(lane);  // (a vocabulary of 262144 has 64 chunks)
+        double total = verify_wave_sum(first);
+        for (int c0 = 64; c0 < a.chunks; c0 += 64) total += verify_wave_sum(weight_of(c0 + lane));
+        const double target = (double)number * total;
         double before = 0., before_chunk = 0.;
         int chunk = -1, last = 0;
         for (int c0 = 0; c0 < a.chunks && chunk < 0; c0 += 64) {
-            const double w = weight_of(c0 + lane);
-            double upto = w;
-            for (int off = 1; off < 64; off <<= 1) {
-                const double o = __shfl_up(upto, off);
-                if (lane >= off) upto += o;
-            }
+            const double w = c0 == 0 ? first : weight_of(c0 + lane), upto = verify_wave_scan(w);
             const unsigned long long past = __ballot(before + upto > target), some = __ballot(w > 0.);
             if (past) {
                 const int at = __ffsll((long long)past) - 1;
@@ -272,37 +309,32 @@ __global__ void __launch_bounds__(VERIFY_DRAW_THREADS) verify_draw_kernel(const 
     __syncthreads();
     // ---- the index in it: every thread eight neighbours
     const int i0 = chosen_chunk * VERIFY_CHUNK + tid * VERIFY_DRAW_VALUES;
-    double w[VERIFY_DRAW_VALUES], sum = 0.;
+    float l[VERIFY_DRAW_VALUES], d[VERIFY_DRAW_VALUES];
 #pragma unroll
     for (int u = 0; u < VERIFY_DRAW_VALUES; ++u) {
         const int i = min(i0 + u, a.vocab - 1);
-        const float l = row[i], d = q ? q[i] : 0.f;
-        w[u] = i0 + u < a.vocab && i0 + u != x ? verify_share(l, d, e, rate) : 0.;
+        l[u] = row[i];
+        d[u] = q ? q[i] : 0.f;
+    }
+    double w[VERIFY_DRAW_VALUES], sum = 0.;
+#pragma unroll
+    for (int u = 0; u < VERIFY_DRAW_VALUES; ++u) {
+        w[u] = i0 + u < a.vocab && i0 + u != x ? fmax(fma(weight.any(l[u]), share, -(double)d[u]), 0.) : 0.;
         sum += w[u];
     }
-    double upto = sum;
-    for (int off = 1; off < 64; off <<= 1) {
-        const double o = __shfl_up(upto, off);
-        if (lane >= off) upto += o;
-    }
+    const double upto = verify_wave_scan(sum);
     if (lane == 63) sum_of[wave] = upto;
     __syncthreads();
-    double before = 0.;
-    for (int v = 0; v < wave; ++v) before += sum_of[v];
-    before += upto - sum;
+    double c = upto - sum;
+    for (int v = 0; v < wave; ++v) c += sum_of[v];
     // the first index whose cumulative sum is past what is left; where rounding or a number of 1 leaves none, the last with any weight
-    int mine = -1;
-    double c = before;
+    int mine = -1, last = -1;
 #pragma unroll
     for (int u = 0; u < VERIFY_DRAW_VALUES; ++u) {
         c += w[u];
         if (mine < 0 && w[u] > 0. && c > left) mine = i0 + u;
-    }
-    __shared__ int first_at[WAVES], last_at[WAVES];
-    int last = -1;
-#pragma unroll
-    for (int u = 0; u < VERIFY_DRAW_VALUES; ++u)
         if (w[u] > 0.) last = i0 + u;
+    }
     const unsigned long long hit = __ballot(mine >= 0), any = __ballot(last >= 0);
     const int hit_at = hit ? __shfl(mine, __ffsll((long long)hit) - 1) : -1, any_at = any ? __shfl(last, 63 - __clzll((long long)any)) : -1;
     if (lane == 0) {
