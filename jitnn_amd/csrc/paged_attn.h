@@ -28,7 +28,6 @@
 namespace jitnn {
 
 constexpr int PA_THREADS = 256, PA_WAVES = 4;
-constexpr int PA_SEARCH = 1024;  // sequences whose starts a workgroup keeps in LDS
 constexpr float PA_WEIGHT = 6.f, PA_LAG = 8.f;  // weights are 2^(score - m + 6), m at most 8 below the maximum: up to 2^14, inside FP16
 
 typedef float f32x4v __attribute__((ext_vector_type(4)));
@@ -68,17 +67,6 @@ __device__ __forceinline__ float pa_sum4(float v) {
 __device__ __forceinline__ bool pa_finite(_Float16 x) { return (__builtin_bit_cast(unsigned short, x) & 0x7c00) != 0x7c00; }
 __device__ __forceinline__ bool pa_finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 
-// The sequence of token t in ascending starts[0 .. sequences]
-__device__ __forceinline__ int pa_sequence(const int *starts, int sequences, int t) {
-    int lo = 0, hi = sequences;  // the first s with starts[s + 1] > t
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (starts[mid + 1] > t) hi = mid;
-        else lo = mid + 1;
-    }
-    return lo;
-}
-
 // The sequence of token t, its length and the token behind its last; one wave (or every wave) with the same t.  Lengths come with the starts, in one
 // round trip for each 64 sequences.
 struct RowPlace {
@@ -104,7 +92,10 @@ __device__ __forceinline__ RowPlace row_place(const int *__restrict__ starts, co
 template <class T, int D, int R>
 struct PaRows {
     static constexpr int E = D / 16;
-    int rows, row0, t0;    // rows of the part, the wave's first, the first row's token
+    int rows, row0, t0;    // rows of the part, the wave's first, the part's first token
+    int group, token0, rem0;  // query heads per key/value head; the wave's first row as a token behind t0 and a head of the group
+    float per_group;
+    int begins, ends, lens, base;  // sequence base + lane: its first token, the one behind its last, its length
     int lim[R];            // the last position of the span that row n sees
     bool over[R];          // ... of a sequence longer than it may be
     int first, last;       // the least and the largest lim
@@ -119,54 +110,113 @@ struct PaRows {
     u32x4 ph[R], pl[R];  // weights (FP16): slot 4 t + i
     float pf[R][4];      // (FP32)
 
-    // Four steps, so that what they wait for is asked for together: begin (false: the workgroup has nothing to do), fetch (queries, and the starts and
-    // lens to LDS), a barrier, find (the rows' positions), take (the queries as operands).
+    // In steps, so that what they wait for is asked for together: begin (false: the workgroup has nothing to do), fetch (queries), find (the rows'
+    // positions), take (the queries as operands).
     __device__ __forceinline__ bool begin(const AttnArgs &a, const bool ahead, const int seq, const int row0_of_wave, const int row0_of_block, const int key0) {
+        group = a.heads / a.kv;
+        per_group = 1.f / (float)group;
+        // (the first 64 sequences' ends and lengths, a lane each, for find)
+        base = 0;
+        if (ahead) sequences_at(a);
         t0 = max(a.starts[ahead ? 0 : seq], 0);
-        rows = max(min(a.starts[ahead ? a.sequences : seq + 1], a.tokens) - t0, 0) * (a.heads / a.kv);
+        rows = max(min(a.starts[ahead ? a.sequences : seq + 1], a.tokens) - t0, 0) * group;
         row0 = row0_of_wave;
         // (a span that no row of the sequence reaches; where there is one span in all, its rows are still to be written)
         return row0_of_block < rows && (ahead || key0 == 0 || a.lens[seq] > key0);
     }
+    __device__ __forceinline__ void sequences_at(const AttnArgs &a) {
+        const int i = min(base + (int)(threadIdx.x & 63), a.sequences - 1);
+        begins = a.starts[i];
+        ends = a.starts[i + 1];
+        lens = a.lens[i];
+    }
+    // the row behind the wave's first by `in` < 32 as a token behind t0 and a head of the group: whole numbers below 2^17, for which the FP32 quotient of a
+    // number and a half has the right whole part
+    __device__ __forceinline__ int2 place(const int in) const {
+        const int x = rem0 + in, q = (int)(((float)x + 0.5f) * per_group);
+        return make_int2(token0 + q, x - q * group);
+    }
     // queries: 8 g + j of each 32 values (FP16), 4 g + j of each 16 (FP32) of row n
-    __device__ __forceinline__ void fetch(const AttnArgs &a, const bool ahead, const int kvh, int *search) {
-        const int tid = threadIdx.x, n = tid & 15, g = (tid & 63) >> 4, group = a.heads / a.kv;
+    __device__ __forceinline__ void fetch(const AttnArgs &a, const int kvh) {
+        const int n = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
+        token0 = __builtin_amdgcn_readfirstlane(row0 / group);
+        rem0 = row0 - token0 * group;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            const int row = min(row0 + 16 * r + n, rows - 1), t = t0 + row / group, h = kvh * group + row % group;
-            const float *q = a.q + (size_t)t * a.q_stride + (size_t)h * D;
+            const int2 at = place(max(min(16 * r + n, rows - 1 - row0), 0));  // (a wave without rows reads behind them: of a token that exists)
+            const float *q = a.q + (size_t)min(t0 + at.x, a.tokens - 1) * a.q_stride + (size_t)(kvh * group + at.y) * D;
 #pragma unroll
             for (int s = 0; s < D / 16; ++s) qf[r][s] = *reinterpret_cast<const f32x4v_a4 *>(q + (sizeof(T) == 2 ? 32 * (s >> 1) + 8 * g + 4 * (s & 1) : 16 * s + 4 * g));
         }
-        if (ahead && a.sequences <= PA_SEARCH) {
-            for (int i = tid; i <= a.sequences; i += PA_THREADS) search[i] = a.starts[i];
-            for (int i = tid; i < a.sequences; i += PA_THREADS) search[a.sequences + 1 + i] = a.lens[i];
-        }
     }
-    __device__ __forceinline__ void find(const AttnArgs &a, const bool ahead, const int seq, const int key1, const int *search) {
-        const bool near = ahead && a.sequences <= PA_SEARCH;
-        const int *starts = near ? search : a.starts, *lens = near ? search + a.sequences + 1 : a.lens;
-        const int n = threadIdx.x & 15, group = a.heads / a.kv;
+    // The positions of the rows' tokens.  Of a sequence they follow one another.  Of the whole batch: where no sequence ends inside the span - a vote over
+    // all of them -, all rows see all of it; otherwise token by token, in scalar registers: a token's sequence is how many ends are at or below it.
+    __device__ __forceinline__ void find(const AttnArgs &a, const bool ahead, const int seq, const int key1) {
+        const int n = threadIdx.x & 15, lane = threadIdx.x & 63;
         last = -1;
         first = badkey = 0x7fffffff;
+        int token[R];
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            const int row = row0 + 16 * r + n, t = t0 + row / group;
             lim[r] = -1;
             over[r] = false;
-            if (row < rows) {
-                const int s = ahead ? min(pa_sequence(starts, a.sequences, t), a.sequences - 1) : seq;
-                over[r] = lens[s] > a.max_len;
-                if (!over[r]) {
-                    lim[r] = min(lens[s] - starts[s + 1] + t, key1 - 1);
-                    last = max(last, lim[r]);
-                    first = min(first, lim[r]);
-                }
-            }
+            token[r] = row0 + 16 * r + n < rows ? place(16 * r + n).x : -1;
         }
-        for (int off = 1; off < 16; off <<= 1) {
-            last = max(last, __shfl_xor(last, off));
-            first = min(first, __shfl_xor(first, off));
+        const int count = min(16 * R, rows - row0);  // of the wave's rows
+        if (count <= 0) return;
+        const int end_token = token0 + (rem0 + count - 1) / group;
+        if (!ahead) {
+            const int len = a.lens[seq], behind = len - a.starts[seq + 1] + t0;
+            const bool long_one = len > a.max_len;
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                over[r] = long_one && token[r] >= 0;
+                if (!long_one && token[r] >= 0) lim[r] = min(behind + token[r], key1 - 1);
+            }
+            if (!long_one) {
+                first = min(behind + token0, key1 - 1);
+                last = min(behind + end_token, key1 - 1);
+            }
+            return;
+        }
+        bool all = true;
+        for (;;) {
+            const bool whole = lens <= a.max_len && lens - (ends - begins) >= key1 - 1;
+            all = all && __ballot(base + lane < a.sequences && !whole) == 0;
+            if (base + 64 >= a.sequences) break;
+            base += 64;
+            sequences_at(a);
+        }
+        if (all) {
+            first = last = key1 - 1;
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+                if (token[r] >= 0) lim[r] = key1 - 1;
+            return;
+        }
+        if (base > 0) {
+            base = 0;
+            sequences_at(a);
+        }
+        for (int k = token0; k <= end_token; ++k) {
+            int below;
+            while ((below = __popcll(__ballot(base + lane < a.sequences && ends <= t0 + k))) == 64 && base + 64 < a.sequences) {
+                base += 64;  // (the tokens to come are not in front of these either)
+                sequences_at(a);
+            }
+            const int len = __builtin_amdgcn_readlane(lens, min(below, 63)), end = __builtin_amdgcn_readlane(ends, min(below, 63));
+            const bool long_one = len > a.max_len;
+            const int pos = min(len - end + t0 + k, key1 - 1);
+            if (!long_one) {
+                last = max(last, pos);
+                first = min(first, pos);
+            }
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+                if (token[r] == k) {
+                    over[r] = long_one;
+                    lim[r] = long_one ? -1 : pos;
+                }
         }
         last = __builtin_amdgcn_readfirstlane(last);
         first = __builtin_amdgcn_readfirstlane(first);
@@ -306,35 +356,39 @@ struct PaRows {
     // the sum of row n's weights over the four lanes that hold it; NaN for a row that is to be NaN
     __device__ __forceinline__ float total(const int r) const { return over[r] || lim[r] >= badkey ? NAN : pa_sum4(l[r]); }
     __device__ __forceinline__ void spread_badkey() {
+        if (!__ballot(badkey != 0x7fffffff)) return;
         for (int off = 1; off < 64; off <<= 1) badkey = min(badkey, __shfl_xor(badkey, off));
     }
 };
 
-// Pages of the steps of a wave or workgroup, looked up 64 steps at a time, and the tiles of 16 keys in them, as descriptors whose extent ends behind the
-// last key: what lies behind reads as zero without a branch or a mask, and a tile that does not exist (behind the last key, behind the last
-// step, on a page that the cache does not have) costs nothing.
+// Where the tiles of 16 keys of the steps of a wave or workgroup lie, looked up and laid out for 64 steps at a time, a lane to each: in the loop a
+// tile's descriptors are two lane reads and a few scalar additions (worked out there from the page's number they were a quarter of its instructions).
+// A descriptor's extent ends behind the last key: what lies behind reads as zero without a branch or a mask, and a tile that does not exist
+// (behind the last key, on a page that the cache does not have) costs nothing.
 template <int TILES, int KEYS, int ROW>
 struct PaPages {
-    int ids[TILES];  // lane u: the pages of step `first of the 64` + u, -1: none
-    // the pages of the steps step0 + stride * lane, of keys below `end` (which may be asked for before it is known how many of them are seen: then check)
+    int lo[TILES], hi[TILES];  // lane u: bytes from the pool's start (48 bits) and, in the top bits, keys; first the pages' numbers in lo
+    // the pages of the steps step0 + stride * lane, of keys below `end` (which may be asked for before it is known how many of them are seen: then settle)
     __device__ __forceinline__ void fetch(const AttnArgs &a, const int *table, const int key0, const int end, const int step0, const int stride) {
         const int lane = threadIdx.x & 63;
 #pragma unroll
         for (int t = 0; t < TILES; ++t) {
             const int key = key0 + (step0 + lane * stride) * KEYS + 16 * t;
-            ids[t] = key < end ? table[key >> a.page_shift] : -1;
+            lo[t] = key < end ? table[key >> a.page_shift] : -1;
         }
     }
-    __device__ __forceinline__ void check(const AttnArgs &a, const int key0, const int kend, const int step0, const int stride, int &badkey) {
+    __device__ __forceinline__ void settle(const AttnArgs &a, const int key0, const int kend, const int step0, const int stride, int &badkey) {
         const int lane = threadIdx.x & 63;
+        const size_t page_bytes = ((size_t)a.kv << a.page_shift) * ROW;
         int bad = 0x7fffffff;
 #pragma unroll
         for (int t = 0; t < TILES; ++t) {
             const int key = key0 + (step0 + lane * stride) * KEYS + 16 * t;
-            if ((unsigned)ids[t] >= (unsigned)a.pages) {
-                if (key < kend) bad = min(bad, key);
-                ids[t] = -1;
-            }
+            const bool seen = key < kend, there = (unsigned)lo[t] < (unsigned)a.pages;
+            if (seen && !there) bad = min(bad, key);
+            const size_t at = seen && there ? (size_t)lo[t] * page_bytes + (size_t)((key & ((1 << a.page_shift) - 1)) * ROW) : 0;
+            lo[t] = (int)(unsigned)at;
+            hi[t] = (int)(unsigned)(at >> 32) | (seen && there ? min(kend - key, 16) << 16 : 0);
         }
         if (__ballot(bad != 0x7fffffff)) {
             for (int off = 1; off < 64; off <<= 1) bad = min(bad, __shfl_xor(bad, off));
@@ -343,24 +397,30 @@ struct PaPages {
     }
     __device__ __forceinline__ void look_up(const AttnArgs &a, const int *table, const int key0, const int kend, const int step0, const int stride, int &badkey) {
         fetch(a, table, key0, kend, step0, stride);
-        check(a, key0, kend, step0, stride, badkey);
+        settle(a, key0, kend, step0, stride, badkey);
     }
-    __device__ __forceinline__ __amdgpu_buffer_rsrc_t tile(const AttnArgs &a, const uint8_t *pages, const int key0, const int kend, const int step, const int u, const int t) const {
-        const int key = key0 + step * KEYS + 16 * t;
-        int id = __builtin_amdgcn_readlane(ids[0], u);
+    struct Place {
+        size_t at;
+        int extent;
+    };
+    __device__ __forceinline__ Place tile(const int u, const int t) const {
+        unsigned l = __builtin_amdgcn_readlane(lo[0], u), h = __builtin_amdgcn_readlane(hi[0], u);
 #pragma unroll
         for (int i = 1; i < TILES; ++i)
-            if (t == i) id = __builtin_amdgcn_readlane(ids[i], u);
-        const size_t at = (size_t)(id < 0 ? 0 : id) * (((size_t)a.kv << a.page_shift) * ROW) + (size_t)(key & ((1 << a.page_shift) - 1)) * ROW;
-        // (in a scalar register by force: of the clamp the compiler makes a vector instruction, and of a descriptor in vector registers a loop)
-        const int extent = __builtin_amdgcn_readfirstlane(id < 0 ? 0 : max(min(kend - key, 16), 0) * ROW);
-        return __builtin_amdgcn_make_buffer_rsrc((void *)(pages + at), 0, extent, 0x00020000);
+            if (t == i) {
+                l = __builtin_amdgcn_readlane(lo[i], u);
+                h = __builtin_amdgcn_readlane(hi[i], u);
+            }
+        return Place{((size_t)(h & 0xffffu) << 32) | l, (int)(h >> 16) * ROW};
+    }
+    static __device__ __forceinline__ __amdgpu_buffer_rsrc_t source(const uint8_t *pages, const Place &p) {
+        return __builtin_amdgcn_make_buffer_rsrc((void *)(pages + p.at), 0, p.extent, 0x00020000);
     }
 };
 
 // ---- few rows: every wave streams keys of its own
 
-// LDS of a workgroup: outputs [wave][16 R][D + 4], maxima and sums [wave][16 R], then starts and lens
+// LDS of a workgroup: outputs [wave][16 R][D + 4], maxima and sums [wave][16 R]
 template <int D, int R>
 constexpr size_t pa_stream_floats() {
     return (size_t)PA_WAVES * 16 * R * (D + 4) + 2 * PA_WAVES * 16 * R;
@@ -373,26 +433,24 @@ __device__ __forceinline__ void pa_stream(const AttnArgs &a, const AttnPart &par
     using Tile = PaTile<T, D>;
     constexpr int KEYS = Tile::KEYS, TILES = Tile::TILES, E = Tile::E, ROW = D * (int)sizeof(T);
     const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int group = a.heads / a.kv, key_waves = part.key_waves, row_waves = PA_WAVES / key_waves;
+    const int key_waves = part.key_waves, row_waves = PA_WAVES / key_waves;
     const int wr = wave & (row_waves - 1), wk = wave / row_waves;
     const int *table = a.tables + (size_t)(ahead ? 0 : seq) * a.table_stride;
-    int *const search = reinterpret_cast<int *>(lds + pa_stream_floats<D, R>());
     PaRows<T, D, R> w;
     PaPages<TILES, KEYS, ROW> pages;
-    if (!w.begin(a, ahead, seq, (block * row_waves + wr) * 16 * R, block * row_waves * 16 * R, key0)) return;
     pages.fetch(a, table, key0, key1, wk, key_waves);
-    w.fetch(a, ahead, kvh, search);
-    if (ahead) __syncthreads();
-    w.find(a, ahead, seq, key1, search);
+    if (!w.begin(a, ahead, seq, (block * row_waves + wr) * 16 * R, block * row_waves * 16 * R, key0)) return;
+    w.fetch(a, kvh);
+    w.find(a, ahead, seq, key1);
     const int kend = w.last + 1;  // keys key0 .. kend - 1
     const int steps = kend > key0 ? (kend - key0 + KEYS - 1) / KEYS : 0;
     const uint8_t *const kbase = (const uint8_t *)a.k + ((size_t)kvh << a.page_shift) * ROW, *const vbase = (const uint8_t *)a.v + ((size_t)kvh << a.page_shift) * ROW;
     const int koff = n * ROW + 16 * g, voff = 4 * g * ROW + E * n * (int)sizeof(T);
     Tile x;
-    auto load_k = [&](int step, int u) {
+    auto load_k = [&](int u) {
 #pragma unroll
         for (int t = 0; t < TILES; ++t) {
-            const auto p = pages.tile(a, kbase, key0, kend, step, u, t);
+            const auto p = pages.source(kbase, pages.tile(u, t));
             if constexpr (sizeof(T) == 2) {
 #pragma unroll
                 for (int s = 0; s < D / 32; ++s) x.k[t][s] = __builtin_bit_cast(f16x8, __builtin_amdgcn_raw_buffer_load_b128(p, koff + 64 * s, 0, 0));
@@ -402,10 +460,10 @@ __device__ __forceinline__ void pa_stream(const AttnArgs &a, const AttnPart &par
             }
         }
     };
-    auto load_v = [&](int step, int u) {
+    auto load_v = [&](int u) {
 #pragma unroll
         for (int t = 0; t < TILES; ++t) {
-            const auto p = pages.tile(a, vbase, key0, kend, step, u, t);
+            const auto p = pages.source(vbase, pages.tile(u, t));
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 constexpr int W = E * sizeof(T) % 16 == 0 ? 16 : 8;  // bytes of a load
@@ -420,11 +478,11 @@ __device__ __forceinline__ void pa_stream(const AttnArgs &a, const AttnPart &par
         }
     };
 
-    int step = wk, u = 0;  // u: lane of the ids that holds the pages of `step`
+    int step = wk, u = 0;  // u: the lane that holds the places of `step`
     if (step < steps) {
-        pages.check(a, key0, kend, step, key_waves, w.badkey);
-        load_k(step, 0);
-        load_v(step, 0);
+        pages.settle(a, key0, kend, step, key_waves, w.badkey);
+        load_k(0);
+        load_v(0);
     }
     w.take(a);
     while (step < steps) {
@@ -451,16 +509,16 @@ __device__ __forceinline__ void pa_stream(const AttnArgs &a, const AttnPart &par
         // the keys of the next step, into the registers that the products have read (no branch may stand between the products and the first use of their
         // result: the compiler has been seen to leave out the wait it needs there)
         const int next = step + key_waves;
-        load_k(next, (u + 1) & 63);
+        load_k((u + 1) & 63);
         const bool partial = base + KEYS - 1 > w.first;  // some row does not see all of them
         if (partial && w.first < w.last) w.clean(x.v, base);  // ... and others see more
         w.weigh(sc, base, partial);
 #pragma unroll
         for (int e = 0; e < E; ++e) w.sum(x.v, e);
         u = (u + 1) & 63;
-        load_v(next, u);
+        load_v(u);
         step = next;
-        if (u == 63 && step + key_waves < steps) pages.look_up(a, table, key0, kend, step + key_waves, key_waves, w.badkey);  // (what is under way has its pages)
+        if (u == 63) pages.look_up(a, table, key0, kend, step + key_waves, key_waves, w.badkey);  // (what is under way has its places)
     }
 
     // ---- the waves' sums meet in LDS
@@ -481,10 +539,10 @@ __device__ __forceinline__ void pa_stream(const AttnArgs &a, const AttnPart &par
         }
     }
     __syncthreads();
+    const int first_row = block * row_waves * 16 * R, token_of_first = first_row / w.group, rem_of_first = first_row - token_of_first * w.group;
     for (int at = tid; at < row_waves * 16 * R * (D / 4); at += PA_THREADS) {
         const int rr = at / (D / 4), e = 4 * (at - rr * (D / 4)), wv = rr / (16 * R), in = rr - wv * 16 * R;  // wave wv + row_waves j holds row `in` of the keys' share j
-        const int row = block * row_waves * 16 * R + rr;
-        if (row >= w.rows) break;  // (rr grows with at)
+        if (first_row + rr >= w.rows) break;  // (rr grows with at)
         float top = -INFINITY, sum = 0.f;
         f32x4v acc = {0.f, 0.f, 0.f, 0.f};
         for (int j = 0; j < key_waves; ++j) top = fmaxf(top, lm[(wv + row_waves * j) * 16 * R + in]);
@@ -495,13 +553,13 @@ __device__ __forceinline__ void pa_stream(const AttnArgs &a, const AttnPart &par
             sum += ll[src] == ll[src] ? ll[src] * f : NAN;
             acc += *reinterpret_cast<const f32x4v *>(lo + (size_t)src * (D + 4) + e) * f;
         }
-        const int t = w.t0 + row / group, h = kvh * group + row % group;
         if (slots == 1) {
+            const int q = (int)(((float)(rem_of_first + rr) + 0.5f) * w.per_group), t = w.t0 + token_of_first + q, h = kvh * w.group + rem_of_first + rr - q * w.group;
             // (a row that sees nothing is zero)
             const float f = sum == 0.f ? 0.f : 1.f / sum;
             *reinterpret_cast<f32x4v_a4 *>(a.y + (size_t)t * a.y_stride + (size_t)h * D + e) = acc * f;
         } else {
-            const size_t at_slot = ((size_t)t * a.heads + h) * slots + slot;
+            const size_t at_slot = (((size_t)kvh * a.tokens + w.t0) * w.group + first_row + rr) * slots + slot;
             *reinterpret_cast<f32x4v *>(a.part + at_slot * D + e) = acc;
             if (e == 0) *reinterpret_cast<float2 *>(a.stat + 2 * at_slot) = make_float2(top, sum);
         }
@@ -536,23 +594,15 @@ __device__ __forceinline__ void pa_wide(const AttnArgs &a, const bool ahead, con
     using Tile = typename W::Tile;
     constexpr int KEYS = Tile::KEYS, TILES = Tile::TILES, E = Tile::E, ROW = D * (int)sizeof(T), PIECES = W::PIECES, COPIES = W::COPIES;
     const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int group = a.heads / a.kv;
-    __shared__ int last_of[PA_WAVES];
     const int *table = a.tables + (size_t)(ahead ? 0 : seq) * a.table_stride;
-    int *const search = reinterpret_cast<int *>(reinterpret_cast<uint8_t *>(lds) + W::LDS);
     PaRows<T, D, R> w;
     PaPages<TILES, KEYS, ROW> pages;
-    if (!w.begin(a, ahead, seq, (block * PA_WAVES + wave) * 16 * R, block * PA_WAVES * 16 * R, key0)) return;
     pages.fetch(a, table, key0, key1, 0, 1);
-    w.fetch(a, ahead, kvh, search);
-    if (ahead) __syncthreads();
-    w.find(a, ahead, seq, key1, search);
-    if (lane == 0) last_of[wave] = w.last;
-    __syncthreads();
-    int kend = 0;  // keys key0 .. kend - 1: what any row of the workgroup sees
-#pragma unroll
-    for (int i = 0; i < PA_WAVES; ++i) kend = max(kend, last_of[i] + 1);
-    kend = __builtin_amdgcn_readfirstlane(kend);
+    if (!w.begin(a, ahead, seq, (block * PA_WAVES + wave) * 16 * R, block * PA_WAVES * 16 * R, key0)) return;
+    w.fetch(a, kvh);
+    w.find(a, ahead, seq, key1);
+    // keys key0 .. kend - 1: what any row of the workgroup may see, and some of the shared ones perhaps that none does
+    const int kend = ahead ? key1 : min(key1, a.lens[seq]);
     const int steps = kend > key0 ? (kend - key0 + KEYS - 1) / KEYS : 0;
     const uint8_t *const kbase = (const uint8_t *)a.k + ((size_t)kvh << a.page_shift) * ROW, *const vbase = (const uint8_t *)a.v + ((size_t)kvh << a.page_shift) * ROW;
     // copy i of this thread: LDS piece tid + 256 i of the step, i.e. piece (..) % PIECES of row (..) / PIECES; all of a wave's are in one tile
@@ -565,17 +615,14 @@ __device__ __forceinline__ void pa_wide(const AttnArgs &a, const bool ahead, con
     }
     u32x4 kr[W::AHEAD][COPIES], vr[W::AHEAD][COPIES];
     uint8_t *const sm = reinterpret_cast<uint8_t *>(lds);  // [2][keys, values][STEP][16]
-    auto request = [&](auto slot_c, int step, int u) {
+    auto request = [&](auto slot_c, int u) {
         constexpr int S = decltype(slot_c)::value;
 #pragma unroll
         for (int i = 0; i < COPIES; ++i) {
-            const int t = TILES == 1 ? 0 : (wave + PA_WAVES * i) * 64 / (16 * PIECES);
-            kr[S][i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(pages.tile(a, kbase, key0, kend, step, u, t), koff[i], 0, 0));
-        }
-#pragma unroll
-        for (int i = 0; i < COPIES; ++i) {
-            const int t = TILES == 1 ? 0 : (wave + PA_WAVES * i) * 64 / (16 * PIECES);
-            vr[S][i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(pages.tile(a, vbase, key0, kend, step, u, t), voff[i], 0, 0));
+            constexpr int TILE = 16 * PIECES;
+            const auto p = pages.tile(u, TILES == 1 ? 0 : TILE % PA_THREADS == 0 ? i * PA_THREADS / TILE : (wave + PA_WAVES * i) * 64 / TILE);
+            kr[S][i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(pages.source(kbase, p), koff[i], 0, 0));
+            vr[S][i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(pages.source(vbase, p), voff[i], 0, 0));
         }
     };
     auto store = [&](auto slot_c, int buffer) {
@@ -596,11 +643,15 @@ __device__ __forceinline__ void pa_wide(const AttnArgs &a, const bool ahead, con
         for (int t = 0; t < TILES; ++t)
 #pragma unroll
             for (int r = 0; r < R; ++r) sc[r][t] = f32x4v{0.f, 0.f, 0.f, 0.f};
+        u32x4 keys[PIECES / 4][TILES];  // (all requested before the first is used, in the registers that the values take afterwards)
+#pragma unroll
+        for (int s = 0; s < PIECES / 4; ++s)
+#pragma unroll
+            for (int t = 0; t < TILES; ++t) keys[s][t] = *reinterpret_cast<const u32x4 *>(ks + (size_t)(16 * t + n) * ROW + 16 * pa_piece<PIECES>(4 * s + g, n));
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int s = 0; s < PIECES / 4; ++s) {
-            u32x4 k[TILES];
-#pragma unroll
-            for (int t = 0; t < TILES; ++t) k[t] = *reinterpret_cast<const u32x4 *>(ks + (size_t)(16 * t + n) * ROW + 16 * pa_piece<PIECES>(4 * s + g, n));
+            const u32x4(&k)[TILES] = keys[s];
             if constexpr (sizeof(T) == 2) {
 #pragma unroll
                 for (int t = 0; t < TILES; ++t)
@@ -640,15 +691,15 @@ __device__ __forceinline__ void pa_wide(const AttnArgs &a, const bool ahead, con
     constexpr std::integral_constant<int, 0> c0{};
     constexpr std::integral_constant<int, 1> c1{};
     if (steps > 0) {
-        pages.check(a, key0, kend, 0, 1, w.badkey);
-        request(c0, 0, 0);
-        request(c1, 1, 1);
+        pages.settle(a, key0, kend, 0, 1, w.badkey);
+        request(c0, 0);
+        request(c1, 1);
     }
     w.take(a);
     if (steps > 0) store(c0, 0);
     auto turn = [&](auto mine, auto other, int step) {  // step's registers were `mine`
-        if ((step & 63) == 62 && step + 2 < steps) pages.look_up(a, table, key0, kend, step + 2, 1, w.badkey);
-        request(mine, step + 2, (step + 2) & 63);
+        if ((step & 63) == 62) pages.look_up(a, table, key0, kend, step + 2, 1, w.badkey);
+        request(mine, (step + 2) & 63);
         __syncthreads();
         product(step);
         store(other, (step + 1) & 1);
@@ -658,31 +709,57 @@ __device__ __forceinline__ void pa_wide(const AttnArgs &a, const bool ahead, con
         if (step + 1 < steps) turn(c1, c0, step + 1);
     }
 
+    // ---- the outputs, turned in LDS so that a row goes out in one piece (a lane holds E values of it at four places)
     w.spread_badkey();
+    __syncthreads();
+    float *const mine = lds + (size_t)wave * 16 * (D + 4);
+    const size_t first_slot = (((size_t)kvh * a.tokens + w.t0) * w.group + w.row0) * slots + slot;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        const float sum = w.total(r);
-        const int row = w.row0 + 16 * r + n;
-        if (row < w.rows) {
-            const int t = w.t0 + row / group, h = kvh * group + row % group;
-            const size_t at_slot = ((size_t)t * a.heads + h) * slots + slot;
-            const float f = slots > 1 ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
-            float *p = (slots > 1 ? a.part + at_slot * D : a.y + (size_t)t * a.y_stride + (size_t)h * D) + 4 * E * g;
+        const float sum = w.total(r), f = slots > 1 ? 1.f : sum == 0.f ? 0.f : 1.f / sum;  // (a row that sees nothing is zero)
+        float *p = mine + n * (D + 4) + 4 * E * g;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int e = 0; e < E; e += 4)
-                    *reinterpret_cast<f32x4v_a4 *>(p + E * i + e) = f32x4v{w.o[r][e][i], w.o[r][e + 1][i], w.o[r][e + 2][i], w.o[r][e + 3][i]} * f;
-            if (slots > 1 && g == 0) *reinterpret_cast<float2 *>(a.stat + 2 * at_slot) = make_float2(w.m[r], sum);
+            for (int e = 0; e < E; e += 4)
+                *reinterpret_cast<f32x4v *>(p + E * i + e) = f32x4v{w.o[r][e][i], w.o[r][e + 1][i], w.o[r][e + 2][i], w.o[r][e + 3][i]} * f;
+        const int row_n = w.row0 + 16 * r + n;
+        if (slots > 1 && g == 0 && row_n < w.rows) {
+            *reinterpret_cast<float2 *>(a.stat + 2 * (first_slot + (size_t)(16 * r + n) * slots)) = make_float2(w.m[r], sum);
         }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+        for (int i = 0; i < 16 * (D / 4) / 64; ++i) {
+            const int piece = lane + 64 * i, in = piece / (D / 4), e = 4 * (piece - in * (D / 4));
+            const f32x4v v = *reinterpret_cast<const f32x4v *>(mine + in * (D + 4) + e);
+            if (w.row0 + 16 * r + in < w.rows) {
+                float *to = a.part + (first_slot + (size_t)(16 * r + in) * slots) * D;
+                if (slots == 1) {
+                    const int2 at = w.place(16 * r + in);
+                    to = a.y + (size_t)(w.t0 + at.x) * a.y_stride + (size_t)(kvh * w.group + at.y) * D;
+                }
+                *reinterpret_cast<f32x4v_a4 *>(to + e) = v;
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
 }
 
 template <class T, int D, int R>
 __device__ __forceinline__ void pa_attend(const AttnArgs &a, const AttnPart &part, const bool ahead, const int seq, const int block, const int kvh, const int key0,
                                           const int key1, const int slot, const int slots, float *lds) {
-    if (part.key_waves == 1) pa_wide<T, D, R>(a, ahead, seq, block, kvh, key0, key1, slot, slots, lds);
-    else pa_stream<T, D, R>(a, part, ahead, seq, block, kvh, key0, key1, slot, slots, lds);
+    if (part.key_waves == 1) {
+        pa_wide<T, D, R>(a, ahead, seq, block, kvh, key0, key1, slot, slots, lds);
+        return;
+    }
+    if constexpr (R == 2) {
+        // (of a ragged batch: a sequence whose rows fill one tile takes no product for the other)
+        if (!ahead && part.key_waves == PA_WAVES && (a.starts[seq + 1] - a.starts[seq]) * (a.heads / a.kv) <= 16) {
+            pa_stream<T, D, 1>(a, part, ahead, seq, block, kvh, key0, key1, slot, slots, lds);
+            return;
+        }
+    }
+    pa_stream<T, D, R>(a, part, ahead, seq, block, kvh, key0, key1, slot, slots, lds);
 }
 
 // The workgroups: `chunk` of the shared positions, as many of the sequences' own, and so on until one kind is used up - the first are bound by the matrix
@@ -733,7 +810,9 @@ __global__ void __launch_bounds__(PA_MERGE) paged_merge_kernel(const AttnArgs a)
     const int first_own = a.ahead.spans;
     const int ahead = min(first_own, a.shared > 0 ? lim / a.ahead.span + 1 : 0), own = lim >= a.shared ? (lim - a.shared) / a.own.span + 1 : 0;
     const int count = ahead + own;  // at most PA_MERGE (paged_attn_plan)
-    auto slot_of = [&](int i) { return (size_t)row * slots + (i < ahead ? i : first_own + i - ahead); };
+    const int group = a.heads / a.kv, kvh = h / group;
+    const size_t first_slot = (((size_t)kvh * a.tokens + t) * group + h - kvh * group) * slots;
+    auto slot_of = [&](int i) { return first_slot + (i < ahead ? i : first_own + i - ahead); };
     f32x4v acc = {0.f, 0.f, 0.f, 0.f}, x[U];
     auto request = [&](int i0) {
 #pragma unroll
@@ -775,12 +854,10 @@ constexpr size_t pa_lds_bytes() {
 }
 template <class T, int D, int RA, int RO>
 static void paged_attn_run(unsigned blocks, hipStream_t s, const AttnArgs &a) {
-    constexpr int R = RA > RO ? RA : RO;
+    constexpr size_t lds = pa_lds_bytes<T, D, (RA > RO ? RA : RO)>();
     // (more than 64 KiB must be asked for, once; a refusal shows at the launch)
-    static const hipError_t asked = hipFuncSetAttribute((const void *)paged_attn_kernel<T, D, RA, RO>, hipFuncAttributeMaxDynamicSharedMemorySize,
-                                                        (int)(pa_lds_bytes<T, D, R>() + (2 * PA_SEARCH + 1) * sizeof(int)));
+    static const hipError_t asked = hipFuncSetAttribute((const void *)paged_attn_kernel<T, D, RA, RO>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     (void)asked;
-    const size_t lds = pa_lds_bytes<T, D, R>() + (a.ahead.spans > 0 && a.sequences <= PA_SEARCH ? (size_t)(2 * a.sequences + 1) * sizeof(int) : 0);
     hipLaunchKernelGGL((paged_attn_kernel<T, D, RA, RO>), dim3(blocks), dim3(PA_THREADS), lds, s, a);
 }
 template <class T>
