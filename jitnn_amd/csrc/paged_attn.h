@@ -50,11 +50,11 @@ struct PaTile<float, D> {
 
 // maximum / sum over the lanes 16, 32 and 48 away
 __device__ __forceinline__ float pa_max4(float v) {
-    float a = v, b = v;
-    asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(a), "+v"(b));
-    a = b = fmaxf(a, b);
-    asm("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(a), "+v"(b));
-    return fmaxf(a, b);
+    float a = v, b = v;  // (the maxima in assembly too: of what comes out of one, the compiler first makes both operands quiet)
+    asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1\n\ts_nop 1\n\tv_max_f32 %0, %0, %1" : "+v"(a), "+v"(b));
+    b = a;
+    asm("s_nop 1\n\tv_permlane16_swap_b32 %0, %1\n\ts_nop 1\n\tv_max_f32 %0, %0, %1" : "+v"(a), "+v"(b));
+    return a;
 }
 __device__ __forceinline__ float pa_sum4(float v) {
     float a = v, b = v;
@@ -649,6 +649,8 @@ __device__ __forceinline__ void pa_wide(const AttnArgs &a, const bool ahead, con
 #pragma unroll
             for (int t = 0; t < TILES; ++t) keys[s][t] = *reinterpret_cast<const u32x4 *>(ks + (size_t)(16 * t + n) * ROW + 16 * pa_piece<PIECES>(4 * s + g, n));
         __builtin_amdgcn_sched_barrier(0);
+        // (a wave with operands for the matrix cores goes before one that works on weights: 8192 rows against 131072 positions 277 us, so and with pa_max4 265)
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int s = 0; s < PIECES / 4; ++s) {
             const u32x4(&k)[TILES] = keys[s];
@@ -668,6 +670,7 @@ __device__ __forceinline__ void pa_wide(const AttnArgs &a, const bool ahead, con
                     for (int r = 0; r < R; ++r) sc[r][0] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(f32x4v, k[0])[j], w.qf[r][s][j], sc[r][0], 0, 0, 0);
             }
         }
+        __builtin_amdgcn_s_setprio(0);
         const bool partial = base + KEYS - 1 > w.first;
         w.weigh(sc, base, partial);
         T v[TILES][4][E] __attribute__((aligned(16)));
@@ -684,8 +687,10 @@ __device__ __forceinline__ void pa_wide(const AttnArgs &a, const bool ahead, con
                 }
             }
         if (partial) w.clean(v, base);
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int e = 0; e < E; ++e) w.sum(v, e);
+        __builtin_amdgcn_s_setprio(0);
     };
     // steps s and s + 1 are requested, s is stored, from then on: barrier, request s + 2, store s + 1, product s
     constexpr std::integral_constant<int, 0> c0{};
@@ -787,9 +792,66 @@ __global__ void __launch_bounds__(PA_THREADS, D <= 128 ? 2 : 1) paged_attn_kerne
     }
 }
 
-// y of every row (token, head) from its spans, a workgroup per row: groups of D / 4 threads take a span each, all of a group's requested before the
-// first is used.  Spans that begin behind the row's position were not written.
+// ---- y of every row (token, head) from its spans.  Spans that begin behind the row's position were not written.
 constexpr int PA_MERGE = 256;
+
+// What token t's rows see: spans of the shared positions and of the sequence's own; false where y is already right or has been made so (`rows` rows of it from y
+// on, this thread's four values of each group of D / 4 threads).
+struct MergeRow {
+    int ahead, count;
+};
+template <int D>
+__device__ __forceinline__ bool merge_row(const AttnArgs &a, const int t, const bool writes, f32x4v_a4 *y, MergeRow &m) {
+    const RowPlace at = row_place(a.starts, a.lens, a.sequences, t);
+    if (at.sequence >= a.sequences || t < a.starts[0]) return false;  // behind the last sequence
+    const int lim = at.len - at.end + t;
+    if (lim < 0 || at.len > a.max_len) {
+        const float f = at.len > a.max_len ? NAN : 0.f;
+        if (writes) *y = f32x4v{f, f, f, f};
+        return false;
+    }
+    m.ahead = min(a.ahead.spans, a.shared > 0 ? lim / a.ahead.span + 1 : 0);
+    m.count = m.ahead + (lim >= a.shared ? (lim - a.shared) / a.own.span + 1 : 0);
+    return true;
+}
+
+// Few spans: D / 4 threads take a row, a workgroup PA_MERGE / (D / 4) rows of a token.
+constexpr int PA_FEW = 8;
+template <int D>
+__global__ void __launch_bounds__(PA_MERGE) paged_merge_few_kernel(const AttnArgs a) {
+    constexpr int LANES = D / 4, GROUPS = PA_MERGE / LANES;
+    const int tid = threadIdx.x, grp = tid / LANES, in = tid - grp * LANES, t = blockIdx.x, h = blockIdx.y * GROUPS + grp;
+    const bool mine = grp < GROUPS && h < a.heads;
+    f32x4v_a4 *y = reinterpret_cast<f32x4v_a4 *>(a.y + (size_t)t * a.y_stride + (size_t)h * D) + in;
+    MergeRow m;
+    if (!merge_row<D>(a, t, mine, y, m) || !mine) return;
+    const int group = a.heads / a.kv, kvh = h / group;
+    const size_t first_slot = (((size_t)kvh * a.tokens + t) * group + h - kvh * group) * (a.ahead.spans + a.own.spans);
+    f32x4v x[PA_FEW];
+    float2 st[PA_FEW];
+#pragma unroll
+    for (int u = 0; u < PA_FEW; ++u)
+        if (u < m.count) {
+            const size_t slot = first_slot + (u < m.ahead ? u : a.ahead.spans + u - m.ahead);
+            st[u] = *reinterpret_cast<const float2 *>(a.stat + 2 * slot);
+            x[u] = *reinterpret_cast<const f32x4v *>(a.part + slot * D + 4 * in);
+        }
+    float top = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int u = 0; u < PA_FEW; ++u)
+        if (u < m.count) top = fmaxf(top, st[u].x);
+    f32x4v acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int u = 0; u < PA_FEW; ++u)
+        if (u < m.count) {
+            const float f = st[u].x > -INFINITY ? __builtin_amdgcn_exp2f(st[u].x - top) : 0.f;
+            sum += st[u].y == st[u].y ? st[u].y * f : NAN;
+            acc += x[u] * f;
+        }
+    *y = acc * (sum == 0.f ? 0.f : 1.f / sum);
+}
+
+// Many: a workgroup per row, groups of D / 4 threads take a span each, all of a group's requested before the first is used.
 template <int D>
 __global__ void __launch_bounds__(PA_MERGE) paged_merge_kernel(const AttnArgs a) {
     constexpr int LANES = D / 4, GROUPS = PA_MERGE / LANES, U = 8;
@@ -798,18 +860,10 @@ __global__ void __launch_bounds__(PA_MERGE) paged_merge_kernel(const AttnArgs a)
     const int tid = threadIdx.x, wave = tid >> 6, grp = tid / LANES, in = tid - grp * LANES;
     const long long row = blockIdx.x;
     const int t = (int)(row / a.heads), h = (int)(row - (long long)t * a.heads), slots = a.ahead.spans + a.own.spans;
-    const RowPlace at = row_place(a.starts, a.lens, a.sequences, t);
-    if (at.sequence >= a.sequences || t < a.starts[0]) return;  // behind the last sequence
-    const int lim = at.len - at.end + t;
     f32x4v_a4 *y = reinterpret_cast<f32x4v_a4 *>(a.y + (size_t)t * a.y_stride + (size_t)h * D);
-    if (lim < 0 || at.len > a.max_len) {
-        const float f = at.len > a.max_len ? NAN : 0.f;
-        if (grp == 0) y[in] = f32x4v{f, f, f, f};
-        return;
-    }
-    const int first_own = a.ahead.spans;
-    const int ahead = min(first_own, a.shared > 0 ? lim / a.ahead.span + 1 : 0), own = lim >= a.shared ? (lim - a.shared) / a.own.span + 1 : 0;
-    const int count = ahead + own;  // at most PA_MERGE (paged_attn_plan)
+    MergeRow m;
+    if (!merge_row<D>(a, t, grp == 0, y + in, m)) return;
+    const int first_own = a.ahead.spans, ahead = m.ahead, count = m.count;  // at most PA_MERGE (paged_attn_plan)
     const int group = a.heads / a.kv, kvh = h / group;
     const size_t first_slot = (((size_t)kvh * a.tokens + t) * group + h - kvh * group) * slots;
     auto slot_of = [&](int i) { return first_slot + (i < ahead ? i : first_own + i - ahead); };
