@@ -5,7 +5,7 @@
 // cumulative sum exceeds u1 times the total.  Such a draw is a whole number that another summation must reproduce, so weights and sums are held
 // in FP64: a cumulative sum of 128256 FP32 weights is off by 1e-5 of a token's share, one of FP64 weights by 1e-14.
 //   verify_stats_kernel   chunks of a row: largest logit (lowest index among equals), sum of exp((l - largest) / T)
-//   verify_rest_kernel    (with draft probabilities) the refused row's sum of max(p - q, 0) per chunk
+//   verify_rest_kernel    (with draft probabilities, more than VERIFY_FEW chunks) the refused row's sum of max(p - q, 0) per chunk
 //   verify_draw_kernel    one workgroup per sequence: which tokens are kept, the chunk the draw falls in, the index in it
 // All rows are judged whether or not an earlier one is refused: they are read once, side by side.
 #pragma once
@@ -176,11 +176,18 @@ struct VerifyEnd {
     bool refused;               // it draws from what its draft left, and is not behind the last draft
     float temperature;
     VerifyStat stat;            // of that row
+    int draft;                  // the token it refused, -1 where that is none
+    float draft_logit, number;  // ... and its random number
 };
 constexpr int VERIFY_ROWS = 32;  // rows whose sums are kept
+struct VerifyRow {
+    VerifyStat stat;
+    int draft;
+    float draft_logit, number;
+};
 struct VerifyShared {
     int first_refused;
-    VerifyStat row[VERIFY_ROWS + 1];
+    VerifyRow row[VERIFY_ROWS + 1];
     double table[32];
 };
 template <int WAVES>
@@ -193,34 +200,36 @@ __device__ __forceinline__ VerifyEnd verify_end(const VerifyArgs &a, int s, Veri
     if (tid == 0) sh.first_refused = count - 1;
     VerifyWeight::fill(sh.table);
     __syncthreads();
-    for (int j = wave; j < count; j += WAVES) {
+    auto judge = [&](const int j, const int slot) {
         const int r = e.first + j;
         const bool drafted = j + 1 < count;
         const int x = drafted ? a.tokens[r + 1] : -1;
         const bool known = x >= 0 && x < a.vocab;  // (a draft that is no token is never kept)
-        const float u = a.uniforms[2 * (size_t)r], lx = known ? a.logits[(size_t)r * a.logits_stride + x] : 0.f,
+        const float u = a.uniforms[2 * (size_t)r], number = a.uniforms[2 * (size_t)r + 1], lx = known ? a.logits[(size_t)r * a.logits_stride + x] : 0.f,
                     qx = known && a.draft_probs ? a.draft_probs[(size_t)r * a.draft_stride + x] : 1.f;
         const VerifyStat t = verify_row((const VerifyStat *)a.part + (size_t)r * a.chunks, a.chunks, sh.table, e.temperature);
         const VerifyWeight weight(sh.table, e.temperature, t.largest);
         const bool keep = known && (e.temperature > 0.f ? t.largest > -INFINITY && (double)u * (double)qx < weight.any(lx) / t.sum : x == t.index);
         if ((tid & 63) == 0) {
-            if (j < VERIFY_ROWS) sh.row[j] = t;
+            if (slot <= VERIFY_ROWS) sh.row[slot] = VerifyRow{t, known ? x : -1, lx, number};
             if (drafted && !keep) atomicMin(&sh.first_refused, j);
         }
-    }
+    };
+    for (int j = wave; j < count; j += WAVES) judge(j, j < VERIFY_ROWS ? j : VERIFY_ROWS + 1);
     __syncthreads();
     e.kept = max(sh.first_refused, 0);
     e.row = count > 0 ? e.first + e.kept : -1;
     e.refused = e.kept < count - 1;
     if (count <= 0) return e;
     if (e.kept >= VERIFY_ROWS) {
-        if (wave == 0) {
-            const VerifyStat t = verify_row((const VerifyStat *)a.part + (size_t)e.row * a.chunks, a.chunks, sh.table, e.temperature);
-            if (tid == 0) sh.row[VERIFY_ROWS] = t;
-        }
+        if (wave == 0) judge(e.kept, VERIFY_ROWS);
         __syncthreads();
     }
-    e.stat = sh.row[min(e.kept, VERIFY_ROWS)];
+    const VerifyRow &at = sh.row[min(e.kept, VERIFY_ROWS)];
+    e.stat = at.stat;
+    e.draft = at.draft;
+    e.draft_logit = at.draft_logit;
+    e.number = at.number;
     return e;
 }
 
@@ -237,10 +246,16 @@ __global__ void __launch_bounds__(VERIFY_THREADS) verify_rest_kernel(const Verif
     const VerifyWeight weight(sh.table, e.temperature, e.stat.largest);
     const double share = 1. / e.stat.sum;
     double sum = 0.;
+    auto add = [&](double w, float q) {
+        const double rest = fma(w, share, -(double)q);
+        sum += rest > 0. && q > -INFINITY ? rest : 0.;  // (behind the row's end q is -inf)
+    };
+    if (fabsf(e.stat.largest) < INFINITY) {
 #pragma unroll
-    for (int u = 0; u < VERIFY_VALUES; ++u) {
-        const double rest = fma(weight.any(l[u]), share, -(double)q[u]);
-        sum += rest > 0. && q[u] > -INFINITY ? rest : 0.;  // (behind the row's end q is -inf)
+        for (int u = 0; u < VERIFY_VALUES; ++u) add(weight(l[u]), q[u]);
+    } else {
+#pragma unroll
+        for (int u = 0; u < VERIFY_VALUES; ++u) add(weight.any(l[u]), q[u]);
     }
     sum = verify_wave_sum(sum);
     if ((tid & 63) == 0) sum_of[tid >> 6] = sum;
@@ -248,14 +263,41 @@ __global__ void __launch_bounds__(VERIFY_THREADS) verify_rest_kernel(const Verif
     if (tid == 0) ((double *)((VerifyStat *)a.part + (size_t)a.rows * a.chunks))[(size_t)s * a.chunks + blockIdx.x] = (sum_of[0] + sum_of[1]) + (sum_of[2] + sum_of[3]);
 }
 
-// grid (sequences)
-constexpr int VERIFY_DRAW_THREADS = 512, VERIFY_DRAW_VALUES = VERIFY_CHUNK / VERIFY_DRAW_THREADS;
-static_assert(VERIFY_DRAW_VALUES % 4 == 0, "whole loads");
+// grid (sequences).  Of few chunks it sums what the refused draft left by itself, 1 us each: all three kernels over 4 x 5 rows took 23 us at four
+// chunks, 17 us so; at five 21 us.
+constexpr int VERIFY_FEW = 4;
+constexpr int VERIFY_DRAW_THREADS = VERIFY_CHUNK / 4;  // four neighbours each, in one load (eight in eight by half as many threads took 3 us longer)
+// what the draw of a row leaves to each of four neighbours: p, without a draft's q or the draft x
+__device__ __forceinline__ void verify_left(const VerifyArgs &a, const VerifyEnd &e, const VerifyWeight &weight, const double share, const float *q, const int x, const int i0,
+                                            double (&w)[4]) {
+    const float *row = a.logits + (size_t)e.row * a.logits_stride;
+    f32x4_a4 l, d = {0.f, 0.f, 0.f, 0.f};
+    if (i0 + 4 <= a.vocab) {
+        l = *reinterpret_cast<const f32x4_a4 *>(row + i0);
+        if (q) d = *reinterpret_cast<const f32x4_a4 *>(q + i0);
+    } else {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const bool there = i0 + u < a.vocab;
+            l[u] = there ? row[i0 + u] : -INFINITY;
+            if (q) d[u] = there ? q[i0 + u] : INFINITY;
+        }
+    }
+    if (fabsf(e.stat.largest) < INFINITY) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) w[u] = weight(l[u]);
+    } else {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) w[u] = weight.any(l[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) w[u] = i0 + u != x ? fmax(fma(w[u], share, -(double)d[u]), 0.) : 0.;
+}
 __global__ void __launch_bounds__(VERIFY_DRAW_THREADS) verify_draw_kernel(const VerifyArgs a) {
     constexpr int WAVES = VERIFY_DRAW_THREADS / 64;
     __shared__ VerifyShared sh;
     __shared__ int chosen_chunk, first_at[WAVES], last_at[WAVES];
-    __shared__ double left, sum_of[WAVES];
+    __shared__ double left, sum_of[WAVES], rest_of[VERIFY_FEW][WAVES];
     const int s = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const VerifyEnd e = verify_end<WAVES>(a, s, sh);
     if (tid == 0) a.accepted[s] = e.row < 0 ? 0 : e.kept;
@@ -268,25 +310,38 @@ __global__ void __launch_bounds__(VERIFY_DRAW_THREADS) verify_draw_kernel(const 
     }
     const VerifyWeight weight(sh.table, e.temperature, e.stat.largest);
     const double share = 1. / e.stat.sum;
-    const int x = e.refused && !a.draft_probs ? a.tokens[e.row + 1] : -1;  // drafted with probability 1: the rest is p without it
-    const float *row = a.logits + (size_t)e.row * a.logits_stride, *q = e.refused && a.draft_probs ? a.draft_probs + (size_t)e.row * a.draft_stride : nullptr;
+    const int x = e.refused && !a.draft_probs ? e.draft : -1;  // drafted with probability 1: the rest is p without it
+    const float *q = e.refused && a.draft_probs ? a.draft_probs + (size_t)e.row * a.draft_stride : nullptr;
+    if (q && a.chunks <= VERIFY_FEW) {
+#pragma unroll 1
+        for (int c = 0; c < a.chunks; ++c) {
+            double w[4];
+            verify_left(a, e, weight, share, q, -1, c * VERIFY_CHUNK + 4 * tid, w);
+            const double sum = verify_wave_sum((w[0] + w[1]) + (w[2] + w[3]));
+            if (lane == 0) rest_of[c][wave] = sum;
+        }
+        __syncthreads();
+    }
     // ---- the chunk: one wave, 64 chunks at a time
     if (wave == 0) {
         const VerifyStat *st = (const VerifyStat *)a.part + (size_t)e.row * a.chunks;
         const double *rest = (const double *)((const VerifyStat *)a.part + (size_t)a.rows * a.chunks) + (size_t)s * a.chunks;
-        const float lx = x >= 0 && x < a.vocab ? row[x] : -INFINITY;
-        const float number = a.uniforms[2 * (size_t)e.row + 1];
         auto weight_of = [&](int c) {
             if (c >= a.chunks) return 0.;
+            if (q && a.chunks <= VERIFY_FEW) {
+                double w = 0.;
+                for (int v = 0; v < WAVES; ++v) w += rest_of[c][v];
+                return w;
+            }
             if (q) return rest[c];
             double w = st[c].largest > -INFINITY ? st[c].sum * weight.any(st[c].largest) : 0.;
-            if (x >= 0 && x / VERIFY_CHUNK == c) w = fmax(w - weight.any(lx), 0.);
+            if (x >= 0 && x / VERIFY_CHUNK == c) w = fmax(w - weight.any(e.draft_logit), 0.);
             return w * share;
         };
         const double first = weight_of(lane);  // (a vocabulary of 262144 has 64 chunks)
         double total = verify_wave_sum(first);
         for (int c0 = 64; c0 < a.chunks; c0 += 64) total += verify_wave_sum(weight_of(c0 + lane));
-        const double target = (double)number * total;
+        const double target = (double)e.number * total;
         double before = 0., before_chunk = 0.;
         int chunk = -1, last = 0;
         for (int c0 = 0; c0 < a.chunks && chunk < 0; c0 += 64) {
@@ -307,21 +362,11 @@ __global__ void __launch_bounds__(VERIFY_DRAW_THREADS) verify_draw_kernel(const 
         }
     }
     __syncthreads();
-    // ---- the index in it: every thread eight neighbours
-    const int i0 = chosen_chunk * VERIFY_CHUNK + tid * VERIFY_DRAW_VALUES;
-    float l[VERIFY_DRAW_VALUES], d[VERIFY_DRAW_VALUES];
-#pragma unroll
-    for (int u = 0; u < VERIFY_DRAW_VALUES; ++u) {
-        const int i = min(i0 + u, a.vocab - 1);
-        l[u] = row[i];
-        d[u] = q ? q[i] : 0.f;
-    }
-    double w[VERIFY_DRAW_VALUES], sum = 0.;
-#pragma unroll
-    for (int u = 0; u < VERIFY_DRAW_VALUES; ++u) {
-        w[u] = i0 + u < a.vocab && i0 + u != x ? fmax(fma(weight.any(l[u]), share, -(double)d[u]), 0.) : 0.;
-        sum += w[u];
-    }
+    // ---- the index in it
+    const int i0 = chosen_chunk * VERIFY_CHUNK + 4 * tid;
+    double w[4];
+    verify_left(a, e, weight, share, q, x, i0, w);
+    const double sum = (w[0] + w[1]) + (w[2] + w[3]);
     const double upto = verify_wave_scan(sum);
     if (lane == 63) sum_of[wave] = upto;
     __syncthreads();
@@ -330,7 +375,7 @@ __global__ void __launch_bounds__(VERIFY_DRAW_THREADS) verify_draw_kernel(const 
     // the first index whose cumulative sum is past what is left; where rounding or a number of 1 leaves none, the last with any weight
     int mine = -1, last = -1;
 #pragma unroll
-    for (int u = 0; u < VERIFY_DRAW_VALUES; ++u) {
+    for (int u = 0; u < 4; ++u) {
         c += w[u];
         if (mine < 0 && w[u] > 0. && c > left) mine = i0 + u;
         if (w[u] > 0.) last = i0 + u;
