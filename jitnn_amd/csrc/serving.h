@@ -46,6 +46,7 @@ struct AttnPart {
     int tiles = 1;      // of 16 rows, per wave
     int span = 0;
     int spans = 0;      // results per row that this part leaves
+    int beside = 8;     // units (span, sequence, key/value head) whose row blocks alternate in the order of the workgroups; a multiple of 8
 };
 struct AttnArgs {
     const void *k, *v;  // of the layer: [pages, kv, page, D]

@@ -50,6 +50,30 @@ static AttnPart rows_shape(long long rows, int D) {
     return p;
 }
 
+// Spans of a part whose waves share their keys and that is alone: the number for which the workgroups and the merge of what they leave, modelled in
+// microseconds, take least; of nearly equal ones the fewest.  A step of a workgroup is its products at 1100 (FP16) or 140 (FP32) TFLOP/s, on top of which it
+// waits 0.35 us and 3.5 ns a value of the head, two thirds of that where the CU has another one to work on; before the first it takes 5 (2.5).  The
+// merge is a launch, and what is written and read again of each row and span at 4.2 TB/s.  Heads of 128, FP16, 32 of them: 2000 tokens' own positions, one span
+// 91 us, two 119; 512 tokens behind 3584 others, one 158, two 99, four 86, eight 101.
+static int wide_spans(bool half, int D, long long rows_all, const AttnPart &q, long long units, int keys, double len, double seen, int cus) {
+    const int per_cu = D <= 128 ? 2 : 1;
+    const double product = (half ? 0.00167 : 0.0067) * D * q.tiles;
+    int best = 1;
+    double least = 1e30;
+    for (int n = 1; n <= 120 && (n - 1) * keys < len; n = std::max(n + 1, n * 5 / 4)) {
+        const double longest = std::ceil(len / n / keys), mean = std::max(seen / n / keys, 0.5), rounds = std::ceil((double)units * n / cus);
+        const bool two = per_cu == 2 && rounds > 1;
+        const double wait = (0.35 + 0.0035 * D) * (two ? 0.65 : 1.);
+        const double run = std::max(5 + longest * (product + 0.35 + 0.0035 * D), rounds * ((two ? 2.5 : 5.) + mean * (product + wait)));
+        const double time = run + (n > 1 ? 6 + (double)rows_all * std::min(n * seen / len + 0.5, (double)n) * (D + 2) * 8 / 4.2e6 : 0.);
+        if (time < 0.95 * least) {
+            least = time;
+            best = n;
+        }
+    }
+    return best;
+}
+
 AttnPlan paged_attn_plan(bool half, int D, int heads, int kv, int sequences, long long tokens, int max_tokens, int max_len, int shared, int cus) {
     const int group = heads / kv, keys = half ? 32 : 16;
     AttnPlan p;
@@ -68,14 +92,29 @@ AttnPlan paged_attn_plan(bool half, int D, int heads, int kv, int sequences, lon
         q.span = (int)std::min<double>(std::ceil(want / least) * least, std::ceil(len / least) * least);
         q.spans = (int)((len + q.span - 1) / q.span);
     };
+    // Where a sequence's rows differ much in what they see; where they do not, the fewer units at a time share the more in an XCD's L2 (63 sequences of 40 tokens
+    // behind 360 others 54 us, with these 58).  No more units than there are: the order is dense, and so is their spread over the CUs.
+    auto side_by_side = [&](AttnPart &q) {
+        if (2. * max_tokens < own_len) return;
+        const long long units = ((long long)kv * sequences * q.spans + 7) / 8 * 8;
+        q.beside = (int)std::min<long long>(units, std::max(8, (D <= 128 ? 2 : 1) * cus / q.blocks / 8 * 8));
+    };
+    if (shared == 0 && p.own.key_waves == 1) {
+        const int n = wide_spans(half, D, tokens * heads, p.own, (long long)p.own.blocks * kv * sequences, keys, own_len, std::max(own_len - 0.5 * max_tokens, 1.), cus);
+        p.own.span = (int)std::ceil(own_len / n / keys) * keys;
+        p.own.spans = (int)((own_len + p.own.span - 1) / p.own.span);
+        side_by_side(p.own);
+        return p;
+    }
     if (shared > 0) cut(p.ahead, shared);
     cut(p.own, own_len);
+    side_by_side(p.own);
     return p;
 }
 
 void paged_attn_launch(bool half, int D, int cus, hipStream_t s, AttnArgs a) {
     const unsigned units_ahead = (unsigned)(a.ahead.spans * a.kv), units_own = (unsigned)(a.own.spans * a.kv * a.sequences);
-    const unsigned ahead = (units_ahead + 7) / 8 * 8 * (unsigned)a.ahead.blocks, own = (units_own + 7) / 8 * 8 * (unsigned)a.own.blocks;
+    const unsigned ahead = (units_ahead + a.ahead.beside - 1) / a.ahead.beside * a.ahead.beside * (unsigned)a.ahead.blocks, own = (units_own + a.own.beside - 1) / a.own.beside * a.own.beside * (unsigned)a.own.blocks;
     a.chunk = std::max(8, cus / 8 * 8);  // one to a CU
     a.chunks_ahead = (int)((ahead + a.chunk - 1) / a.chunk);
     a.chunks_own = (int)((own + a.chunk - 1) / a.chunk);
