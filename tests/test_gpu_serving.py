@@ -230,6 +230,23 @@ def test_attention(jn, half, hd, heads, kv, page, counts, lens, shared):
     assert torch.equal(run_attention(jn, b, q, pools, half, scale, layer=1), got)  # and again, to the bit
 
 
+PROMPTS = [
+    # hd, heads, kv, page, counts, lens, shared: many rows, some of which see all and some almost nothing
+    (64, 8, 4, 16, [130, 70, 200, 33, 90], [130, 75, 200, 33, 96], 0),
+    (128, 12, 4, 64, [150, 0, 149, 151, 80], [150, 0, 300, 120, 333], 0),   # (one has rows in front of its first position)
+    (128, 16, 2, 32, [300, 280], [900, 700], 0),                             # few spans of many rows
+    (256, 12, 3, 128, [60, 70, 41], [60, 77, 300], 0),
+    (192, 4, 2, 16, [129], [700], 0),
+    (64, 16, 2, 64, [65, 140], [400, 350], 3),
+]
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("hd,heads,kv,page,counts,lens,shared", PROMPTS)
+def test_attention_of_prompts(jn, half, hd, heads, kv, page, counts, lens, shared):
+    test_attention(jn, half, hd, heads, kv, page, counts, lens, shared)
+
+
 @pytest.mark.parametrize("half", [False, True])
 @pytest.mark.parametrize("hd,shared", [(128, 0), (128, 4), (64, 2), (256, 1)])
 def test_attention_ignores_what_a_row_does_not_see(jn, half, hd, shared):
@@ -470,24 +487,25 @@ def test_verify(jn, with_q, counts, vocab, stride):
         assert np.array_equal(got[1], want[1]) and np.array_equal(got[0], want[0])
 
 
+@pytest.mark.parametrize("vocab", [20000, 9000])  # (of few chunks the draw sums by itself what a draft left)
 @pytest.mark.parametrize("with_q", [False, True])
-def test_verify_of_odd_logits_and_numbers(jn, with_q):
+def test_verify_of_odd_logits_and_numbers(jn, with_q, vocab):
     """Equal largest logits, NaN and infinities, rows of nothing else, random numbers of 0 and just below 1, drafts that are no tokens or have no probability."""
     rng = np.random.default_rng(1)
-    counts, vocab = [4] * 12, 20000
+    counts = [4] * 12
     logits, starts, tokens, q, temps, u = drafts(rng, counts, vocab)
     temps = [0.0, 1.0, 0.7] * 4
     below_one = np.float32(1 - 2.0 ** -24)
     u[0:8] = 0
     u[8:16] = below_one
-    logits[1, [500, 9000, 19999]] = logits[1].max() + 1                     # equal largest ones, in three chunks
+    logits[1, [500, 8192, vocab - 1]] = logits[1].max() + 1                     # equal largest ones, in three chunks
     logits[4:8, ::2] = np.nan
     logits[5, 1::2] = -np.inf                                              # nothing at all
     logits[9, 7777] = np.inf
-    logits[13, [3, 12345]] = np.inf                                        # two that share all the weight
+    logits[13, [3, 8345]] = np.inf                                        # two that share all the weight
     logits[17] = -np.inf
     logits[18] = np.nan
-    logits[19, :19000] = -np.inf
+    logits[19, :vocab - 1000] = -np.inf
     tokens[21], tokens[22], tokens[25], tokens[26] = vocab, -1, 1 << 30, -(1 << 31)
     q[28, tokens[29]] = 0
     logits[32, tokens[33]] = -np.inf
