@@ -293,12 +293,12 @@ JITNN_HIP_API int jitnn_hip_paged_cache_copy_page_dev(const jitnn_hip_paged_cach
 /* The tokens of one pass: `tokens` rows, those of sequence s being rows starts[s] .. starts[s + 1] - 1 (ascending; a sequence may have none), its last
  * `starts[s + 1] - starts[s]` positions of the lens[s] it then has.  Position p of sequence s lies on page tables[s * table_stride + p / page_tokens].
  * The arrays are device memory and read when the work runs, so that a recorded graph can be replayed with others; the numbers are host values:
- * max_tokens and max_len bound a sequence's rows and its lens, shared_pages counts the leading pages that all rows of tables have in common (0:
+ * max_tokens and max_len (at most 2^30) bound a sequence's rows and its lens, shared_pages counts the leading pages that all rows of tables have in common (0:
  * none; attention reads them once for the whole batch, by the first row of tables).
  * What the arrays hold is checked where it is used: rows of x, q, y in front of starts[0] or behind starts[sequences] are left as they were.  A position
  * below 0 (a lens smaller than its rows) is appended nowhere and attends to nothing: a zero row.  A page id outside the cache is neither read nor
- * written, and a sequence whose lens is above max_len is not attended: the rows that would have seen them are NaN.  Rows of a sequence beyond
- * max_tokens may stay as they were. */
+ * written, and a sequence whose lens is above max_len is not attended: the rows that would have seen them are NaN.  What attention makes of a
+ * sequence's rows beyond max_tokens is undefined. */
 typedef struct jitnn_hip_batch {
     int sequences, tokens, max_tokens, max_len;
     int shared_pages, table_stride;
@@ -336,7 +336,8 @@ JITNN_HIP_API int jitnn_hip_paged_attention_dev(const jitnn_hip_paged_cache *c, 
  * that row.  Sums in FP64.  uniforms [rows, 2] in [0, 1).
  * accepted[s]: drafts kept.  out [rows]: per sequence the kept drafts, the drawn token, then -1.  A draft outside [0, vocab) is not kept.  NaN logits
  * have no weight; a row of nothing but NaN and -inf gives its lowest index that is not NaN.  A sequence without rows: accepted 0.  Rows in front of starts[0] and behind
- * starts[sequences] are left as they were.  starts, tokens, draft_probs, temperatures, uniforms, out, accepted: device memory.  Workspace as above. */
+ * starts[sequences] are left as they were.  vocab at most 2^30.  starts, tokens, draft_probs, temperatures, uniforms, out, accepted: device memory, the last two apart from the others.  Workspace
+ * as above. */
 JITNN_HIP_API long long jitnn_hip_verify_workspace(int rows, int sequences, int vocab);
 JITNN_HIP_API int jitnn_hip_verify_drafts_dev(const float *logits_dev, long long logits_stride, int rows, int vocab, const int *starts_dev, int sequences,
                                               const int *tokens_dev, const float *draft_probs_dev, long long draft_stride, const float *temperatures_dev,
@@ -425,7 +426,7 @@ JITNN_HIP_API int jitnn_hip_llama_set_rope(jitnn_hip_llama *m, const jitnn_hip_r
  * rows logit_rows [logit_count] (device memory; a row outside the batch gives NaN): a decode step names every row, a prompt's pass its last.
  * logit_count 0: none.  The rows go through the linears together, as in jitnn_hip_llama_prefill; the model's own cache is not touched.
  * The model's many-token buffers and the attention's workspace belong to it and grow with the largest pass (which waits for the device; such a
- * call cannot be recorded: JITNN_HIP_EINVAL). */
+ * call cannot be recorded: JITNN_HIP_EINVAL).  Once a pass has been recorded, those that larger ones replace live on until the model is freed. */
 JITNN_HIP_API int jitnn_hip_llama_step_dev(jitnn_hip_llama *m, const jitnn_hip_paged_cache *c, const jitnn_hip_batch *batch, const float *x_dev,
                                            const int *logit_rows_dev, int logit_count, float *logits_dev, void *stream);
 

@@ -2061,6 +2061,7 @@ int check_batch(const jitnn_hip_paged_cache *c, const jitnn_hip_batch *b) {
     if (b->sequences < 0 || b->tokens < 0 || b->max_tokens < 0 || b->max_len < 0 || b->shared_pages < 0 || b->table_stride < 0 || b->sequences > 65535)
         return fail(JITNN_HIP_EINVAL, "%d sequences, %d tokens (at most %d each), lengths to %d, %d shared of %d pages", b->sequences, b->tokens, b->max_tokens, b->max_len,
                     b->shared_pages, b->table_stride);
+    if (b->max_len > 1 << 30) return fail(JITNN_HIP_EINVAL, "lengths to %d (at most 2^30)", b->max_len);
     if (b->shared_pages > b->table_stride || (long long)b->max_len > (long long)b->table_stride * c->page_tokens)
         return fail(JITNN_HIP_EINVAL, "lengths to %d and %d shared pages in tables of %d pages of %d", b->max_len, b->shared_pages, b->table_stride, c->page_tokens);
     if (b->tokens > 0 && b->sequences > 0 && (!b->starts || !b->lens || (!b->tables && b->table_stride > 0))) return fail(JITNN_HIP_EINVAL, "NULL array of the batch");
@@ -2236,7 +2237,8 @@ int jitnn_hip_paged_attention_dev(const jitnn_hip_paged_cache *c, int layer, con
         return fail(JITNN_HIP_EINVAL, "a workspace of %lld bytes, %zu are needed (aligned to 16)", workspace_dev ? workspace_bytes : 0ll, need);
     const long long units = (long long)p.own.spans * c->kv * b->sequences * p.own.blocks + (long long)p.ahead.spans * c->kv * p.ahead.blocks,
                     merges = (long long)b->tokens * heads;
-    if (units > (1 << 28) || merges > (1 << 28)) return fail(JITNN_HIP_EINVAL, "%d sequences of up to %d tokens are too many for one pass", b->sequences, b->max_tokens);
+    // (a launch holds fewer than 2^32 threads; the order of the workgroups may leave as many of them empty as there are)
+    if (units > (1 << 22) || merges > (1 << 28) || (need > 0 && merges >= (1 << 24))) return fail(JITNN_HIP_EINVAL, "%d sequences of up to %d tokens are too many for one pass", b->sequences, b->max_tokens);
     AttnArgs a;
     a.k = c->k + (size_t)layer * c->layer_bytes();
     a.v = c->v + (size_t)layer * c->layer_bytes();
@@ -2269,8 +2271,8 @@ int jitnn_hip_paged_attention_dev(const jitnn_hip_paged_cache *c, int layer, con
 // ---- drafted tokens
 
 static int check_drafts(int rows, int sequences, int vocab) {
-    if (rows < 0 || sequences < 0 || vocab < 1 || rows > 65535 || sequences > 65535)
-        return fail(JITNN_HIP_EINVAL, "%d rows of %d sequences (at most 65535) over a vocabulary of %d", rows, sequences, vocab);
+    if (rows < 0 || sequences < 0 || vocab < 1 || rows > 65535 || sequences > 65535 || vocab > 1 << 30)
+        return fail(JITNN_HIP_EINVAL, "%d rows of %d sequences (at most 65535) over a vocabulary of %d (at most 2^30)", rows, sequences, vocab);
     return JITNN_HIP_OK;
 }
 
@@ -2336,6 +2338,11 @@ struct jitnn_hip_llama {
     jitnn_hip_rope *rope;  // what cosv and sinv hold, for positions of a paged cache (the pairing is rope_interleaved)
     void *paged_ws;        // workspace of the attention over a paged cache, grown by jitnn_hip_llama_step_dev
     size_t paged_ws_bytes;
+    bool recorded;         // a pass over a paged cache has been recorded: buffers that its replays use are kept, not freed, where larger ones take their place
+    struct Kept {
+        void *p;
+        Kept *next;
+    } *kept;
     // token embedding table [vocab, d] in ggml type embd_fmt (F32 = 0, F16 = 1 or a block format), owned
     uint8_t *embd;
     int embd_fmt;
@@ -2533,14 +2540,22 @@ int residual_linear_rows(const jitnn_hip_weight *w, const float *x, int rows, co
 }
 
 // The many-token buffers of a model, for at least `tokens` rows.
+// A buffer that a larger one replaces.
+void release_or_keep(jitnn_hip_llama *m, void *p) {
+    if (!p) return;
+    jitnn_hip_llama::Kept *k = m->recorded ? new (std::nothrow) jitnn_hip_llama::Kept{p, m->kept} : nullptr;
+    if (k) m->kept = k;
+    else if (!m->recorded) (void)hipFree(p);  // (no memory to note it: left to the process)
+}
+
 int ensure_prefill(jitnn_hip_llama *m, int tokens) {
     if (tokens <= m->pf_cap) return JITNN_HIP_OK;
     HIP_TRY(hipDeviceSynchronize());  // earlier calls may still use the old buffers
+    m->pf_cap = 0;
     for (float *&b : m->pf) {
-        if (b) (void)hipFree(b);
+        release_or_keep(m, b);
         b = nullptr;
     }
-    m->pf_cap = 0;
     const size_t qd = (size_t)m->heads * m->hd, kd = (size_t)m->kv * m->hd;
     const size_t per[11] = {(size_t)m->d, qd, kd, kd, qd, (size_t)m->d, (size_t)m->d, (size_t)m->ffn, (size_t)m->ffn, (size_t)m->ffn, (size_t)8 * m->d};
     for (int i = 0; i < 11; ++i) {
@@ -2796,6 +2811,12 @@ int jitnn_hip_llama_free(jitnn_hip_llama *m) {
         if (b) (void)hipFree(b);
     if (m->packed) (void)hipFree(m->packed);
     if (m->paged_ws) (void)hipFree(m->paged_ws);
+    while (m->kept) {
+        jitnn_hip_llama::Kept *k = m->kept;
+        m->kept = k->next;
+        (void)hipFree(k->p);
+        delete k;
+    }
     rope_drop(m->rope);
     if (m->embd) (void)hipFree(m->embd);
     if (m->tok_dev) (void)hipFree(m->tok_dev);
@@ -3005,10 +3026,11 @@ int jitnn_hip_llama_step_dev(jitnn_hip_llama *m, const jitnn_hip_paged_cache *c,
     if (need < 0) return (int)need;
     if ((T > m->pf_cap || (size_t)need > m->paged_ws_bytes) && stream_recording(st))
         return fail(JITNN_HIP_EINVAL, "a pass of %d tokens needs larger buffers than the model has, which a recording cannot allocate", T);
+    if (stream_recording(st)) m->recorded = true;
     if (int rc = ensure_prefill(m, T)) return rc;
     if ((size_t)need > m->paged_ws_bytes) {
         HIP_TRY(hipDeviceSynchronize());  // earlier passes may still use the old one
-        if (m->paged_ws) (void)hipFree(m->paged_ws);
+        release_or_keep(m, m->paged_ws);
         m->paged_ws = nullptr;
         m->paged_ws_bytes = 0;
         if (hipMalloc(&m->paged_ws, (size_t)need) != hipSuccess) {

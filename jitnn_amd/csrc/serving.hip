@@ -146,7 +146,7 @@ size_t verify_workspace(int rows, int sequences, int vocab) {
 }
 void verify_launch(VerifyArgs a, hipStream_t s) {
     a.chunks = verify_chunks(a.vocab);
-    hipLaunchKernelGGL(verify_stats_kernel, dim3(a.chunks, a.rows), dim3(VERIFY_THREADS), 0, s, a);
+    if (a.rows > 0) hipLaunchKernelGGL(verify_stats_kernel, dim3(a.chunks, a.rows), dim3(VERIFY_THREADS), 0, s, a);
     if (a.draft_probs && a.chunks > VERIFY_FEW) hipLaunchKernelGGL(verify_rest_kernel, dim3(a.chunks, a.sequences), dim3(VERIFY_THREADS), 0, s, a);
     hipLaunchKernelGGL(verify_draw_kernel, dim3(a.sequences), dim3(VERIFY_DRAW_THREADS), 0, s, a);
 }

@@ -437,7 +437,7 @@ def test_serving_refusals_of_sizes(jn):
 
 # ---------------------------------------------------------------------------------------------- drafted tokens
 
-def run_verify(jn, logits, starts, tokens, q, temps, uniforms, stride=0):
+def run_verify(jn, logits, starts, tokens, q, temps, uniforms, stride=0, rows_of_call=None):
     rows, vocab = logits.shape
     wide = np.zeros((rows, vocab + stride), dtype=np.float32)
     wide[:, :vocab] = logits
@@ -449,6 +449,7 @@ def run_verify(jn, logits, starts, tokens, q, temps, uniforms, stride=0):
         dq = dev(wq)
     out = torch.full((rows,), -7, dtype=torch.int32, device="cuda")
     acc = torch.full((len(temps),), -7, dtype=torch.int32, device="cuda")
+    rows = rows if rows_of_call is None else rows_of_call
     n = jn.verify_workspace(rows, len(temps), vocab)
     ws = torch.full((n // 4 + 4,), float("nan"), device="cuda")
     jn.verify_drafts_dev(keep[0].data_ptr(), rows, vocab, keep[1].data_ptr(), len(temps), keep[2].data_ptr(), keep[3].data_ptr(), keep[4].data_ptr(), out.data_ptr(),
@@ -514,6 +515,13 @@ def test_verify_of_odd_logits_and_numbers(jn, with_q, vocab):
     want = ref.verify(logits, starts, tokens, q if with_q else None, [0.0 if not t > 0 else t for t in temps], u)
     got = run_verify(jn, logits, starts, tokens, q if with_q else None, temps, u)
     assert np.array_equal(got[1], want[1]) and np.array_equal(got[0], want[0]), (np.argwhere(got[0] != want[0]), got[0], want[0])
+
+
+def test_verify_of_no_rows(jn):
+    """Sequences without rows, with and without draft probabilities: nothing kept, and nothing else written."""
+    for q in (None, np.zeros((1, 9000), np.float32)):
+        out, acc = run_verify(jn, np.zeros((1, 9000), np.float32), [0, 0, 0], [0], q, [1.0, 0.0], np.zeros((1, 2), np.float32), rows_of_call=0)
+        assert list(acc) == [0, 0] and list(out) == [-7]
 
 
 def test_verify_follows_the_target(jn):

@@ -212,14 +212,20 @@ def test_files_that_scale_their_positions(jn, tmp_path, monkeypatch):
     cases = {"plain": ({}, []), "linear": ({"llama.rope.scaling.type": "linear", "llama.rope.scaling.factor": 4.0}, []),
              "yarn": ({"llama.rope.scaling.type": "yarn", "llama.rope.scaling.factor": 4.0, "llama.rope.scaling.original_context_length": 16}, []),
              "factors": ({}, [("rope_freqs.weight", (32,), 0, factors)]), "part": ({"llama.rope.dimension_count": 32}, []),
+             "magnitude": ({"llama.rope.scaling.attn_factor": 1.5}, []),
+             "yarn with one": ({"llama.rope.scaling.type": "yarn", "llama.rope.scaling.factor": 4.0, "llama.rope.scaling.original_context_length": 16,
+                                "llama.rope.scaling.attn_factor": 0.5, "llama.rope.scaling.yarn_beta_fast": 8.0}, []),
              "whole": ({"llama.rope.dimension_count": 64, "llama.rope.scaling.type": "none"}, [])}
-    want = {"linear": dict(kind="linear", factor=4.0), "yarn": dict(kind="yarn", factor=4.0, original=16), "factors": dict(factors=factors)}
+    want = {"linear": dict(kind="linear", factor=4.0), "yarn": dict(kind="yarn", factor=4.0, original=16), "factors": dict(factors=factors),
+            "yarn with one": dict(kind="yarn", factor=4.0, original=16, beta_fast=8.0)}
+    gain = {"magnitude": 1.5, "yarn with one": 0.5}  # (on top of the scaling's own)
     for name, (meta, tensors) in cases.items():
         monkeypatch.setattr(test_llm, "write_gguf", lambda p, m, t: write_gguf(p, {**m, **meta}, t + tensors))
         path = tmp_path / f"{name}.gguf"
         test_llm.write_model(path, "llama", 11)
         rot = 32 if name == "part" else 64
         f, m = ref.rope_frequencies(rot, 10000.0, **want.get(name, {}))
+        m *= gain.get(name, 1.0)
         with jn.Llm.load(path) as llm:
             dec = llm.model()
             x = dec.embed([7])[0]
@@ -230,8 +236,11 @@ def test_files_that_scale_their_positions(jn, tmp_path, monkeypatch):
             assert np.abs(dec.kv_read(0, 29, 1)[0][0] - ref.rotate(raw[None], [29], f, m, True)[0]).max() <= 1e-5 * np.abs(raw).max(), name
     monkeypatch.setattr(test_llm, "write_gguf", lambda p, m, t: write_gguf(p, {**m, "llama.rope.scaling.type": "longrope"}, t))
     test_llm.write_model(tmp_path / "other.gguf", "llama", 11)
-    with pytest.raises(ValueError, match="longrope"):
-        jn.Llm.load(tmp_path / "other.gguf")
+    with pytest.warns(UserWarning, match="longrope"), jn.Llm.load(tmp_path / "other.gguf") as other, jn.Llm.load(tmp_path / "plain.gguf") as plain:
+        x = plain.model().embed([7])[0]
+        for llm in (other, plain):
+            llm.model().decode(x, 29)
+        assert np.array_equal(other.model().kv_read(0, 29, 1)[0], plain.model().kv_read(0, 29, 1)[0])
 
 
 def test_recorded_step(jn, model_file):
@@ -272,6 +281,20 @@ def test_recorded_step(jn, model_file):
                 rc = _lib.lib.jitnn_hip_llama_step_dev(dec.handle, cache.handle, wide, x.data_ptr(), None, 0, None, side.cuda_stream)
                 y.add_(0)  # (a recording of something)
             assert rc == _lib.EINVAL and "recording" in _lib.last_error()
+            # an eager pass that takes larger buffers, and a replay on those it was recorded with
+            many = torch.zeros(900, 256, device="cuda")
+            large = jn.Batch(1, 900, 900, 48, keep[0].data_ptr(), b.width, keep[1].data_ptr(), keep[2].data_ptr())
+            dec.step_dev(cache, large, many.data_ptr(), 0, 0, 0, side.cuda_stream)
+            side.synchronize()
+            filler = [torch.full((1 << 20,), float("nan"), device="cuda") for _ in range(8)]
+            for _ in range(2):
+                x.normal_()
+                graph.replay()
+                side.synchronize()
+                step(z, side)
+                side.synchronize()
+                assert torch.equal(y, z) and torch.isfinite(y).all()
+            del filler
 
 
 def test_step_refusals(jn, model_file):

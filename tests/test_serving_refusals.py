@@ -47,7 +47,7 @@ def test_batches_and_arguments(lib):
         return lib.lib.jitnn_hip_paged_attention_dev(h, layer, batch, heads, a["q"], a["qs"], a["scale"], a["y"], a["ys"], None, 0, None)
 
     for bad in (dict(sequences=-1), dict(tokens=-1), dict(max_tokens=-1), dict(max_len=-1), dict(max_len=49), dict(shared_pages=4), dict(shared_pages=-1), dict(table_stride=-1),
-                dict(tables_ptr=0), dict(starts_ptr=0), dict(lens_ptr=0), dict(sequences=65536)):
+                dict(tables_ptr=0), dict(starts_ptr=0), dict(lens_ptr=0), dict(sequences=65536), dict(max_len=(1 << 30) + 1, table_stride=1 << 27)):
         b = Batch(**{**good, **bad})
         assert append(b) == lib.EINVAL and attend(b) == lib.EINVAL, bad
         assert lib.lib.jitnn_hip_paged_attention_workspace(h, b, 4) == lib.EINVAL
@@ -85,8 +85,9 @@ def test_null_handles(lib):
 
 def test_workspace_of_drafts(lib):
     n = lib.lib.jitnn_hip_verify_workspace
-    assert n(1, 1, 1) == 24 and n(5, 2, 8192) == 96 and n(5, 2, 8193) == 192
+    assert n(1, 1, 1) == 24 and n(5, 2, 4096) == 96 and n(5, 2, 4097) == 192
     assert n(-1, 1, 1) == lib.EINVAL and n(1, -1, 1) == lib.EINVAL and n(1, 1, 0) == lib.EINVAL and n(65536, 1, 10) == lib.EINVAL
+    assert n(1, 1, (1 << 30) + 1) == lib.EINVAL and n(1, 1, 1 << 30) == (24 + 8 - 8) * (1 << 18) and n(0, 3, 1) == 24
 
 
 def test_requests_with_drafts():
