@@ -153,8 +153,8 @@ __global__ void __launch_bounds__(VERIFY_THREADS) verify_stats_kernel(const Veri
     }
 }
 
-// A row's largest logit, its index and the sum of its weights, from the chunks'; one wave, every lane receives them.
-__device__ __forceinline__ VerifyStat verify_row(const VerifyStat *__restrict__ st, int chunks, const double *table, float temperature) {
+// A row's largest logit, its index and the sum of its weights, from the chunks'; one wave, every lane receives them.  first: chunk `lane`'s part of the sum.
+__device__ __forceinline__ VerifyStat verify_row(const VerifyStat *__restrict__ st, int chunks, const double *table, float temperature, double &first) {
     const int lane = threadIdx.x & 63;
     VerifyStat t{0., -INFINITY, 0x7fffffff}, mine{0., -INFINITY, 0x7fffffff};
     if (lane < chunks) mine = st[lane];
@@ -162,7 +162,8 @@ __device__ __forceinline__ VerifyStat verify_row(const VerifyStat *__restrict__ 
     for (int c = lane + 64; c < chunks; c += 64) verify_take(st[c].largest, st[c].index, t.largest, t.index);
     verify_wave_best(t.largest, t.index);
     const VerifyWeight weight(table, temperature, t.largest);
-    if (mine.largest > -INFINITY) t.sum = mine.sum * weight.any(mine.largest);
+    first = mine.largest > -INFINITY ? mine.sum * weight.any(mine.largest) : 0.;
+    t.sum = first;
     for (int c = lane + 64; c < chunks; c += 64)
         if (st[c].largest > -INFINITY) t.sum += st[c].sum * weight.any(st[c].largest);
     t.sum = verify_wave_sum(t.sum);
@@ -178,6 +179,7 @@ struct VerifyEnd {
     VerifyStat stat;            // of that row
     int draft;                  // the token it refused, -1 where that is none
     float draft_logit, number;  // ... and its random number
+    const double *parts;
 };
 constexpr int VERIFY_ROWS = 32;  // rows whose sums are kept
 struct VerifyRow {
@@ -190,8 +192,9 @@ struct VerifyShared {
     VerifyRow row[VERIFY_ROWS + 1];
     double table[32];
 };
+// parts [VERIFY_ROWS + 1][64] (or nullptr): what the first 64 chunks of each row hold of its sum; e.parts is the drawing row's.
 template <int WAVES>
-__device__ __forceinline__ VerifyEnd verify_end(const VerifyArgs &a, int s, VerifyShared &sh) {
+__device__ __forceinline__ VerifyEnd verify_end(const VerifyArgs &a, int s, VerifyShared &sh, double *parts) {
     VerifyEnd e;
     e.first = min(max(a.starts[s], 0), a.rows);
     e.end = min(max(a.starts[s + 1], e.first), a.rows);
@@ -207,7 +210,9 @@ __device__ __forceinline__ VerifyEnd verify_end(const VerifyArgs &a, int s, Veri
         const bool known = x >= 0 && x < a.vocab;  // (a draft that is no token is never kept)
         const float u = a.uniforms[2 * (size_t)r], number = a.uniforms[2 * (size_t)r + 1], lx = known ? a.logits[(size_t)r * a.logits_stride + x] : 0.f,
                     qx = known && a.draft_probs ? a.draft_probs[(size_t)r * a.draft_stride + x] : 1.f;
-        const VerifyStat t = verify_row((const VerifyStat *)a.part + (size_t)r * a.chunks, a.chunks, sh.table, e.temperature);
+        double first;
+        const VerifyStat t = verify_row((const VerifyStat *)a.part + (size_t)r * a.chunks, a.chunks, sh.table, e.temperature, first);
+        if (parts && slot <= VERIFY_ROWS) parts[64 * slot + (tid & 63)] = first;
         const VerifyWeight weight(sh.table, e.temperature, t.largest);
         const bool keep = known && (e.temperature > 0.f ? t.largest > -INFINITY && (double)u * (double)qx < weight.any(lx) / t.sum : x == t.index);
         if ((tid & 63) == 0) {
@@ -225,7 +230,9 @@ __device__ __forceinline__ VerifyEnd verify_end(const VerifyArgs &a, int s, Veri
         if (wave == 0) judge(e.kept, VERIFY_ROWS);
         __syncthreads();
     }
-    const VerifyRow &at = sh.row[min(e.kept, VERIFY_ROWS)];
+    const int slot = min(e.kept, VERIFY_ROWS);
+    const VerifyRow &at = sh.row[slot];
+    e.parts = parts ? parts + 64 * slot : nullptr;
     e.stat = at.stat;
     e.draft = at.draft;
     e.draft_logit = at.draft_logit;
@@ -238,7 +245,7 @@ __global__ void __launch_bounds__(VERIFY_THREADS) verify_rest_kernel(const Verif
     __shared__ VerifyShared sh;
     __shared__ double sum_of[VERIFY_THREADS / 64];
     const int s = blockIdx.y, c0 = blockIdx.x * VERIFY_CHUNK, tid = threadIdx.x;
-    const VerifyEnd e = verify_end<VERIFY_THREADS / 64>(a, s, sh);
+    const VerifyEnd e = verify_end<VERIFY_THREADS / 64>(a, s, sh, nullptr);
     if (e.row < 0 || !e.refused || !(e.temperature > 0.f)) return;
     float l[VERIFY_VALUES], q[VERIFY_VALUES];
     verify_load(a.logits + (size_t)e.row * a.logits_stride, c0, a.vocab, l);
@@ -297,9 +304,12 @@ __global__ void __launch_bounds__(VERIFY_DRAW_THREADS) verify_draw_kernel(const 
     constexpr int WAVES = VERIFY_DRAW_THREADS / 64;
     __shared__ VerifyShared sh;
     __shared__ int chosen_chunk, first_at[WAVES], last_at[WAVES];
-    __shared__ double left, sum_of[WAVES], rest_of[VERIFY_FEW][WAVES];
+    __shared__ double left, sum_of[WAVES], rest_of[VERIFY_FEW][WAVES], parts[(VERIFY_ROWS + 1) * 64];
     const int s = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const VerifyEnd e = verify_end<WAVES>(a, s, sh);
+    const double *rest = (const double *)((const VerifyStat *)a.part + (size_t)a.rows * a.chunks) + (size_t)s * a.chunks;
+    // (asked for before it is known whether it is needed; without a refused draft nobody has written it)
+    const double first_rest = a.draft_probs && a.chunks > VERIFY_FEW && lane < a.chunks ? rest[lane] : 0.;
+    const VerifyEnd e = verify_end<WAVES>(a, s, sh, parts);
     if (tid == 0) a.accepted[s] = e.row < 0 ? 0 : e.kept;
     if (e.row < 0) return;
     for (int r = e.first + tid; r < e.end; r += VERIFY_DRAW_THREADS)
@@ -325,7 +335,6 @@ __global__ void __launch_bounds__(VERIFY_DRAW_THREADS) verify_draw_kernel(const 
     // ---- the chunk: one wave, 64 chunks at a time
     if (wave == 0) {
         const VerifyStat *st = (const VerifyStat *)a.part + (size_t)e.row * a.chunks;
-        const double *rest = (const double *)((const VerifyStat *)a.part + (size_t)a.rows * a.chunks) + (size_t)s * a.chunks;
         auto weight_of = [&](int c) {
             if (c >= a.chunks) return 0.;
             if (q && a.chunks <= VERIFY_FEW) {
@@ -333,8 +342,8 @@ __global__ void __launch_bounds__(VERIFY_DRAW_THREADS) verify_draw_kernel(const 
                 for (int v = 0; v < WAVES; ++v) w += rest_of[c][v];
                 return w;
             }
-            if (q) return rest[c];
-            double w = st[c].largest > -INFINITY ? st[c].sum * weight.any(st[c].largest) : 0.;
+            if (q) return c < 64 ? first_rest : rest[c];
+            double w = c < 64 ? e.parts[c] : st[c].largest > -INFINITY ? st[c].sum * weight.any(st[c].largest) : 0.;
             if (x >= 0 && x / VERIFY_CHUNK == c) w = fmax(w - weight.any(e.draft_logit), 0.);
             return w * share;
         };
