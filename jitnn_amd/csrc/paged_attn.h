@@ -10,9 +10,13 @@
 //   * of the values the lane loads, for the very keys 4 g + i, the D / 16 neighbours from D / 16 n on: all a row of V, so that the loads of
 //     16 lanes are one row in one piece, and the A operand of V^T needs no more than the lane's own registers - its tile e takes the e-th value
 //     of each key, row n of that tile being value D / 16 n + e.
-//   A wave so streams keys and values from memory at its own pace, without a barrier.
+//   A wave so streams keys and values from memory at its own pace, without a barrier (pa_stream): for few rows, which memory bounds.  8 sequences of up to 2000
+//   positions, 32 heads of 128 in FP16: 148 MB in 33.8 us (4.4 TB/s).  Where the rows fill several waves, each wave's own stream of the same keys
+//   is what bounds: there the waves share them through LDS (pa_wide).  64 sequences behind 16384 shared positions, 32 heads over 8: 126 us with streams
+//   alone, 58 so, and the merge 8.6: the matrix cores at 1.04 PFLOP/s over the shared part, two parts of every product counted.
 // FP16 pages: keys and values are operands as they are; queries (scaled so that a row's largest is near 2^13) and weights (times 2^6 to 2^14) go in two FP16
-// parts, 22 bits together, so that the result is as good as in FP32.  FP32 pages: the FP32 matrix instruction.
+// parts, 22 bits together, so that the result is as good as in FP32 (one part of 11 bits would leave 2^-12 of every weight).  FP32 pages: the FP32
+// matrix instruction, an eighth of the rate; 24 sequences of up to 5 rows behind 992 shared positions, 33.8 us and the merge 7.4.
 // Sums, maxima and outputs are FP32.
 //
 // What a row does not see: its scores are masked; values past the last key that any row of the tile sees are cleared, and of those that only some see
@@ -798,7 +802,8 @@ __global__ void __launch_bounds__(PA_THREADS, D <= 128 ? 2 : 1) paged_attn_kerne
     }
 }
 
-// ---- y of every row (token, head) from its spans.  Spans that begin behind the row's position were not written.
+// ---- y of every row (token, head) from its spans, y = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i with m the largest m_i: bound by the latency of a chain (the
+// token's sequence, the statistics, the sums) where rows are few, 4 us, and by memory where they are many.  Spans that begin behind the row's position were not written.
 constexpr int PA_MERGE = 256;
 
 // What token t's rows see: spans of the shared positions and of the sequence's own; false where y is already right or has been made so (`rows` rows of it from y
