@@ -50,76 +50,92 @@ static AttnPart rows_shape(long long rows, int D) {
     return p;
 }
 
-// Spans of a part whose waves share their keys and that is alone: the number for which the workgroups and the merge of what they leave, modelled in
-// microseconds, take least; of nearly equal ones the fewest.  A step of a workgroup is its products at 1100 (FP16) or 140 (FP32) TFLOP/s, on top of which it
-// waits 0.35 us and 3.5 ns a value of the head, two thirds of that where the CU has another one to work on; before the first it takes 5 (2.5).  The
-// merge is a launch, and what is written and read again of each row and span at 4.2 TB/s.  Heads of 128, FP16, 32 of them: 2000 tokens' own positions, one span
-// 91 us, two 119; 512 tokens behind 3584 others, one 158, two 99, four 86, eight 101.
-static int wide_spans(bool half, int D, long long rows_all, const AttnPart &q, long long units, int keys, double len, double seen, int cus) {
-    const int per_cu = D <= 128 ? 2 : 1;
-    const double product = (half ? 0.00167 : 0.0067) * D * q.tiles;
-    int best = 1;
-    double least = 1e30;
-    for (int n = 1; n <= 120 && (n - 1) * keys < len; n = std::max(n + 1, n * 5 / 4)) {
-        const double longest = std::ceil(len / n / keys), mean = std::max(seen / n / keys, 0.5), rounds = std::ceil((double)units * n / cus);
-        const bool two = per_cu == 2 && rounds > 1;
-        const double wait = (0.35 + 0.0035 * D) * (two ? 0.65 : 1.);
-        const double run = std::max(5 + longest * (product + 0.35 + 0.0035 * D), rounds * ((two ? 2.5 : 5.) + mean * (product + wait)));
-        const double time = run + (n > 1 ? 6 + (double)rows_all * std::min(n * seen / len + 0.5, (double)n) * (D + 2) * 8 / 4.2e6 : 0.);
-        if (time < 0.95 * least) {
-            least = time;
-            best = n;
-        }
-    }
-    return best;
+// What a part takes when it is cut into spans of `steps` steps of a wave, in microseconds: its longest workgroup alone on a CU, and a workgroup's share of a CU that has
+// others (as long as that where a CU holds no second one, heads of more than 128 values).  A step is its products at 1100 (FP16) or 140 (FP32) TFLOP/s and what it
+// waits for; 40 GB/s and CU come from memory and the L2s.
+struct PartTime {
+    int span = 0, spans = 0;
+    double alone = 0, busy = 0, load = 0, groups = 0;  // load: of a CU that takes its turn of them all
+};
+// (whole numbers: a call takes as long as its launch, and this is part of it)
+static PartTime part_time(const AttnPart &q, bool half, int D, int keys, int len, double mean, long long units, int n, int cus) {
+    PartTime t;
+    const int least = keys * q.key_waves, all = (len + least - 1) / least, steps = (all + n - 1) / n;
+    t.span = steps * least;
+    t.spans = (all + steps - 1) / steps;
+    const long long groups = units * t.spans * q.blocks;
+    t.groups = (double)groups;
+    const bool wide = q.key_waves == 1;
+    const double product = (half ? 0.00167 : 0.0067) * D * q.tiles, bytes = 2. * least * D * (half ? 2 : 4);
+    t.alone = (wide ? 3.7 : 1.9) + steps * (product + (wide ? 0.2 : 0.) + 0.003 * D);
+    t.busy = (wide ? 4.4 : 2.7) + mean / (t.spans * least) * std::max(product + 0.04, bytes * (1. / 40e3));
+    if (D > 128) t.busy = std::max(t.busy, 0.92 * t.alone);
+    t.load = t.busy * (groups < 3ll * cus ? (double)((groups + cus - 1) / cus) : t.groups / cus + 0.7);
+    return t;
 }
 
+// Spans of the shared positions and of the sequences' own: the numbers for which the modelled time is least.  While there are no more workgroups than CUs, the longest;
+// beyond, a CU has one of each kind after the other as often as it takes (they go round the CUs), and those that do not find a place at once, the sequences', end
+// later.  The merge is 5 us and what is written and read again of each row and span, at 4.6 TB/s.  A batch's lengths are taken to lie evenly up to the longest.  Of 260 batches with head sizes, types, rows and
+// lengths of all kinds, the chosen numbers took 2 % longer than the best of a sweep on average; equal times of the workgroups, with two to a CU, took 12 %.
 AttnPlan paged_attn_plan(bool half, int D, int heads, int kv, int sequences, long long tokens, int max_tokens, int max_len, int shared, int cus) {
     const int group = heads / kv, keys = half ? 32 : 16;
     AttnPlan p;
     if (shared > 0) p.ahead = rows_shape(tokens * group, D);
     p.own = rows_shape((long long)max_tokens * group, D);
-    // Spans of about equal time: for two workgroups to a CU, as many as run at once, where some share their keys (each leaves its rows' sums in memory, so that
-    // more of them cost more than their balance gains: 64 sequences behind 16384 shared positions 70 us with two, 96 with three, 93 with four); for
-    // four where all stream (8 sequences of up to 2000 positions 38.1 us, with two 38.7).
-    auto step = [](const AttnPart &q) { return q.tiles == 2 ? 1.6 : 1.0; };  // of a wave, in units of one tile's
-    const double own_len = std::max(max_len - shared, 1);
-    auto work = [&](const AttnPart &q, double n, double len) { return n * q.blocks * kv * len / q.key_waves * step(q); };
-    const double all = (shared > 0 ? work(p.ahead, 1, shared) : 0) + work(p.own, sequences, own_len), each = all / ((p.own.key_waves == 1 || (shared > 0 && p.ahead.key_waves == 1) ? 2. : 4.) * cus);
-    auto cut = [&](AttnPart &q, double len) {
-        const int least = keys * q.key_waves;  // one step of every wave
-        const double want = std::max(each * q.key_waves / step(q), len / 120);  // (at most 128 spans of each part: PA_MERGE)
-        q.span = (int)std::min<double>(std::ceil(want / least) * least, std::ceil(len / least) * least);
-        q.spans = (int)((len + q.span - 1) / q.span);
-    };
-    // Where a sequence's rows differ much in what they see; where they do not, the fewer units at a time share the more in an XCD's L2 (63 sequences of 40 tokens
-    // behind 360 others 54 us, with these 58).  No more units than there are: the order is dense, and so is their spread over the CUs.
-    auto side_by_side = [&](AttnPart &q) {
-        if (2. * max_tokens < own_len) return;
-        const long long units = ((long long)kv * sequences * q.spans + 7) / 8 * 8;
-        q.beside = (int)std::min<long long>(units, std::max(8, (D <= 128 ? 2 : 1) * cus / q.blocks / 8 * 8));
-    };
-    if (shared == 0 && p.own.key_waves == 1) {
-        const int n = wide_spans(half, D, tokens * heads, p.own, (long long)p.own.blocks * kv * sequences, keys, own_len, std::max(own_len - 0.5 * max_tokens, 1.), cus);
-        p.own.span = (int)std::ceil(own_len / n / keys) * keys;
-        p.own.spans = (int)((own_len + p.own.span - 1) / p.own.span);
-        side_by_side(p.own);
-        return p;
+    const int own_len = std::max(max_len - shared, 1);
+    const double own_mean = std::max(0.5 * own_len * (1 + 1. / sequences) - 0.5 * max_tokens, 1.);
+    static constexpr int NUMBERS[] = {1, 2, 3, 4, 5, 6, 8, 11, 14, 16, 20, 22, 24, 32, 40, 45, 48, 64, 96, 120}, COUNT = sizeof(NUMBERS) / sizeof(int);  // (two below PA_MERGE)
+    PartTime ahead[COUNT], own[COUNT];
+    int aheads = 0, owns = 0;
+    long long before = 0;  // (the first number that leaves every wave one step is the last)
+    for (int n : NUMBERS) {
+        if (before * keys * p.ahead.key_waves < shared) ahead[aheads++] = part_time(p.ahead, half, D, keys, shared, shared, kv, n, cus);
+        if (before * keys * p.own.key_waves < own_len) own[owns++] = part_time(p.own, half, D, keys, own_len, own_mean, (long long)kv * sequences, n, cus);
+        before = n;
     }
-    if (shared > 0) cut(p.ahead, shared);
-    cut(p.own, own_len);
-    side_by_side(p.own);
+    if (aheads == 0) aheads = 1;  // (no workgroups, no time)
+    const int resident = (D <= 128 ? 2 : 1) * cus;
+    const double merge = (double)tokens * heads * (D + 2) * (8 / 4.6e6);
+    double least = 1e30;
+    const PartTime *best_ahead = ahead, *best_own = own;
+    for (int i = 0; i < aheads; ++i)
+        for (int j = 0; j < owns; ++j) {
+            const PartTime &a = ahead[i], &o = own[j];
+            const double load = a.groups + o.groups <= cus ? std::max(a.busy, o.busy) : a.load + o.load;
+            const int spans = a.spans + o.spans;
+            const double time = std::max(std::max(a.alone, o.alone), load) + (a.groups + o.groups > resident ? 0.43 * o.alone : 0.) + (spans > 1 ? 4.9 + merge * spans : 0.);
+            if (time < least) {
+                least = time;
+                best_ahead = &a;
+                best_own = &o;
+            }
+        }
+    p.ahead.span = best_ahead->span;
+    p.ahead.spans = best_ahead->spans;
+    p.own.span = best_own->span;
+    p.own.spans = best_own->spans;
+    // How many units are taken together (paged_attn_kernel).  Eight, a unit to an XCD, so that its row blocks share the keys in that XCD's L2 (63 sequences of 40 tokens
+    // behind 360 others 54 us, with as many units as run at once 58); these where a sequence's rows differ much in what they see.  Units that are no multiple
+    // of eight and all run at once go all together: rounded up they would leave XCDs idle (one prompt of 204 tokens on one key/value head ran on one).
+    auto order = [&](AttnPart &q, long long of, bool prompts) {
+        const long long units = of * kv * q.spans, whole = units % 8 != 0 && units * q.blocks <= resident ? units : (units + 7) / 8 * 8;
+        q.beside = (int)std::min<long long>(whole, prompts ? std::max(8, resident / q.blocks / 8 * 8) : whole % 8 != 0 ? whole : 8);
+    };
+    if (shared > 0) order(p.ahead, 1, false);
+    order(p.own, sequences, 2ll * max_tokens >= own_len);
     return p;
 }
 
 void paged_attn_launch(bool half, int D, int cus, hipStream_t s, AttnArgs a) {
     const unsigned units_ahead = (unsigned)(a.ahead.spans * a.kv), units_own = (unsigned)(a.own.spans * a.kv * a.sequences);
     const unsigned ahead = (units_ahead + a.ahead.beside - 1) / a.ahead.beside * a.ahead.beside * (unsigned)a.ahead.blocks, own = (units_own + a.own.beside - 1) / a.own.beside * a.own.beside * (unsigned)a.own.blocks;
-    a.chunk = std::max(8, cus / 8 * 8);  // one to a CU
+    // one to a CU, and where there are no more than CUs in all, the own behind the shared ones without a gap
+    a.chunk = ahead > 0 && ahead + own <= (unsigned)cus ? (int)ahead : std::max(8, cus / 8 * 8);
     a.chunks_ahead = (int)((ahead + a.chunk - 1) / a.chunk);
     a.chunks_own = (int)((own + a.chunk - 1) / a.chunk);
     a.pairs = std::min(a.chunks_ahead, a.chunks_own);
-    const unsigned blocks = (unsigned)(a.chunks_ahead + a.chunks_own) * (unsigned)a.chunk;
+    const unsigned blocks = a.chunk == (int)ahead ? ahead + own : (unsigned)(a.chunks_ahead + a.chunks_own) * (unsigned)a.chunk;
     if (half) paged_attn_launch_f16(D, blocks, s, a);
     else paged_attn_launch_f32(D, blocks, s, a);
     if (a.ahead.spans + a.own.spans == 1) return;
