@@ -238,6 +238,8 @@ PROMPTS = [
     (256, 12, 3, 128, [60, 70, 41], [60, 77, 300], 0),
     (192, 4, 2, 16, [129], [700], 0),
     (64, 16, 2, 64, [65, 140], [400, 350], 3),
+    (64, 5, 1, 16, [90], [90], 0),                                           # fewer units of work than XCDs
+    (128, 8, 1, 32, [40, 24, 11], [120, 500, 90], 2),
 ]
 
 
@@ -415,7 +417,7 @@ def test_recorded_pass_follows_its_arrays(jn):
 
 def test_serving_refusals_of_sizes(jn):
     from jitnn_amd import _lib
-    b = ref.Batch(np.random.default_rng(0), [1], [300], 16)
+    b = ref.Batch(np.random.default_rng(0), [1], [6000], 16)
     cache = jn.PagedCache(1, 2, 64, b.pages, 16, 1)
     nb, keep = batch_of(jn, b)
     x = torch.zeros(4096, device="cuda")
