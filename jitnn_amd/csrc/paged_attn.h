@@ -2,7 +2,7 @@
 // in pages that a table names.  The leading pages may be everybody's: the workgroups that take their positions take the rows - (token, query
 // head) pairs of one key/value head - of the whole batch, so that they are read once and not once per sequence; the other positions go
 // to workgroups of their sequence.  Every workgroup leaves, for its span of keys, the largest score, the sum of the weights and the weighted sum
-// of the values, and paged_merge_kernel joins a row's spans.
+// of the values, and paged_merge_kernel joins a row's spans; where there is one span in all, its workgroups write the outputs.
 //
 // The products run on the matrix cores, transposed, S^T = K Q^T and O^T = V^T P^T, and nothing but the last sums goes through LDS:
 //   * lane n + 16 g holds for the scores key n of a tile of 16 (16 bytes of its row per load), receives the scores of ROW n against the keys
@@ -11,12 +11,12 @@
 //     16 lanes are one row in one piece, and the A operand of V^T needs no more than the lane's own registers - its tile e takes the e-th value
 //     of each key, row n of that tile being value D / 16 n + e.
 //   A wave so streams keys and values from memory at its own pace, without a barrier (pa_stream): for few rows, which memory bounds.  8 sequences of up to 2000
-//   positions, 32 heads of 128 in FP16: 148 MB in 33.8 us (4.4 TB/s).  Where the rows fill several waves, each wave's own stream of the same keys
+//   positions, 32 heads of 128 in FP16: 148 MB in 34.6 us, one launch (4.3 TB/s).  Where the rows fill several waves, each wave's own stream of the same keys
 //   is what bounds: there the waves share them through LDS (pa_wide).  64 sequences behind 16384 shared positions, 32 heads over 8: 126 us with streams
-//   alone, 58 so, and the merge 8.6: the matrix cores at 1.04 PFLOP/s over the shared part, two parts of every product counted.
+//   alone, 59 so, and the merge 7: the matrix cores at 1.04 PFLOP/s over the shared part, two parts of every product counted.
 // FP16 pages: keys and values are operands as they are; queries (scaled so that a row's largest is near 2^13) and weights (times 2^6 to 2^14) go in two FP16
 // parts, 22 bits together, so that the result is as good as in FP32 (one part of 11 bits would leave 2^-12 of every weight).  FP32 pages: the FP32
-// matrix instruction, an eighth of the rate; 24 sequences of up to 5 rows behind 992 shared positions, 33.8 us and the merge 7.4.
+// matrix instruction, an eighth of the rate; 24 sequences of up to 5 rows behind 992 shared positions, 35 us and the merge 7.5.
 // Sums, maxima and outputs are FP32.
 //
 // What a row does not see: its scores are masked; values past the last key that any row of the tile sees are cleared, and of those that only some see

@@ -142,8 +142,8 @@ void paged_attn_launch(bool half, int D, int cus, hipStream_t s, AttnArgs a) {
     if (a.ahead.spans + a.own.spans == 1) return;
     auto merge = [&](auto d) {
         constexpr int DD = decltype(d)::value, ROWS = PA_MERGE / (DD / 4);
-        // (few spans and rows for every CU: 512 tokens of one sequence behind 4096, 16384 rows of 5 spans, 85 us against 95 with a workgroup to each row; of 8
-        // sequences' 256 rows, 8 spans, 38.6 against 37.8)
+        // (few spans and rows for every CU: 512 tokens of one sequence behind 3584, 16384 rows of 4 spans, 85 us against 95 with a workgroup to each row; 256 rows of 8
+        // spans are 0.8 us slower with it)
         if (a.ahead.spans + a.own.spans <= PA_FEW && (long long)a.tokens * a.heads >= (long long)ROWS * cus) hipLaunchKernelGGL(paged_merge_few_kernel<DD>, dim3(a.tokens, (a.heads + ROWS - 1) / ROWS), dim3(PA_MERGE), 0, s, a);
         else hipLaunchKernelGGL(paged_merge_kernel<DD>, dim3((unsigned)((long long)a.tokens * a.heads)), dim3(PA_MERGE), 0, s, a);
     };
