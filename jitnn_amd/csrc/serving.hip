@@ -86,7 +86,9 @@ AttnPlan paged_attn_plan(bool half, int D, int heads, int kv, int sequences, lon
     p.own = rows_shape((long long)max_tokens * group, D);
     const int own_len = std::max(max_len - shared, 1);
     const double own_mean = std::max(0.5 * own_len * (1 + 1. / sequences) - 0.5 * max_tokens, 1.);
-    static constexpr int NUMBERS[] = {1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12, 14, 16, 18, 20, 22, 24, 28, 32, 36, 40, 45, 50, 56, 64, 80, 96, 120}, COUNT = sizeof(NUMBERS) / sizeof(int);  // (two below PA_MERGE)
+    // (the largest two together below PA_MERGE)
+    static constexpr int NUMBERS[] = {1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12, 14, 16, 18, 20, 22, 24, 28, 32, 36, 40, 45, 50, 56, 64, 80, 96, 120};
+    constexpr int COUNT = sizeof(NUMBERS) / sizeof(int);
     PartTime ahead[COUNT], own[COUNT];
     int aheads = 0, owns = 0;
     long long before = 0;  // (the first number that leaves every wave one step is the last)
@@ -130,7 +132,8 @@ AttnPlan paged_attn_plan(bool half, int D, int heads, int kv, int sequences, lon
 
 void paged_attn_launch(bool half, int D, int cus, hipStream_t s, AttnArgs a) {
     const unsigned units_ahead = (unsigned)(a.ahead.spans * a.kv), units_own = (unsigned)(a.own.spans * a.kv * a.sequences);
-    const unsigned ahead = (units_ahead + a.ahead.beside - 1) / a.ahead.beside * a.ahead.beside * (unsigned)a.ahead.blocks, own = (units_own + a.own.beside - 1) / a.own.beside * a.own.beside * (unsigned)a.own.blocks;
+    auto groups = [](unsigned units, const AttnPart &q) { return (units + q.beside - 1) / q.beside * q.beside * (unsigned)q.blocks; };
+    const unsigned ahead = groups(units_ahead, a.ahead), own = groups(units_own, a.own);
     // one to a CU, and where there are no more than CUs in all, the own behind the shared ones without a gap
     a.chunk = ahead > 0 && ahead + own <= (unsigned)cus ? (int)ahead : std::max(8, cus / 8 * 8);
     a.chunks_ahead = (int)((ahead + a.chunk - 1) / a.chunk);
@@ -144,8 +147,10 @@ void paged_attn_launch(bool half, int D, int cus, hipStream_t s, AttnArgs a) {
         constexpr int DD = decltype(d)::value, ROWS = PA_MERGE / (DD / 4);
         // (few spans and rows for every CU: 512 tokens of one sequence behind 3584, 16384 rows of 4 spans, 85 us against 95 with a workgroup to each row; 256 rows of 8
         // spans are 0.8 us slower with it)
-        if (a.ahead.spans + a.own.spans <= PA_FEW && (long long)a.tokens * a.heads >= (long long)ROWS * cus) hipLaunchKernelGGL(paged_merge_few_kernel<DD>, dim3(a.tokens, (a.heads + ROWS - 1) / ROWS), dim3(PA_MERGE), 0, s, a);
-        else hipLaunchKernelGGL(paged_merge_kernel<DD>, dim3((unsigned)((long long)a.tokens * a.heads)), dim3(PA_MERGE), 0, s, a);
+        if (a.ahead.spans + a.own.spans <= PA_FEW && (long long)a.tokens * a.heads >= (long long)ROWS * cus)
+            hipLaunchKernelGGL(paged_merge_few_kernel<DD>, dim3(a.tokens, (a.heads + ROWS - 1) / ROWS), dim3(PA_MERGE), 0, s, a);
+        else
+            hipLaunchKernelGGL(paged_merge_kernel<DD>, dim3((unsigned)((long long)a.tokens * a.heads)), dim3(PA_MERGE), 0, s, a);
     };
     switch (D) {
     case 64: merge(std::integral_constant<int, 64>{}); break;
