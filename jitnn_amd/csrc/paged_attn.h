@@ -84,8 +84,8 @@ __device__ __forceinline__ RowPlace row_place(const int *__restrict__ starts, co
         const int below = __popcll(__ballot(i0 + lane < sequences && end <= t));
         p.sequence += below;
         if (below < 64) {
-            p.len = __shfl(len, below);
-            p.end = __shfl(end, below);
+            p.len = __builtin_amdgcn_readlane(len, below);
+            p.end = __builtin_amdgcn_readlane(end, below);
             break;
         }
     }

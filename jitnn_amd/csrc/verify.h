@@ -64,17 +64,31 @@ struct VerifyWeight {
     // the same where the largest may be infinite: equal infinities share all the weight
     __device__ __forceinline__ double any(float l) const { return fabsf(largest) < INFINITY ? (*this)(l) : l == largest ? 1. : 0.; }
 };
-__device__ __forceinline__ double verify_wave_sum(double v) {
-    for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off);
-    return v;
+// Across a wave without the trip through LDS that a shuffle takes (half a dozen of them in a row were 1.5 us of the draw's 7): within rows of 16 lanes from the lanes
+// 1, 2, 4 and 8 before, then the last lane of a row to the next row, then that of the first half to the second.  What no lane sends is `none`.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int verify_from(int v, int none) {
+    return __builtin_amdgcn_update_dpp(none, v, CTRL, ROWS, 0xf, false);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double verify_from(double v) {
+    return __hiloint2double(verify_from<CTRL, ROWS>(__double2hiint(v), 0), verify_from<CTRL, ROWS>(__double2loint(v), 0));
+}
+__device__ __forceinline__ double verify_lane(double v, int lane) {  // the same lane for all
+    return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(v), lane), __builtin_amdgcn_readlane(__double2loint(v), lane));
 }
 __device__ __forceinline__ double verify_wave_scan(double v) {  // the sum up to this lane
-    const int lane = threadIdx.x & 63;
-    for (int off = 1; off < 64; off <<= 1) {
-        const double o = __shfl_up(v, off);
-        if (lane >= off) v += o;
-    }
+    v += verify_from<0x111, 0xf>(v);
+    v += verify_from<0x112, 0xf>(v);
+    v += verify_from<0x114, 0xf>(v);
+    v += verify_from<0x118, 0xf>(v);
+    v += verify_from<0x142, 0xa>(v);
+    v += verify_from<0x143, 0xc>(v);
     return v;
+}
+__device__ __forceinline__ double verify_wave_sum(double v) {
+    v = verify_wave_scan(v);
+    return verify_lane(v, 63);
 }
 __device__ __forceinline__ void verify_take(float v, int i, float &best, int &index) {
     if (v > best || (v == best && i < index)) {
@@ -82,12 +96,20 @@ __device__ __forceinline__ void verify_take(float v, int i, float &best, int &in
         index = i;
     }
 }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ void verify_best_from(float &best, int &index) {
+    const float v = __int_as_float(verify_from<CTRL, ROWS>(__float_as_int(best), __float_as_int(-INFINITY)));
+    verify_take(v, verify_from<CTRL, ROWS>(index, 0x7fffffff), best, index);
+}
 __device__ __forceinline__ void verify_wave_best(float &best, int &index) {
-    for (int off = 32; off > 0; off >>= 1) {
-        const float v = __shfl_xor(best, off);
-        const int i = __shfl_xor(index, off);
-        verify_take(v, i, best, index);
-    }
+    verify_best_from<0x111, 0xf>(best, index);
+    verify_best_from<0x112, 0xf>(best, index);
+    verify_best_from<0x114, 0xf>(best, index);
+    verify_best_from<0x118, 0xf>(best, index);
+    verify_best_from<0x142, 0xa>(best, index);
+    verify_best_from<0x143, 0xc>(best, index);
+    best = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(best), 63));
+    index = __builtin_amdgcn_readlane(index, 63);
 }
 // VERIFY_VALUES values of a chunk per thread, four neighbours at a time; behind the row's end -inf
 __device__ __forceinline__ void verify_load(const float *__restrict__ row, int c0, int vocab, float (&v)[VERIFY_VALUES]) {
@@ -362,11 +384,11 @@ __global__ void __launch_bounds__(VERIFY_DRAW_THREADS) verify_draw_kernel(const 
             if (past) {
                 const int at = __ffsll((long long)past) - 1;
                 chunk = c0 + at;
-                before_chunk = before + (__shfl(upto, at) - __shfl(w, at));
+                before_chunk = before + (verify_lane(upto, at) - verify_lane(w, at));
             } else if (some) {
                 last = c0 + 63 - __clzll((long long)some);
             }
-            before += __shfl(upto, 63);
+            before += verify_lane(upto, 63);
         }
         if (lane == 0) {
             chosen_chunk = chunk >= 0 ? chunk : last;
@@ -393,19 +415,17 @@ __global__ void __launch_bounds__(VERIFY_DRAW_THREADS) verify_draw_kernel(const 
         if (w[u] > 0.) last = i0 + u;
     }
     const unsigned long long hit = __ballot(mine >= 0), any = __ballot(last >= 0);
-    const int hit_at = hit ? __shfl(mine, __ffsll((long long)hit) - 1) : -1, any_at = any ? __shfl(last, 63 - __clzll((long long)any)) : -1;
+    const int hit_at = hit ? __builtin_amdgcn_readlane(mine, __ffsll((long long)hit) - 1) : -1, any_at = any ? __builtin_amdgcn_readlane(last, 63 - __clzll((long long)any)) : -1;
     if (lane == 0) {
         first_at[wave] = hit_at;
         last_at[wave] = any_at;
     }
     __syncthreads();
-    if (tid == 0) {
-        int found = -1, end_at = -1;
-        for (int v = 0; v < WAVES; ++v) {
-            if (found < 0 && first_at[v] >= 0) found = first_at[v];
-            if (last_at[v] >= 0) end_at = last_at[v];
-        }
-        a.out[e.row] = found >= 0 ? found : end_at >= 0 ? end_at : e.stat.index;
+    if (wave == 0) {
+        const int f = lane < WAVES ? first_at[lane] : -1, l = lane < WAVES ? last_at[lane] : -1;
+        const unsigned long long found = __ballot(f >= 0), some = __ballot(l >= 0);
+        const int at = found ? __builtin_amdgcn_readlane(f, __ffsll((long long)found) - 1) : some ? __builtin_amdgcn_readlane(l, 63 - __clzll((long long)some)) : e.stat.index;
+        if (lane == 0) a.out[e.row] = at;
     }
 }
 
