@@ -7,9 +7,9 @@
 //   verify_stats_kernel   chunks of a row: largest logit (lowest index among equals), sum of exp((l - largest) / T)
 //   verify_rest_kernel    (with draft probabilities, more than VERIFY_FEW chunks) the refused row's sum of max(p - q, 0) per chunk
 //   verify_draw_kernel    one workgroup per sequence: which tokens are kept, the chunk the draw falls in, the index in it
-// Measured, us per kernel: 16 x 9 ragged rows of 128256, a draft with certainty, stats 16.7 and draw 7.9; 32 x 5 rows with draft probabilities, stats 25.6, rest 11.3, draw
-// 7.7; 5 rows of 32000, 5.2 and 7.2.  The stats read 82 MB in 18.3 us where the temperature is 0 (4.5 TB/s); the FP64 weights of 20 million logits
-// are the other 7.  The rest and the draw are chains of dependent reads - starts, drafts and chunks' sums, the draft's logit, the chunk - of about 1 us each.
+// Measured, us per kernel: 16 x 9 ragged rows of 128256, a draft with certainty, stats 16.0 and draw 6.6; 32 x 5 rows with draft probabilities, stats 24.2, rest 10.0, draw
+// 6.3; 5 rows of 32000, 4.9 and 5.7.  The stats read 82 MB in 18.3 us where the temperature is 0 (4.5 TB/s); the FP64 weights of 20 million logits
+// are the other 6.  The rest and the draw are chains of dependent reads - starts, drafts and chunks' sums, the draft's logit, the chunk - of about 1 us each.
 // All rows are judged whether or not an earlier one is refused: they are read once, side by side.
 #pragma once
 #include "common.h"
@@ -296,7 +296,7 @@ __global__ void __launch_bounds__(VERIFY_THREADS) verify_rest_kernel(const Verif
 }
 
 // grid (sequences).  Of few chunks it sums what the refused draft left by itself, 1 us each: all three kernels over 4 x 5 rows took 23 us at four
-// chunks, 17 us so; at five 21 us.
+// chunks, 15 us so; at five 18 us.
 constexpr int VERIFY_FEW = 4;
 constexpr int VERIFY_DRAW_THREADS = VERIFY_CHUNK / 4;  // four neighbours each, in one load (eight in eight by half as many threads took 3 us longer)
 // what the draw of a row leaves to each of four neighbours: p, without a draft's q or the draft x
