@@ -71,6 +71,21 @@ __device__ __forceinline__ float pa_sum4(float v) {
 __device__ __forceinline__ bool pa_finite(_Float16 x) { return (__builtin_bit_cast(unsigned short, x) & 0x7c00) != 0x7c00; }
 __device__ __forceinline__ bool pa_finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 
+// n / by and what is left of it, m = reciprocal(by): less than one below 2^32 / by, so that the product is at most one too small.
+__device__ __forceinline__ unsigned pa_div(unsigned n, unsigned by, unsigned m, unsigned &rest) {
+    unsigned d = __umulhi(n, m);
+    rest = n - d * by;
+    if (rest >= by) {
+        ++d;
+        rest -= by;
+    }
+    return d;
+}
+__device__ __forceinline__ int pa_div(int n, int by, unsigned m) {  // n >= 0
+    unsigned rest;
+    return (int)pa_div((unsigned)n, (unsigned)by, m, rest);
+}
+
 // The sequence of token t, its length and the token behind its last; one wave (or every wave) with the same t.  Lengths come with the starts, in one
 // round trip for each 64 sequences.
 struct RowPlace {
@@ -117,8 +132,8 @@ struct PaRows {
     // In steps, so that what they wait for is asked for together: begin (false: the workgroup has nothing to do), fetch (queries), find (the rows'
     // positions), take (the queries as operands).
     __device__ __forceinline__ bool begin(const AttnArgs &a, const bool ahead, const int seq, const int row0_of_wave, const int row0_of_block, const int key0) {
-        group = a.heads / a.kv;
-        per_group = 1.f / (float)group;
+        group = a.group;
+        per_group = a.per_group;
         // (the first 64 sequences' ends and lengths, a lane each, for find)
         base = 0;
         if (ahead) sequences_at(a);
@@ -143,7 +158,7 @@ struct PaRows {
     // queries: 8 g + j of each 32 values (FP16), 4 g + j of each 16 (FP32) of row n
     __device__ __forceinline__ void fetch(const AttnArgs &a, const int kvh) {
         const int n = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
-        token0 = __builtin_amdgcn_readfirstlane(row0 / group);
+        token0 = __builtin_amdgcn_readfirstlane(pa_div(row0, group, a.by_group));
         rem0 = row0 - token0 * group;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
@@ -168,7 +183,7 @@ struct PaRows {
         }
         const int count = min(16 * R, rows - row0);  // of the wave's rows
         if (count <= 0) return;
-        const int end_token = token0 + (rem0 + count - 1) / group;
+        const int end_token = place(count - 1).x;
         if (!ahead) {
             const int len = a.lens[seq], behind = len - a.starts[seq + 1] + t0;
             const bool long_one = len > a.max_len;
@@ -437,8 +452,8 @@ __device__ __forceinline__ void pa_stream(const AttnArgs &a, const AttnPart &par
     using Tile = PaTile<T, D>;
     constexpr int KEYS = Tile::KEYS, TILES = Tile::TILES, E = Tile::E, ROW = D * (int)sizeof(T);
     const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int key_waves = part.key_waves, row_waves = PA_WAVES / key_waves;
-    const int wr = wave & (row_waves - 1), wk = wave / row_waves;
+    const int key_waves = part.key_waves, row_waves = key_waves == PA_WAVES ? 1 : 2;  // (4 or 2 of the four)
+    const int wr = wave & (row_waves - 1), wk = row_waves == 1 ? wave : wave >> 1;
     const int *table = a.tables + (size_t)(ahead ? 0 : seq) * a.table_stride;
     PaRows<T, D, R> w;
     PaPages<TILES, KEYS, ROW> pages;
@@ -543,7 +558,7 @@ __device__ __forceinline__ void pa_stream(const AttnArgs &a, const AttnPart &par
         }
     }
     __syncthreads();
-    const int first_row = block * row_waves * 16 * R, token_of_first = first_row / w.group, rem_of_first = first_row - token_of_first * w.group;
+    const int first_row = block * row_waves * 16 * R, token_of_first = pa_div(first_row, a.group, a.by_group), rem_of_first = first_row - token_of_first * w.group;
     for (int at = tid; at < row_waves * 16 * R * (D / 4); at += PA_THREADS) {
         const int rr = at / (D / 4), e = 4 * (at - rr * (D / 4)), wv = rr / (16 * R), in = rr - wv * 16 * R;  // wave wv + row_waves j holds row `in` of the keys' share j
         if (first_row + rr >= w.rows) break;  // (rr grows with at)
@@ -608,8 +623,8 @@ __device__ __forceinline__ void pa_wide(const AttnArgs &a, const bool ahead, con
     // keys key0 .. kend - 1: what any row of the workgroup may see, and some of the shared ones perhaps that none does
     int kend = key1;
     if (!ahead) {
-        const int len = a.lens[seq], last_token = min((block + 1) * PA_WAVES * 16 * R, w.rows) / w.group;  // ... or the one behind it
-        kend = min(key1, len - (a.starts[seq + 1] - w.t0) + min(last_token + 1, w.rows / w.group));
+        const int len = a.lens[seq], last_token = pa_div(min((block + 1) * PA_WAVES * 16 * R, w.rows), a.group, a.by_group);  // ... or the one behind it
+        kend = min(key1, len - (a.starts[seq + 1] - w.t0) + min(last_token + 1, pa_div(w.rows, a.group, a.by_group)));
         if (slots > 1 && kend <= key0) return;  // (a span that begins behind a row's position is not read)
     }
     const int steps = kend > key0 ? (kend - key0 + KEYS - 1) / KEYS : 0;
@@ -768,7 +783,7 @@ __device__ __forceinline__ void pa_attend(const AttnArgs &a, const AttnPart &par
     }
     if constexpr (R == 2) {
         // (of a ragged batch: a sequence whose rows fill one tile takes no product for the other)
-        if (!ahead && part.key_waves == PA_WAVES && (a.starts[seq + 1] - a.starts[seq]) * (a.heads / a.kv) <= 16) {
+        if (!ahead && part.key_waves == PA_WAVES && (a.starts[seq + 1] - a.starts[seq]) * a.group <= 16) {
             pa_stream<T, D, 1>(a, part, ahead, seq, block, kvh, key0, key1, slot, slots, lds);
             return;
         }
@@ -784,21 +799,26 @@ __device__ __forceinline__ void pa_attend(const AttnArgs &a, const AttnPart &par
 template <class T, int D, int RA, int RO>
 __global__ void __launch_bounds__(PA_THREADS, D <= 128 ? 2 : 1) paged_attn_kernel(const AttnArgs a) {
     extern __shared__ __align__(16) float pa_lds[];
-    const unsigned kv = (unsigned)a.kv, seqs = (unsigned)a.sequences, chunk = (unsigned)a.chunk, c = blockIdx.x / chunk, in = blockIdx.x - c * chunk;
+    const unsigned kv = (unsigned)a.kv, seqs = (unsigned)a.sequences, chunk = (unsigned)a.chunk;
+    unsigned in, of, side, kvh;
+    const unsigned c = pa_div(blockIdx.x, chunk, a.by_chunk, in);
     const bool own = c < 2 * (unsigned)a.pairs ? (c & 1) != 0 : a.chunks_own > a.chunks_ahead;
     const unsigned b = (c < 2 * (unsigned)a.pairs ? c / 2 : c - (unsigned)a.pairs) * chunk + in;
     const int slots = a.ahead.spans + a.own.spans;
     if (!own) {
-        const unsigned beside = (unsigned)a.ahead.beside, per = beside * (unsigned)a.ahead.blocks, u = b / per * beside + b % beside;
+        const unsigned beside = (unsigned)a.ahead.beside, first = pa_div(b, beside * (unsigned)a.ahead.blocks, a.by_ahead, of) * beside;
+        const unsigned block = pa_div(of, beside, a.by_ahead_beside, side), u = first + side;
         if (u >= kv * (unsigned)a.ahead.spans) return;
-        const int span = (int)(u / kv), kvh = (int)(u % kv);
-        pa_attend<T, D, RA>(a, a.ahead, true, 0, (int)(b % per / beside), kvh, span * a.ahead.span, min((span + 1) * a.ahead.span, a.shared), span, slots, pa_lds);
+        const int span = (int)pa_div(u, kv, a.by_kv, kvh);
+        pa_attend<T, D, RA>(a, a.ahead, true, 0, (int)block, (int)kvh, span * a.ahead.span, min((span + 1) * a.ahead.span, a.shared), span, slots, pa_lds);
     } else {
-        const unsigned beside = (unsigned)a.own.beside, per = beside * (unsigned)a.own.blocks, u = b / per * beside + b % beside;
+        const unsigned beside = (unsigned)a.own.beside, first = pa_div(b, beside * (unsigned)a.own.blocks, a.by_own, of) * beside;
+        const unsigned block = pa_div(of, beside, a.by_own_beside, side), u = first + side;
         if (u >= kv * seqs * (unsigned)a.own.spans) return;
-        const int kvh = (int)(u % kv), seq = (int)(u / kv % seqs), span = (int)(u / kv / seqs);
+        unsigned seq;
+        const int span = (int)pa_div(pa_div(u, kv, a.by_kv, kvh), seqs, a.by_sequences, seq);
         const int key0 = a.shared + span * a.own.span;
-        pa_attend<T, D, RO>(a, a.own, false, seq, a.own.blocks - 1 - (int)(b % per / beside), kvh, key0, min(key0 + a.own.span, a.max_len), a.ahead.spans + span, slots, pa_lds);
+        pa_attend<T, D, RO>(a, a.own, false, (int)seq, a.own.blocks - 1 - (int)block, (int)kvh, key0, min(key0 + a.own.span, a.max_len), a.ahead.spans + span, slots, pa_lds);
     }
 }
 
@@ -821,8 +841,8 @@ __device__ __forceinline__ bool merge_row(const AttnArgs &a, const int t, const 
         if (writes) *y = f32x4v{f, f, f, f};
         return false;
     }
-    m.ahead = min(a.ahead.spans, a.shared > 0 ? lim / a.ahead.span + 1 : 0);
-    m.count = m.ahead + (lim >= a.shared ? (lim - a.shared) / a.own.span + 1 : 0);
+    m.ahead = min(a.ahead.spans, a.shared > 0 ? pa_div(lim, a.ahead.span, a.by_ahead_span) + 1 : 0);
+    m.count = m.ahead + (lim >= a.shared ? pa_div(lim - a.shared, a.own.span, a.by_own_span) + 1 : 0);
     return true;
 }
 
@@ -836,7 +856,7 @@ __global__ void __launch_bounds__(PA_MERGE) paged_merge_few_kernel(const AttnArg
     f32x4v_a4 *y = reinterpret_cast<f32x4v_a4 *>(a.y + (size_t)t * a.y_stride + (size_t)h * D) + in;
     MergeRow m;
     if (!merge_row<D>(a, t, mine, y, m) || !mine) return;
-    const int group = a.heads / a.kv, kvh = h / group;
+    const int group = a.group, kvh = pa_div(h, group, a.by_group);
     const size_t first_slot = (((size_t)kvh * a.tokens + t) * group + h - kvh * group) * (a.ahead.spans + a.own.spans);
     f32x4v x[PA_FEW];
     float2 st[PA_FEW];
@@ -869,13 +889,12 @@ __global__ void __launch_bounds__(PA_MERGE) paged_merge_kernel(const AttnArgs a)
     __shared__ float weight[PA_MERGE], top_of[PA_MERGE / 64], sum_of[PA_MERGE / 64];
     __shared__ f32x4v part_of[GROUPS][LANES];
     const int tid = threadIdx.x, wave = tid >> 6, grp = tid / LANES, in = tid - grp * LANES;
-    const long long row = blockIdx.x;
-    const int t = (int)(row / a.heads), h = (int)(row - (long long)t * a.heads), slots = a.ahead.spans + a.own.spans;
+    const int t = blockIdx.x, h = blockIdx.y, slots = a.ahead.spans + a.own.spans;
     f32x4v_a4 *y = reinterpret_cast<f32x4v_a4 *>(a.y + (size_t)t * a.y_stride + (size_t)h * D);
     MergeRow m;
     if (!merge_row<D>(a, t, grp == 0, y + in, m)) return;
     const int first_own = a.ahead.spans, ahead = m.ahead, count = m.count;  // at most PA_MERGE (paged_attn_plan)
-    const int group = a.heads / a.kv, kvh = h / group;
+    const int group = a.group, kvh = pa_div(h, group, a.by_group);
     const size_t first_slot = (((size_t)kvh * a.tokens + t) * group + h - kvh * group) * slots;
     auto slot_of = [&](int i) { return first_slot + (i < ahead ? i : first_own + i - ahead); };
     f32x4v acc = {0.f, 0.f, 0.f, 0.f}, x[U];

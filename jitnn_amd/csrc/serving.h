@@ -48,6 +48,8 @@ struct AttnPart {
     int spans = 0;      // results per row that this part leaves
     int beside = 8;     // units (span, sequence, key/value head) whose row blocks alternate in the order of the workgroups; a multiple of 8
 };
+// For division by a number that the host knows.  A kernel's own division takes some 150 cycles, and a workgroup has nine before its first load.
+inline unsigned reciprocal(unsigned by) { return 0xffffffffu / by; }
 struct AttnArgs {
     const void *k, *v;  // of the layer: [pages, kv, page, D]
     const float *q;
@@ -56,10 +58,12 @@ struct AttnArgs {
     const int *tables, *starts, *lens;
     long long q_stride, y_stride;
     float scale;         // with log2 e
-    int tokens, sequences, heads, kv, pages, page_shift, table_stride, max_len;
+    int tokens, sequences, heads, kv, group, pages, page_shift, table_stride, max_len;
     int shared;          // positions
     AttnPart ahead, own;
     int chunk, chunks_ahead, chunks_own, pairs;  // the order of the workgroups: see paged_attn_kernel
+    float per_group;
+    unsigned by_group, by_kv, by_sequences, by_chunk, by_ahead, by_ahead_beside, by_own, by_own_beside, by_ahead_span, by_own_span;  // reciprocals
 };
 struct AttnPlan {
     AttnPart ahead, own;

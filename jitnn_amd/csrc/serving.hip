@@ -139,6 +139,20 @@ void paged_attn_launch(bool half, int D, int cus, hipStream_t s, AttnArgs a) {
     a.chunks_ahead = (int)((ahead + a.chunk - 1) / a.chunk);
     a.chunks_own = (int)((own + a.chunk - 1) / a.chunk);
     a.pairs = std::min(a.chunks_ahead, a.chunks_own);
+    a.group = a.heads / a.kv;
+    a.per_group = 1.f / (float)a.group;
+    a.by_group = reciprocal(a.group);
+    a.by_kv = reciprocal(a.kv);
+    a.by_sequences = reciprocal(a.sequences);
+    a.by_chunk = reciprocal(a.chunk);
+    a.by_own_beside = reciprocal(a.own.beside);
+    a.by_own = reciprocal(a.own.beside * a.own.blocks);
+    a.by_own_span = reciprocal(a.own.span);
+    if (ahead > 0) {
+        a.by_ahead_beside = reciprocal(a.ahead.beside);
+        a.by_ahead = reciprocal(a.ahead.beside * a.ahead.blocks);
+        a.by_ahead_span = reciprocal(a.ahead.span);
+    }
     const unsigned blocks = a.chunk == (int)ahead ? ahead + own : (unsigned)(a.chunks_ahead + a.chunks_own) * (unsigned)a.chunk;
     if (half) paged_attn_launch_f16(D, blocks, s, a);
     else paged_attn_launch_f32(D, blocks, s, a);
@@ -150,7 +164,7 @@ void paged_attn_launch(bool half, int D, int cus, hipStream_t s, AttnArgs a) {
         if (a.ahead.spans + a.own.spans <= PA_FEW && (long long)a.tokens * a.heads >= (long long)ROWS * cus)
             hipLaunchKernelGGL(paged_merge_few_kernel<DD>, dim3(a.tokens, (a.heads + ROWS - 1) / ROWS), dim3(PA_MERGE), 0, s, a);
         else
-            hipLaunchKernelGGL(paged_merge_kernel<DD>, dim3((unsigned)((long long)a.tokens * a.heads)), dim3(PA_MERGE), 0, s, a);
+            hipLaunchKernelGGL(paged_merge_kernel<DD>, dim3(a.tokens, a.heads), dim3(PA_MERGE), 0, s, a);
     };
     switch (D) {
     case 64: merge(std::integral_constant<int, 64>{}); break;
