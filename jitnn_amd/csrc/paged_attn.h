@@ -16,7 +16,7 @@
 //   alone, 59 so, and the merge 7: the matrix cores at 1.04 PFLOP/s over the shared part, two parts of every product counted.
 // FP16 pages: keys and values are operands as they are; queries (scaled so that a row's largest is near 2^13) and weights (times 2^6 to 2^14) go in two FP16
 // parts, 22 bits together, so that the result is as good as in FP32 (one part of 11 bits would leave 2^-12 of every weight).  FP32 pages: the FP32
-// matrix instruction, an eighth of the rate; 24 sequences of up to 5 rows behind 992 shared positions, 35 us and the merge 7.5.
+// matrix instruction, an eighth of the rate; 24 sequences of up to 5 rows behind 992 shared positions, 35 us and the merge 6.7.
 // Sums, maxima and outputs are FP32.
 //
 // What a row does not see: its scores are masked; values past the last key that any row of the tile sees are cleared, and of those that only some see
