@@ -4,7 +4,7 @@
 // not kept a token is drawn from max(p - q, 0), behind the last kept one from p, by the inverse of the distribution: the first index whose
 // cumulative sum exceeds u1 times the total.  Such a draw is a whole number that another summation must reproduce, so weights and sums are held
 // in FP64: a cumulative sum of 128256 FP32 weights is off by 1e-5 of a token's share, one of FP64 weights by 1e-14.
-//   verify_stats_kernel   chunks of a row: largest logit (lowest index among equals), sum of exp((l - largest) / T)
+//   verify_stats_kernel   chunks of a row: largest logit (lowest index among equals), sum of exp((l - largest) / T) over all but the row's draft
 //   verify_rest_kernel    (with draft probabilities, more than VERIFY_FEW chunks) the refused row's sum of max(p - q, 0) per chunk
 //   verify_draw_kernel    one workgroup per sequence: which tokens are kept, the chunk the draw falls in, the index in it
 // Measured, us per kernel: 16 x 9 ragged rows of 128256, a draft with certainty, stats 16.0 and draw 6.6; 32 x 5 rows with draft probabilities, stats 24.2, rest 10.0, draw
@@ -21,7 +21,7 @@ namespace jitnn {
 constexpr int VERIFY_THREADS = 256, VERIFY_VALUES = 16, VERIFY_CHUNK = VERIFY_THREADS * VERIFY_VALUES;
 
 struct VerifyStat {
-    double sum;  // of exp((l - largest) / T); T <= 0: unused
+    double sum;  // of exp((l - largest) / T) without the row's draft (of a row: with it); T <= 0: unused
     float largest;
     int index;
 };
@@ -127,7 +127,9 @@ __device__ __forceinline__ void verify_load(const float *__restrict__ row, int c
     }
 }
 
-// grid (chunks, rows)
+// grid (chunks, rows).  A draft is left out of its chunk's sum and joined where it is judged: what is left when it is refused is so a sum and not a difference.  (Of a token with
+// all but 6e-8 of the weight, the largest share that can be refused, a difference has the error of the whole, 2e-9 of what is left, and nothing of what is
+// below 1e-16.)
 __global__ void __launch_bounds__(VERIFY_THREADS) verify_stats_kernel(const VerifyArgs a) {
     __shared__ float best_of[VERIFY_THREADS / 64];
     __shared__ int index_of[VERIFY_THREADS / 64];
@@ -136,9 +138,11 @@ __global__ void __launch_bounds__(VERIFY_THREADS) verify_stats_kernel(const Veri
     float v[VERIFY_VALUES];
     verify_load(a.logits + (size_t)r * a.logits_stride, c0, a.vocab, v);
     VerifyWeight::fill(table);
-    const int s = batch_sequence(a.starts, a.sequences, r);
+    const int s = __builtin_amdgcn_readfirstlane(batch_sequence(a.starts, a.sequences, r));
     if (s >= a.sequences || r < a.starts[0]) return;  // a row of no sequence
     const float temperature = a.temperatures[s];
+    const int end = min(a.starts[s + 1], a.rows), next = a.tokens[min(r + 1, a.rows - 1)];
+    const int draft = r + 1 < end ? next - c0 : -1;  // as a place of the chunk
     float best = -INFINITY;
     int index = 0x7fffffff;
 #pragma unroll
@@ -159,6 +163,10 @@ __global__ void __launch_bounds__(VERIFY_THREADS) verify_stats_kernel(const Veri
     double sum = 0.;
     if (temperature > 0.f && best > -INFINITY) {
         const VerifyWeight weight(table, temperature, best);
+        if (draft >= 0 && draft < VERIFY_CHUNK) {
+#pragma unroll
+            for (int u = 0; u < VERIFY_VALUES; ++u) v[u] = draft == 4 * ((u >> 2) * VERIFY_THREADS + tid) + (u & 3) ? -INFINITY : v[u];
+        }
         if (best < INFINITY) {
 #pragma unroll
             for (int u = 0; u < VERIFY_VALUES; ++u) sum += weight(v[u]);
@@ -178,7 +186,7 @@ __global__ void __launch_bounds__(VERIFY_THREADS) verify_stats_kernel(const Veri
     }
 }
 
-// A row's largest logit, its index and the sum of its weights, from the chunks'; one wave, every lane receives them.  first: chunk `lane`'s part of the sum.
+// A row's largest logit, its index and the sum of its weights but for its draft's, from the chunks'; one wave, every lane receives them.  first: chunk `lane`'s part of the sum.
 __device__ __forceinline__ VerifyStat verify_row(const VerifyStat *__restrict__ st, int chunks, const double *table, float temperature, double &first) {
     const int lane = threadIdx.x & 63;
     VerifyStat t{0., -INFINITY, 0x7fffffff}, mine{0., -INFINITY, 0x7fffffff};
@@ -203,21 +211,22 @@ struct VerifyEnd {
     float temperature;
     VerifyStat stat;            // of that row
     int draft;                  // the token it refused, -1 where that is none
-    float draft_logit, number;  // ... and its random number
+    float number;               // its random number
     const double *parts;
 };
 constexpr int VERIFY_ROWS = 32;  // rows whose sums are kept
 struct VerifyRow {
     VerifyStat stat;
     int draft;
-    float draft_logit, number;
+    float number;
 };
 struct VerifyShared {
     int first_refused;
     VerifyRow row[VERIFY_ROWS + 1];
     double table[32];
 };
-// parts [VERIFY_ROWS + 1][64] (or nullptr): what the first 64 chunks of each row hold of its sum; e.parts is the drawing row's.
+// parts [VERIFY_ROWS + 1][64] (or nullptr): what the first 64 chunks of each row hold of its sum, its draft left out; e.parts is the drawing row's, which has refused
+// its draft or has none.
 template <int WAVES>
 __device__ __forceinline__ VerifyEnd verify_end(const VerifyArgs &a, int s, VerifyShared &sh, double *parts) {
     VerifyEnd e;
@@ -236,12 +245,14 @@ __device__ __forceinline__ VerifyEnd verify_end(const VerifyArgs &a, int s, Veri
         const float u = a.uniforms[2 * (size_t)r], number = a.uniforms[2 * (size_t)r + 1], lx = known ? a.logits[(size_t)r * a.logits_stride + x] : 0.f,
                     qx = known && a.draft_probs ? a.draft_probs[(size_t)r * a.draft_stride + x] : 1.f;
         double first;
-        const VerifyStat t = verify_row((const VerifyStat *)a.part + (size_t)r * a.chunks, a.chunks, sh.table, e.temperature, first);
+        VerifyStat t = verify_row((const VerifyStat *)a.part + (size_t)r * a.chunks, a.chunks, sh.table, e.temperature, first);
         if (parts && slot <= VERIFY_ROWS) parts[64 * slot + (tid & 63)] = first;
         const VerifyWeight weight(sh.table, e.temperature, t.largest);
-        const bool keep = known && (e.temperature > 0.f ? t.largest > -INFINITY && (double)u * (double)qx < weight.any(lx) / t.sum : x == t.index);
+        const double wx = known ? weight.any(lx) : 0.;
+        t.sum += wx;
+        const bool keep = known && (e.temperature > 0.f ? t.largest > -INFINITY && (double)u * (double)qx < wx / t.sum : x == t.index);
         if ((tid & 63) == 0) {
-            if (slot <= VERIFY_ROWS) sh.row[slot] = VerifyRow{t, known ? x : -1, lx, number};
+            if (slot <= VERIFY_ROWS) sh.row[slot] = VerifyRow{t, known ? x : -1, number};
             if (drafted && !keep) atomicMin(&sh.first_refused, j);
         }
     };
@@ -260,7 +271,6 @@ __device__ __forceinline__ VerifyEnd verify_end(const VerifyArgs &a, int s, Veri
     e.parts = parts ? parts + 64 * slot : nullptr;
     e.stat = at.stat;
     e.draft = at.draft;
-    e.draft_logit = at.draft_logit;
     e.number = at.number;
     return e;
 }
@@ -368,9 +378,7 @@ __global__ void __launch_bounds__(VERIFY_DRAW_THREADS) verify_draw_kernel(const 
                 return w;
             }
             if (q) return c < 64 ? first_rest : rest[c];
-            double w = c < 64 ? e.parts[c] : st[c].largest > -INFINITY ? st[c].sum * weight.any(st[c].largest) : 0.;
-            if (x >= 0 && x / VERIFY_CHUNK == c) w = fmax(w - weight.any(e.draft_logit), 0.);
-            return w * share;
+            return share * (c < 64 ? e.parts[c] : st[c].largest > -INFINITY ? st[c].sum * weight.any(st[c].largest) : 0.);
         };
         const double first = weight_of(lane);  // (a vocabulary of 262144 has 64 chunks)
         double total = verify_wave_sum(first);

@@ -1,0 +1,59 @@
+"""Operators of a served batch where sums nearly cancel, positions are far and batches are long, against plain implementations in 64 bits or more."""
+import numpy as np
+import pytest
+import torch
+
+import serving_reference as ref
+import test_gpu_serving as served
+
+pytestmark = pytest.mark.gpu
+
+BELOW_ONE = np.float32(1 - 2.0 ** -24)
+
+
+@pytest.fixture(scope="module")
+def jn():
+    import jitnn_amd
+    jitnn_amd.init()
+    return jitnn_amd
+
+
+# ---------------------------------------------------------------------------------------------- drafted tokens
+
+@pytest.mark.parametrize("vocab", [4096, 9000, 50000])
+def test_verify_of_a_refused_draft_that_had_nearly_all_the_weight(jn, vocab):
+    """Looked-up drafts of probability 1 - 7e-8 and less, refused by the largest number below one: the token behind them is drawn from what little is left.  A number of
+    0 takes the first index with any weight, though that is 4e-18 of the draft's and shares its chunk; others stand next to the border of every cumulative sum (the border's distance
+    is 2^-25 of the sum at most, and 64-bit sums without the draft are good to 2^-45 of it)."""
+    rng = np.random.default_rng(vocab)
+    count = 60
+    logits, tokens, u = np.full((2 * count, vocab), -np.inf, dtype=np.float32), np.zeros(2 * count, dtype=np.int64), np.zeros((2 * count, 2), dtype=np.float32)
+    for s in range(count):
+        r, zero = 2 * s, s % 3 == 0
+        x = int(rng.integers(10, 4000 if zero else vocab - 100))
+        chunk, end = x // 4096 * 4096, min(x // 4096 * 4096 + 4096, vocab)
+        tokens[r + 1] = x
+        logits[r, x] = 5.0
+        # the rest, 1e-7 to 1e-6 of the draft's weight: over the tokens of its chunk and all others, or all behind its chunk where there are more
+        near = [] if zero else rng.integers(chunk, end, 9)
+        far = rng.integers(end if zero and end < vocab else x + 1 if zero else 0, vocab, 9)
+        for at in np.unique(np.concatenate([near, far]).astype(int)):
+            if at != x:
+                logits[r, at] = np.float32(5.0 - 16.5 + 1.5 * rng.random())
+        if zero:
+            logits[r, x - 5] = 5.0 - 40.0
+        logits[r + 1] = rng.standard_normal(vocab).astype(np.float32)
+        u[r, 0], u[r + 1] = BELOW_ONE, rng.random(2)
+        w = np.exp(logits[r].astype(np.float64) - 5.0)
+        w[x] = 0
+        c = np.cumsum(w)
+        if not zero:  # the nearest number to a border, on either side of it
+            border = c[rng.choice(np.nonzero(w)[0][:-1])] / c[-1]
+            u[r, 1] = min(np.float32(border), BELOW_ONE)
+            if s % 3 == 2:
+                u[r, 1] = np.nextafter(u[r, 1], np.float32(0 if np.float64(u[r, 1]) > border else 1))
+    starts, temps = np.arange(0, 2 * count + 1, 2), np.ones(count)
+    want = ref.verify(logits, starts, tokens, None, temps, u)
+    assert list(want[1]) == [0] * count and all(want[0][2 * s] == tokens[2 * s + 1] - 5 for s in range(0, count, 3))
+    got = served.run_verify(jn, logits, starts, tokens, None, temps, u)
+    assert np.array_equal(got[1], want[1]) and np.array_equal(got[0], want[0]), np.argwhere(got[0] != want[0])
