@@ -423,7 +423,7 @@ JITNN_HIP_API int jitnn_hip_llama_set_rope(jitnn_hip_llama *m, const jitnn_hip_r
 
 /* One pass of a batch of sequences over a paged cache (layers, kv_heads and head_dim of the model): x [batch->tokens, d_model] are the embeddings of
  * the batch's rows; every row's keys and values are appended, turned by the model's rotary positions, and logits [logit_count, vocab] are those of the
- * rows logit_rows [logit_count] (device memory; a row outside the batch gives NaN): a decode step names every row, a prompt's pass its last.
+ * rows logit_rows [logit_count] (device memory; a row outside the batch or of no sequence gives NaN): a decode step names every row, a prompt's pass its last.
  * logit_count 0: none.  The rows go through the linears together, as in jitnn_hip_llama_prefill; the model's own cache is not touched.
  * The model's many-token buffers and the attention's workspace belong to it and grow with the largest pass (which waits for the device; such a
  * call cannot be recorded: JITNN_HIP_EINVAL).  Once a pass has been recorded, those that larger ones replace live on until the model is freed. */

@@ -1071,4 +1071,14 @@ __global__ void __launch_bounds__(256) embed_plain_rows_kernel(const void *__res
                                         : __half2float(reinterpret_cast<const __half *>(table)[row + i]);
 }
 
+// y[i, :] = row rows[i] of a pass's x [tokens, d], for its logits.  A row of no sequence - outside starts[0] .. starts[sequences] - has no hidden state that means
+// anything, as the attention leaves what it has of it alone: NaN.  grid = rows asked for.
+__global__ void __launch_bounds__(256) batch_rows_kernel(const float *__restrict__ x, const int *__restrict__ rows, const int *__restrict__ starts, int sequences, int tokens,
+                                                         float *__restrict__ y, int d) {
+    const int r = rows[blockIdx.x];
+    const bool there = r >= 0 && r < tokens && sequences > 0 && r >= starts[0] && r < starts[sequences];
+    float *to = y + (size_t)blockIdx.x * d;
+    for (int i = threadIdx.x; i < d; i += 256) to[i] = there ? x[(size_t)r * d + i] : __builtin_nanf("");
+}
+
 }  // namespace jitnn

@@ -3018,7 +3018,7 @@ int jitnn_hip_llama_step_dev(jitnn_hip_llama *m, const jitnn_hip_paged_cache *c,
         return fail(JITNN_HIP_EINVAL, "logits of %d rows of %d", logit_count, b->tokens);
     if (m->d % 4 != 0) return fail(JITNN_HIP_EUNSUPPORTED, "d_model %d is not a multiple of 4", m->d);
     if (m->rope->rot % 8 != 0) return fail(JITNN_HIP_EUNSUPPORTED, "rot_dim %d is not a multiple of 8", m->rope->rot);
-    if (b->tokens == 0 || b->sequences == 0) return JITNN_HIP_OK;
+    if (b->tokens == 0 || (b->sequences == 0 && logit_count == 0)) return JITNN_HIP_OK;
     if (!x_dev) return fail(JITNN_HIP_EINVAL, "input is NULL");
     hipStream_t st = (hipStream_t)stream;
     const int d = m->d, T = b->tokens;
@@ -3045,15 +3045,15 @@ int jitnn_hip_llama_step_dev(jitnn_hip_llama *m, const jitnn_hip_paged_cache *c,
     prefill_reserve(m, T, st);
     const long long qd = (long long)m->heads * m->hd, kd = (long long)m->kv * m->hd;
     const float scale = 1.0f / sqrtf((float)m->hd);
-    const float *x = nullptr;
-    const int rc = run_layers(m, x_dev, T, false, st, &x, [&](int l, float *q, const float *k, const float *v, float *att, PfGroupPending &) {
+    const float *x = x_dev;  // (of no sequence at all, only the logits are to be said to be none)
+    const int rc = b->sequences == 0 ? JITNN_HIP_OK : run_layers(m, x_dev, T, false, st, &x, [&](int l, float *q, const float *k, const float *v, float *att, PfGroupPending &) {
         if (int arc = append_rows(c, l, b, m->rope, m->rope_interleaved != 0, q, qd, m->heads, q, qd, k, kd, v, kd, st)) return arc;
         return jitnn_hip_paged_attention_dev(c, l, b, m->heads, q, qd, scale, att, qd, m->paged_ws, (long long)m->paged_ws_bytes, stream);
     });
     if (rc) return rc;
     if (logit_count > 0) {
         float *rows = m->pf[5], *xn = m->pf[0];  // (free behind the last layer)
-        hipLaunchKernelGGL(embed_plain_rows_kernel, dim3((unsigned)logit_count), dim3(256), 0, st, (const void *)x, 0, logit_rows_dev, rows, d, T);
+        hipLaunchKernelGGL(batch_rows_kernel, dim3((unsigned)logit_count), dim3(256), 0, st, x, logit_rows_dev, b->starts, b->sequences, T, rows, d);
         const jitnn_hip_weight *ws[1] = {m->w_out};
         float *ys[1] = {logits_dev};
         const float *nw = m->norms + (size_t)m->layers * 2 * d;

@@ -1,0 +1,87 @@
+"""Rows of a pass that belong to no sequence, and sequences that cannot be attended, beside others: what they leave behind and that they reach nobody else."""
+import numpy as np
+import pytest
+import torch
+
+import serving_reference as ref
+import test_llm
+from helpers import norm_err
+
+pytestmark = pytest.mark.gpu
+
+TWICE = {False: 2e-4, True: 1e-2}  # the bars of few-row and many-row linears, for two results that may both be off by one
+
+
+@pytest.fixture(scope="module")
+def jn():
+    import jitnn_amd
+    jitnn_amd.init()
+    return jitnn_amd
+
+
+@pytest.fixture(scope="module")
+def model_file(tmp_path_factory):
+    path = tmp_path_factory.mktemp("rows") / "tiny.gguf"
+    test_llm.write_model(path, "llama", 11)
+    return path
+
+
+# rows in front, rows of each sequence, rows behind: few-row linears, many-row ones, and a pass of nobody's rows alone
+@pytest.mark.parametrize("front,counts,behind", [(0, [3, 1], 2), (2, [1, 4], 3), (5, [30, 25, 1], 4), (7, [90, 60], 9), (1, [1], 0), (3, [0, 0], 2), (40, [], 60)])
+def test_rows_of_no_sequence_have_no_logits(jn, model_file, front, counts, behind):
+    """NaN, whatever an earlier pass left in the model's buffers; and what they hold themselves reaches no row of a sequence."""
+    rng = np.random.default_rng(front + behind)
+    with jn.Llm.load(model_file) as llm:
+        dec, vocab = llm.model(), llm.info().vocab
+        table = torch.from_numpy(dec.embed(np.arange(vocab))).cuda()
+        rows = front + sum(counts) + behind
+        own = list(range(front, front + sum(counts)))
+        b = ref.Batch(rng, counts, [c + 5 for c in counts], 16, max_len=128)
+        starts = (b.starts + front).astype(np.int32)
+        first = None
+        for fill in (0.0, 3.0, float("nan"), float("inf")):
+            pool = [torch.ones(2, b.pages, 2, 16, 64, device="cuda") * 0.1 for _ in range(2)]
+            cache = jn.PagedCache.wrap_dev(pool[0].data_ptr(), pool[1].data_ptr(), 2, 2, 64, b.pages, 16, 0)
+            x = torch.full((rows, 256), fill, device="cuda")
+            if own:
+                x[own] = table[torch.arange(len(own), device="cuda") * 7 % vocab]
+            keep = [torch.from_numpy(np.ascontiguousarray(a)).cuda() for a in (b.tables, starts, np.array(b.lens, dtype=np.int32), np.arange(rows, dtype=np.int32))]
+            nb = jn.Batch(len(counts), rows, max([1] + counts), 128, keep[0].data_ptr(), b.width, keep[1].data_ptr(), keep[2].data_ptr())
+            logits = torch.full((rows, vocab), 7.0, device="cuda")
+            dec.step_dev(cache, nb, x.data_ptr(), keep[3].data_ptr(), rows, logits.data_ptr())
+            torch.cuda.synchronize()
+            stray = [r for r in range(rows) if r not in own]
+            assert torch.isnan(logits[stray]).all()
+            assert torch.isfinite(logits[own]).all()
+            first = logits[own].clone() if first is None else first
+            if np.isfinite(fill):
+                assert torch.equal(logits[own], first)
+            elif own:  # (a linear may take another way to the same result beside a row that is not finite)
+                assert norm_err(logits[own].cpu().numpy(), first.cpu().numpy()) <= TWICE[rows > 64]
+
+
+@pytest.mark.parametrize("counts", [[3, 1, 2], [30, 25, 40]])
+def test_a_sequence_on_a_bad_page_reaches_no_other(jn, model_file, counts):
+    """Its own rows are NaN through all layers; the logits of the other sequences' rows are those of a pass in which it is sound."""
+    rng = np.random.default_rng(5)
+    with jn.Llm.load(model_file) as llm:
+        dec, vocab = llm.model(), llm.info().vocab
+        table = torch.from_numpy(dec.embed(np.arange(vocab))).cuda()
+        b = ref.Batch(rng, counts, [c + 20 for c in counts], 16, max_len=64)
+        bad = list(range(int(b.starts[1]), int(b.starts[2])))
+        out = []
+        for page in (None, b.pages):
+            pool = [torch.ones(2, b.pages, 2, 16, 64, device="cuda") * 0.1 for _ in range(2)]
+            cache = jn.PagedCache.wrap_dev(pool[0].data_ptr(), pool[1].data_ptr(), 2, 2, 64, b.pages, 16, 0)
+            tables = b.tables.copy()
+            if page is not None:
+                tables[1, 0] = page
+            keep = [torch.from_numpy(np.ascontiguousarray(a)).cuda() for a in (tables, b.starts, np.array(b.lens, dtype=np.int32), np.arange(b.tokens, dtype=np.int32))]
+            nb = jn.Batch(3, b.tokens, max(counts), 64, keep[0].data_ptr(), b.width, keep[1].data_ptr(), keep[2].data_ptr())
+            x, logits = table[torch.arange(b.tokens, device="cuda") * 5 % vocab].contiguous(), torch.empty(b.tokens, vocab, device="cuda")
+            dec.step_dev(cache, nb, x.data_ptr(), keep[3].data_ptr(), b.tokens, logits.data_ptr())
+            torch.cuda.synchronize()
+            out.append(logits)
+        others = [r for r in range(b.tokens) if r not in bad]
+        assert torch.isnan(out[1][bad]).all() and torch.isfinite(out[0]).all()
+        assert norm_err(out[1][others].cpu().numpy(), out[0][others].cpu().numpy()) <= TWICE[b.tokens > 64]
