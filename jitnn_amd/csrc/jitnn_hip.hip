@@ -1939,27 +1939,32 @@ int rope_build(int rot, bool interleaved, double theta, const jitnn_hip_rope_sca
     r->rot = rot;
     r->interleaved = interleaved;
     const int kind = sc ? sc->kind : JITNN_HIP_ROPE_PLAIN;
-    constexpr double two_pi = 6.283185307179586476925;
+    constexpr long double two_pi = 6.283185307179586476925286766559L;
     double lo = 0, hi = 0;
     if (kind == JITNN_HIP_ROPE_YARN) {
         // the pair that turns beta times in the original context
-        auto pair_of = [&](double beta) { return rot * log(sc->original_context / (two_pi * beta)) / (2.0 * log(theta)); };
+        auto pair_of = [&](double beta) { return rot * log(sc->original_context / ((double)two_pi * beta)) / (2.0 * log(theta)); };
         lo = std::max(0.0, floor(pair_of(sc->beta_fast)));
         hi = std::min((double)rot - 1, ceil(pair_of(sc->beta_slow)));
         r->magnitude = 0.1 * log(sc->factor) + 1.0;
     }
     if (sc && sc->attention_factor != 0.0) r->magnitude = sc->attention_factor;
     for (int i = 0; i < rot / 2; ++i) {
-        double f = pow(theta, -2.0 * i / rot);
+        double f = pow(theta, -2.0 * i / rot), ramp = 0;
         if (factors) f /= (double)factors[i];
         if (kind == JITNN_HIP_ROPE_LINEAR) f /= sc->factor;
         if (kind == JITNN_HIP_ROPE_YARN) {
-            const double ramp = std::min(1.0, std::max(0.0, (i - lo) / std::max(hi - lo, 0.001)));
+            ramp = std::min(1.0, std::max(0.0, (i - lo) / std::max(hi - lo, 0.001)));
             f = f * (1.0 - ramp) + f / sc->factor * ramp;
         }
         r->frequency[i] = f;
-        const double turn = f / two_pi, part = turn - floor(turn);  // (positions are whole: whole turns of a frequency are none)
-        turns[i] = (unsigned long long)std::min(ldexp(part, 64), 18446744073709549568.0);
+        // All 64 bits of the fraction of a turn, from the same formulas in 80-bit numbers: the 53 of a double are off by 2.6e-7 at position 2^31.
+        long double whole = powl((long double)theta, -2.0L * i / rot);
+        if (factors) whole /= (long double)factors[i];
+        if (kind == JITNN_HIP_ROPE_LINEAR) whole /= (long double)sc->factor;
+        if (kind == JITNN_HIP_ROPE_YARN) whole = whole * (1.0L - ramp) + whole / (long double)sc->factor * ramp;
+        const long double turn = whole / two_pi, part = turn - floorl(turn);  // (positions are whole: whole turns of a frequency are none)
+        turns[i] = part > 0 ? (unsigned long long)fminl(ldexpl(part, 64) + 0.5L, 18446744073709551615.0L) : 0;
     }
     const size_t bytes = turns.size() * sizeof(turns[0]);
     if (hipMalloc(&r->turns, bytes) != hipSuccess) {

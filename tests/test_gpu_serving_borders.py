@@ -1,4 +1,6 @@
 """Operators of a served batch where sums nearly cancel, positions are far and batches are long, against plain implementations in 64 bits or more."""
+from decimal import Decimal, localcontext
+
 import numpy as np
 import pytest
 import torch
@@ -57,3 +59,37 @@ def test_verify_of_a_refused_draft_that_had_nearly_all_the_weight(jn, vocab):
     assert list(want[1]) == [0] * count and all(want[0][2 * s] == tokens[2 * s + 1] - 5 for s in range(0, count, 3))
     got = served.run_verify(jn, logits, starts, tokens, None, temps, u)
     assert np.array_equal(got[1], want[1]) and np.array_equal(got[0], want[0]), np.argwhere(got[0] != want[0])
+
+
+# ---------------------------------------------------------------------------------------------- rotary positions
+
+def turned(theta, rot, divisor, positions):
+    """Cosines and sines [positions, rot / 2] of position theta^(-2 i / rot) / divisor, the angle to 40 digits and reduced before it is a double."""
+    with localcontext() as ctx:
+        ctx.prec = 60
+        tan = []  # arctangents of 1/5 and 1/239: pi = 16 and -4 of them (Machin)
+        for n in (5, 239):
+            term, total, k = Decimal(1) / n, Decimal(0), 1
+            while abs(term) > Decimal(10) ** -58:
+                total, term, k = total + term / k, -term / (n * n), k + 2
+            tan.append(total)
+        whole = 2 * (16 * tan[0] - 4 * tan[1])
+        f = [(-(Decimal(2) * i / rot) * Decimal(theta).ln()).exp() / Decimal(divisor) for i in range(rot // 2)]
+        angle = np.array([[float((p * x).remainder_near(whole)) for x in f] for p in positions])
+    return np.cos(angle), np.sin(angle)
+
+
+@pytest.mark.parametrize("theta,rot,factor", [(10000, 128, 1.0), (500000, 128, 1.0), (500000, 64, 3.0), (1000000, 250, 1.0)])
+def test_rope_at_the_far_end_of_its_positions(jn, theta, rot, factor):
+    """Pairs (1, 0), so that cosines and sines come out as they are.  Their angle x, up to pi / 4, is off by 2^-24 of itself for each of its conversion, its constant and its product,
+    which x cos x <= 0.56 of it makes 1.7 x 2^-24 of a sine or cosine; the fraction of a turn by 2^-32, the series' last step by 2^-25, the steps before it by 0.2 x 2^-24, the terms left
+    out by 2e-9: below 2.5 x 2^-24."""
+    rope = jn.Rope(rot, theta=float(theta), interleaved=True, scaling="linear" if factor != 1.0 else None, factor=factor)
+    pos = np.array([(1 << 31) - 1 - 977 * i for i in range(100)] + [-(1 << 31) + 1013 * i for i in range(100)] + [0, 1, -1, 131071, 1 << 27, -(1 << 27)], dtype=np.int64)
+    c, s = turned(theta, rot, factor, [int(p) for p in pos])
+    x = torch.zeros(len(pos), rot, device="cuda")
+    x[:, 0::2] = 1
+    p = torch.from_numpy(pos.astype(np.int32)).cuda()
+    rope.apply_dev(x.data_ptr(), p.data_ptr(), len(pos), 1, rot, x.data_ptr())
+    got = x.double().cpu().numpy()
+    assert np.abs(got[:, 0::2] - c).max() <= 2.5 * 2.0 ** -24 and np.abs(got[:, 1::2] - s).max() <= 2.5 * 2.0 ** -24
