@@ -201,7 +201,6 @@ class SharedPrompt:
         self._dec.step_dev(self._cache, batch, self._x.ptr, rows.ptr, len(logit_rows), self._logits.ptr)
 
     def _step(self, which, tokens):
-        which = list(which)
         if not which or len(set(which)) != len(which) or len(tokens) != len(which) or any(not 0 < len(t) <= self._rows for t in tokens):
             raise ValueError(f"sequences {which} with {[len(t) for t in tokens]} tokens (1 to {self._rows} each)")
         if any(not 0 <= t < self._vocab for ts in tokens for t in ts):
@@ -214,6 +213,7 @@ class SharedPrompt:
 
     def step(self, which, tokens) -> np.ndarray:
         """The next tokens of the sequences `which` (a list per sequence): appended, and the logits [rows, vocab] after each of them."""
+        which = list(which)
         lens = self._step(which, tokens)
         for i, n in zip(which, lens):
             self.lens[i] = n
@@ -223,6 +223,7 @@ class SharedPrompt:
     def verify(self, which, tokens, temperatures, uniforms):
         """The same for sequences whose tokens after the first are drafted: [(drafts kept, the token drawn after them)].  Of each sequence the first token and the kept
         drafts are appended.  uniforms [rows, 2]: two random numbers in [0, 1) for each token."""
+        which = list(which)
         self._step(which, tokens)
         count, rows = len(self._tables), len(self._tables) * self._rows
         if self._verify is None:

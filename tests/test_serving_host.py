@@ -1,0 +1,30 @@
+"""The host side of a served batch: what a shared prompt's steps take and refuse before anything is launched.  No device needed."""
+import numpy as np
+import pytest
+
+
+@pytest.fixture
+def run():
+    """Three sequences behind a prompt of 20 tokens whose passes are only written down."""
+    from jitnn_amd.serving import SharedPrompt
+
+    class Logits:
+        ptr = 0
+
+        @staticmethod
+        def get(n):
+            return np.zeros(n, dtype=np.float32)
+
+    s = SharedPrompt.__new__(SharedPrompt)
+    s._vocab, s._rows, s.max_len, s.shared = 50, 4, 40, 1
+    s._tables, s._verify, s._logits = np.zeros((3, 3), dtype=np.int32), None, Logits
+    s.lens, s.passes = [20, 20, 20], []
+    s._pass = lambda which, tokens, lens, shared, rows: s.passes.append((list(which), tokens, lens))
+    return s
+
+
+def test_a_step_advances_the_sequences_that_an_iterator_names(run):
+    assert run.step(iter([2, 0]), [[1, 2], [3]]).shape == (3, 50)
+    assert run.lens == [21, 20, 22] and [p[2] for p in run.passes] == [[22, 21]]
+    run.step((i for i in (0, 1)), [[1], [2]])
+    assert run.lens == [22, 21, 22]
