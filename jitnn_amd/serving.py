@@ -222,19 +222,21 @@ class SharedPrompt:
 
     def verify(self, which, tokens, temperatures, uniforms):
         """The same for sequences whose tokens after the first are drafted: [(drafts kept, the token drawn after them)].  Of each sequence the first token and the kept
-        drafts are appended.  uniforms [rows, 2]: two random numbers in [0, 1) for each token."""
-        which = list(which)
+        drafts are appended.  temperatures: one for each of these sequences; uniforms [rows, 2]: two random numbers in [0, 1) for each token."""
+        which, rows = list(which), sum(len(t) for t in tokens)
+        temperatures, uniforms = np.asarray(temperatures, dtype=np.float32), np.asarray(uniforms, dtype=np.float32)
+        if temperatures.shape != (len(which),) or uniforms.shape != (rows, 2):
+            raise ValueError(f"temperatures {temperatures.shape} and uniforms {uniforms.shape} of {len(which)} sequences with {rows} tokens")
         self._step(which, tokens)
-        count, rows = len(self._tables), len(self._tables) * self._rows
+        count, most = len(self._tables), len(self._tables) * self._rows
         if self._verify is None:
-            n = verify_workspace(rows, count, self._vocab)
-            self._verify = [DeviceArray(count, np.float32), DeviceArray(2 * rows, np.float32), DeviceArray(rows, np.int32), DeviceArray(count, np.int32), DeviceArray(n, np.uint8)]
+            n = verify_workspace(most, count, self._vocab)
+            self._verify = [DeviceArray(count, np.float32), DeviceArray(2 * most, np.float32), DeviceArray(most, np.int32), DeviceArray(count, np.int32), DeviceArray(n, np.uint8)]
         temps, nums, out, accepted, space = self._verify
-        n = sum(len(t) for t in tokens)
         temps.put(temperatures)
         nums.put(uniforms)
-        verify_drafts_dev(self._logits.ptr, n, self._vocab, self._ints[1].ptr, len(tokens), self._tok.ptr, temps.ptr, nums.ptr, out.ptr, accepted.ptr, space.ptr, space.count)
-        got, kept, at, result = out.get(n), accepted.get(len(tokens)), 0, []
+        verify_drafts_dev(self._logits.ptr, rows, self._vocab, self._ints[1].ptr, len(tokens), self._tok.ptr, temps.ptr, nums.ptr, out.ptr, accepted.ptr, space.ptr, space.count)
+        got, kept, at, result = out.get(rows), accepted.get(len(tokens)), 0, []
         for i, ts, k in zip(which, tokens, kept):
             result.append((int(k), int(got[at + k])))
             self.lens[i] += 1 + int(k)

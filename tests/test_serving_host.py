@@ -28,3 +28,12 @@ def test_a_step_advances_the_sequences_that_an_iterator_names(run):
     assert run.lens == [21, 20, 22] and [p[2] for p in run.passes] == [[22, 21]]
     run.step((i for i in (0, 1)), [[1], [2]])
     assert run.lens == [22, 21, 22]
+
+
+@pytest.mark.parametrize("temperatures,uniforms", [([1.0], np.zeros((3, 2))), ([1.0, 0.5, 0.2], np.zeros((3, 2))), ([], np.zeros((3, 2))), ([1.0, 0.5], np.zeros((2, 2))),
+                                                   ([1.0, 0.5], np.zeros((4, 2))), ([1.0, 0.5], np.zeros(5)), ([1.0, 0.5], np.zeros((3, 1))), ([1.0, 0.5], np.zeros((2, 3)))])
+def test_verification_refuses_other_numbers_of_numbers(run, temperatures, uniforms):
+    """Before the pass: too few would leave those of an earlier call in use."""
+    with pytest.raises(ValueError, match="temperatures"):
+        run.verify([0, 2], [[1, 2], [3]], temperatures, uniforms)
+    assert run.passes == [] and run.lens == [20, 20, 20]
