@@ -307,7 +307,7 @@ class Llm:
                     continue
                 tokens = [[texts[i].known[-1]] + look_up_draft(texts[i].known, drafts) for i in live]
                 numbers = np.concatenate([texts[i].rng.random((len(ts), 2)) for i, ts in zip(live, tokens)])
-                got = run.verify(live, tokens, [0.0 if greedy else rq.temperature] * len(live), np.minimum(numbers.astype(np.float32), np.float32(1 - 2.0 ** -24)))
+                got = run.verify(live, tokens, [0.0 if greedy else rq.temperature] * len(live), numbers)
                 for i, ts, (kept, token) in zip(live, tokens, got):
                     for t in ts[1:1 + kept] + [token]:
                         if texts[i].reason is None:

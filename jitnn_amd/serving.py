@@ -227,6 +227,7 @@ class SharedPrompt:
         temperatures, uniforms = np.asarray(temperatures, dtype=np.float32), np.asarray(uniforms, dtype=np.float32)
         if temperatures.shape != (len(which),) or uniforms.shape != (rows, 2):
             raise ValueError(f"temperatures {temperatures.shape} and uniforms {uniforms.shape} of {len(which)} sequences with {rows} tokens")
+        uniforms = np.minimum(uniforms, np.float32(1 - 2.0 ** -24))  # (64-bit numbers below 1 may have become 1, which keeps no draft)
         self._step(which, tokens)
         count, most = len(self._tables), len(self._tables) * self._rows
         if self._verify is None:

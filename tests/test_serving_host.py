@@ -37,3 +37,27 @@ def test_verification_refuses_other_numbers_of_numbers(run, temperatures, unifor
     with pytest.raises(ValueError, match="temperatures"):
         run.verify([0, 2], [[1, 2], [3]], temperatures, uniforms)
     assert run.passes == [] and run.lens == [20, 20, 20]
+
+
+def test_numbers_just_below_one_stay_below_it(run, monkeypatch):
+    """64-bit numbers in [0, 1) that 32 bits would round up to 1, which no longer keeps a certain draft."""
+    from jitnn_amd import serving
+    seen = {}
+
+    class Array:
+        def __init__(self, count, dtype):
+            self.count, self.ptr = count, 0
+
+        def put(self, values):
+            seen[self.count] = np.array(values)
+            return self
+
+        def get(self, n):
+            return np.zeros(n, dtype=np.int32)
+
+    monkeypatch.setattr(serving, "DeviceArray", Array)
+    monkeypatch.setattr(serving, "verify_workspace", lambda *a: 999)
+    monkeypatch.setattr(serving, "verify_drafts_dev", lambda *a: None)
+    run._ints, run._tok = [Array(1, np.int32)] * 4, Array(1, np.int32)
+    run.verify([0], [[1, 2]], [1.0], [[1 - 2.0 ** -30, 0.25], [0.5, 1 - 2.0 ** -53]])
+    assert seen[24].dtype == np.float32 and seen[24].max() == np.float32(1 - 2.0 ** -24) and seen[24].shape == (2, 2)
