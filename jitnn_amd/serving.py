@@ -200,6 +200,9 @@ class SharedPrompt:
         _lib.check(_lib.lib.jitnn_hip_llama_embed_dev(self._dec.handle, self._tok.ptr, len(flat), self._x.ptr, None), "jitnn_hip_llama_embed_dev")
         self._dec.step_dev(self._cache, batch, self._x.ptr, rows.ptr, len(logit_rows), self._logits.ptr)
 
+    def _named(self, which):
+        return [range(len(self._tables))[i] for i in which]
+
     def _step(self, which, tokens):
         if not which or len(set(which)) != len(which) or len(tokens) != len(which) or any(not 0 < len(t) <= self._rows for t in tokens):
             raise ValueError(f"sequences {which} with {[len(t) for t in tokens]} tokens (1 to {self._rows} each)")
@@ -213,7 +216,7 @@ class SharedPrompt:
 
     def step(self, which, tokens) -> np.ndarray:
         """The next tokens of the sequences `which` (a list per sequence): appended, and the logits [rows, vocab] after each of them."""
-        which = list(which)
+        which = self._named(which)
         lens = self._step(which, tokens)
         for i, n in zip(which, lens):
             self.lens[i] = n
@@ -223,9 +226,9 @@ class SharedPrompt:
     def verify(self, which, tokens, temperatures, uniforms):
         """The same for sequences whose tokens after the first are drafted: [(drafts kept, the token drawn after them)].  Of each sequence the first token and the kept
         drafts are appended.  temperatures: one for each of these sequences; uniforms [rows, 2]: two random numbers in [0, 1) for each token."""
-        which, rows = list(which), sum(len(t) for t in tokens)
+        which, rows = self._named(which), sum(len(t) for t in tokens)
         temperatures, uniforms = np.asarray(temperatures, dtype=np.float32), np.asarray(uniforms, dtype=np.float32)
-        if temperatures.shape != (len(which),) or uniforms.shape != (rows, 2):
+        if temperatures.shape != (len(which),) or uniforms.shape not in ((rows, 2), (2 * rows,)):
             raise ValueError(f"temperatures {temperatures.shape} and uniforms {uniforms.shape} of {len(which)} sequences with {rows} tokens")
         uniforms = np.minimum(uniforms, np.float32(1 - 2.0 ** -24))  # (64-bit numbers below 1 may have become 1, which keeps no draft)
         self._step(which, tokens)

@@ -30,6 +30,18 @@ def test_a_step_advances_the_sequences_that_an_iterator_names(run):
     assert run.lens == [22, 21, 22]
 
 
+def test_a_sequence_counted_from_the_end_is_the_same_one(run):
+    """Named twice, once so and once so, it would write two tokens to one position."""
+    for call in (lambda w, t: run.step(w, t), lambda w, t: run.verify(w, t, [0.0] * 2, np.zeros((2, 2)))):
+        with pytest.raises(ValueError, match="sequences"):
+            call([-1, 2], [[1], [2]])
+        with pytest.raises(IndexError):
+            call([0, 3], [[1], [2]])
+    assert run.passes == []
+    run.step([-1], [[1]])
+    assert run.lens == [20, 20, 21] and run.passes[0][0] == [2]
+
+
 @pytest.mark.parametrize("temperatures,uniforms", [([1.0], np.zeros((3, 2))), ([1.0, 0.5, 0.2], np.zeros((3, 2))), ([], np.zeros((3, 2))), ([1.0, 0.5], np.zeros((2, 2))),
                                                    ([1.0, 0.5], np.zeros((4, 2))), ([1.0, 0.5], np.zeros(5)), ([1.0, 0.5], np.zeros((3, 1))), ([1.0, 0.5], np.zeros((2, 3)))])
 def test_verification_refuses_other_numbers_of_numbers(run, temperatures, uniforms):
