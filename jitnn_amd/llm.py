@@ -225,23 +225,26 @@ class Llm:
     @staticmethod
     def _rope(f: GgufFile, arch: str, head_dim: int, theta: float):
         """The rotary positions that the file asks for, None where they are the plain ones: a part of the head (rope.dimension_count), linear or YaRN scaling
-        (rope.scaling.*), factors of the frequencies (rope_freqs.weight).  Of a kind that is not built: a warning, and the plain ones."""
-        rot = f.integer(f"{arch}.rope.dimension_count", head_dim)
-        kind = f.get(f"{arch}.rope.scaling.type") if f.has(f"{arch}.rope.scaling.type") else "none"
-        factors = f.raw("rope_freqs.weight").view(np.float32) if f.has_tensor("rope_freqs.weight") else None
-        magnitude = f.float_value(f"{arch}.rope.scaling.attn_factor", 0.0)
-        if rot == head_dim and kind == "none" and factors is None and magnitude in (0.0, 1.0):
+        (rope.scaling.*), factors of the frequencies (rope_freqs.weight).  Of a kind that is not built, or of numbers that nothing can turn by: a warning, and the plain ones."""
+        try:
+            rot = f.integer(f"{arch}.rope.dimension_count", head_dim)
+            kind = f.get(f"{arch}.rope.scaling.type") if f.has(f"{arch}.rope.scaling.type") else "none"
+            factors = f.raw("rope_freqs.weight").view(np.float32) if f.has_tensor("rope_freqs.weight") else None
+            magnitude = f.float_value(f"{arch}.rope.scaling.attn_factor", 0.0)
+            if rot == head_dim and kind == "none" and factors is None and magnitude in (0.0, 1.0):
+                return None
+            interleaved = arch in INTERLEAVED_ROPE_ARCHS
+            if kind not in ("none", "linear", "yarn") or rot > head_dim or rot % 2 or (rot < head_dim and not interleaved) or (factors is not None and factors.size != rot // 2):
+                raise ValueError(f"rotary scaling {kind!r} of {rot} of {head_dim} values is not built")
+            factor = f.float_value(f"{arch}.rope.scaling.factor", 1.0) or 1.0
+            if magnitude and kind == "yarn":
+                magnitude *= 0.1 * math.log(factor) + 1.0  # (the file's factor goes on top of the scaling's own)
+            return Rope(rot, theta, interleaved, None if kind == "none" else kind, factor,
+                        f.integer(f"{arch}.rope.scaling.original_context_length", f.integer(f"{arch}.context_length", 2048)),
+                        f.float_value(f"{arch}.rope.scaling.yarn_beta_fast", 32.0), f.float_value(f"{arch}.rope.scaling.yarn_beta_slow", 1.0), magnitude, factors)
+        except ValueError as e:
+            warnings.warn(f"{arch}: the file's rotary positions are not built ({e}); the positions are the plain ones")
             return None
-        interleaved = arch in INTERLEAVED_ROPE_ARCHS
-        if kind not in ("none", "linear", "yarn") or rot > head_dim or rot % 2 or (rot < head_dim and not interleaved) or (factors is not None and factors.size != rot // 2):
-            warnings.warn(f"{arch}: rotary scaling {kind!r} of {rot} of {head_dim} values is not built; the positions are the plain ones")
-            return None
-        factor = f.float_value(f"{arch}.rope.scaling.factor", 1.0) or 1.0
-        if magnitude and kind == "yarn":
-            magnitude *= 0.1 * math.log(factor) + 1.0  # (the file's factor goes on top of the scaling's own)
-        return Rope(rot, theta, interleaved, None if kind == "none" else kind, factor,
-                    f.integer(f"{arch}.rope.scaling.original_context_length", f.integer(f"{arch}.context_length", 2048)),
-                    f.float_value(f"{arch}.rope.scaling.yarn_beta_fast", 32.0), f.float_value(f"{arch}.rope.scaling.yarn_beta_slow", 1.0), magnitude, factors)
 
     def generate(self, prompt, max_new_tokens: int | None = None, on_text=None):
         """generate(prompt, max_new_tokens[, on_text]): the greedy (temperature 0) continuation of `prompt` as a string, at most
