@@ -2544,7 +2544,6 @@ int residual_linear_rows(const jitnn_hip_weight *w, const float *x, int rows, co
     return JITNN_HIP_OK;
 }
 
-// The many-token buffers of a model, for at least `tokens` rows.
 // A buffer that a larger one replaces.
 void release_or_keep(jitnn_hip_llama *m, void *p) {
     if (!p) return;
@@ -2553,6 +2552,7 @@ void release_or_keep(jitnn_hip_llama *m, void *p) {
     else if (!m->recorded) (void)hipFree(p);  // (no memory to note it: left to the process)
 }
 
+// The many-token buffers of a model, for at least `tokens` rows.
 int ensure_prefill(jitnn_hip_llama *m, int tokens) {
     if (tokens <= m->pf_cap) return JITNN_HIP_OK;
     HIP_TRY(hipDeviceSynchronize());  // earlier calls may still use the old buffers
@@ -2738,24 +2738,31 @@ int run_layers(jitnn_hip_llama *m, const float *x_dev, int T, bool defer, hipStr
 
 // cos/sin of t * base^(-2i/D) in double, stored FP32: Rope.tables (core/ops/Rope.java:86-102); other frequencies and a magnitude where the model has
 // been given some.  Pairs behind the rotated part do not turn.
-bool rope_tables(jitnn_hip_llama *m, const jitnn_hip_rope *r) {
+// The tables stay where they are, and change together or not at all: they come to the device aside, and go to their places when both are there.
+int rope_tables(jitnn_hip_llama *m, const jitnn_hip_rope *r) {
     const int half = m->hd / 2;
-    float *c = new (std::nothrow) float[(size_t)m->max_ctx * half], *s = new (std::nothrow) float[(size_t)m->max_ctx * half];
-    bool ok = c && s;
-    if (ok) {
-        for (int t = 0; t < m->max_ctx; ++t)
-            for (int i = 0; i < half; ++i) {
-                const bool turns = i < r->rot / 2;
-                const double angle = turns ? t * r->frequency[i] : 0.0, magnitude = turns ? r->magnitude : 1.0;
-                c[(size_t)t * half + i] = (float)(magnitude * cos(angle));
-                s[(size_t)t * half + i] = (float)(magnitude * sin(angle));
-            }
-        ok = hipMemcpy(m->cosv, c, (size_t)m->max_ctx * half * 4, hipMemcpyHostToDevice) == hipSuccess &&
-             hipMemcpy(m->sinv, s, (size_t)m->max_ctx * half * 4, hipMemcpyHostToDevice) == hipSuccess;
+    const size_t n = (size_t)m->max_ctx * half;
+    float *host = new (std::nothrow) float[2 * n], *aside = nullptr;
+    if (!host) return fail(JITNN_HIP_ENOMEM, "out of host memory");
+    for (int t = 0; t < m->max_ctx; ++t)
+        for (int i = 0; i < half; ++i) {
+            const bool turns = i < r->rot / 2;
+            const double angle = turns ? t * r->frequency[i] : 0.0, magnitude = turns ? r->magnitude : 1.0;
+            host[(size_t)t * half + i] = (float)(magnitude * cos(angle));
+            host[n + (size_t)t * half + i] = (float)(magnitude * sin(angle));
+        }
+    if (hipMalloc(&aside, 2 * n * sizeof(float)) != hipSuccess) {
+        (void)hipGetLastError();
+        delete[] host;
+        return fail(JITNN_HIP_ENOMEM, "no %zu bytes of device memory for the rotary tables", 2 * n * sizeof(float));
     }
-    delete[] c;
-    delete[] s;
-    return ok;
+    hipError_t e = hipMemcpy(aside, host, 2 * n * sizeof(float), hipMemcpyHostToDevice);
+    delete[] host;
+    if (e == hipSuccess) e = hipMemcpy(m->cosv, aside, n * sizeof(float), hipMemcpyDeviceToDevice);
+    if (e == hipSuccess) e = hipMemcpy(m->sinv, aside + n, n * sizeof(float), hipMemcpyDeviceToDevice);
+    if (e == hipSuccess) e = hipDeviceSynchronize();
+    (void)hipFree(aside);
+    return e == hipSuccess ? JITNN_HIP_OK : fail(JITNN_HIP_EDEVICE, "copying the rotary tables: %s", hipGetErrorString(e));
 }
 
 }  // namespace
@@ -2798,7 +2805,7 @@ int jitnn_hip_llama_create(int layers, int d_model, int heads, int kv_heads, int
         m->k = m->q + qd;
         m->v = m->k + kd;
     }
-    ok = ok && rope_build(head_dim, false, (double)rope_theta, nullptr, nullptr, &m->rope) == JITNN_HIP_OK && rope_tables(m, m->rope);
+    ok = ok && rope_build(head_dim, false, (double)rope_theta, nullptr, nullptr, &m->rope) == JITNN_HIP_OK && rope_tables(m, m->rope) == JITNN_HIP_OK;
     if (!ok) {
         jitnn_hip_llama_free(m);
         return fail(JITNN_HIP_ENOMEM, "allocating the model buffers (%zu bytes of KV cache) failed", 2 * cache * sizeof(float));
@@ -3002,9 +3009,9 @@ int jitnn_hip_llama_set_rope(jitnn_hip_llama *m, const jitnn_hip_rope *r) {
         return fail(JITNN_HIP_ENOMEM, "no %zu bytes of device memory for the rotary frequencies", bytes);
     }
     const hipError_t e = hipMemcpy(copy->turns, r->turns, bytes, hipMemcpyDeviceToDevice);
-    if (e != hipSuccess || !rope_tables(m, copy)) {
+    if (const int rc = e == hipSuccess ? rope_tables(m, copy) : fail(JITNN_HIP_EDEVICE, "copying the rotary frequencies: %s", hipGetErrorString(e))) {
         rope_drop(copy);
-        return fail(JITNN_HIP_EDEVICE, "copying the rotary tables: %s", hipGetErrorString(e));
+        return rc;
     }
     rope_drop(m->rope);
     m->rope = copy;
