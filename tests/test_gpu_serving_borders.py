@@ -61,6 +61,29 @@ def test_verify_of_a_refused_draft_that_had_nearly_all_the_weight(jn, vocab):
     assert np.array_equal(got[1], want[1]) and np.array_equal(got[0], want[0]), np.argwhere(got[0] != want[0])
 
 
+@pytest.mark.parametrize("with_q", [False, True])
+@pytest.mark.parametrize("vocab", [700, 30000])
+def test_verify_of_more_rows_than_the_sums_kept(jn, with_q, vocab):
+    """Sequences of 32 and more rows whose first refused draft stands around the 32nd and behind it, or nowhere; greedy ones among them."""
+    rng = np.random.default_rng(vocab)
+    counts, ends = [32, 33, 34, 40, 70, 70, 70, 33, 2, 64, 65], [None, None, 32, 31, 32, 33, 60, 0, None, 62, None]
+    rows, starts = sum(counts), np.concatenate([[0], np.cumsum(counts)])
+    logits, tokens = (2 * rng.standard_normal((rows, vocab))).astype(np.float32), rng.integers(0, vocab, rows)
+    temps = [0.0 if s % 4 == 3 else 0.8 for s in range(len(counts))]
+    q = np.zeros((rows, vocab), dtype=np.float32)
+    for s, (c, end) in enumerate(zip(counts, ends)):
+        for j in range(c - 1):
+            r, x = starts[s] + j, tokens[starts[s] + j + 1]
+            logits[r, x] = 40.0 if j != end else -np.inf
+            q[r] = 0.5 / vocab
+            q[r, x] = 0.5
+    u = rng.random((rows, 2)).astype(np.float32)
+    want = ref.verify(logits, starts, tokens, q if with_q else None, temps, u)
+    assert list(want[1]) == [c - 1 if e is None else e for c, e in zip(counts, ends)]
+    got = served.run_verify(jn, logits, starts, tokens, q if with_q else None, temps, u)
+    assert np.array_equal(got[1], want[1]) and np.array_equal(got[0], want[0])
+
+
 # ---------------------------------------------------------------------------------------------- rotary positions
 
 def turned(theta, rot, divisor, positions):
@@ -93,3 +116,21 @@ def test_rope_at_the_far_end_of_its_positions(jn, theta, rot, factor):
     rope.apply_dev(x.data_ptr(), p.data_ptr(), len(pos), 1, rot, x.data_ptr())
     got = x.double().cpu().numpy()
     assert np.abs(got[:, 0::2] - c).max() <= 2.5 * 2.0 ** -24 and np.abs(got[:, 1::2] - s).max() <= 2.5 * 2.0 ** -24
+
+
+# ---------------------------------------------------------------------------------------------- attention
+
+LONG_BATCHES = [
+    # hd, heads, kv, page, counts, lens, shared: more sequences than a wave has lanes, some of which have no rows, see only a part of what is shared or nothing else
+    (64, 2, 1, 16, [1] * 65, [100 + i for i in range(65)], 4),
+    (64, 4, 2, 32, [1, 2] * 64, [200 + 3 * i if i < 90 else 100 + i for i in range(128)], 5),
+    (128, 4, 1, 16, [0] * 66 + [3] * 70 + [0, 1], [0] * 66 + [250 + i for i in range(70)] + [7, 200], 12),
+    (64, 4, 4, 16, [1] * 200, [1 + (37 * i) % 240 for i in range(200)], 0),
+    (192, 2, 2, 64, [2] * 129, [130 + i for i in range(129)], 2),
+]
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("hd,heads,kv,page,counts,lens,shared", LONG_BATCHES)
+def test_attention_of_long_batches(jn, half, hd, heads, kv, page, counts, lens, shared):
+    served.test_attention(jn, half, hd, heads, kv, page, counts, lens, shared)
