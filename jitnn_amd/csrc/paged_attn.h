@@ -1,7 +1,7 @@
 // Attention of a batch over a paged cache: token t of sequence s, at position p, attends to the positions 0 .. p of s, whose keys and values lie
 // in pages that a table names.  The leading pages may be everybody's: the workgroups that take their positions take the rows - (token, query
 // head) pairs of one key/value head - of the whole batch, so that they are read once and not once per sequence; the other positions go
-// to workgroups of their sequence.  Every workgroup leaves, for its span of keys, the largest score, the sum of the weights and the weighted sum
+// to workgroups of their sequence.  Every workgroup leaves, for its span of keys, what its weights count in, their sum and the weighted sum
 // of the values, and paged_merge_kernel joins a row's spans; where there is one span in all, its workgroups write the outputs.
 //
 // The products run on the matrix cores, transposed, S^T = K Q^T and O^T = V^T P^T, and nothing but the last sums goes through LDS:
@@ -124,7 +124,7 @@ struct PaRows {
     float qs[R];
     f32x4v o[R][E];
     float m[R], l[R];
-    float less[R];       // PA_WEIGHT - m
+    float less[R];       // what scores are less by as exponents of weights: PA_WEIGHT - m, or -m where FP32 does not hold that (scores beyond 2^25)
     float minus;         // -1, which the compiler does not know: it would take the FP16 part off the weight in two instructions and not in one
     u32x4 ph[R], pl[R];  // weights (FP16): slot 4 t + i
     float pf[R][4];      // (FP32)
@@ -272,7 +272,8 @@ struct PaRows {
         asm("v_mov_b32 %0, -1.0" : "=v"(minus));
     }
 
-    // Scores sc[r][t][i] of row n (in units of 1 / qs), key base + 16 t + 4 g + i, to weights 2^(score - m + PA_WEIGHT).  m follows the maximum only when that
+    // Scores sc[r][t][i] of row n (in units of 1 / qs), key base + 16 t + 4 g + i, to weights 2^(score - m + PA_WEIGHT).  PA_WEIGHT - m is exact or does without PA_WEIGHT: rounded by
+    // a few units, as beyond 2^25, it would take weights out of FP16 and other waves' weights apart from these.  m follows the maximum only when that
     // is more than PA_LAG above it: the rescaling of the output, which a wave of 32 rows would need in nearly every step of a short span, is left to the
     // first.
     template <int TILES>
@@ -297,12 +298,13 @@ struct PaRows {
             if constexpr (sizeof(T) == 2) top *= qs[r];
             if (__ballot(top > m[r] + PA_LAG)) {
                 top = fmaxf(m[r], top);
-                const float f = top > -INFINITY ? __builtin_amdgcn_exp2f(m[r] - top) : 1.f;
+                const float full = PA_WEIGHT - top, now = top > -INFINITY ? (full + top == PA_WEIGHT ? full : -top) : 0.f;
+                const float f = m[r] > -INFINITY ? __builtin_amdgcn_exp2f(now - less[r]) : 1.f;
                 l[r] *= f;
 #pragma unroll
                 for (int e = 0; e < E; ++e) o[r][e] *= f;
                 m[r] = top;
-                less[r] = top > -INFINITY ? PA_WEIGHT - top : 0.f;
+                less[r] = now;
             }
 #pragma unroll
             for (int t = 0; t < TILES; ++t)
@@ -372,6 +374,8 @@ struct PaRows {
         }
     }
 
+    // what the weights are of: 2^unit of what a weight of 1 stands for, -inf where there are none
+    __device__ __forceinline__ float unit(const int r) const { return m[r] > -INFINITY ? -less[r] : -INFINITY; }
     // the sum of row n's weights over the four lanes that hold it; NaN for a row that is to be NaN
     __device__ __forceinline__ float total(const int r) const { return over[r] || lim[r] >= badkey ? NAN : pa_sum4(l[r]); }
     __device__ __forceinline__ void spread_badkey() {
@@ -553,7 +557,7 @@ __device__ __forceinline__ void pa_stream(const AttnArgs &a, const AttnPart &par
                 *reinterpret_cast<f32x4v *>(p + E * i + e) = f32x4v{w.o[r][e][i], w.o[r][e + 1][i], w.o[r][e + 2][i], w.o[r][e + 3][i]};
         const float sum = w.total(r);
         if (g == 0) {
-            lm[wave * 16 * R + 16 * r + n] = w.m[r];
+            lm[wave * 16 * R + 16 * r + n] = w.unit(r);
             ll[wave * 16 * R + 16 * r + n] = sum;
         }
     }
@@ -568,7 +572,7 @@ __device__ __forceinline__ void pa_stream(const AttnArgs &a, const AttnPart &par
         for (int j = 0; j < key_waves; ++j) {
             const int src = (wv + row_waves * j) * 16 * R + in;
             const float mm = lm[src], f = mm > -INFINITY ? __builtin_amdgcn_exp2f(mm - top) : 0.f;
-            // (a wave without a key has no weight; one whose rows are to be NaN has, wherever its maximum stands)
+            // (a wave without a key has no weight; one whose rows are to be NaN has, whatever its unit)
             sum += ll[src] == ll[src] ? ll[src] * f : NAN;
             acc += *reinterpret_cast<const f32x4v *>(lo + (size_t)src * (D + 4) + e) * f;
         }
@@ -754,7 +758,7 @@ __device__ __forceinline__ void pa_wide(const AttnArgs &a, const bool ahead, con
                 *reinterpret_cast<f32x4v *>(p + E * i + e) = f32x4v{w.o[r][e][i], w.o[r][e + 1][i], w.o[r][e + 2][i], w.o[r][e + 3][i]} * f;
         const int row_n = w.row0 + 16 * r + n;
         if (slots > 1 && g == 0 && row_n < w.rows) {
-            *reinterpret_cast<float2 *>(a.stat + 2 * (first_slot + (size_t)(16 * r + n) * slots)) = make_float2(w.m[r], sum);
+            *reinterpret_cast<float2 *>(a.stat + 2 * (first_slot + (size_t)(16 * r + n) * slots)) = make_float2(w.unit(r), sum);
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
@@ -822,7 +826,7 @@ __global__ void __launch_bounds__(PA_THREADS, D <= 128 ? 2 : 1) paged_attn_kerne
     }
 }
 
-// ---- y of every row (token, head) from its spans, y = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i with m the largest m_i: bound by the latency of a chain (the
+// ---- y of every row (token, head) from its spans, y = sum_i 2^(u_i - u) o_i / sum_i 2^(u_i - u) l_i with u_i the units of their weights (PaRows::unit) and u the largest: bound by the latency of a chain (the
 // token's sequence, the statistics, the sums) where rows are few, 4 us, and by memory where they are many.  Spans that begin behind the row's position were not written.
 constexpr int PA_MERGE = 256;
 

@@ -134,3 +134,33 @@ LONG_BATCHES = [
 @pytest.mark.parametrize("hd,heads,kv,page,counts,lens,shared", LONG_BATCHES)
 def test_attention_of_long_batches(jn, half, hd, heads, kv, page, counts, lens, shared):
     served.test_attention(jn, half, hd, heads, kv, page, counts, lens, shared)
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("rise", [2, 4, 8, 16])
+@pytest.mark.parametrize("top", [23, 24, 25, 26, 27, 28])
+def test_attention_of_scores_far_beyond_what_weights_hold(jn, half, rise, top):
+    """Scores of 2^top and `rise` above it (to the base 2, all of them exact), the lower ones first: the higher key has 2^rise of the weight of a lower one, and no finite input makes a NaN.
+    Where FP32 has no room for the rise the scores are equal."""
+    rng = np.random.default_rng(top)
+    hd, heads, kv, page, n = 64, 2, 1, 16, 700
+    b = ref.Batch(rng, [1, 1], [n, n - 100], page)
+    keys, values = np.zeros((n, hd), dtype=np.float32), rng.standard_normal((n, hd)).astype(np.float32).astype(np.float16).astype(np.float32)
+    keys[:, 0] = 1024
+    keys[n // 2:, 1] = 1
+    kind = torch.float16 if half else torch.float32
+    pools = [torch.zeros(1, b.pages, kv, page, hd, device="cuda", dtype=kind) for _ in range(2)]
+    for s in range(2):
+        for p in range(b.lens[s]):
+            for pool, rows in zip(pools, (keys, values)):
+                pool[0, int(b.tables[s, p // page]), 0, p % page] = torch.from_numpy(rows[p]).to(kind)
+    q = torch.zeros(2, heads, hd, device="cuda")
+    q[:, :, 0], q[:, :, 1] = 2.0 ** (top - 10), rise
+    got = served.run_attention(jn, b, q, pools, half, float(np.log(2.0))).double().cpu().numpy()
+    scores = (np.float32(2.0 ** top) + np.float32(rise) * keys[:, 1]).astype(np.float32).astype(np.float64)
+    for s in range(2):
+        z = scores[:b.lens[s]]
+        w = np.exp2(z - z.max())
+        want = (w / w.sum()) @ values[:b.lens[s]].astype(np.float64)
+        # (weights to 2^-21, up to 700 terms added)
+        assert np.abs(got[s] - want).max() <= (2.0 ** -20 + 64 * 2.0 ** -24) * np.abs(values).max()
