@@ -296,7 +296,7 @@ struct PaRows {
                 for (int i = 0; i < 4; ++i) top = fmaxf(top, sc[r][t][i]);
             top = pa_max4(top);
             if constexpr (sizeof(T) == 2) top *= qs[r];
-            if (__ballot(top > m[r] + PA_LAG)) {
+            if (__ballot(top - m[r] > PA_LAG)) {  // (the difference of neighbours is exact, a sum beyond 2^24 is not)
                 top = fmaxf(m[r], top);
                 const float full = PA_WEIGHT - top, now = top > -INFINITY ? (full + top == PA_WEIGHT ? full : -top) : 0.f;
                 const float f = m[r] > -INFINITY ? __builtin_amdgcn_exp2f(now - less[r]) : 1.f;

@@ -137,16 +137,15 @@ def test_attention_of_long_batches(jn, half, hd, heads, kv, page, counts, lens, 
 
 
 @pytest.mark.parametrize("half", [False, True])
-@pytest.mark.parametrize("rise", [2, 4, 8, 16])
-@pytest.mark.parametrize("top", [23, 24, 25, 26, 27, 28])
-def test_attention_of_scores_far_beyond_what_weights_hold(jn, half, rise, top):
-    """Scores of 2^top and `rise` above it (to the base 2, all of them exact), the lower ones first: the higher key has 2^rise of the weight of a lower one, and no finite input makes a NaN.
-    Where FP32 has no room for the rise the scores are equal."""
+@pytest.mark.parametrize("top,rise,odd", [(top, rise, odd) for top in range(23, 29) for rise in (2, 4, 8, 16, 32, 64) for odd in (0, 1) if not odd or rise >= 2 ** (top - 23)])
+def test_attention_of_scores_far_beyond_what_weights_hold(jn, half, top, rise, odd):
+    """Scores of 2^top, or one step of FP32 above it, and `rise` above that (to the base 2), the lower ones first: the higher key has 2^rise of the weight of a lower one, and no finite
+    input makes a NaN.  Where FP32 has no room for the rise the scores are equal."""
     rng = np.random.default_rng(top)
     hd, heads, kv, page, n = 64, 2, 1, 16, 700
     b = ref.Batch(rng, [1, 1], [n, n - 100], page)
     keys, values = np.zeros((n, hd), dtype=np.float32), rng.standard_normal((n, hd)).astype(np.float32).astype(np.float16).astype(np.float32)
-    keys[:, 0] = 1024
+    keys[:, 0], keys[:, 2] = 1024, 1
     keys[n // 2:, 1] = 1
     kind = torch.float16 if half else torch.float32
     pools = [torch.zeros(1, b.pages, kv, page, hd, device="cuda", dtype=kind) for _ in range(2)]
@@ -155,9 +154,10 @@ def test_attention_of_scores_far_beyond_what_weights_hold(jn, half, rise, top):
             for pool, rows in zip(pools, (keys, values)):
                 pool[0, int(b.tables[s, p // page]), 0, p % page] = torch.from_numpy(rows[p]).to(kind)
     q = torch.zeros(2, heads, hd, device="cuda")
-    q[:, :, 0], q[:, :, 1] = 2.0 ** (top - 10), rise
+    q[:, :, 0], q[:, :, 1], q[:, :, 2] = 2.0 ** (top - 10), rise, odd * 2.0 ** (top - 23)
     got = served.run_attention(jn, b, q, pools, half, float(np.log(2.0))).double().cpu().numpy()
-    scores = (np.float32(2.0 ** top) + np.float32(rise) * keys[:, 1]).astype(np.float32).astype(np.float64)
+    base = np.float32(2.0 ** top + odd * 2.0 ** (top - 23))
+    scores = (base + np.float32(rise) * keys[:, 1]).astype(np.float32).astype(np.float64)
     for s in range(2):
         z = scores[:b.lens[s]]
         w = np.exp2(z - z.max())
