@@ -316,7 +316,7 @@ JITNN_HIP_API int jitnn_hip_paged_append_dev(const jitnn_hip_paged_cache *c, int
                                              const float *v_dev, long long v_stride, void *stream);
 
 /* y [tokens, heads, head_dim] = softmax(scale q K^T) V over the positions up to the row's own, query head h reading key/value head h / (heads / kv_heads)
- * (F.scaledDotProductAttentionBTHD with F.repeatHeads, core/F.java:588-624).  FP32-grade with both cache types.  Keys and values that a row sees must be
+ * (F.scaledDotProductAttentionBTHD with F.repeatHeads, core/F.java:588-624).  FP32-grade with both cache types (F16: each weight within 2^-22 of itself or 2^-36 of the largest).  Keys and values that a row sees must be
  * finite (a row that sees others is not); what it does not see - later tokens, the rest of a page - may hold anything.  A row whose scores are all
  * -inf is zero.  The workspace is device memory of at least jitnn_hip_paged_attention_workspace bytes (0 where it returns 0; 16-byte aligned), used until the work has run: calls that may
  * overlap in time, recorded graphs among them, need one each.  Allocates nothing; may be recorded. */

@@ -14,9 +14,9 @@
 //   positions, 32 heads of 128 in FP16: 148 MB in 34.6 us, one launch (4.3 TB/s).  Where the rows fill several waves, each wave's own stream of the same keys
 //   is what bounds: there the waves share them through LDS (pa_wide).  64 sequences behind 16384 shared positions, 32 heads over 8: 126 us with streams
 //   alone, 59 so, and the merge 7: the matrix cores at 1.04 PFLOP/s over the shared part, two parts of every product counted.
-// FP16 pages: keys and values are operands as they are; queries (scaled so that a row's largest is near 2^13) and weights (times 2^6 to 2^14) go in two FP16
-// parts, 22 bits together, so that the result is as good as in FP32 (one part of 11 bits would leave 2^-12 of every weight).  FP32 pages: the FP32
-// matrix instruction, an eighth of the rate; 24 sequences of up to 5 rows behind 992 shared positions, 35 us and the merge 6.7.
+// FP16 pages: keys and values are operands as they are; queries (scaled so that a row's largest is near 2^13) and weights (the largest 2^11 to 2^16) go in two FP16
+// parts: each within 2^-22 of itself, or 2^-36 of the largest where that is more.  The result is as good as in FP32 but for keys of less weight than 2^-14, which may be off by 2^-36 each
+// (one part of 11 bits would leave 2^-12 of every weight).  FP32 pages: the FP32 matrix instruction, an eighth of the rate; 24 sequences of up to 5 rows behind 992 shared positions, 35 us and the merge 6.7.
 // Sums, maxima and outputs are FP32.
 //
 // What a row does not see: its scores are masked; values past the last key that any row of the tile sees are cleared, and of those that only some see
@@ -24,6 +24,7 @@
 // lie on a page that the cache does not have.
 #pragma once
 #include <algorithm>
+#include <cfloat>
 #include <type_traits>
 
 #include "common.h"
@@ -32,7 +33,9 @@
 namespace jitnn {
 
 constexpr int PA_THREADS = 256, PA_WAVES = 4;
-constexpr float PA_WEIGHT = 6.f, PA_LAG = 8.f;  // weights are 2^(score - m + 6), m at most 8 below the maximum: up to 2^14, inside FP16
+// A row's largest weight is 2^11.5 to 2^15.5 (and 1/4 in the exponent): inside FP16, whose steps of 2^-24 at the lower end are then 2^-35 of it at most.  (At 2^6 to 2^14 they were 2^-30, and
+// 16384 keys of 2^-31 each off by a quarter of their sum, 2.6e-6.)
+constexpr float PA_WEIGHT = 11.5f, PA_LAG = 4.f;
 
 typedef float f32x4v __attribute__((ext_vector_type(4)));
 typedef float f32x4v_a4 __attribute__((ext_vector_type(4), aligned(4)));  // (rows of y start anywhere)
@@ -123,8 +126,8 @@ struct PaRows {
     f32x4v qf[R][D / 16];  // (FP16: until they are operands)
     float qs[R];
     f32x4v o[R][E];
-    float m[R], l[R];
-    float less[R];       // what scores are less by as exponents of weights: PA_WEIGHT - m, or -m where FP32 does not hold that (scores beyond 2^25)
+    float l[R];
+    float less[R];       // a weight is 2^(score + less): PA_WEIGHT minus about the largest score so far, FLT_MAX before the first
     float minus;         // -1, which the compiler does not know: it would take the FP16 part off the weight in two instructions and not in one
     u32x4 ph[R], pl[R];  // weights (FP16): slot 4 t + i
     float pf[R][4];      // (FP32)
@@ -264,18 +267,18 @@ struct PaRows {
                         ql[r][s][j] = (_Float16)(y - (float)qh[r][s][j]);
                     }
             }
-            m[r] = -INFINITY;
-            l[r] = less[r] = 0.f;
+            less[r] = FLT_MAX;
+            l[r] = 0.f;
 #pragma unroll
             for (int e = 0; e < E; ++e) o[r][e] = f32x4v{0.f, 0.f, 0.f, 0.f};
         }
         asm("v_mov_b32 %0, -1.0" : "=v"(minus));
     }
 
-    // Scores sc[r][t][i] of row n (in units of 1 / qs), key base + 16 t + 4 g + i, to weights 2^(score - m + PA_WEIGHT).  PA_WEIGHT - m is exact or does without PA_WEIGHT: rounded by
-    // a few units, as beyond 2^25, it would take weights out of FP16 and other waves' weights apart from these.  m follows the maximum only when that
-    // is more than PA_LAG above it: the rescaling of the output, which a wave of 32 rows would need in nearly every step of a short span, is left to the
-    // first.
+    // Scores sc[r][t][i] of row n (in units of 1 / qs), key base + 16 t + 4 g + i, to weights 2^(score + less).  Only where the largest would be above 2^(PA_WEIGHT + PA_LAG) does less
+    // follow the scores: the rescaling of the output, which a wave of 32 rows would need in nearly every step of a short span, is left to the
+    // first.  It need not be PA_WEIGHT minus the maximum to the bit, only the same for all of a row's weights here and, as their unit, for whoever joins them with others; where FP32 cannot hold
+    // it within 1/4 (scores beyond 2^23), it does without PA_WEIGHT.
     template <int TILES>
     __device__ __forceinline__ void weigh(f32x4v (&sc)[R][TILES], const int base, const bool partial) {
         const int g = (threadIdx.x & 63) >> 4;
@@ -296,14 +299,12 @@ struct PaRows {
                 for (int i = 0; i < 4; ++i) top = fmaxf(top, sc[r][t][i]);
             top = pa_max4(top);
             if constexpr (sizeof(T) == 2) top *= qs[r];
-            if (__ballot(top - m[r] > PA_LAG)) {  // (the difference of neighbours is exact, a sum beyond 2^24 is not)
-                top = fmaxf(m[r], top);
-                const float full = PA_WEIGHT - top, now = top > -INFINITY ? (full + top == PA_WEIGHT ? full : -top) : 0.f;
-                const float f = m[r] > -INFINITY ? __builtin_amdgcn_exp2f(now - less[r]) : 1.f;
+            if (__ballot(top + less[r] > PA_WEIGHT + PA_LAG)) {
+                const float full = PA_WEIGHT - top, now = fminf(less[r], fabsf(full + top - PA_WEIGHT) <= 0.25f ? full : -top);
+                const float f = __builtin_amdgcn_exp2f(now - less[r]);
                 l[r] *= f;
 #pragma unroll
                 for (int e = 0; e < E; ++e) o[r][e] *= f;
-                m[r] = top;
                 less[r] = now;
             }
 #pragma unroll
@@ -374,8 +375,8 @@ struct PaRows {
         }
     }
 
-    // what the weights are of: 2^unit of what a weight of 1 stands for, -inf where there are none
-    __device__ __forceinline__ float unit(const int r) const { return m[r] > -INFINITY ? -less[r] : -INFINITY; }
+    // the score of a weight of 1; -inf where there are no weights
+    __device__ __forceinline__ float unit(const int r) const { return less[r] < FLT_MAX ? -less[r] : -INFINITY; }
     // the sum of row n's weights over the four lanes that hold it; NaN for a row that is to be NaN
     __device__ __forceinline__ float total(const int r) const { return over[r] || lim[r] >= badkey ? NAN : pa_sum4(l[r]); }
     __device__ __forceinline__ void spread_badkey() {

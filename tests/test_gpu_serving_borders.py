@@ -164,3 +164,28 @@ def test_attention_of_scores_far_beyond_what_weights_hold(jn, half, top, rise, o
         want = (w / w.sum()) @ values[:b.lens[s]].astype(np.float64)
         # (weights to 2^-21, up to 700 terms added)
         assert np.abs(got[s] - want).max() <= (2.0 ** -20 + 64 * 2.0 ** -24) * np.abs(values).max()
+
+
+@pytest.mark.parametrize("shift", [0.0, -7.0703125, 5.5625, -1000.5, 900.25])
+def test_attention_of_many_keys_far_below_one(jn, shift):
+    """FP16 pages, rows enough that spans are long: one key with all but 1e-5 of the weight in front of thousands that have 6e-10 of it each, which are the whole output.  Weights are held to
+    2^-36 of the largest at least, and all of them off the same way at worst: 2^-36 a key; sums and scores 2^-12 of the result.  All scores
+    are `shift` higher."""
+    hd, heads, page, shared, n = 64, 64, 256, 64, 512
+    long = shared * page
+    rng = np.random.default_rng(0)
+    b = ref.Batch(rng, [1] * n, [long + 1] * n, page, shared)
+    low = -21.203125
+    keys, values = torch.zeros(1, b.pages, 1, page, hd, device="cuda").half(), torch.zeros(1, b.pages, 1, page, hd, device="cuda").half()
+    keys[..., 0], keys[..., 1], values[..., :] = low, shift, 1.0
+    first = int(b.tables[0, 0])
+    keys[0, first, 0, 0, 0], values[0, first, 0, 0] = 0.0, 0.0
+    q = torch.zeros(n, heads, hd, device="cuda")
+    q[..., :2] = 1.0
+    nb, keep = served.batch_of(jn, b)
+    cache = jn.PagedCache.wrap_dev(keys.data_ptr(), values.data_ptr(), 1, 1, hd, b.pages, page, 1)
+    assert cache.attention_workspace(nb, heads) <= n * heads * 6 * (hd + 2) * 4  # (a few spans)
+    got = served.run_attention(jn, b, q, [keys, values], True, 1.0).double()
+    w = np.exp(low)
+    want = long * w / (1 + long * w)
+    assert (got - want).abs().max().item() <= long * 2.0 ** -36 + want * 2.0 ** -12
