@@ -85,3 +85,18 @@ def test_a_sequence_on_a_bad_page_reaches_no_other(jn, model_file, counts):
         others = [r for r in range(b.tokens) if r not in bad]
         assert torch.isnan(out[1][bad]).all() and torch.isfinite(out[0]).all()
         assert norm_err(out[1][others].cpu().numpy(), out[0][others].cpu().numpy()) <= TWICE[b.tokens > 64]
+
+
+@pytest.mark.parametrize("length", [512, 513, 700])
+def test_a_prompt_of_several_passes(jn, model_file, monkeypatch, length):
+    """As many rows a pass as the default, and 16 of them: the same logits of the token after it, and of one more of each sequence (few-row linears on one side, many-row ones on the other)."""
+    rng = np.random.default_rng(length)
+    with jn.Llm.load(model_file) as llm:
+        dec, vocab = llm.model(), llm.info().vocab
+        prompt = [int(t) for t in rng.integers(0, vocab, length)]
+        out = []
+        for rows in (jn.SharedPrompt.PROMPT_ROWS, 16):
+            monkeypatch.setattr(jn.SharedPrompt, "PROMPT_ROWS", rows)
+            run = jn.SharedPrompt(dec, prompt, 3, length + 20, page_tokens=32, ggml_type=0)
+            out.append((run.prompt_logits, run.step([0, 1, 2], [[5], [6], [7]])))
+        assert norm_err(out[0][0], out[1][0]) <= TWICE[True] and norm_err(out[0][1], out[1][1]) <= TWICE[True]
