@@ -100,3 +100,35 @@ def test_a_prompt_of_several_passes(jn, model_file, monkeypatch, length):
             run = jn.SharedPrompt(dec, prompt, 3, length + 20, page_tokens=32, ggml_type=0)
             out.append((run.prompt_logits, run.step([0, 1, 2], [[5], [6], [7]])))
         assert norm_err(out[0][0], out[1][0]) <= TWICE[True] and norm_err(out[0][1], out[1][1]) <= TWICE[True]
+
+
+@pytest.mark.parametrize("sequences", [4, 16, 90])
+def test_a_pass_recorded_on_another_stream_than_it_ran_on(jn, model_file, sequences):
+    """Run on the default stream, recorded on a stream of its own, replayed there, with eager passes on the default stream in between: every replay against an eager pass."""
+    rng = np.random.default_rng(sequences)
+    with jn.Llm.load(model_file) as llm:
+        dec, vocab = llm.model(), llm.info().vocab
+        b = ref.Batch(rng, [1] * sequences, [9 + i % 30 for i in range(sequences)], 16, max_len=48)
+        pool = [torch.randn(2, b.pages, 2, 16, 64, device="cuda") for _ in range(2)]
+        cache = jn.PagedCache.wrap_dev(pool[0].data_ptr(), pool[1].data_ptr(), 2, 2, 64, b.pages, 16, 0)
+        keep = [torch.from_numpy(a).cuda() for a in (b.tables, b.starts, np.array(b.lens, dtype=np.int32), np.arange(sequences, dtype=np.int32))]
+        nb = jn.Batch(sequences, sequences, 1, 48, keep[0].data_ptr(), b.width, keep[1].data_ptr(), keep[2].data_ptr())
+        x, y, z = torch.randn(sequences, 256, device="cuda"), torch.empty(sequences, vocab, device="cuda"), torch.empty(sequences, vocab, device="cuda")
+
+        def step(out):
+            dec.step_dev(cache, nb, x.data_ptr(), keep[3].data_ptr(), sequences, out.data_ptr(), torch.cuda.current_stream().cuda_stream)
+
+        step(z)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step(y)
+        for _ in range(4):
+            x.normal_()
+            y.fill_(float("nan"))
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            step(z)
+            torch.cuda.synchronize()
+            assert torch.equal(y, z) and torch.isfinite(y).all()
