@@ -189,3 +189,69 @@ def test_attention_of_many_keys_far_below_one(jn, shift):
     w = np.exp(low)
     want = long * w / (1 + long * w)
     assert (got - want).abs().max().item() <= long * 2.0 ** -36 + want * 2.0 ** -12
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("hd,heads,kv,counts,shared", [(64, 8, 2, [1] * 40, 6), (128, 8, 1, [3, 1, 30, 2], 4), (256, 4, 2, [2] * 9, 5), (128, 4, 4, [1, 1, 1], 0)])
+def test_attention_beside_queries_that_are_not_numbers(jn, half, hd, heads, kv, counts, shared):
+    """NaN, infinities and the largest finite number in some rows' queries: every other row is what it is beside ordinary ones, to the bit."""
+    rng = np.random.default_rng(hd)
+    page = 32
+    b = ref.Batch(rng, counts, [shared * page + 40 + 11 * i for i in range(len(counts))], page, shared)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    pools = [torch.randn(1, b.pages, kv, page, hd, device="cuda", generator=g).to(torch.float16 if half else torch.float32) for _ in range(2)]
+    q = torch.randn(b.tokens, heads, hd, device="cuda", generator=g)
+    want = served.run_attention(jn, b, q, pools, half, 0.1)
+    odd = sorted(set(int(t) for t in rng.integers(0, b.tokens, max(1, b.tokens // 6))))
+    for value in (float("nan"), float("inf"), float("-inf"), torch.finfo(torch.float32).max):
+        other = q.clone()
+        other[odd, :, ::3] = value
+        got = served.run_attention(jn, b, other, pools, half, 0.1)
+        rest = [r for r in range(b.tokens) if r not in odd]
+        assert torch.equal(got[rest], want[rest])
+        assert np.isfinite(value) or torch.isnan(got[odd]).all()
+
+
+def test_two_batches_at_once(jn):
+    """Append, attention and verification of two batches on two streams, each with its own cache and workspaces, beside one another: what each gives alone."""
+    rng = np.random.default_rng(7)
+    runs = []
+    for hd, heads, kv, counts, lens, shared in ((128, 32, 8, [1] * 30, [700 + i for i in range(30)], 8), (64, 8, 2, [90, 3], [500, 40], 1)):
+        b = ref.Batch(rng, counts, lens, 32, shared)
+        pools = [torch.randn(1, b.pages, kv, 32, hd, device="cuda").half() for _ in range(2)]
+        cache = jn.PagedCache.wrap_dev(pools[0].data_ptr(), pools[1].data_ptr(), 1, kv, hd, b.pages, 32, 1)
+        nb, keep = served.batch_of(jn, b)
+        rows, vocab = b.tokens, 20000
+        qkv, q, y = torch.randn(rows, heads + 2 * kv, hd, device="cuda"), torch.empty(rows, heads, hd, device="cuda"), torch.empty(rows, heads, hd, device="cuda")
+        ws = torch.empty(cache.attention_workspace(nb, heads) // 4 + 4, device="cuda")
+        vs = torch.empty(jn.verify_workspace(rows, len(counts), vocab) // 4 + 4, device="cuda")
+        logits, tokens = torch.randn(rows, vocab, device="cuda") * 3, torch.randint(0, vocab, (rows,), device="cuda", dtype=torch.int32)
+        temps, numbers = torch.ones(len(counts), device="cuda"), torch.rand(rows, 2, device="cuda")
+        out, accepted = torch.empty(rows, device="cuda", dtype=torch.int32), torch.empty(len(counts), device="cuda", dtype=torch.int32)
+        rope, row = jn.Rope(hd), (heads + 2 * kv) * hd
+
+        def run(stream, cache=cache, nb=nb, keep=keep, pools=pools, heads=heads, kv=kv, hd=hd, rows=rows, qkv=qkv, q=q, y=y, ws=ws, vs=vs, logits=logits, tokens=tokens, temps=temps,
+                numbers=numbers, out=out, accepted=accepted, rope=rope, row=row, vocab=vocab, n=len(counts)):
+            st = stream.cuda_stream
+            cache.append_dev(0, nb, rope, heads, qkv.data_ptr(), q.data_ptr(), qkv.data_ptr() + 4 * heads * hd, qkv.data_ptr() + 4 * (heads + kv) * hd, row, 0, row, row, st)
+            cache.attention_dev(0, nb, heads, q.data_ptr(), 0.1, y.data_ptr(), ws.data_ptr(), 4 * ws.numel(), stream_ptr=st)
+            jn.verify_drafts_dev(logits.data_ptr(), rows, vocab, keep[1].data_ptr(), n, tokens.data_ptr(), temps.data_ptr(), numbers.data_ptr(), out.data_ptr(), accepted.data_ptr(),
+                                 vs.data_ptr(), 4 * vs.numel(), stream_ptr=st)
+
+        runs.append((run, (y, out, accepted)))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    alone = []
+    for (run, outs), stream in zip(runs, streams):
+        run(stream)
+        torch.cuda.synchronize()
+        alone.append([o.clone() for o in outs])
+    for _ in range(10):
+        for o in [o for _, outs in runs for o in outs]:
+            o.zero_()
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for (run, _), stream in zip(runs, streams):
+                run(stream)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, o) for (_, outs), was in zip(runs, alone) for a, o in zip(was, outs))
