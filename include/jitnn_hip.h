@@ -320,7 +320,7 @@ JITNN_HIP_API int jitnn_hip_paged_append_dev(const jitnn_hip_paged_cache *c, int
  * finite (a row that sees others is not); what it does not see - later tokens, the rest of a page - may hold anything.  A row whose scores are all
  * -inf is zero.  The workspace is device memory of at least jitnn_hip_paged_attention_workspace bytes (0 where it returns 0; 16-byte aligned), used until the work has run: calls that may
  * overlap in time, recorded graphs among them, need one each.  Allocates nothing; may be recorded.  Passes whose tokens x heads reach 2^24, or whose
- * sequences x kv_heads and spans pass 2^22 workgroups, are refused (JITNN_HIP_EINVAL). */
+ * sequences x kv_heads and spans pass 2^22 workgroups, may be refused (JITNN_HIP_EINVAL). */
 JITNN_HIP_API long long jitnn_hip_paged_attention_workspace(const jitnn_hip_paged_cache *c, const jitnn_hip_batch *batch, int heads);
 JITNN_HIP_API int jitnn_hip_paged_attention_dev(const jitnn_hip_paged_cache *c, int layer, const jitnn_hip_batch *batch, int heads, const float *q_dev,
                                                 long long q_stride, float scale, float *y_dev, long long y_stride, void *workspace_dev, long long workspace_bytes,
