@@ -344,6 +344,51 @@ JITNN_HIP_API int jitnn_hip_verify_drafts_dev(const float *logits_dev, long long
                                               const int *tokens_dev, const float *draft_probs_dev, long long draft_stride, const float *temperatures_dev,
                                               const float *uniforms_dev, int *out_dev, int *accepted_dev, void *workspace_dev, long long workspace_bytes, void *stream);
 
+/* ---- mixtures of experts ------------------------------------------------------------------------- */
+
+/* The activations of a feed-forward layer: max(v, 0); v / (1 + exp(-v)); v times the normal distribution's integral up to v; its approximation by tanh
+ * (Hendrycks, Gimpel, "Gaussian Error Linear Units", 2016). */
+#define JITNN_HIP_ACT_NONE 0
+#define JITNN_HIP_ACT_RELU 1
+#define JITNN_HIP_ACT_SILU 2
+#define JITNN_HIP_ACT_GELU 3
+#define JITNN_HIP_ACT_GELU_TANH 4
+
+/* The router of a layer of experts (Shazeer et al., "Outrageously Large Neural Networks: The Sparsely-Gated Mixture-of-Experts Layer", 2017), which the
+ * reference does not have: l = x W^T, p = softmax(l) over all experts or sigmoid(l), the `used` experts with the largest l - with a selection bias, the
+ * largest p + bias - and their weights scale * p, normalise: divided by the sum of those chosen.  Sums and p in FP64, the same choice whatever the order of
+ * a sum; ties go to the lowest index, logits that are not numbers come last.  Weights [experts, d_model] and bias [experts] are copied from host memory;
+ * immutable afterwards and usable by any number of threads.  experts at most 512, used at most 64, d_model a multiple of 4. */
+typedef struct jitnn_hip_router jitnn_hip_router;
+#define JITNN_HIP_GATING_SOFTMAX 0
+#define JITNN_HIP_GATING_SIGMOID 1
+JITNN_HIP_API int jitnn_hip_router_create(int experts, int d_model, int used, int gating, int normalise, float scale, const float *weights_host,
+                                          const float *selection_bias_host, jitnn_hip_router **out);
+JITNN_HIP_API int jitnn_hip_router_free(jitnn_hip_router *r);
+/* ids and weights [tokens, used] of x [tokens, d_model], in the order of choice.  tokens 0: nothing is done.  x 16-byte aligned.  Workspace as for the attention over pages:
+ * device memory of at least jitnn_hip_router_workspace bytes (0 where it returns 0; 16-byte aligned), used until the work has run: calls that may overlap in time,
+ * recorded graphs among them, need one each. */
+JITNN_HIP_API long long jitnn_hip_router_workspace(const jitnn_hip_router *r, int tokens);
+JITNN_HIP_API int jitnn_hip_router_dev(const jitnn_hip_router *r, const float *x_dev, int tokens, int *ids_dev, float *weights_dev, void *workspace_dev,
+                                       long long workspace_bytes, void *stream);
+
+/* A layer of experts on quantised weights as GGUF files hold them, one expert after the other: gate and up [experts * ffn, d_model], down [experts * d_model,
+ * ffn] (formats may differ; router and weights are not owned).
+ *   y = residual (or 0) + the sum over a token's experts e of weight_e * down_e (act(gate_e x) * (up_e x))
+ * jitnn_hip_moe_dev routes x [tokens, d_model] itself; jitnn_hip_moe_experts_dev takes ids and weights [tokens, used] that exist: an id outside [0, experts)
+ * counts for nothing, one that stands twice counts twice.  FP32-grade at any number of tokens (error ~1e-6).  x must be finite where it meets an expert: a
+ * token with values that are not gives a row that is not.  y may be x or the residual; tokens 0: nothing is done.  x, residual and y 16-byte aligned.  Workspace as
+ * above (long calls go through the experts in passes of 4096 / used tokens: it does not grow beyond those).  Allocates nothing; may be recorded. */
+typedef struct jitnn_hip_moe jitnn_hip_moe;
+JITNN_HIP_API int jitnn_hip_moe_create(const jitnn_hip_router *router, const jitnn_hip_weight *gate, const jitnn_hip_weight *up, const jitnn_hip_weight *down,
+                                       int activation, jitnn_hip_moe **out);
+JITNN_HIP_API int jitnn_hip_moe_free(jitnn_hip_moe *m);
+JITNN_HIP_API long long jitnn_hip_moe_workspace(const jitnn_hip_moe *m, int tokens);
+JITNN_HIP_API int jitnn_hip_moe_dev(const jitnn_hip_moe *m, const float *x_dev, int tokens, const float *residual_dev, float *y_dev, void *workspace_dev,
+                                    long long workspace_bytes, void *stream);
+JITNN_HIP_API int jitnn_hip_moe_experts_dev(const jitnn_hip_moe *m, const float *x_dev, int tokens, const int *ids_dev, const float *weights_dev,
+                                            const float *residual_dev, float *y_dev, void *workspace_dev, long long workspace_bytes, void *stream);
+
 /* ---- Llama-style decode step on quantised weights --------------------------------------------- */
 
 /* The reference has no quantised Llama and no KV-cache operator; the step is the composition of its operators as

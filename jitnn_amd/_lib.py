@@ -117,6 +117,15 @@ def _bind() -> C.CDLL:
         "jitnn_hip_paged_attention_dev": (i, [vp, i, batch, i, vp, ll, C.c_float, vp, ll, vp, ll, vp]),
         "jitnn_hip_verify_workspace": (ll, [i, i, i]),
         "jitnn_hip_verify_drafts_dev": (i, [vp, ll, i, i, vp, i, vp, vp, ll, vp, vp, vp, vp, vp, ll, vp]),
+        "jitnn_hip_router_create": (i, [i, i, i, i, i, C.c_float, fp, fp, C.POINTER(vp)]),
+        "jitnn_hip_router_free": (i, [vp]),
+        "jitnn_hip_router_workspace": (ll, [vp, i]),
+        "jitnn_hip_router_dev": (i, [vp, vp, i, vp, vp, vp, ll, vp]),
+        "jitnn_hip_moe_create": (i, [vp, vp, vp, vp, i, C.POINTER(vp)]),
+        "jitnn_hip_moe_free": (i, [vp]),
+        "jitnn_hip_moe_workspace": (ll, [vp, i]),
+        "jitnn_hip_moe_dev": (i, [vp, vp, i, vp, vp, vp, ll, vp]),
+        "jitnn_hip_moe_experts_dev": (i, [vp, vp, i, vp, vp, vp, vp, vp, ll, vp]),
         "jitnn_hip_llama_set_rope": (i, [vp, vp]),
         "jitnn_hip_llama_step_dev": (i, [vp, vp, batch, vp, vp, i, vp, vp]),
     }

@@ -1,0 +1,95 @@
+// The experts' products for any block format, the gate and the weighted sum of a token's experts.
+#include "experts.h"
+
+#include <algorithm>
+
+#include "act.h"
+#include "dequant.h"
+
+namespace jitnn {
+
+// One wave per weight row of the slot's expert, every lane dequantises quads of the row.  grid (ceil(n / 4), slots up to 65535, and so on along z).
+template <int FMT>
+__global__ void __launch_bounds__(256) experts_value_kernel(const ExpertWeights w, int experts, const int *__restrict__ ids, int slots, int per_row, const float *__restrict__ x,
+                                                             float *__restrict__ y) {
+    const int lane = threadIdx.x & 63, row = (int)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const long long slot = (long long)blockIdx.z * 65535 + blockIdx.y;
+    if (slot >= slots || row >= w.n) return;
+    const int e = ids[slot];
+    if ((unsigned)e >= (unsigned)experts) return;
+    const uint8_t *wr = w.w + (size_t)e * w.expert_bytes + (size_t)row * ((size_t)(w.k / block_values(FMT)) * block_bytes(FMT));
+    const float *xr = x + (size_t)(slot / per_row) * w.k;
+    float acc = 0.f;
+    for (int f = lane; f < (w.k >> 2); f += 64) {
+        const float4 v = dequant4<FMT>(wr, (size_t)f * 4), xv = reinterpret_cast<const float4 *>(xr)[f];
+        acc = __builtin_fmaf(v.w, xv.w, __builtin_fmaf(v.z, xv.z, __builtin_fmaf(v.y, xv.y, __builtin_fmaf(v.x, xv.x, acc))));
+    }
+    acc = wave_sum(acc);
+    if (lane == 0) y[(size_t)slot * w.n + row] = acc;
+}
+
+template <int FMT>
+static void value(const ExpertWeights &w, int experts, const int *ids, int slots, int per_row, const float *x, float *y, hipStream_t s) {
+    const dim3 grid((w.n + 3) / 4, std::min(slots, 65535), (slots + 65534) / 65535);
+    hipLaunchKernelGGL(experts_value_kernel<FMT>, grid, dim3(256), 0, s, w, experts, ids, slots, per_row, x, y);
+}
+
+void experts_value_launch(const ExpertWeights &w, int experts, const int *ids, int slots, int per_row, const float *x, float *y, hipStream_t s) {
+    switch (w.fmt) {
+    case F_Q4_0: value<F_Q4_0>(w, experts, ids, slots, per_row, x, y, s); break;
+    case F_Q4_1: value<F_Q4_1>(w, experts, ids, slots, per_row, x, y, s); break;
+    case F_Q8_0: value<F_Q8_0>(w, experts, ids, slots, per_row, x, y, s); break;
+    case F_Q4_K: value<F_Q4_K>(w, experts, ids, slots, per_row, x, y, s); break;
+    case F_Q5_K: value<F_Q5_K>(w, experts, ids, slots, per_row, x, y, s); break;
+    case F_Q6_K: value<F_Q6_K>(w, experts, ids, slots, per_row, x, y, s); break;
+    case F_Q5_0: value<F_Q5_0>(w, experts, ids, slots, per_row, x, y, s); break;
+    case F_Q5_1: value<F_Q5_1>(w, experts, ids, slots, per_row, x, y, s); break;
+    case F_Q2_K: value<F_Q2_K>(w, experts, ids, slots, per_row, x, y, s); break;
+    case F_Q3_K: value<F_Q3_K>(w, experts, ids, slots, per_row, x, y, s); break;
+    }
+}
+
+static __global__ void __launch_bounds__(256) experts_gate_kernel(int act, const float *g, const float *__restrict__ u, float *h, size_t count4, unsigned stride) {
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < count4; i += stride) {
+        float4 v = reinterpret_cast<const float4 *>(g)[i];
+        const float4 m = reinterpret_cast<const float4 *>(u)[i];
+        v = make_float4(activate(act, v.x) * m.x, activate(act, v.y) * m.y, activate(act, v.z) * m.z, activate(act, v.w) * m.w);
+        reinterpret_cast<float4 *>(h)[i] = v;
+    }
+}
+
+void experts_gate_launch(int act, const float *g, const float *u, float *h, size_t count, int cus, hipStream_t s) {
+    const size_t count4 = count / 4;
+    const unsigned blocks = (unsigned)std::min<size_t>((count4 + 255) / 256, (size_t)cus * 8);
+    hipLaunchKernelGGL(experts_gate_kernel, dim3(blocks), dim3(256), 0, s, act, g, u, h, count4, blocks * 256);
+}
+
+// grid (ceil(n / 1024), tokens), 256 threads, four values each.  (res may be y)
+static __global__ void __launch_bounds__(256) experts_combine_kernel(const float *__restrict__ part, const int *__restrict__ ids, const float *__restrict__ weights, const float *res,
+                                                                     float *y, int used, int experts, int n) {
+    const int t = (int)blockIdx.y, i = ((int)blockIdx.x * 256 + (int)threadIdx.x) * 4;
+    if (i >= n) return;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int j = 0; j < used; ++j) {
+        const size_t slot = (size_t)t * used + j;
+        if ((unsigned)ids[slot] >= (unsigned)experts) continue;
+        const float w = weights[slot];
+        const float4 p = *reinterpret_cast<const float4 *>(part + slot * n + i);
+        sum.x = __builtin_fmaf(w, p.x, sum.x);
+        sum.y = __builtin_fmaf(w, p.y, sum.y);
+        sum.z = __builtin_fmaf(w, p.z, sum.z);
+        sum.w = __builtin_fmaf(w, p.w, sum.w);
+    }
+    if (res) {
+        const float4 r = *reinterpret_cast<const float4 *>(res + (size_t)t * n + i);
+        sum = make_float4(sum.x + r.x, sum.y + r.y, sum.z + r.z, sum.w + r.w);
+    }
+    *reinterpret_cast<float4 *>(y + (size_t)t * n + i) = sum;
+}
+
+void experts_combine_launch(const float *part, const int *ids, const float *weights, const float *res, float *y, int tokens, int used, int experts, int n, int,
+                            hipStream_t s) {
+    hipLaunchKernelGGL(experts_combine_kernel, dim3((n + 1023) / 1024, tokens), dim3(256), 0, s, part, ids, weights, res, y, used, experts, n);
+}
+
+}  // namespace jitnn

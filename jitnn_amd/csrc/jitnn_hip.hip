@@ -24,6 +24,7 @@
 #include "attn_packed.h"
 #include "attn_split.h"
 #include "dequant.h"
+#include "experts.h"
 #include "gemv.h"
 #include "gemv_mfma.h"
 #include "gemv_tail.h"
@@ -2316,6 +2317,233 @@ int jitnn_hip_verify_drafts_dev(const float *logits_dev, long long logits_stride
     a.chunks = 0;
     verify_launch(a, (hipStream_t)stream);
     HIP_TRY(hipGetLastError());
+    return JITNN_HIP_OK;
+}
+
+}  // extern "C"
+
+// ================================================================================================ mixtures of experts
+
+struct jitnn_hip_router {
+    int experts, d, used;
+    bool sigmoid, normalise;
+    float scale;
+    float *w = nullptr, *bias = nullptr;  // [experts, d], [experts] (one allocation)
+};
+
+struct jitnn_hip_moe {
+    const jitnn_hip_router *router;
+    const jitnn_hip_weight *gate, *up, *down;
+    int act, ffn;
+};
+
+namespace {
+
+constexpr int ROUTER_PASS = 8192;  // tokens of a pass of the router alone
+constexpr int MOE_PASS_SLOTS = 4096;  // places (tokens x used) of a pass through the experts
+
+size_t pad256(size_t b) { return (b + 255) & ~(size_t)255; }
+
+int moe_pass_tokens(const jitnn_hip_moe *m) { return std::max(1, MOE_PASS_SLOTS / m->router->used); }
+
+// What a pass of `tokens` keeps in the workspace, in bytes from its start.
+struct MoeLayout {
+    size_t logits, ids, weights, g, u, part, total;
+};
+MoeLayout moe_layout(const jitnn_hip_moe *m, int tokens) {
+    const jitnn_hip_router *r = m->router;
+    const size_t slots = (size_t)tokens * r->used;
+    MoeLayout l{};
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        const size_t here = at;
+        at += pad256(bytes);
+        return here;
+    };
+    l.logits = take((size_t)tokens * r->experts * sizeof(double));
+    l.ids = take(slots * sizeof(int));
+    l.weights = take(slots * sizeof(float));
+    l.g = take(slots * m->ffn * sizeof(float));
+    l.u = take(slots * m->ffn * sizeof(float));
+    l.part = take(slots * r->d * sizeof(float));
+    l.total = at;
+    return l;
+}
+
+RouterArgs router_args(const jitnn_hip_router *r, const float *x, int tokens, int *ids, float *weights, void *logits) {
+    RouterArgs a{};
+    a.x = x;
+    a.w = r->w;
+    a.bias = r->bias;
+    a.logits = (double *)logits;
+    a.ids = ids;
+    a.weights = weights;
+    a.tokens = tokens;
+    a.experts = r->experts;
+    a.d = r->d;
+    a.used = r->used;
+    a.sigmoid = r->sigmoid;
+    a.normalise = r->normalise;
+    a.scale = r->scale;
+    return a;
+}
+
+ExpertWeights expert_weights(const jitnn_hip_weight *w, int experts) {
+    return {w->fmt, w->n / experts, w->k, w->dev, (size_t)(w->n / experts) * (size_t)(w->k / block_values(w->fmt)) * block_bytes(w->fmt)};
+}
+
+int check_moe_call(const jitnn_hip_moe *m, const float *x, int tokens, const float *res, const float *y, const void *ws, long long ws_bytes) {
+    if (!m) return fail(JITNN_HIP_EINVAL, "the layer is NULL");
+    if (tokens < 0) return fail(JITNN_HIP_EINVAL, "tokens = %d", tokens);
+    if (tokens == 0) return JITNN_HIP_OK;
+    if (!x || !y) return fail(JITNN_HIP_EINVAL, "input or output is NULL");
+    if ((((uintptr_t)x | (uintptr_t)y | (uintptr_t)res) & 15) != 0) return fail(JITNN_HIP_EINVAL, "input, residual and output must be 16-byte aligned");
+    const long long need = jitnn_hip_moe_workspace(m, tokens);
+    if (need < 0) return (int)need;
+    if (!ws || ((uintptr_t)ws & 15) != 0 || ws_bytes < need) return fail(JITNN_HIP_EINVAL, "workspace of %lld bytes, 16-byte aligned, needed; got %lld", need, ws ? ws_bytes : 0);
+    return check_ready();
+}
+
+// One pass: the experts of `tokens` tokens for given choices.
+int moe_experts(const jitnn_hip_moe *m, const float *x, int tokens, const int *ids, const float *weights, const float *res, float *y, uint8_t *ws, const MoeLayout &l,
+                hipStream_t s) {
+    const jitnn_hip_router *r = m->router;
+    const int slots = tokens * r->used;
+    float *gb = (float *)(ws + l.g), *ub = (float *)(ws + l.u), *part = (float *)(ws + l.part);
+    experts_value_launch(expert_weights(m->gate, r->experts), r->experts, ids, slots, r->used, x, gb, s);
+    experts_value_launch(expert_weights(m->up, r->experts), r->experts, ids, slots, r->used, x, ub, s);
+    experts_gate_launch(m->act, gb, ub, gb, (size_t)slots * m->ffn, g.cus, s);
+    experts_value_launch(expert_weights(m->down, r->experts), r->experts, ids, slots, 1, gb, part, s);
+    experts_combine_launch(part, ids, weights, res, y, tokens, r->used, r->experts, r->d, g.cus, s);
+    HIP_TRY(hipGetLastError());
+    return JITNN_HIP_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int jitnn_hip_router_create(int experts, int d_model, int used, int gating, int normalise, float scale, const float *weights_host, const float *selection_bias_host,
+                            jitnn_hip_router **out) {
+    if (!out) return fail(JITNN_HIP_EINVAL, "out is NULL");
+    *out = nullptr;
+    if (experts < 1 || experts > MAX_EXPERTS) return fail(JITNN_HIP_EINVAL, "%d experts (1 to %d)", experts, MAX_EXPERTS);
+    if (used < 1 || used > experts || used > MAX_USED) return fail(JITNN_HIP_EINVAL, "%d of %d experts (at most %d)", used, experts, MAX_USED);
+    if (d_model < 4 || d_model % 4 != 0) return fail(JITNN_HIP_EINVAL, "d_model %d (a multiple of 4)", d_model);
+    if (gating != JITNN_HIP_GATING_SOFTMAX && gating != JITNN_HIP_GATING_SIGMOID) return fail(JITNN_HIP_EINVAL, "gating %d", gating);
+    if (!std::isfinite(scale)) return fail(JITNN_HIP_EINVAL, "scale %g", (double)scale);
+    if (!weights_host) return fail(JITNN_HIP_EINVAL, "weights are NULL");
+    if (int rc = check_ready()) return rc;
+    jitnn_hip_router *r = new (std::nothrow) jitnn_hip_router{experts, d_model, used, gating == JITNN_HIP_GATING_SIGMOID, normalise != 0, scale};
+    if (!r) return fail(JITNN_HIP_ENOMEM, "out of host memory");
+    const size_t count = (size_t)experts * d_model, bytes = (count + experts) * sizeof(float);
+    if (hipMalloc(&r->w, bytes) != hipSuccess) {
+        (void)hipGetLastError();
+        delete r;
+        return fail(JITNN_HIP_ENOMEM, "no %zu bytes of device memory for the router", bytes);
+    }
+    hipError_t e = hipMemcpy(r->w, weights_host, count * sizeof(float), hipMemcpyHostToDevice);
+    if (e == hipSuccess && selection_bias_host) {
+        r->bias = r->w + count;
+        e = hipMemcpy(r->bias, selection_bias_host, (size_t)experts * sizeof(float), hipMemcpyHostToDevice);
+    }
+    if (e != hipSuccess) {
+        (void)hipFree(r->w);
+        delete r;
+        return fail(JITNN_HIP_EDEVICE, "copying the router: %s", hipGetErrorString(e));
+    }
+    *out = r;
+    return JITNN_HIP_OK;
+}
+
+int jitnn_hip_router_free(jitnn_hip_router *r) {
+    if (!r) return JITNN_HIP_OK;
+    (void)hipFree(r->w);
+    delete r;
+    return JITNN_HIP_OK;
+}
+
+long long jitnn_hip_router_workspace(const jitnn_hip_router *r, int tokens) {
+    if (!r) return fail(JITNN_HIP_EINVAL, "the router is NULL");
+    if (tokens < 0) return fail(JITNN_HIP_EINVAL, "tokens = %d", tokens);
+    long long most = 0;  // (a shorter last pass may need what a longer one does not)
+    for (const int t : {std::min(tokens, ROUTER_PASS), tokens % ROUTER_PASS})
+        if (t && router_needs_logits(t, r->experts, r->d, false)) most = std::max(most, (long long)t * r->experts * (long long)sizeof(double));
+    return most;
+}
+
+int jitnn_hip_router_dev(const jitnn_hip_router *r, const float *x_dev, int tokens, int *ids_dev, float *weights_dev, void *workspace_dev, long long workspace_bytes,
+                         void *stream) {
+    if (!r) return fail(JITNN_HIP_EINVAL, "the router is NULL");
+    if (tokens < 0) return fail(JITNN_HIP_EINVAL, "tokens = %d", tokens);
+    if (tokens == 0) return JITNN_HIP_OK;
+    if (!x_dev || !ids_dev || !weights_dev) return fail(JITNN_HIP_EINVAL, "input or output is NULL");
+    if (((uintptr_t)x_dev & 15) != 0) return fail(JITNN_HIP_EINVAL, "the input must be 16-byte aligned");
+    const long long need = jitnn_hip_router_workspace(r, tokens);
+    if (need > 0 && (!workspace_dev || ((uintptr_t)workspace_dev & 15) != 0 || workspace_bytes < need))
+        return fail(JITNN_HIP_EINVAL, "workspace of %lld bytes, 16-byte aligned, needed; got %lld", need, workspace_dev ? workspace_bytes : 0);
+    if (int rc = check_ready()) return rc;
+    for (int t = 0; t < tokens; t += ROUTER_PASS)
+        router_launch(router_args(r, x_dev + (size_t)t * r->d, std::min(ROUTER_PASS, tokens - t), ids_dev + (size_t)t * r->used, weights_dev + (size_t)t * r->used, workspace_dev),
+                      (hipStream_t)stream);
+    HIP_TRY(hipGetLastError());
+    return JITNN_HIP_OK;
+}
+
+int jitnn_hip_moe_create(const jitnn_hip_router *router, const jitnn_hip_weight *gate, const jitnn_hip_weight *up, const jitnn_hip_weight *down, int activation,
+                         jitnn_hip_moe **out) {
+    if (!out) return fail(JITNN_HIP_EINVAL, "out is NULL");
+    *out = nullptr;
+    if (!router || !gate || !up || !down) return fail(JITNN_HIP_EINVAL, "router or weight is NULL");
+    if (activation < 0 || activation >= ACT_COUNT) return fail(JITNN_HIP_EINVAL, "activation %d", activation);
+    const int e = router->experts, d = router->d, ffn = down->k;
+    if (gate->k != d || up->k != d || (long long)e * ffn != gate->n || gate->n != up->n || (long long)e * d != down->n)
+        return fail(JITNN_HIP_EINVAL, "experts of shapes gate [%d, %d], up [%d, %d], down [%d, %d] for a router of %d experts on %d values", gate->n, gate->k, up->n, up->k, down->n,
+                    down->k, e, d);
+    jitnn_hip_moe *m = new (std::nothrow) jitnn_hip_moe{router, gate, up, down, activation, ffn};
+    if (!m) return fail(JITNN_HIP_ENOMEM, "out of host memory");
+    *out = m;
+    return JITNN_HIP_OK;
+}
+
+int jitnn_hip_moe_free(jitnn_hip_moe *m) {
+    delete m;
+    return JITNN_HIP_OK;
+}
+
+long long jitnn_hip_moe_workspace(const jitnn_hip_moe *m, int tokens) {
+    if (!m) return fail(JITNN_HIP_EINVAL, "the layer is NULL");
+    if (tokens < 0) return fail(JITNN_HIP_EINVAL, "tokens = %d", tokens);
+    return tokens == 0 ? 0 : (long long)moe_layout(m, std::min(tokens, moe_pass_tokens(m))).total;
+}
+
+int jitnn_hip_moe_dev(const jitnn_hip_moe *m, const float *x_dev, int tokens, const float *residual_dev, float *y_dev, void *workspace_dev, long long workspace_bytes, void *stream) {
+    if (int rc = check_moe_call(m, x_dev, tokens, residual_dev, y_dev, workspace_dev, workspace_bytes)) return rc;
+    const int pass = moe_pass_tokens(m);
+    uint8_t *ws = (uint8_t *)workspace_dev;
+    for (int t = 0; t < tokens; t += pass) {
+        const int count = std::min(pass, tokens - t), d = m->router->d;
+        const MoeLayout l = moe_layout(m, count);
+        const float *x = x_dev + (size_t)t * d;
+        router_launch(router_args(m->router, x, count, (int *)(ws + l.ids), (float *)(ws + l.weights), ws + l.logits), (hipStream_t)stream);
+        if (int rc = moe_experts(m, x, count, (const int *)(ws + l.ids), (const float *)(ws + l.weights), residual_dev ? residual_dev + (size_t)t * d : nullptr, y_dev + (size_t)t * d,
+                                 ws, l, (hipStream_t)stream))
+            return rc;
+    }
+    return JITNN_HIP_OK;
+}
+
+int jitnn_hip_moe_experts_dev(const jitnn_hip_moe *m, const float *x_dev, int tokens, const int *ids_dev, const float *weights_dev, const float *residual_dev, float *y_dev,
+                              void *workspace_dev, long long workspace_bytes, void *stream) {
+    if (int rc = check_moe_call(m, x_dev, tokens, residual_dev, y_dev, workspace_dev, workspace_bytes)) return rc;
+    if (tokens > 0 && (!ids_dev || !weights_dev)) return fail(JITNN_HIP_EINVAL, "ids or weights are NULL");
+    const int pass = moe_pass_tokens(m);
+    for (int t = 0; t < tokens; t += pass) {
+        const int count = std::min(pass, tokens - t), d = m->router->d, used = m->router->used;
+        if (int rc = moe_experts(m, x_dev + (size_t)t * d, count, ids_dev + (size_t)t * used, weights_dev + (size_t)t * used,
+                                 residual_dev ? residual_dev + (size_t)t * d : nullptr, y_dev + (size_t)t * d, (uint8_t *)workspace_dev, moe_layout(m, count), (hipStream_t)stream))
+            return rc;
+    }
     return JITNN_HIP_OK;
 }
 

@@ -57,6 +57,18 @@ class Tensor:
                    "jitnn_hip_weight_upload")
         return Tensor(dims, dtype, handle=h)
 
+    @staticmethod
+    def wrap_dev(dtype: DType, ptr: int, *dims) -> "Tensor":
+        """The same around blocks that are in device memory already, at address ptr (16-byte aligned); the caller keeps them alive."""
+        if not dtype.is_block_quantized() or len(dims) == 0 or dims[-1] % dtype.block_values() != 0:
+            raise ValueError(f"no {dtype.name} weight of shape {list(dims)}")
+        n, k = int(np.prod(dims[:-1], dtype=np.int64)), int(dims[-1])
+        _lib.init()
+        h = C.c_void_p()
+        _lib.check(_lib.lib.jitnn_hip_weight_wrap_dev(dtype.ggml_id, ptr or None, n * k // dtype.block_values() * dtype.block_bytes(), n, k, C.byref(h)),
+                   "jitnn_hip_weight_wrap_dev")
+        return Tensor(dims, dtype, handle=h)
+
     # ---- accessors
     def dtype(self) -> DType:
         return self._dtype
