@@ -156,6 +156,21 @@ JITNN_HIP_API int jitnn_hip_linear_noalloc_dev(const jitnn_hip_weight *w, const 
                                                void *stream);
 JITNN_HIP_API long long jitnn_hip_noalloc_scratch_bytes(void);
 
+/* The activations of a feed-forward layer: max(v, 0); v / (1 + exp(-v)); v times the normal distribution's integral up to v; its approximation by tanh
+ * (Hendrycks, Gimpel, "Gaussian Error Linear Units", 2016). */
+#define JITNN_HIP_ACT_NONE 0
+#define JITNN_HIP_ACT_RELU 1
+#define JITNN_HIP_ACT_SILU 2
+#define JITNN_HIP_ACT_GELU 3
+#define JITNN_HIP_ACT_GELU_TANH 4
+
+/* y = act(x W^T (+ bias)) (+ residual [rows, n]): jitnn_hip_linear with an epilogue, which the reference runs as operators of their own (core/F.java:1159-1161).
+ * Accuracy, routes and scratch are those of jitnn_hip_linear; bias and residual may be NULL, residual and y may not overlap. */
+JITNN_HIP_API int jitnn_hip_linear_act(const jitnn_hip_weight *w, const float *x_host, int rows, const float *bias_host, int activation, const float *residual_host,
+                                       float *y_host);
+JITNN_HIP_API int jitnn_hip_linear_act_dev(const jitnn_hip_weight *w, const float *x_dev, int rows, const float *bias_dev, int activation,
+                                           const float *residual_dev, float *y_dev, void *stream);
+
 /* Which of the two kernels above a launch of more than 64 rows takes: 0 the one that decodes as it goes, otherwise the
  * weight rows of a tile (256, 192 or 128) of the one that multiplies weights dequantised before it.  `count` (up to three)
  * weights [n[i], k] on one activation, as the model steps launch q, k and v; gate_up: two weights whose product is formed as
@@ -345,14 +360,6 @@ JITNN_HIP_API int jitnn_hip_verify_drafts_dev(const float *logits_dev, long long
                                               const float *uniforms_dev, int *out_dev, int *accepted_dev, void *workspace_dev, long long workspace_bytes, void *stream);
 
 /* ---- mixtures of experts ------------------------------------------------------------------------- */
-
-/* The activations of a feed-forward layer: max(v, 0); v / (1 + exp(-v)); v times the normal distribution's integral up to v; its approximation by tanh
- * (Hendrycks, Gimpel, "Gaussian Error Linear Units", 2016). */
-#define JITNN_HIP_ACT_NONE 0
-#define JITNN_HIP_ACT_RELU 1
-#define JITNN_HIP_ACT_SILU 2
-#define JITNN_HIP_ACT_GELU 3
-#define JITNN_HIP_ACT_GELU_TANH 4
 
 /* The router of a layer of experts (Shazeer et al., "Outrageously Large Neural Networks: The Sparsely-Gated Mixture-of-Experts Layer", 2017), which the
  * reference does not have: l = x W^T, p = softmax(l) over all experts or sigmoid(l), the `used` experts with the largest l - with a selection bias, the

@@ -6,7 +6,7 @@ benchmark.  Importing it requires the built library.
 """
 from ._lib import JitnnError, device_info, init, stats, stats_reset  # noqa: F401
 from .dtype import DType  # noqa: F401
-from .ops import F, Gguf, Quant  # noqa: F401
+from .ops import F, Gguf, Quant, linear_dev  # noqa: F401
 from .tensor import Tensor  # noqa: F401
 from .llama import LlamaDecoder  # noqa: F401
 from .gguf_file import GgufFile, GgufTensorInfo  # noqa: F401

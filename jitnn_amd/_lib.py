@@ -64,6 +64,8 @@ def _bind() -> C.CDLL:
         "jitnn_hip_dequantize_dev": (i, [vp, vp, vp]),
         "jitnn_hip_linear": (i, [vp, vp, i, vp, vp]),
         "jitnn_hip_linear_dev": (i, [vp, vp, i, vp, vp, vp]),
+        "jitnn_hip_linear_act": (i, [vp, vp, i, vp, i, vp, vp]),
+        "jitnn_hip_linear_act_dev": (i, [vp, vp, i, vp, i, vp, vp, vp]),
         "jitnn_hip_linear_noalloc_dev": (i, [vp, vp, i, vp, vp, vp]),
         "jitnn_hip_noalloc_scratch_bytes": (ll, []),
         "jitnn_hip_many_row_tile": (i, [C.POINTER(i), C.POINTER(i), i, i, i, i, i, i]),
@@ -164,6 +166,16 @@ def init(device: int = 0) -> None:
     if not _initialised:
         check(lib.jitnn_hip_init(device), "jitnn_hip_init")
         _initialised = True
+
+
+ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
+
+
+def activation_id(name) -> int:
+    """JITNN_HIP_ACT_* of an activation's name."""
+    if name not in ACTIVATIONS:
+        raise ValueError(f"activation {name!r} (None, 'relu', 'silu', 'gelu' and 'gelu_tanh' are built)")
+    return ACTIVATIONS[name]
 
 
 def device_info() -> dict:

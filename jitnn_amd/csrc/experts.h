@@ -44,4 +44,7 @@ void experts_gate_launch(int act, const float *g, const float *u, float *h, size
 void experts_combine_launch(const float *part, const int *ids, const float *weights, const float *res, float *y, int tokens, int used, int experts, int n, int cus,
                             hipStream_t s);
 
+// ---- the epilogue of a linear, where its kernel has none: y [count] = act(y) + res (or 0)
+void linear_epilogue_launch(int act, const float *res, float *y, size_t count, int cus, hipStream_t s);
+
 }  // namespace jitnn

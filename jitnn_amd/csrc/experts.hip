@@ -92,4 +92,17 @@ void experts_combine_launch(const float *part, const int *ids, const float *weig
     hipLaunchKernelGGL(experts_combine_kernel, dim3((n + 1023) / 1024, tokens), dim3(256), 0, s, part, ids, weights, res, y, used, experts, n);
 }
 
+// (any alignment: outputs and residuals of linears need none)
+static __global__ void __launch_bounds__(256) linear_epilogue_kernel(int act, const float *__restrict__ res, float *__restrict__ y, size_t count, unsigned stride) {
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < count; i += stride) {
+        const float v = activate(act, y[i]);
+        y[i] = res ? v + res[i] : v;
+    }
+}
+
+void linear_epilogue_launch(int act, const float *res, float *y, size_t count, int cus, hipStream_t s) {
+    const unsigned blocks = (unsigned)std::min<size_t>((count + 255) / 256, (size_t)cus * 16);
+    hipLaunchKernelGGL(linear_epilogue_kernel, dim3(blocks), dim3(256), 0, s, act, res, y, count, blocks * 256);
+}
+
 }  // namespace jitnn

@@ -1609,12 +1609,33 @@ int linear_dev(const jitnn_hip_weight *w, const float *x_dev, int rows, const fl
     return JITNN_HIP_OK;
 }
 
+// What an epilogue adds to the checks of a linear (which come after these): y apart from the residual, which a launch may read after another has written y.
+int check_linear_act(const jitnn_hip_weight *w, int rows, int activation, const float *residual, const float *y) {
+    if (activation < 0 || activation >= ACT_COUNT) return fail(JITNN_HIP_EINVAL, "activation %d", activation);
+    if (w && rows > 0 && residual && y) {
+        const size_t bytes = (size_t)rows * w->n * sizeof(float);
+        if ((uintptr_t)residual < (uintptr_t)y + bytes && (uintptr_t)y < (uintptr_t)residual + bytes) return fail(JITNN_HIP_EINVAL, "the output overlaps the residual");
+    }
+    return JITNN_HIP_OK;
+}
+
 }  // namespace
 
 extern "C" {
 
 int jitnn_hip_linear_dev(const jitnn_hip_weight *w, const float *x_dev, int rows, const float *bias_dev, float *y_dev, void *stream) {
     return linear_dev(w, x_dev, rows, bias_dev, y_dev, (hipStream_t)stream, SCRATCH_THREAD);
+}
+
+int jitnn_hip_linear_act_dev(const jitnn_hip_weight *w, const float *x_dev, int rows, const float *bias_dev, int activation, const float *residual_dev, float *y_dev, void *stream) {
+    if (int rc = check_linear_act(w, rows, activation, residual_dev, y_dev)) return rc;
+    hipStream_t s = (hipStream_t)stream;
+    if (int rc = linear_dev(w, x_dev, rows, bias_dev, y_dev, s, SCRATCH_THREAD)) return rc;
+    if (activation != JITNN_HIP_ACT_NONE || residual_dev) {
+        linear_epilogue_launch(activation, residual_dev, y_dev, (size_t)rows * w->n, g.cus, s);
+        HIP_TRY(hipGetLastError());
+    }
+    return JITNN_HIP_OK;
 }
 
 int jitnn_hip_linear_noalloc_dev(const jitnn_hip_weight *w, const float *x_dev, int rows, const float *bias_dev, float *y_dev, void *stream) {
@@ -1649,15 +1670,26 @@ int jitnn_hip_few_rows_slices(int fmt, int n, int k, int rows, int adds, int com
     return rows_path(&w, rows) ? rows_plan(&w, rows, adds != 0, compute_units).slices : 0;
 }
 
+static int linear_host(const jitnn_hip_weight *w, const float *x_host, int rows, const float *bias_host, int activation, const float *residual_host, float *y_host);
+
 long long jitnn_hip_noalloc_scratch_bytes(void) { return (long long)JITNN_HIP_SCRATCH_BYTES; }
 
 int jitnn_hip_linear(const jitnn_hip_weight *w, const float *x_host, int rows, const float *bias_host, float *y_host) {
+    return linear_host(w, x_host, rows, bias_host, JITNN_HIP_ACT_NONE, nullptr, y_host);
+}
+
+int jitnn_hip_linear_act(const jitnn_hip_weight *w, const float *x_host, int rows, const float *bias_host, int activation, const float *residual_host, float *y_host) {
+    if (int rc = check_linear_act(w, rows, activation, nullptr, nullptr)) return rc;
+    return linear_host(w, x_host, rows, bias_host, activation, residual_host, y_host);
+}
+
+static int linear_host(const jitnn_hip_weight *w, const float *x_host, int rows, const float *bias_host, int activation, const float *residual_host, float *y_host) {
     if (!w || !x_host || !y_host) return fail(JITNN_HIP_EINVAL, "weight, input or output is NULL");
     if (rows < 1) return fail(JITNN_HIP_EINVAL, "rows = %d", rows);
     if (int rc = check_ready()) return rc;
-    // layout of both staging buffers: [x | bias | y], x and bias going up in one copy, y coming back in one
-    const size_t xb = (size_t)rows * w->k * 4, yb = (size_t)rows * w->n * 4, bb = bias_host ? (size_t)w->n * 4 : 0;
-    const size_t bo = (xb + 255) & ~(size_t)255, yo = bo + ((bb + 255) & ~(size_t)255), total = yo + yb;
+    // layout of both staging buffers: [x | bias | residual | y], x, bias and residual going up in one copy, y coming back in one
+    const size_t xb = (size_t)rows * w->k * 4, yb = (size_t)rows * w->n * 4, bb = bias_host ? (size_t)w->n * 4 : 0, rb = residual_host ? yb : 0;
+    const size_t bo = (xb + 255) & ~(size_t)255, ro = bo + ((bb + 255) & ~(size_t)255), yo = ro + ((rb + 255) & ~(size_t)255), total = yo + yb;
     const bool keep = total <= STAGE_KEEP_MAX;  // small calls go through pinned memory (one DMA each way, no page locking per call)
     if (int rc = stage_reserve(keep ? total : 0, total)) return rc;
     HostStage &st = g_thread.stage;
@@ -1671,14 +1703,17 @@ int jitnn_hip_linear(const jitnn_hip_weight *w, const float *x_host, int rows, c
     if (keep) {
         memcpy(st.pinned, x_host, xb);
         if (bias_host) memcpy(st.pinned + bo, bias_host, bb);
-        const size_t up = bias_host ? bo + bb : xb;
+        if (residual_host) memcpy(st.pinned + ro, residual_host, rb);
+        const size_t up = residual_host ? ro + rb : bias_host ? bo + bb : xb;
         if (by_kernel) copy16(st.dev, st.pinned_dev, up);
         else HIP_TRY(hipMemcpyAsync(st.dev, st.pinned, up, hipMemcpyHostToDevice, st.stream));
     } else {
         HIP_TRY(hipMemcpyAsync(st.dev, x_host, xb, hipMemcpyHostToDevice, st.stream));
         if (bias_host) HIP_TRY(hipMemcpyAsync(st.dev + bo, bias_host, bb, hipMemcpyHostToDevice, st.stream));
+        if (residual_host) HIP_TRY(hipMemcpyAsync(st.dev + ro, residual_host, rb, hipMemcpyHostToDevice, st.stream));
     }
-    int rc = jitnn_hip_linear_dev(w, (const float *)st.dev, rows, bias_host ? (const float *)(st.dev + bo) : nullptr, (float *)(st.dev + yo), st.stream);
+    int rc = jitnn_hip_linear_act_dev(w, (const float *)st.dev, rows, bias_host ? (const float *)(st.dev + bo) : nullptr, activation,
+                                      residual_host ? (const float *)(st.dev + ro) : nullptr, (float *)(st.dev + yo), st.stream);
     if (rc == JITNN_HIP_OK) {
         if (by_kernel) {
             copy16(st.pinned_dev + yo, st.dev + yo, yb);

@@ -13,13 +13,6 @@ from .serving import DeviceArray
 from .tensor import Tensor
 
 GATINGS = {"softmax": 0, "sigmoid": 1}
-ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
-
-
-def activation_id(name) -> int:
-    if name not in ACTIVATIONS:
-        raise ValueError(f"activation {name!r} (None, 'relu', 'silu', 'gelu' and 'gelu_tanh' are built)")
-    return ACTIVATIONS[name]
 
 
 def _bytes(n: int, what: str) -> int:
@@ -82,7 +75,7 @@ class Moe:
         if gate.shape() != up.shape() or gate.dim(2) != d or down.dim(1) != d or down.dim(2) != gate.dim(1):
             raise ValueError(f"experts of shapes {list(gate.shape())}, {list(up.shape())}, {list(down.shape())} on {d} values")
         h = C.c_void_p()
-        _lib.check(_lib.lib.jitnn_hip_moe_create(router.handle, gate.handle, up.handle, down.handle, activation_id(activation), C.byref(h)), "jitnn_hip_moe_create")
+        _lib.check(_lib.lib.jitnn_hip_moe_create(router.handle, gate.handle, up.handle, down.handle, _lib.activation_id(activation), C.byref(h)), "jitnn_hip_moe_create")
         self.router, self.d_model, self.ffn, self._keep, self._h = router, d, gate.dim(1), (gate, up, down), h
         weakref.finalize(self, _lib.lib.jitnn_hip_moe_free, h)
 

@@ -18,7 +18,7 @@ def _f32(x: Tensor, what: str) -> None:
         raise ValueError(f"{what} needs an FP32 input, got {x.dtype().name}")
 
 
-def _linear(x: Tensor, w: Tensor, bias: Tensor | None, what: str) -> Tensor:
+def _linear(x: Tensor, w: Tensor, bias: Tensor | None, what: str, activation: str | None = None, residual: Tensor | None = None) -> Tensor:
     if w.rank() != 2 or x.rank() < 1 or x.dim(-1) != w.dim(1):
         raise ValueError(f"{what}: input {list(x.shape())} and weight {list(w.shape())}")
     n, k = w.dim(0), w.dim(1)
@@ -27,14 +27,27 @@ def _linear(x: Tensor, w: Tensor, bias: Tensor | None, what: str) -> Tensor:
         _f32(bias, what)
         if bias.numel() != n:
             raise ValueError(f"{what}: bias {list(bias.shape())} for {n} outputs")
+    act = _lib.activation_id(activation)
+    if residual is not None:
+        _f32(residual, what)
+        if residual.shape() != x.shape()[:-1] + (n,):
+            raise ValueError(f"{what}: residual {list(residual.shape())} for an output {list(x.shape()[:-1] + (n,))}")
     xa = np.ascontiguousarray(x.numpy(), dtype=np.float32)
     ba = None if bias is None else np.ascontiguousarray(bias.numpy(), dtype=np.float32)
     y = np.empty(x.shape()[:-1] + (n,), dtype=np.float32)
     if rows > 0:
-        _lib.check(_lib.lib.jitnn_hip_linear(w.handle, xa.ctypes.data_as(C.c_void_p), rows,
-                                             None if ba is None else ba.ctypes.data_as(C.c_void_p), y.ctypes.data_as(C.c_void_p)),
-                   "jitnn_hip_linear")
+        ra = None if residual is None else np.ascontiguousarray(residual.numpy(), dtype=np.float32)
+        _lib.check(_lib.lib.jitnn_hip_linear_act(w.handle, xa.ctypes.data_as(C.c_void_p), rows, None if ba is None else ba.ctypes.data_as(C.c_void_p), act,
+                                                 None if ra is None else ra.ctypes.data_as(C.c_void_p), y.ctypes.data_as(C.c_void_p)), "jitnn_hip_linear_act")
     return Tensor.of(y)
+
+
+def linear_dev(w: Tensor, x_ptr: int, rows: int, y_ptr: int, bias_ptr: int = 0, activation: str | None = None, residual_ptr: int = 0, stream_ptr: int = 0) -> None:
+    """y [rows, n] = act(x W^T + bias) + residual on addresses in device memory (jitnn_hip_linear_act_dev): x [rows, k], bias [n], residual [rows, n] apart from y.
+    Only enqueues, on the hipStream_t stream_ptr (0: the null stream)."""
+    rc = _lib.lib.jitnn_hip_linear_act_dev(w.handle, x_ptr or None, rows, bias_ptr or None, _lib.activation_id(activation), residual_ptr or None, y_ptr or None, stream_ptr)
+    if rc:
+        _lib.check(rc, "jitnn_hip_linear_act_dev")
 
 
 class Quant:
@@ -59,11 +72,11 @@ class Quant:
         return Tensor.of(q.to_float_array(), *q.shape())
 
     @staticmethod
-    def linear(x: Tensor, w: Tensor, bias: Tensor | None = None) -> Tensor:
+    def linear(x: Tensor, w: Tensor, bias: Tensor | None = None, activation: str | None = None, residual: Tensor | None = None) -> Tensor:
         _f32(x, "Q8_0 linear")
         if w.dtype() != DType.Q8_0:
             raise ValueError(f"Q8_0 linear: input {list(x.shape())} and weight {list(w.shape())} {w.dtype().name}")
-        return _linear(x, w, bias, "Q8_0 linear")
+        return _linear(x, w, bias, "Q8_0 linear", activation, residual)
 
 
 class Gguf:
@@ -76,14 +89,15 @@ class Gguf:
         return Tensor.of(w.to_float_array(), *w.shape())
 
     @staticmethod
-    def linear(x: Tensor, w: Tensor, bias: Tensor | None = None) -> Tensor:
-        """y = x W^T + b, W [N, K] in a GGUF format, x FP32 [..., K]; b may be None."""
+    def linear(x: Tensor, w: Tensor, bias: Tensor | None = None, activation: str | None = None, residual: Tensor | None = None) -> Tensor:
+        """y = act(x W^T + b) + r, W [N, K] in a GGUF format, x FP32 [..., K]; b and r (of y's shape) may be None, activation None, "relu", "silu", "gelu" or
+        "gelu_tanh"."""
         _f32(x, "linear")
         if w.dtype() == DType.Q8_0:
-            return Quant.linear(x, w, bias)
+            return Quant.linear(x, w, bias, activation, residual)
         if not w.dtype().is_block_quantized():
             raise ValueError(f"not a GGUF block format: {w.dtype().name}")
-        return _linear(x, w, bias, f"{w.dtype().name} linear")
+        return _linear(x, w, bias, f"{w.dtype().name} linear", activation, residual)
 
 
 class F:

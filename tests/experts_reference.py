@@ -12,10 +12,10 @@ def dequantised(fmt, raw, *shape):
 
 
 def activate(name, v):
-    from scipy.special import ndtr
+    from scipy.special import expit, ndtr
     with np.errstate(over="ignore"):
         return {None: lambda z: z, "none": lambda z: z, "relu": lambda z: np.maximum(z, 0), "silu": lambda z: z / (1 + np.exp(-z)), "gelu": lambda z: z * ndtr(z),
-                "gelu_tanh": lambda z: 0.5 * z * (1 + np.tanh(math.sqrt(2 / math.pi) * (z + 0.044715 * z ** 3)))}[name](v)
+                "gelu_tanh": lambda z: z * expit(2 * math.sqrt(2 / math.pi) * (z + 0.044715 * z ** 3))}[name](v)
 
 
 def route(x, w, used, gating="softmax", normalise=True, scale=1.0, bias=None):
@@ -36,6 +36,7 @@ class Layer:
     def __init__(self, rng, experts, used, d, ffn, up="Q4_K", down="Q6_K", gate=None, activation="silu", **routing):
         self.experts, self.used, self.d, self.ffn, self.activation, self.routing = experts, used, d, ffn, activation, routing
         self.formats = (gate or up, up, down)
+        self.tolerance = tolerance(self.formats)
         self.shapes = ((experts, ffn, d), (experts, ffn, d), (experts, d, ffn))
         self.raw = [random_valid_blocks(rng, f, s[0] * s[1], s[2]) for f, s in zip(self.formats, self.shapes)]
         # (random blocks of any format: the rows brought to about one, so that the gates are neither open nor shut)
@@ -67,13 +68,24 @@ class Layer:
         return y
 
 
+# How many times the terms of a product with an offset are what they leave (2-norm): quants around 32, 8 or 7.5 less that offset, 2 at most for blocks of
+# quants that are spread over their whole range.  Q3_K blocks run as Q6_K blocks whose quants are 28 to 35: sqrt(mean of q^2 / mean of (q - 32)^2) =
+# sqrt(1029.5 / 5.5) = 13.7 with q spread evenly.
+OFFSET = {"Q3_K": 14}
+
+
+def offset(fmt):
+    return OFFSET.get(fmt, 4)
+
+
 # How far a layer may be off (2-norm over 2-norm).  The operands of a product hold a value to 2^-20 of itself (two FP16 parts, both cut) or to 2^-22 of the
-# largest of 64 (three bytes), FP32 sums of some hundred terms add as much again; block formats with offsets have terms up to four times the
-# sum they leave; three products follow one another, errors of the first two meet in one.
-TOLERANCE = 3 * 2 * 4 * 2.0 ** -22
+# largest of 64 (three bytes), FP32 sums of some hundred terms add as much again, both count as often as offset() says; three products follow one
+# another, errors of the first two meet in one.
+def tolerance(formats):
+    return 2 * sum(offset(f) for f in formats) * 2.0 ** -22
 
 
-def close(got, want, tolerance=TOLERANCE):
+def close(got, want, tolerance):
     got, want = np.asarray(got, dtype=np.float64), np.asarray(want, dtype=np.float64)
     norm = np.linalg.norm(want)
     assert np.isfinite(got).all()

@@ -40,7 +40,7 @@ def test_host_side():
         jitnn_amd.Router(np.zeros(8), 2)
     with pytest.raises(ValueError, match="biases"):
         jitnn_amd.Router(np.zeros((4, 8)), 2, selection_bias=np.zeros(5))
-    from jitnn_amd.experts import activation_id
+    from jitnn_amd._lib import activation_id
     assert activation_id(None) == 0 and activation_id("gelu_tanh") == 4
     with pytest.raises(ValueError, match="activation"):
         activation_id("swish")

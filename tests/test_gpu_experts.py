@@ -144,7 +144,7 @@ def test_formats(jn, up, down, tokens):
     moe = layer.make(jn)
     x = layer.input(rng, tokens)
     res = 0.1 * rng.standard_normal(x.shape).astype(np.float32)
-    ref.close(Call(moe, x, res).result(), layer.experts_of(x, *layer.route(x), res))
+    ref.close(Call(moe, x, res).result(), layer.experts_of(x, *layer.route(x), res), layer.tolerance)
 
 
 @pytest.mark.parametrize("experts,used,d,ffn,up,down", [
@@ -157,7 +157,7 @@ def test_shapes(jn, experts, used, d, ffn, up, down, tokens):
     layer = ref.Layer(rng, experts, used, d, ffn, up, down, gating="sigmoid", normalise=True, scale=2.5, bias=(0.1 * rng.standard_normal(experts)).astype(np.float32))
     moe = layer.make(jn)
     x = layer.input(rng, tokens)
-    ref.close(Call(moe, x).result(), layer.experts_of(x, *layer.route(x)))
+    ref.close(Call(moe, x).result(), layer.experts_of(x, *layer.route(x)), layer.tolerance)
 
 
 @pytest.mark.parametrize("activation", [None, "relu", "silu", "gelu", "gelu_tanh"])
@@ -166,7 +166,7 @@ def test_activations(jn, activation, tokens):
     rng = np.random.default_rng(3)
     layer = ref.Layer(rng, 4, 2, 512, 768, activation=activation, normalise=False)
     x = 3 * layer.input(rng, tokens)
-    ref.close(Call(layer.make(jn), x).result(), layer.experts_of(x, *layer.route(x)))
+    ref.close(Call(layer.make(jn), x).result(), layer.experts_of(x, *layer.route(x)), layer.tolerance)
 
 
 @pytest.mark.parametrize("tokens", [1, 11, 90])
@@ -174,7 +174,7 @@ def test_gate_and_up_of_two_formats(jn, tokens):
     rng = np.random.default_rng(4)
     layer = ref.Layer(rng, 4, 2, 512, 512, up="Q6_K", gate="Q4_K", down="Q8_0")
     x = layer.input(rng, tokens)
-    ref.close(Call(layer.make(jn), x).result(), layer.experts_of(x, *layer.route(x)))
+    ref.close(Call(layer.make(jn), x).result(), layer.experts_of(x, *layer.route(x)), layer.tolerance)
 
 
 @pytest.mark.parametrize("tokens", [1, 4, 33, 200])
@@ -188,12 +188,12 @@ def test_given_choices(jn, tokens):
     ids[0] = [3, 3, 3, -1]
     weights = rng.standard_normal((tokens, 4)).astype(np.float32)
     res = rng.standard_normal(x.shape).astype(np.float32)
-    ref.close(Call(moe, x, res, ids, weights).result(), layer.experts_of(x, ids, weights, res))
+    ref.close(Call(moe, x, res, ids, weights).result(), layer.experts_of(x, ids, weights, res), layer.tolerance)
     ids[:] = [9, -1, 1 << 30, -(1 << 31)]
     assert np.array_equal(Call(moe, x, res, ids, weights).result(), res)
     assert not Call(moe, x, None, ids, weights).result().any()
     ids[:] = 2
-    ref.close(Call(moe, x, None, ids, weights).result(), layer.experts_of(x, ids, weights))
+    ref.close(Call(moe, x, None, ids, weights).result(), layer.experts_of(x, ids, weights), layer.tolerance)
 
 
 def test_rows_behind_the_last_and_passes(jn):
@@ -206,7 +206,7 @@ def test_rows_behind_the_last_and_passes(jn):
     got = call.result()
     assert (call.y[-2:] == 7).all()
     some = [0, 1, 100, 511, 512, 513, 772]
-    ref.close(got[some], layer.experts_of(x[some], *layer.route(x[some])))
+    ref.close(got[some], layer.experts_of(x[some], *layer.route(x[some])), layer.tolerance)
     assert moe.workspace(512 + 261) == moe.workspace(512) == moe.workspace(100000)
 
 
@@ -251,8 +251,8 @@ def test_large_and_small_inputs(jn):
     x = layer.input(rng, 5)
     for s in (2.0 ** -60, 2.0 ** -20, 2.0 ** 20, 2.0 ** 40):
         z = (x * np.float32(s)).astype(np.float32)
-        ref.close(Call(moe, z, None, ids, weights).result() / s ** 2, layer.experts_of(x, ids, weights))
-        ref.close(Call(moe, z[:1], None, ids[:1], weights[:1]).result() / s ** 2, layer.experts_of(x[:1], ids[:1], weights[:1]))
+        ref.close(Call(moe, z, None, ids, weights).result() / s ** 2, layer.experts_of(x, ids, weights), layer.tolerance)
+        ref.close(Call(moe, z[:1], None, ids[:1], weights[:1]).result() / s ** 2, layer.experts_of(x[:1], ids[:1], weights[:1]), layer.tolerance)
     assert not Call(moe, np.zeros_like(x)).result().any()
 
 
