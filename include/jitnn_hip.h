@@ -380,7 +380,7 @@ JITNN_HIP_API int jitnn_hip_router_dev(const jitnn_hip_router *r, const float *x
                                        long long workspace_bytes, void *stream);
 
 /* A layer of experts on quantised weights as GGUF files hold them, one expert after the other: gate and up [experts * ffn, d_model], down [experts * d_model,
- * ffn] (formats may differ; router and weights are not owned).
+ * ffn] (formats may differ; d_model and ffn at most 131072; router and weights are not owned).
  *   y = residual (or 0) + the sum over a token's experts e of weight_e * down_e (act(gate_e x) * (up_e x))
  * jitnn_hip_moe_dev routes x [tokens, d_model] itself; jitnn_hip_moe_experts_dev takes ids and weights [tokens, used] that exist: an id outside [0, experts)
  * counts for nothing, one that stands twice counts twice.  FP32-grade at any number of tokens (error ~1e-6).  x must be finite where it meets an expert: a

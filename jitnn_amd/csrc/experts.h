@@ -6,6 +6,8 @@
 #include <cstddef>
 #include <cstdint>
 
+#include "tu.h"
+
 namespace jitnn {
 
 enum : int { ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3, ACT_GELU_TANH = 4, ACT_COUNT = 5 };
@@ -13,14 +15,21 @@ enum : int { ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3, ACT_GELU_TA
 constexpr int MAX_EXPERTS = 512, MAX_USED = 64;
 
 // ---- router.h
+// The slots (token x used + place) of each expert, one expert's after the other, and their chunks of at most chunk_rows: [0].x their number, then
+// {expert, place of the first slot in the list, slots, 0} each.
+struct ExpertLists {
+    int *list = nullptr;   // [slots]; nullptr: not wanted
+    int4 *chunks = nullptr;  // [1 + chunks_most()]
+    int chunk_rows = 8;
+    static int chunks_most(int slots, int experts, int chunk_rows) { return (slots < experts ? slots : experts) + slots / chunk_rows; }
+};
 struct RouterArgs {
     const float *x, *w;  // [tokens, d], [experts, d]
     const float *bias;   // [experts] or nullptr: added for the choice, not for the weights
     double *logits;      // [tokens, experts]
     int *ids;            // [tokens, used]
     float *weights;      // [tokens, used]
-    // the slots (token x used + place) of each expert: list[offsets[e]] .. list[offsets[e + 1] - 1]; nullptr: not wanted
-    int *offsets, *list;  // [experts + 1], [tokens x used]
+    ExpertLists lists;
     int tokens, experts, d, used;
     bool sigmoid, normalise;
     float scale;
@@ -28,14 +37,38 @@ struct RouterArgs {
 bool router_needs_logits(int tokens, int experts, int d, bool lists);  // whether a launch of this size reads and writes `logits`
 void router_launch(const RouterArgs &a, hipStream_t s);
 // the lists of choices that somebody else made; an id outside [0, experts) is on none
-void expert_lists_launch(const int *ids, int slots, int experts, int *offsets, int *list, hipStream_t s);
+void expert_lists_launch(const int *ids, int slots, int experts, const ExpertLists &lists, hipStream_t s);
 
-// ---- experts.hip
 struct ExpertWeights {
     int fmt, n, k;  // of one expert: [n, k]
     const uint8_t *w;
     size_t expert_bytes;
 };
+// ---- experts_rows.h: the same on the matrix cores
+struct ExpertRowsArgs {
+    const uint8_t *w, *w2;  // [experts][n rows]
+    size_t expert_bytes;
+    const uint8_t *ops;     // the prepared rows (experts_prepare_launch), in the layout of the format
+    const float *inv;
+    const int *list;
+    const int4 *chunks;
+    float *y;               // [slots, n]
+    int n, k, experts, per_row, act, nblocks, groups;
+};
+size_t experts_ops_bytes(size_t rows, int k);  // the operands of so many rows, and their scales behind them
+// x [rows, k] -> the layouts (GR_LAYOUT_*) that have a place
+void experts_prepare_launch(const float *x, int rows, int k, uint8_t *const *places, hipStream_t s);
+KernelRef experts_rows_kernel_ref(int fmt, int groups, bool dual);
+// w2: y = act(w x) * (w2 x); nullptr: y = w x.  chunks_most: no more of them are there
+void experts_rows_launch(int fmt, ExpertRowsArgs a, int chunks_most, hipStream_t s);
+void experts_rows_launch_k(int fmt, const ExpertRowsArgs &a, unsigned blocks, bool dual, hipStream_t s);    // experts_rows_k.hip: Q4_K, Q5_K
+void experts_rows_launch_k6(int fmt, const ExpertRowsArgs &a, unsigned blocks, bool dual, hipStream_t s);   // experts_rows_k6.hip: Q6_K, Q2_K
+void experts_rows_launch_q32(int fmt, const ExpertRowsArgs &a, unsigned blocks, bool dual, hipStream_t s);  // experts_rows_q32.hip: Q8_0, Q4_0, Q4_1, Q5_1
+KernelRef experts_rows_ref_k(int fmt, int groups, bool dual);
+KernelRef experts_rows_ref_k6(int fmt, int groups, bool dual);
+KernelRef experts_rows_ref_q32(int fmt, int groups, bool dual);
+
+// ---- experts.hip
 // y [slots, n] = the product of each slot's expert with row slot / per_row of x, in FP32 on the dequantiser's values: any format
 void experts_value_launch(const ExpertWeights &w, int experts, const int *ids, int slots, int per_row, const float *x, float *y, hipStream_t s);
 // h [count] = act(g) * u (h may be g)

@@ -5,6 +5,7 @@
 
 #include "act.h"
 #include "dequant.h"
+#include "experts_rows.h"
 
 namespace jitnn {
 
@@ -47,6 +48,39 @@ void experts_value_launch(const ExpertWeights &w, int experts, const int *ids, i
     case F_Q2_K: value<F_Q2_K>(w, experts, ids, slots, per_row, x, y, s); break;
     case F_Q3_K: value<F_Q3_K>(w, experts, ids, slots, per_row, x, y, s); break;
     }
+}
+
+// ---- on the matrix cores
+
+size_t experts_ops_bytes(size_t rows, int k) {
+    const size_t columns = rows * ((k + 255) / 256);
+    return columns * (ER_OP_BYTES + sizeof(float));
+}
+
+void experts_prepare_launch(const float *x, int rows, int k, uint8_t *const *places, hipStream_t s) {
+    const int ncol = (k + 255) / 256;
+    ExpertPrepareOut o{};
+    for (int l = 0; l < GR_LAYOUTS; ++l) {
+        if (!places[l]) continue;
+        o.ops[l] = places[l];
+        o.inv[l] = reinterpret_cast<float *>(places[l] + (size_t)rows * ncol * ER_OP_BYTES);
+    }
+    hipLaunchKernelGGL(experts_prepare_kernel, dim3(ncol, (rows + 7) / 8), dim3(64), 0, s, x, rows, k, o);
+}
+
+KernelRef experts_rows_kernel_ref(int fmt, int groups, bool dual) {
+    return fmt == F_Q4_K || fmt == F_Q5_K ? experts_rows_ref_k(fmt, groups, dual) : fmt == F_Q6_K || fmt == F_Q2_K ? experts_rows_ref_k6(fmt, groups, dual)
+                                                                                                                   : experts_rows_ref_q32(fmt, groups, dual);
+}
+
+void experts_rows_launch(int fmt, ExpertRowsArgs a, int chunks_most, hipStream_t s) {
+    const bool dual = a.w2 != nullptr;
+    const int per_block = ER_WAVES * (dual ? 1 : ER_T);
+    a.nblocks = (a.n / 16 + per_block - 1) / per_block;
+    const unsigned blocks = (unsigned)a.nblocks * (unsigned)chunks_most;
+    if (fmt == F_Q4_K || fmt == F_Q5_K) experts_rows_launch_k(fmt, a, blocks, dual, s);
+    else if (fmt == F_Q6_K || fmt == F_Q2_K) experts_rows_launch_k6(fmt, a, blocks, dual, s);
+    else experts_rows_launch_q32(fmt, a, blocks, dual, s);
 }
 
 static __global__ void __launch_bounds__(256) experts_gate_kernel(int act, const float *g, const float *__restrict__ u, float *h, size_t count4, unsigned stride) {

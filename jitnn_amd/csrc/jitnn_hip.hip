@@ -2376,14 +2376,26 @@ namespace {
 
 constexpr int ROUTER_PASS = 8192;  // tokens of a pass of the router alone
 constexpr int MOE_PASS_SLOTS = 4096;  // places (tokens x used) of a pass through the experts
+constexpr int MOE_MAX_VALUES = 1 << 17;  // of a row: the operands of a pass's rows are found by 32-bit offsets, 4096 rows x 512 columns x 1152 bytes
 
 size_t pad256(size_t b) { return (b + 255) & ~(size_t)255; }
 
 int moe_pass_tokens(const jitnn_hip_moe *m) { return std::max(1, MOE_PASS_SLOTS / m->router->used); }
 
+bool experts_on_rows(const jitnn_hip_weight *w) { return gemv_rows_supported(w->fmt); }  // (Q5_0 and Q3_K blocks that were not rewritten have no operands)
+
+// Groups of eight rows in a chunk of an expert's: what most experts have where every one is as likely as any other, so that their weights are read
+// once; at most five, whose operands LDS holds twice.
+int moe_groups(const jitnn_hip_moe *m, int tokens) {
+    const double mean = (double)tokens * m->router->used / m->router->experts;
+    return std::max(1, std::min(5, (int)std::ceil((mean + 2 * std::sqrt(mean)) / 8)));
+}
+
 // What a pass of `tokens` keeps in the workspace, in bytes from its start.
 struct MoeLayout {
-    size_t logits, ids, weights, g, u, part, total;
+    size_t logits, ids, weights, list, chunks, ops[GR_LAYOUTS], h_ops, g, u, part, total;
+    bool layouts[GR_LAYOUTS];  // of x that gate and up ask for
+    int groups, chunks_most;
 };
 MoeLayout moe_layout(const jitnn_hip_moe *m, int tokens) {
     const jitnn_hip_router *r = m->router;
@@ -2395,9 +2407,17 @@ MoeLayout moe_layout(const jitnn_hip_moe *m, int tokens) {
         at += pad256(bytes);
         return here;
     };
+    l.groups = moe_groups(m, tokens);
+    l.chunks_most = ExpertLists::chunks_most((int)slots, r->experts, 8 * l.groups);
     l.logits = take((size_t)tokens * r->experts * sizeof(double));
     l.ids = take(slots * sizeof(int));
     l.weights = take(slots * sizeof(float));
+    l.list = take(slots * sizeof(int));
+    l.chunks = take(((size_t)l.chunks_most + 1) * sizeof(int4));
+    for (const jitnn_hip_weight *w : {m->gate, m->up})
+        if (experts_on_rows(w)) l.layouts[gemv_rows_layout(w->fmt)] = true;
+    for (int i = 0; i < GR_LAYOUTS; ++i) l.ops[i] = l.layouts[i] ? take(experts_ops_bytes(tokens, r->d)) : 0;
+    l.h_ops = take(experts_on_rows(m->down) ? experts_ops_bytes(slots, m->ffn) : 0);
     l.g = take(slots * m->ffn * sizeof(float));
     l.u = take(slots * m->ffn * sizeof(float));
     l.part = take(slots * r->d * sizeof(float));
@@ -2423,6 +2443,14 @@ RouterArgs router_args(const jitnn_hip_router *r, const float *x, int tokens, in
     return a;
 }
 
+ExpertLists moe_lists(uint8_t *ws, const MoeLayout &l) {
+    ExpertLists lists;
+    lists.list = (int *)(ws + l.list);
+    lists.chunks = (int4 *)(ws + l.chunks);
+    lists.chunk_rows = 8 * l.groups;
+    return lists;
+}
+
 ExpertWeights expert_weights(const jitnn_hip_weight *w, int experts) {
     return {w->fmt, w->n / experts, w->k, w->dev, (size_t)(w->n / experts) * (size_t)(w->k / block_values(w->fmt)) * block_bytes(w->fmt)};
 }
@@ -2439,16 +2467,58 @@ int check_moe_call(const jitnn_hip_moe *m, const float *x, int tokens, const flo
     return check_ready();
 }
 
-// One pass: the experts of `tokens` tokens for given choices.
+// One pass: the experts of `tokens` tokens for given choices, whose lists are made.
 int moe_experts(const jitnn_hip_moe *m, const float *x, int tokens, const int *ids, const float *weights, const float *res, float *y, uint8_t *ws, const MoeLayout &l,
                 hipStream_t s) {
     const jitnn_hip_router *r = m->router;
     const int slots = tokens * r->used;
     float *gb = (float *)(ws + l.g), *ub = (float *)(ws + l.u), *part = (float *)(ws + l.part);
-    experts_value_launch(expert_weights(m->gate, r->experts), r->experts, ids, slots, r->used, x, gb, s);
-    experts_value_launch(expert_weights(m->up, r->experts), r->experts, ids, slots, r->used, x, ub, s);
-    experts_gate_launch(m->act, gb, ub, gb, (size_t)slots * m->ffn, g.cus, s);
-    experts_value_launch(expert_weights(m->down, r->experts), r->experts, ids, slots, 1, gb, part, s);
+    // out [slots, n] = the products of w (with w2: of both, gated) with rows [rows, k], whose operands stand at ops
+    auto rows = [&](const jitnn_hip_weight *w, const jitnn_hip_weight *w2, const uint8_t *ops, int count, int per_row, float *out) -> int {
+        const ExpertWeights e = expert_weights(w, r->experts);
+        ExpertRowsArgs a{};
+        a.w = w->dev;
+        a.w2 = w2 ? w2->dev : nullptr;
+        a.expert_bytes = e.expert_bytes;
+        a.ops = ops;
+        a.inv = (const float *)(ops + (experts_ops_bytes(count, w->k) - (size_t)count * ((w->k + 255) / 256) * sizeof(float)));
+        a.list = (const int *)(ws + l.list);
+        a.chunks = (const int4 *)(ws + l.chunks);
+        a.y = out;
+        a.n = e.n;
+        a.k = e.k;
+        a.experts = r->experts;
+        a.per_row = per_row;
+        a.act = m->act;
+        a.groups = l.groups;
+        const KernelRef k = experts_rows_kernel_ref(w->fmt, l.groups, w2 != nullptr);
+        if (int rc = allow_lds(k.fn, k.lds)) return rc;
+        experts_rows_launch(w->fmt, a, l.chunks_most, s);
+        return JITNN_HIP_OK;
+    };
+    uint8_t *places[GR_LAYOUTS] = {};
+    for (int i = 0; i < GR_LAYOUTS; ++i) places[i] = l.layouts[i] ? ws + l.ops[i] : nullptr;
+    if (places[0] || places[1] || places[2]) experts_prepare_launch(x, tokens, r->d, places, s);
+    const bool pair = experts_on_rows(m->gate) && m->gate->fmt == m->up->fmt;
+    if (pair) {
+        if (int rc = rows(m->gate, m->up, places[gemv_rows_layout(m->gate->fmt)], tokens, r->used, gb)) return rc;
+    } else {
+        const jitnn_hip_weight *ws2[2] = {m->gate, m->up};
+        float *outs[2] = {gb, ub};
+        for (int i = 0; i < 2; ++i) {
+            if (!experts_on_rows(ws2[i])) experts_value_launch(expert_weights(ws2[i], r->experts), r->experts, ids, slots, r->used, x, outs[i], s);
+            else if (int rc = rows(ws2[i], nullptr, places[gemv_rows_layout(ws2[i]->fmt)], tokens, r->used, outs[i])) return rc;
+        }
+        experts_gate_launch(m->act, gb, ub, gb, (size_t)slots * m->ffn, g.cus, s);
+    }
+    if (experts_on_rows(m->down)) {
+        uint8_t *h_places[GR_LAYOUTS] = {};
+        h_places[gemv_rows_layout(m->down->fmt)] = ws + l.h_ops;
+        experts_prepare_launch(gb, slots, m->ffn, h_places, s);
+        if (int rc = rows(m->down, nullptr, ws + l.h_ops, slots, 1, part)) return rc;
+    } else {
+        experts_value_launch(expert_weights(m->down, r->experts), r->experts, ids, slots, 1, gb, part, s);
+    }
     experts_combine_launch(part, ids, weights, res, y, tokens, r->used, r->experts, r->d, g.cus, s);
     HIP_TRY(hipGetLastError());
     return JITNN_HIP_OK;
@@ -2535,6 +2605,7 @@ int jitnn_hip_moe_create(const jitnn_hip_router *router, const jitnn_hip_weight 
     if (gate->k != d || up->k != d || (long long)e * ffn != gate->n || gate->n != up->n || (long long)e * d != down->n)
         return fail(JITNN_HIP_EINVAL, "experts of shapes gate [%d, %d], up [%d, %d], down [%d, %d] for a router of %d experts on %d values", gate->n, gate->k, up->n, up->k, down->n,
                     down->k, e, d);
+    if (d > MOE_MAX_VALUES || ffn > MOE_MAX_VALUES) return fail(JITNN_HIP_EINVAL, "experts on %d and %d values (at most %d)", d, ffn, MOE_MAX_VALUES);
     jitnn_hip_moe *m = new (std::nothrow) jitnn_hip_moe{router, gate, up, down, activation, ffn};
     if (!m) return fail(JITNN_HIP_ENOMEM, "out of host memory");
     *out = m;
@@ -2549,7 +2620,11 @@ int jitnn_hip_moe_free(jitnn_hip_moe *m) {
 long long jitnn_hip_moe_workspace(const jitnn_hip_moe *m, int tokens) {
     if (!m) return fail(JITNN_HIP_EINVAL, "the layer is NULL");
     if (tokens < 0) return fail(JITNN_HIP_EINVAL, "tokens = %d", tokens);
-    return tokens == 0 ? 0 : (long long)moe_layout(m, std::min(tokens, moe_pass_tokens(m))).total;
+    if (tokens == 0) return 0;
+    const int pass = moe_pass_tokens(m);
+    long long most = (long long)moe_layout(m, std::min(tokens, pass)).total;
+    if (tokens > pass && tokens % pass) most = std::max(most, (long long)moe_layout(m, tokens % pass).total);  // (more, smaller chunks)
+    return most;
 }
 
 int jitnn_hip_moe_dev(const jitnn_hip_moe *m, const float *x_dev, int tokens, const float *residual_dev, float *y_dev, void *workspace_dev, long long workspace_bytes, void *stream) {
@@ -2560,7 +2635,9 @@ int jitnn_hip_moe_dev(const jitnn_hip_moe *m, const float *x_dev, int tokens, co
         const int count = std::min(pass, tokens - t), d = m->router->d;
         const MoeLayout l = moe_layout(m, count);
         const float *x = x_dev + (size_t)t * d;
-        router_launch(router_args(m->router, x, count, (int *)(ws + l.ids), (float *)(ws + l.weights), ws + l.logits), (hipStream_t)stream);
+        RouterArgs a = router_args(m->router, x, count, (int *)(ws + l.ids), (float *)(ws + l.weights), ws + l.logits);
+        a.lists = moe_lists(ws, l);
+        router_launch(a, (hipStream_t)stream);
         if (int rc = moe_experts(m, x, count, (const int *)(ws + l.ids), (const float *)(ws + l.weights), residual_dev ? residual_dev + (size_t)t * d : nullptr, y_dev + (size_t)t * d,
                                  ws, l, (hipStream_t)stream))
             return rc;
@@ -2575,8 +2652,11 @@ int jitnn_hip_moe_experts_dev(const jitnn_hip_moe *m, const float *x_dev, int to
     const int pass = moe_pass_tokens(m);
     for (int t = 0; t < tokens; t += pass) {
         const int count = std::min(pass, tokens - t), d = m->router->d, used = m->router->used;
-        if (int rc = moe_experts(m, x_dev + (size_t)t * d, count, ids_dev + (size_t)t * used, weights_dev + (size_t)t * used,
-                                 residual_dev ? residual_dev + (size_t)t * d : nullptr, y_dev + (size_t)t * d, (uint8_t *)workspace_dev, moe_layout(m, count), (hipStream_t)stream))
+        const MoeLayout l = moe_layout(m, count);
+        const int *ids = ids_dev + (size_t)t * used;
+        expert_lists_launch(ids, count * used, m->router->experts, moe_lists((uint8_t *)workspace_dev, l), (hipStream_t)stream);
+        if (int rc = moe_experts(m, x_dev + (size_t)t * d, count, ids, weights_dev + (size_t)t * used, residual_dev ? residual_dev + (size_t)t * d : nullptr,
+                                 y_dev + (size_t)t * d, (uint8_t *)workspace_dev, l, (hipStream_t)stream))
             return rc;
     }
     return JITNN_HIP_OK;

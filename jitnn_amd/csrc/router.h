@@ -169,12 +169,12 @@ __device__ __forceinline__ void store_choice(const RouterArgs &a, int t, int lan
     }
 }
 
-// The lists of each expert's slots, by one workgroup of 1024 threads: counted, summed up, handed out.  (In what order a list holds its slots is
-// no part of any result: each row of a product is computed by itself.)  hist: [MAX_EXPERTS + 1] in LDS.
+// The lists of each expert's slots and their chunks, by one workgroup of 1024 threads: counted, summed up, handed out.  (In what order a list holds its slots
+// is no part of any result: each row of a product is computed by itself.)  hist: [MAX_EXPERTS] in LDS.
 template <class Id>
-__device__ __forceinline__ void make_lists(Id &&id_of, int slots, int experts, int *__restrict__ offsets, int *__restrict__ list, int *hist) {
+__device__ __forceinline__ void make_lists(Id &&id_of, int slots, int experts, const ExpertLists &lists, int *hist) {
     const int tid = threadIdx.x, lane = tid & 63;
-    for (int e = tid; e <= experts; e += 1024) hist[e] = 0;
+    for (int e = tid; e < experts; e += 1024) hist[e] = 0;
     __syncthreads();
     for (int i = tid; i < slots; i += 1024) {
         const int e = id_of(i);
@@ -182,27 +182,31 @@ __device__ __forceinline__ void make_lists(Id &&id_of, int slots, int experts, i
     }
     __syncthreads();
     if (tid < 64) {
-        int run = 0;
+        int run = 0, made = 0;
         for (int e0 = 0; e0 < experts; e0 += 64) {
-            const int mine = e0 + lane < experts ? hist[e0 + lane] : 0;
-            int sum = mine;
+            const int e = e0 + lane, mine = e < experts ? hist[e] : 0, chunks = (mine + lists.chunk_rows - 1) / lists.chunk_rows;
+            int sum = mine, chunk_sum = chunks;
 #pragma unroll
             for (int o = 1; o < 64; o <<= 1) {
-                const int below = __shfl_up(sum, o);
+                const int below = __shfl_up(sum, o), chunk_below = __shfl_up(chunk_sum, o);
                 sum += lane >= o ? below : 0;
+                chunk_sum += lane >= o ? chunk_below : 0;
             }
-            if (e0 + lane < experts) {
-                hist[e0 + lane] = run + sum - mine;
-                offsets[e0 + lane] = run + sum - mine;
+            const int first = run + sum - mine;
+            if (e < experts) hist[e] = first;
+            for (int i = 0; i < chunks; ++i) {  // (as even as whole rows allow)
+                const int from = (int)((long long)mine * i / chunks), to = (int)((long long)mine * (i + 1) / chunks);
+                lists.chunks[1 + made + chunk_sum - chunks + i] = int4{e, first + from, to - from, 0};
             }
             run += __shfl(sum, 63);
+            made += __shfl(chunk_sum, 63);
         }
-        if (lane == 0) offsets[experts] = run;
+        if (lane == 0) lists.chunks[0] = int4{made, 0, 0, 0};
     }
     __syncthreads();
     for (int i = tid; i < slots; i += 1024) {
         const int e = id_of(i);
-        if ((unsigned)e < (unsigned)experts) list[atomicAdd(&hist[e], 1)] = i;
+        if ((unsigned)e < (unsigned)experts) lists.list[atomicAdd(&hist[e], 1)] = i;
     }
 }
 
@@ -226,7 +230,7 @@ static __global__ void __launch_bounds__(256) choose_kernel(const RouterArgs a) 
 constexpr int CHOOSE_FEW = 64;
 static __global__ void __launch_bounds__(1024) choose_few_kernel(const RouterArgs a, int waves) {
     extern __shared__ __align__(16) double choose_smem[];
-    __shared__ int ids[CHOOSE_FEW * MAX_USED], hist[MAX_EXPERTS + 1];
+    __shared__ int ids[CHOOSE_FEW * MAX_USED], hist[MAX_EXPERTS];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     double *l = choose_smem + (size_t)wave * 2 * a.experts;
     for (int t = wave; wave < waves && t < a.tokens; t += waves) {
@@ -242,12 +246,12 @@ static __global__ void __launch_bounds__(1024) choose_few_kernel(const RouterArg
         __builtin_amdgcn_wave_barrier();
     }
     __syncthreads();
-    make_lists([&](int i) { return ids[i]; }, a.tokens * a.used, a.experts, a.offsets, a.list, hist);
+    make_lists([&](int i) { return ids[i]; }, a.tokens * a.used, a.experts, a.lists, hist);
 }
 
-static __global__ void __launch_bounds__(1024) expert_lists_kernel(const int *__restrict__ ids, int slots, int experts, int *offsets, int *list) {
-    __shared__ int hist[MAX_EXPERTS + 1];
-    make_lists([&](int i) { return ids[i]; }, slots, experts, offsets, list, hist);
+static __global__ void __launch_bounds__(1024) expert_lists_kernel(const int *__restrict__ ids, int slots, int experts, const ExpertLists lists) {
+    __shared__ int hist[MAX_EXPERTS];
+    make_lists([&](int i) { return ids[i]; }, slots, experts, lists, hist);
 }
 
 // A router whose weights one workgroup reads in about the time that a second launch would take: logits and choice of a token, 1024 threads.

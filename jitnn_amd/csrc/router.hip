@@ -11,7 +11,7 @@ static bool one_launch(int tokens, int experts, int d, bool lists) { return !lis
 bool router_needs_logits(int tokens, int experts, int d, bool lists) { return !one_launch(tokens, experts, d, lists); }
 
 void router_launch(const RouterArgs &a, hipStream_t s) {
-    const bool lists = a.offsets != nullptr;
+    const bool lists = a.lists.list != nullptr;
     if (one_launch(a.tokens, a.experts, a.d, lists)) {
         hipLaunchKernelGGL(router_one_kernel, dim3(a.tokens), dim3(1024), 0, s, a);
         return;
@@ -24,11 +24,11 @@ void router_launch(const RouterArgs &a, hipStream_t s) {
         return;
     }
     hipLaunchKernelGGL(choose_kernel, dim3((a.tokens + 3) / 4), dim3(256), (size_t)64 * a.experts, s, a);
-    if (lists) expert_lists_launch(a.ids, a.tokens * a.used, a.experts, a.offsets, a.list, s);
+    if (lists) expert_lists_launch(a.ids, a.tokens * a.used, a.experts, a.lists, s);
 }
 
-void expert_lists_launch(const int *ids, int slots, int experts, int *offsets, int *list, hipStream_t s) {
-    hipLaunchKernelGGL(expert_lists_kernel, dim3(1), dim3(1024), 0, s, ids, slots, experts, offsets, list);
+void expert_lists_launch(const int *ids, int slots, int experts, const ExpertLists &lists, hipStream_t s) {
+    hipLaunchKernelGGL(expert_lists_kernel, dim3(1), dim3(1024), 0, s, ids, slots, experts, lists);
 }
 
 }  // namespace jitnn
