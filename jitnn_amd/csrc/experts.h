@@ -68,6 +68,29 @@ KernelRef experts_rows_ref_k(int fmt, int groups, bool dual);
 KernelRef experts_rows_ref_k6(int fmt, int groups, bool dual);
 KernelRef experts_rows_ref_q32(int fmt, int groups, bool dual);
 
+// ---- experts_few.h: few tokens, INT8 products
+struct ExpertFewArgs {
+    const uint8_t *w, *w2;  // [experts][n rows of k values]; up: gate and up, down: w2 not used
+    size_t expert_bytes;
+    const float *x;         // up: [tokens, k]; down: [tokens, used, k]
+    const int *ids;         // [tokens, used]
+    const float *weights;   // down: [tokens, used]
+    const float *res;       // down: [tokens, n] or nullptr
+    float *y;               // up: [tokens, used, n]; down: [tokens, n] (may be res)
+    int n, k, used, experts, act, blocks;
+    unsigned by_rows;       // up: reciprocal of n / 4
+};
+// whether rows of k values (up) and `used` of ffn values behind one another (down) have a kernel
+bool experts_few_up_supported(int fmt, int k);
+bool experts_few_down_supported(int fmt, int ffn, int used);
+void experts_few_up_launch(int fmt, ExpertFewArgs a, int tokens, int cus, hipStream_t s);
+void experts_few_down_launch(int fmt, ExpertFewArgs a, int tokens, int cus, hipStream_t s);
+typedef void (*ExpertFewKernel)(const ExpertFewArgs);
+ExpertFewKernel experts_few_up_k(int fmt, bool aligned, int waves);     // experts_few_k.hip: Q4_K, Q5_K, Q6_K, Q2_K
+ExpertFewKernel experts_few_up_q32(int fmt, int waves);                 // experts_few_q32.hip: Q8_0, Q4_0, Q4_1, Q5_1
+ExpertFewKernel experts_few_down_k(int fmt, bool aligned, int stretches, int waves);
+ExpertFewKernel experts_few_down_q32(int fmt, int stretches, int waves);
+
 // ---- experts.hip
 // y [slots, n] = the product of each slot's expert with row slot / per_row of x, in FP32 on the dequantiser's values: any format
 void experts_value_launch(const ExpertWeights &w, int experts, const int *ids, int slots, int per_row, const float *x, float *y, hipStream_t s);

@@ -5,7 +5,9 @@
 
 #include "act.h"
 #include "dequant.h"
+#include "experts_few.h"
 #include "experts_rows.h"
+#include "serving.h"
 
 namespace jitnn {
 
@@ -48,6 +50,41 @@ void experts_value_launch(const ExpertWeights &w, int experts, const int *ids, i
     case F_Q2_K: value<F_Q2_K>(w, experts, ids, slots, per_row, x, y, s); break;
     case F_Q3_K: value<F_Q3_K>(w, experts, ids, slots, per_row, x, y, s); break;
     }
+}
+
+// ---- few tokens
+
+static bool quants32(int fmt) { return block_values(fmt) == 32; }
+
+bool experts_few_up_supported(int fmt, int k) {
+    return (quants32(fmt) ? fmt != F_Q5_0 && k % 64 == 0 : fmt != F_Q3_K) && k <= 1024 * I8_MAX_WAVES;  // (rows of whole chunks of 64 values)
+}
+
+bool experts_few_down_supported(int fmt, int ffn, int used) {
+    return (quants32(fmt) ? fmt != F_Q5_0 && ffn % 64 == 0 : fmt != F_Q3_K) && (long long)used * ffn <= 2 * 1024 * I8_MAX_WAVES;
+}
+
+// Workgroups for `groups` row groups of each of `tokens`, so many waves a CU in all and every workgroup as many turns as the others.
+static int few_blocks(int groups, int tokens, int waves, int cus, int waves_per_cu) {
+    const int most = std::max(1, std::max(1, waves_per_cu / waves) * cus / tokens), turns = (groups + most - 1) / most;
+    return (groups + turns - 1) / turns;
+}
+
+void experts_few_up_launch(int fmt, ExpertFewArgs a, int tokens, int cus, hipStream_t s) {
+    const int waves = (a.k + 1023) / 1024;
+    const bool aligned = a.k % 512 == 0 && (((uintptr_t)a.w | (uintptr_t)a.w2) & 3) == 0;
+    a.blocks = few_blocks(a.used * (a.n / 4), tokens, waves, cus, 8);
+    a.by_rows = reciprocal((unsigned)(a.n / 4));
+    const ExpertFewKernel fn = quants32(fmt) ? experts_few_up_q32(fmt, waves) : experts_few_up_k(fmt, aligned, waves);
+    hipLaunchKernelGGL(fn, dim3(a.blocks, tokens), dim3(64 * waves), (size_t)waves * EF_WAVE_LDS, s, a);
+}
+
+void experts_few_down_launch(int fmt, ExpertFewArgs a, int tokens, int cus, hipStream_t s) {
+    const int all = (int)(((long long)a.used * a.k + 1023) / 1024), stretches = all > I8_MAX_WAVES ? 2 : 1, waves = (all + stretches - 1) / stretches;
+    const bool aligned = a.k % 512 == 0 && ((uintptr_t)a.w & 3) == 0;
+    a.blocks = few_blocks(a.n / 4, tokens, waves, cus, 16);
+    const ExpertFewKernel fn = quants32(fmt) ? experts_few_down_q32(fmt, stretches, waves) : experts_few_down_k(fmt, aligned, stretches, waves);
+    hipLaunchKernelGGL(fn, dim3(a.blocks, tokens), dim3(64 * waves), (size_t)waves * EF_WAVE_LDS, s, a);
 }
 
 // ---- on the matrix cores

@@ -2391,11 +2391,20 @@ int moe_groups(const jitnn_hip_moe *m, int tokens) {
     return std::max(1, std::min(5, (int)std::ceil((mean + 2 * std::sqrt(mean)) / 8)));
 }
 
+// Few tokens: the INT8 products on the raw quants, for weights whose rows are whole chunks of 64 values.
+bool moe_few(const jitnn_hip_moe *m, int tokens) {
+    if (!g.gemv_i8 || tokens > 1 || m->gate->fmt != m->up->fmt) return false;
+    for (const jitnn_hip_weight *w : {m->gate, m->up, m->down})
+        if (w->nbytes >= (1ll << 32) || ((uintptr_t)w->dev & 3) != 0) return false;
+    return experts_few_up_supported(m->gate->fmt, m->router->d) && experts_few_down_supported(m->down->fmt, m->ffn, m->router->used);
+}
+
 // What a pass of `tokens` keeps in the workspace, in bytes from its start.
 struct MoeLayout {
     size_t logits, ids, weights, list, chunks, ops[GR_LAYOUTS], h_ops, g, u, part, total;
     bool layouts[GR_LAYOUTS];  // of x that gate and up ask for
     int groups, chunks_most;
+    bool few;
 };
 MoeLayout moe_layout(const jitnn_hip_moe *m, int tokens) {
     const jitnn_hip_router *r = m->router;
@@ -2407,18 +2416,21 @@ MoeLayout moe_layout(const jitnn_hip_moe *m, int tokens) {
         at += pad256(bytes);
         return here;
     };
+    l.few = moe_few(m, tokens);
     l.groups = moe_groups(m, tokens);
     l.chunks_most = ExpertLists::chunks_most((int)slots, r->experts, 8 * l.groups);
     l.logits = take((size_t)tokens * r->experts * sizeof(double));
     l.ids = take(slots * sizeof(int));
     l.weights = take(slots * sizeof(float));
+    l.g = take(slots * m->ffn * sizeof(float));
+    l.total = at;
+    if (l.few) return l;
     l.list = take(slots * sizeof(int));
     l.chunks = take(((size_t)l.chunks_most + 1) * sizeof(int4));
     for (const jitnn_hip_weight *w : {m->gate, m->up})
         if (experts_on_rows(w)) l.layouts[gemv_rows_layout(w->fmt)] = true;
     for (int i = 0; i < GR_LAYOUTS; ++i) l.ops[i] = l.layouts[i] ? take(experts_ops_bytes(tokens, r->d)) : 0;
     l.h_ops = take(experts_on_rows(m->down) ? experts_ops_bytes(slots, m->ffn) : 0);
-    l.g = take(slots * m->ffn * sizeof(float));
     l.u = take(slots * m->ffn * sizeof(float));
     l.part = take(slots * r->d * sizeof(float));
     l.total = at;
@@ -2473,6 +2485,34 @@ int moe_experts(const jitnn_hip_moe *m, const float *x, int tokens, const int *i
     const jitnn_hip_router *r = m->router;
     const int slots = tokens * r->used;
     float *gb = (float *)(ws + l.g), *ub = (float *)(ws + l.u), *part = (float *)(ws + l.part);
+    if (l.few) {
+        ExpertFewArgs a{};
+        ExpertWeights e = expert_weights(m->gate, r->experts);
+        a.w = m->gate->dev;
+        a.w2 = m->up->dev;
+        a.expert_bytes = e.expert_bytes;
+        a.x = x;
+        a.ids = ids;
+        a.weights = weights;
+        a.y = gb;
+        a.n = e.n;
+        a.k = e.k;
+        a.used = r->used;
+        a.experts = r->experts;
+        a.act = m->act;
+        experts_few_up_launch(m->gate->fmt, a, tokens, g.cus, s);
+        e = expert_weights(m->down, r->experts);
+        a.w = m->down->dev;
+        a.expert_bytes = e.expert_bytes;
+        a.x = gb;
+        a.res = res;
+        a.y = y;
+        a.n = e.n;
+        a.k = e.k;
+        experts_few_down_launch(m->down->fmt, a, tokens, g.cus, s);
+        HIP_TRY(hipGetLastError());
+        return JITNN_HIP_OK;
+    }
     // out [slots, n] = the products of w (with w2: of both, gated) with rows [rows, k], whose operands stand at ops
     auto rows = [&](const jitnn_hip_weight *w, const jitnn_hip_weight *w2, const uint8_t *ops, int count, int per_row, float *out) -> int {
         const ExpertWeights e = expert_weights(w, r->experts);
@@ -2636,7 +2676,7 @@ int jitnn_hip_moe_dev(const jitnn_hip_moe *m, const float *x_dev, int tokens, co
         const MoeLayout l = moe_layout(m, count);
         const float *x = x_dev + (size_t)t * d;
         RouterArgs a = router_args(m->router, x, count, (int *)(ws + l.ids), (float *)(ws + l.weights), ws + l.logits);
-        a.lists = moe_lists(ws, l);
+        if (!l.few) a.lists = moe_lists(ws, l);
         router_launch(a, (hipStream_t)stream);
         if (int rc = moe_experts(m, x, count, (const int *)(ws + l.ids), (const float *)(ws + l.weights), residual_dev ? residual_dev + (size_t)t * d : nullptr, y_dev + (size_t)t * d,
                                  ws, l, (hipStream_t)stream))
@@ -2654,7 +2694,7 @@ int jitnn_hip_moe_experts_dev(const jitnn_hip_moe *m, const float *x_dev, int to
         const int count = std::min(pass, tokens - t), d = m->router->d, used = m->router->used;
         const MoeLayout l = moe_layout(m, count);
         const int *ids = ids_dev + (size_t)t * used;
-        expert_lists_launch(ids, count * used, m->router->experts, moe_lists((uint8_t *)workspace_dev, l), (hipStream_t)stream);
+        if (!l.few) expert_lists_launch(ids, count * used, m->router->experts, moe_lists((uint8_t *)workspace_dev, l), (hipStream_t)stream);
         if (int rc = moe_experts(m, x_dev + (size_t)t * d, count, ids, weights_dev + (size_t)t * used, residual_dev ? residual_dev + (size_t)t * d : nullptr,
                                  y_dev + (size_t)t * d, (uint8_t *)workspace_dev, l, (hipStream_t)stream))
             return rc;
