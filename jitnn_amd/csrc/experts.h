@@ -26,16 +26,19 @@ struct ExpertLists {
 struct RouterArgs {
     const float *x, *w;  // [tokens, d], [experts, d]
     const float *bias;   // [experts] or nullptr: added for the choice, not for the weights
-    double *logits;      // [tokens, experts]
+    double *logits;      // [splits][tokens, experts]
     int *ids;            // [tokens, used]
     float *weights;      // [tokens, used]
     ExpertLists lists;
     int tokens, experts, d, used;
     bool sigmoid, normalise;
     float scale;
+    int splits;  // (set with the launch of the logits)
 };
-bool router_needs_logits(int tokens, int experts, int d, bool lists);  // whether a launch of this size reads and writes `logits`
-void router_launch(const RouterArgs &a, hipStream_t s);
+// what `logits` takes; choice_follows: router_launch without lists, which may need none
+size_t router_logits_bytes(int tokens, int experts, int d, bool choice_follows);
+void router_logits_launch(RouterArgs &a, hipStream_t s);
+void router_launch(RouterArgs a, hipStream_t s);
 // the lists of choices that somebody else made; an id outside [0, experts) is on none
 void expert_lists_launch(const int *ids, int slots, int experts, const ExpertLists &lists, hipStream_t s);
 
@@ -53,20 +56,25 @@ struct ExpertRowsArgs {
     const int *list;
     const int4 *chunks;
     float *y;               // [slots, n]
-    int n, k, experts, per_row, act, nblocks, groups;
+    size_t split_floats;    // from one split's y to the next one's
+    int n, k, experts, per_row, act, nblocks, splits;
+};
+typedef void (*RowsKernel)(const ExpertRowsArgs);
+struct RowsKernelRef {
+    RowsKernel fn;
+    size_t lds;
+    int threads, tiles, groups;  // tiles: of 16 weight rows (of each matrix of a pair) per workgroup; groups: of eight rows per chunk, at most
 };
 size_t experts_ops_bytes(size_t rows, int k);  // the operands of so many rows, and their scales behind them
 // x [rows, k] -> the layouts (GR_LAYOUT_*) that have a place
 void experts_prepare_launch(const float *x, int rows, int k, uint8_t *const *places, hipStream_t s);
-KernelRef experts_rows_kernel_ref(int fmt, int groups, bool dual);
-// w2: y = act(w x) * (w2 x); nullptr: y = w x.  chunks_most: no more of them are there
-void experts_rows_launch(int fmt, ExpertRowsArgs a, int chunks_most, hipStream_t s);
-void experts_rows_launch_k(int fmt, const ExpertRowsArgs &a, unsigned blocks, bool dual, hipStream_t s);    // experts_rows_k.hip: Q4_K, Q5_K
-void experts_rows_launch_k6(int fmt, const ExpertRowsArgs &a, unsigned blocks, bool dual, hipStream_t s);   // experts_rows_k6.hip: Q6_K, Q2_K
-void experts_rows_launch_q32(int fmt, const ExpertRowsArgs &a, unsigned blocks, bool dual, hipStream_t s);  // experts_rows_q32.hip: Q8_0, Q4_0, Q4_1, Q5_1
-KernelRef experts_rows_ref_k(int fmt, int groups, bool dual);
-KernelRef experts_rows_ref_k6(int fmt, int groups, bool dual);
-KernelRef experts_rows_ref_q32(int fmt, int groups, bool dual);
+// the kernel for chunks of so many groups of eight rows (or of the most it has, where they are more).  pair: y = act(w x) * (w2 x)
+RowsKernelRef experts_rows_kernel_ref(int fmt, int groups, bool pair);
+RowsKernelRef experts_rows_ref_k(int fmt, int groups, bool pair);    // experts_rows_k.hip: Q4_K, Q5_K
+RowsKernelRef experts_rows_ref_k6(int fmt, int groups, bool pair);   // experts_rows_k6.hip: Q6_K, Q2_K
+RowsKernelRef experts_rows_ref_q32(int fmt, int groups, bool pair);  // experts_rows_q32.hip: Q8_0, Q4_0, Q4_1, Q5_1
+// chunks_most: no more of them are there
+void experts_rows_launch(const RowsKernelRef &k, ExpertRowsArgs a, int chunks_most, hipStream_t s);
 
 // ---- experts_few.h: few tokens, INT8 products
 struct ExpertFewArgs {
@@ -79,8 +87,10 @@ struct ExpertFewArgs {
     float *y;               // up: [tokens, used, n]; down: [tokens, n] (may be res)
     int n, k, used, experts, act, blocks;
     unsigned by_rows;       // up: reciprocal of n / 4
+    RouterArgs route;       // up: logits that are there, of which every wave makes the choice for itself (and the first one leaves it at ids and weights); logits nullptr: ids are there
 };
 // whether rows of k values (up) and `used` of ffn values behind one another (down) have a kernel
+bool experts_few_chooses(int experts);  // whether the first launch can make the choices
 bool experts_few_up_supported(int fmt, int k);
 bool experts_few_down_supported(int fmt, int ffn, int used);
 void experts_few_up_launch(int fmt, ExpertFewArgs a, int tokens, int cus, hipStream_t s);
@@ -96,8 +106,9 @@ ExpertFewKernel experts_few_down_q32(int fmt, int stretches, int waves);
 void experts_value_launch(const ExpertWeights &w, int experts, const int *ids, int slots, int per_row, const float *x, float *y, hipStream_t s);
 // h [count] = act(g) * u (h may be g)
 void experts_gate_launch(int act, const float *g, const float *u, float *h, size_t count, int cus, hipStream_t s);
-// y [tokens, n] = res (or 0) + the sum over a token's places j of weights[j] * part[token x used + j]; an id outside [0, experts) counts for nothing
-void experts_combine_launch(const float *part, const int *ids, const float *weights, const float *res, float *y, int tokens, int used, int experts, int n, int cus,
+// y [tokens, n] = res (or 0) + the sum over a token's places j of weights[j] * part[token x used + j], part in `splits` arrays to be added up; an id outside
+// [0, experts) counts for nothing
+void experts_combine_launch(const float *part, int splits, const int *ids, const float *weights, const float *res, float *y, int tokens, int used, int experts, int n,
                             hipStream_t s);
 
 // ---- the epilogue of a linear, where its kernel has none: y [count] = act(y) + res (or 0)

@@ -56,6 +56,8 @@ void experts_value_launch(const ExpertWeights &w, int experts, const int *ids, i
 
 static bool quants32(int fmt) { return block_values(fmt) == 32; }
 
+bool experts_few_chooses(int experts) { return experts <= FEW_CHOICE; }
+
 bool experts_few_up_supported(int fmt, int k) {
     return (quants32(fmt) ? fmt != F_Q5_0 && k % 64 == 0 : fmt != F_Q3_K) && k <= 1024 * I8_MAX_WAVES;  // (rows of whole chunks of 64 values)
 }
@@ -105,19 +107,14 @@ void experts_prepare_launch(const float *x, int rows, int k, uint8_t *const *pla
     hipLaunchKernelGGL(experts_prepare_kernel, dim3(ncol, (rows + 7) / 8), dim3(64), 0, s, x, rows, k, o);
 }
 
-KernelRef experts_rows_kernel_ref(int fmt, int groups, bool dual) {
-    return fmt == F_Q4_K || fmt == F_Q5_K ? experts_rows_ref_k(fmt, groups, dual) : fmt == F_Q6_K || fmt == F_Q2_K ? experts_rows_ref_k6(fmt, groups, dual)
-                                                                                                                   : experts_rows_ref_q32(fmt, groups, dual);
+RowsKernelRef experts_rows_kernel_ref(int fmt, int groups, bool pair) {
+    return fmt == F_Q4_K || fmt == F_Q5_K ? experts_rows_ref_k(fmt, groups, pair) : fmt == F_Q6_K || fmt == F_Q2_K ? experts_rows_ref_k6(fmt, groups, pair)
+                                                                                                                   : experts_rows_ref_q32(fmt, groups, pair);
 }
 
-void experts_rows_launch(int fmt, ExpertRowsArgs a, int chunks_most, hipStream_t s) {
-    const bool dual = a.w2 != nullptr;
-    const int per_block = ER_WAVES * (dual ? 1 : ER_T);
-    a.nblocks = (a.n / 16 + per_block - 1) / per_block;
-    const unsigned blocks = (unsigned)a.nblocks * (unsigned)chunks_most;
-    if (fmt == F_Q4_K || fmt == F_Q5_K) experts_rows_launch_k(fmt, a, blocks, dual, s);
-    else if (fmt == F_Q6_K || fmt == F_Q2_K) experts_rows_launch_k6(fmt, a, blocks, dual, s);
-    else experts_rows_launch_q32(fmt, a, blocks, dual, s);
+void experts_rows_launch(const RowsKernelRef &k, ExpertRowsArgs a, int chunks_most, hipStream_t s) {
+    a.nblocks = (a.n / 16 + k.tiles - 1) / k.tiles;
+    hipLaunchKernelGGL(k.fn, dim3((unsigned)a.nblocks * (unsigned)a.splits * (unsigned)chunks_most), dim3(k.threads), k.lds, s, a);
 }
 
 static __global__ void __launch_bounds__(256) experts_gate_kernel(int act, const float *g, const float *__restrict__ u, float *h, size_t count4, unsigned stride) {
@@ -136,7 +133,7 @@ void experts_gate_launch(int act, const float *g, const float *u, float *h, size
 }
 
 // grid (ceil(n / 1024), tokens), 256 threads, four values each.  (res may be y)
-static __global__ void __launch_bounds__(256) experts_combine_kernel(const float *__restrict__ part, const int *__restrict__ ids, const float *__restrict__ weights, const float *res,
+static __global__ void __launch_bounds__(256) experts_combine_kernel(const float *__restrict__ part, int splits, size_t split_floats, const int *__restrict__ ids, const float *__restrict__ weights, const float *res,
                                                                      float *y, int used, int experts, int n) {
     const int t = (int)blockIdx.y, i = ((int)blockIdx.x * 256 + (int)threadIdx.x) * 4;
     if (i >= n) return;
@@ -145,7 +142,11 @@ static __global__ void __launch_bounds__(256) experts_combine_kernel(const float
         const size_t slot = (size_t)t * used + j;
         if ((unsigned)ids[slot] >= (unsigned)experts) continue;
         const float w = weights[slot];
-        const float4 p = *reinterpret_cast<const float4 *>(part + slot * n + i);
+        float4 p = *reinterpret_cast<const float4 *>(part + slot * n + i);
+        for (int z = 1; z < splits; ++z) {
+            const float4 v = *reinterpret_cast<const float4 *>(part + z * split_floats + slot * n + i);
+            p = make_float4(p.x + v.x, p.y + v.y, p.z + v.z, p.w + v.w);
+        }
         sum.x = __builtin_fmaf(w, p.x, sum.x);
         sum.y = __builtin_fmaf(w, p.y, sum.y);
         sum.z = __builtin_fmaf(w, p.z, sum.z);
@@ -158,9 +159,9 @@ static __global__ void __launch_bounds__(256) experts_combine_kernel(const float
     *reinterpret_cast<float4 *>(y + (size_t)t * n + i) = sum;
 }
 
-void experts_combine_launch(const float *part, const int *ids, const float *weights, const float *res, float *y, int tokens, int used, int experts, int n, int,
+void experts_combine_launch(const float *part, int splits, const int *ids, const float *weights, const float *res, float *y, int tokens, int used, int experts, int n,
                             hipStream_t s) {
-    hipLaunchKernelGGL(experts_combine_kernel, dim3((n + 1023) / 1024, tokens), dim3(256), 0, s, part, ids, weights, res, y, used, experts, n);
+    hipLaunchKernelGGL(experts_combine_kernel, dim3((n + 1023) / 1024, tokens), dim3(256), 0, s, part, splits, (size_t)tokens * used * n, ids, weights, res, y, used, experts, n);
 }
 
 // (any alignment: outputs and residuals of linears need none)

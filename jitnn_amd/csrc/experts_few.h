@@ -10,8 +10,11 @@
 #include "common.h"
 #include "experts.h"
 #include "gemv_i8.h"
+#include "router.h"
 
 namespace jitnn {
+
+constexpr int FEW_CHOICE = 128;  // experts of which the first kernel makes the choice itself
 
 // Turns between two joins of the waves' sums, and a wave's LDS: the digits while they are staged, then two windows of sums.
 constexpr int EF_FLUSH = 24;
@@ -66,12 +69,21 @@ __global__ void __launch_bounds__(64 * MAXW, 4) experts_few_up_kernel(const Expe
     const int c = inrow ? wave * 16 + b : chunks - 1;
     const uint32_t rowbytes = (uint32_t)(a.k / block_values(U::FMT)) * block_bytes(U::FMT);
     const typename U::Off off = U::offsets(c, (uint32_t)j * rowbytes);
-    // the token's experts, one a lane; those that are none read nothing
-    const int mine = lane < a.used ? a.ids[(size_t)token * a.used + lane] : -1;
     const float *const x = a.x + (size_t)token * a.k;
     float4 xv[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) xv[i] = reinterpret_cast<const float4 *>(x + U::x_first(c, j))[i];
+    // the token's experts, one a lane; those that are none read nothing
+    int mine;
+    if (a.route.logits) {  // (1.2 us in every wave, where a launch in front would take 4)
+        double l[FEW_CHOICE / 64];
+        load_logits(a.route, token, lane, l);
+        float weight;
+        choose_experts(a.route, l, lane, mine, weight);
+        if (blockIdx.x == 0 && wave == 0) store_choice(a.route, token, lane, mine, weight);
+    } else {
+        mine = lane < a.used ? a.ids[(size_t)token * a.used + lane] : -1;
+    }
     const int per = a.n >> 2, groups = a.used * per;  // groups of four rows: of an expert (its rows are a multiple of 32), of the token
     const int turns = 2 * ((groups + a.blocks - 1) / a.blocks);
     typename U::Raw buf[NB];

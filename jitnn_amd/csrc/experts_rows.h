@@ -14,15 +14,22 @@
 
 namespace jitnn {
 
-constexpr int ER_WAVES = 8, ER_THREADS = ER_WAVES * 64;
 constexpr int ER_OP_CHUNKS = 72;                      // 16-byte pieces of a row's operands of one column: [8 blocks and the sums][hi, lo][lane group]
 constexpr int ER_OP_BYTES = ER_OP_CHUNKS * 16;
-constexpr int ER_T = 2;                               // tiles of 16 weight rows that a wave holds: of gate and up one each
 constexpr int ER_GROUP_CHUNKS = 9 * 64;               // pieces of the operands of a group of eight rows
 
-template <int FMT>
-__host__ __device__ constexpr size_t experts_rows_lds(int groups) {
-    return (size_t)2 * groups * (ER_GROUP_CHUNKS * 16 + 8 * sizeof(float)) + (size_t)groups * 8 * 2 * sizeof(int) + (size_t)ER_WAVES * ER_T * RTile<FMT>::STAGE_BYTES;
+// A workgroup's shape: its waves, the groups of eight rows whose operands are in LDS at a time, and how many such sets a chunk has at most.
+template <int WAVES, int GS, int SETS, int PER_SIMD>
+struct RowsShape {
+    static constexpr int waves = WAVES, threads = 64 * WAVES, gs = GS, sets = SETS, groups = GS * SETS, per_simd = PER_SIMD;
+};
+// Tiles of 16 weight rows that a wave holds: two share the operands that cross LDS, one of Q6_K, which has sixteen operands a tile where the others have eight.
+template <int FMT, class S>
+__host__ __device__ constexpr int er_tiles() { return RTile<FMT>::NOPS > 8 ? 1 : 2; }
+template <int FMT, class S>
+__host__ __device__ constexpr size_t experts_rows_lds() {
+    constexpr size_t ops = (size_t)2 * S::gs * (ER_GROUP_CHUNKS * 16 + 8 * sizeof(float)), gated = er_tiles<FMT, S>() == 1 ? (size_t)S::waves / 2 * S::groups * 64 * sizeof(float2) : 0;
+    return (ops > gated ? ops : gated) + (size_t)S::groups * 8 * 2 * sizeof(int) + (size_t)S::waves * er_tiles<FMT, S>() * RTile<FMT>::STAGE_BYTES;
 }
 
 // Column c of eight rows, as rows_prepare_column, in pieces of a row: operand s (block s of the column; 8: the sums), part and lane group kq at
@@ -115,203 +122,239 @@ __device__ __forceinline__ void load_last_column(typename R::Raw &r, const typen
     if constexpr (R::REST > 0) r.c[R::FULL] = ld128_until(q + p.rest, end);
 }
 
-// grid: a.nblocks x (at least as many as there are chunks); experts_rows_lds<FMT>(a.groups) of dynamic LDS, a.groups <= GM.
-// DUAL: tile i of gate and of up, y = act(gate x) * (up x); otherwise tiles 2 i and 2 i + 1 of w.
-template <int FMT, int GM, bool DUAL>
-__global__ void __launch_bounds__(ER_THREADS) experts_rows_kernel(const ExpertRowsArgs a) {
+// grid: a.nblocks x a.splits x (at least as many as there are chunks); experts_rows_lds() of dynamic LDS, chunks of at most 8 S::groups rows.
+// DUAL: y = act(gate x) * (up x), a wave having a tile of each, or the one or the other, waves 2 i and 2 i + 1 the same rows of the two.  Otherwise a split takes its share
+// of the columns and has a y of its own.
+template <int FMT, class S, bool DUAL>
+__global__ void __launch_bounds__(S::threads, S::per_simd) experts_rows_kernel(const ExpertRowsArgs a) {
     typedef RTile<FMT> R;
-    constexpr int NOPS = R::NOPS, NI = (GM * ER_GROUP_CHUNKS + ER_THREADS - 1) / ER_THREADS;
-    constexpr int HELD = NOPS > 8 && GM > 1 ? 1 : ER_T;  // tiles whose operands a wave has at a time: of Q6_K's sixteen a tile there is room for one beside the rest
+    constexpr int NOPS = R::NOPS, T = er_tiles<FMT, S>(), NI = S::gs * ER_GROUP_CHUNKS / S::threads + 1;
     constexpr bool PARTIAL = R::BLOCK_SCALES;  // (only 32-value blocks have rows that are no whole columns)
     extern __shared__ __attribute__((aligned(16))) uint8_t er_smem[];
-    const int G = a.groups;
-    u32x4 *const ops = reinterpret_cast<u32x4 *>(er_smem);                            // [2][G][9][64]
-    float *const invs = reinterpret_cast<float *>(ops + (size_t)2 * G * ER_GROUP_CHUNKS);  // [2][G * 8]
-    uint32_t *const where = reinterpret_cast<uint32_t *>(invs + 2 * G * 8);           // [G * 8] a row's operands, in columns from the first one's
-    int *const slots = reinterpret_cast<int *>(where + G * 8);                        // [G * 8]
+    uint8_t *stage = er_smem;                                                                    // per wave: T tiles' bytes of a column
+    uint32_t *const where = reinterpret_cast<uint32_t *>(er_smem + (size_t)S::waves * T * R::STAGE_BYTES);  // [groups * 8] a row's operands, in columns from the first one's
+    int *const slots = reinterpret_cast<int *>(where + S::groups * 8);                           // [groups * 8]
+    u32x4 *const ops = reinterpret_cast<u32x4 *>(slots + S::groups * 8);                         // [2][gs][9][64]
+    float *const invs = reinterpret_cast<float *>(ops + (size_t)2 * S::gs * ER_GROUP_CHUNKS);    // [2][gs * 8]
     const int tid = threadIdx.x, lane = tid & 63, kq = lane >> 4, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    uint8_t *const stage = reinterpret_cast<uint8_t *>(slots + G * 8) + (size_t)wave * ER_T * R::STAGE_BYTES;
-    const int u = (int)blockIdx.x / a.nblocks, block = (int)blockIdx.x - u * a.nblocks;
+    stage += (size_t)wave * T * R::STAGE_BYTES;
+    const int per_chunk = a.nblocks * a.splits, u = (int)blockIdx.x / per_chunk, of_chunk = (int)blockIdx.x - u * per_chunk, split = of_chunk / a.nblocks,
+              block = of_chunk - split * a.nblocks;
     if (u >= a.chunks->x) return;
     const int4 ch = a.chunks[1 + u];  // expert, place of its first row in the list, rows
-    const int ncol = (a.k + 255) >> 8, groups = (ch.z + 7) >> 3, items = groups * ER_GROUP_CHUNKS;
+    const int ncol = (a.k + 255) >> 8, groups = (ch.z + 7) >> 3, sets = (groups + S::gs - 1) / S::gs;
+    const int c0 = (int)((long long)ncol * split / a.splits), c1 = (int)((long long)ncol * (split + 1) / a.splits);
 
-    // the weights on their way first: column 0 of this wave's tiles
+    const int slot = a.list[ch.y + min(min(tid, S::groups * 8 - 1), ch.z - 1)];  // (a place without a row takes the last one again: computed, not stored)
+    static_assert(S::groups * 8 <= S::threads, "a thread for each row");
+    // the weights on their way: the first column of this wave's tiles
     const size_t rowbytes = (size_t)(a.k / block_values(FMT)) * block_bytes(FMT);
     const uint8_t *const w0 = a.w + (size_t)ch.x * a.expert_bytes, *const w1 = DUAL ? a.w2 + (size_t)ch.x * a.expert_bytes : w0;
-    const int ntiles = a.n >> 4, tile = (block * ER_WAVES + wave) * (DUAL ? 1 : ER_T);
+    const int ntiles = a.n >> 4, first = block * S::waves + wave;
+    const int tile = DUAL ? (T == 2 ? first : first >> 1) : first * T;  // of this wave (T 2 without DUAL: and the next one)
+    const bool second = DUAL && T == 1 && (wave & 1);                   // a wave with a tile of up
     const uint8_t *const end0 = a.w + (size_t)a.experts * a.expert_bytes, *const end1 = DUAL ? a.w2 + (size_t)a.experts * a.expert_bytes : end0;
-    typename R::Ptr ptr[ER_T];
-    typename R::Raw raw[ER_T];
-    ptr[0] = R::ptr(w0, min(tile, ntiles - 1) * 16, rowbytes, lane);
-    ptr[1] = R::ptr(w1, min(DUAL ? tile : tile + 1, ntiles - 1) * 16, rowbytes, lane);
+    typename R::Ptr ptr[T];
+    typename R::Raw raw[T];
+#pragma unroll
+    for (int t = 0; t < T; ++t) ptr[t] = R::ptr(second || (DUAL && t) ? w1 : w0, min(DUAL ? tile : tile + t, ntiles - 1) * 16, rowbytes, lane);
     const int last_blocks = PARTIAL ? (a.k & 255) >> 5 : 0;  // of the last column, where it is none of eight
     auto fetch = [&](int c) {
         if (PARTIAL && last_blocks && c == ncol - 1) {
-            load_last_column<R>(raw[0], ptr[0], c, end0);
-            load_last_column<R>(raw[1], ptr[1], c, end1);
+#pragma unroll
+            for (int t = 0; t < T; ++t) load_last_column<R>(raw[t], ptr[t], c, second || (DUAL && t) ? end1 : end0);
             return;
         }
-        R::load(raw[0], ptr[0], c);
-        R::load(raw[1], ptr[1], c);
+#pragma unroll
+        for (int t = 0; t < T; ++t) R::load(raw[t], ptr[t], c);
     };
-    fetch(0);
-    if (tid < groups * 8) {  // (a place without a row takes the last one again: computed, not stored)
-        const int slot = a.list[ch.y + min(tid, ch.z - 1)];
+    fetch(c0);
+    if (tid < S::groups * 8) {
         slots[tid] = slot;
         where[tid] = (uint32_t)(slot / a.per_row) * (uint32_t)ncol;
     }
     __syncthreads();
-    // piece i of this thread: lane l of operand s of group g, whose row is that of l's place
-    uint32_t from[NI];
+    // Piece i of this thread: lane l of operand s of group g of a set, whose row is that of l's place.  What the whole rounds leave is shared out over the waves, a few
+    // lanes each, the others doing what the last of those does; and a group that the chunk has not is the last row's again: no load stands behind a condition,
+    // for at the end of one the compiler waits for what was asked for before it.
+    constexpr int ROUNDS = NI - 1, SHARE = (S::gs * ER_GROUP_CHUNKS - ROUNDS * S::threads) / S::waves;
+    static_assert(SHARE >= 1 && SHARE <= 64 && SHARE * S::waves == S::gs * ER_GROUP_CHUNKS - ROUNDS * S::threads, "whole lanes");
+    uint32_t from[NI];   // one set: where it stands in column 0; several: of the row in its set | where in the row's operands << 16
+    int to[NI];
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-        const int idx = min(tid + i * ER_THREADS, items - 1), g = idx / ER_GROUP_CHUNKS, rest = idx - g * ER_GROUP_CHUNKS, s = rest >> 6, l = rest & 63;
-        from[i] = where[g * 8 + ((l & 15) >> 1)] * (uint32_t)ER_OP_BYTES + (uint32_t)(s * 128 + (l & 1) * 64 + (l >> 4) * 16);
+        const int idx = i < ROUNDS ? tid + i * S::threads : ROUNDS * S::threads + wave * SHARE + min(lane, SHARE - 1);
+        const int g = idx / ER_GROUP_CHUNKS, rest = idx - g * ER_GROUP_CHUNKS, s = rest >> 6, l = rest & 63;
+        const uint32_t row = (uint32_t)(g * 8 + ((l & 15) >> 1)), piece = (uint32_t)(s * 128 + (l & 1) * 64 + (l >> 4) * 16);
+        from[i] = S::sets == 1 ? where[row] * (uint32_t)ER_OP_BYTES + piece : row | piece << 16;
+        to[i] = idx;
     }
-    const uint32_t inv_from = tid < groups * 8 ? where[tid] : 0u;
+    const int inv_row = min(tid, S::gs * 8 - 1);
+    const uint32_t inv_from = where[inv_row];
     u32x4 next[NI];
-    float next_inv = 0.f;
-    auto ask = [&](int c) {
+    float next_inv;
+    auto ask = [&](int c, int set) {
 #pragma unroll
-        for (int i = 0; i < NI; ++i)
-            if (i == 0 || wave * 64 + i * ER_THREADS < items) next[i] = *reinterpret_cast<const u32x4 *>(a.ops + from[i] + (size_t)c * ER_OP_BYTES);
-        if (tid < groups * 8) next_inv = a.inv[inv_from + c];
+        for (int i = 0; i < NI; ++i) {
+            if constexpr (S::sets == 1) next[i] = *reinterpret_cast<const u32x4 *>(a.ops + (size_t)c * ER_OP_BYTES + from[i]);
+            else next[i] = *reinterpret_cast<const u32x4 *>(a.ops + (size_t)(where[set * S::gs * 8 + (from[i] & 0xffffu)] + (uint32_t)c) * ER_OP_BYTES + (from[i] >> 16));
+        }
+        next_inv = a.inv[(S::sets == 1 ? inv_from : where[set * S::gs * 8 + inv_row]) + (uint32_t)c];
     };
-    ask(0);
+    ask(c0, 0);
 
-    float2 acc[ER_T][GM];
+    float2 acc[T][S::groups];
 #pragma unroll
-    for (int t = 0; t < ER_T; ++t)
+    for (int t = 0; t < T; ++t)
 #pragma unroll
-        for (int g = 0; g < GM; ++g) acc[t][g] = make_float2(0.f, 0.f);
-    for (int c = 0; c < ncol; ++c) {
-        // this column's operands into the buffer that nobody reads any more: every wave has passed the barrier of the column before, behind its products of the
-        // one before that
-        u32x4 *const op = ops + (size_t)(c & 1) * G * ER_GROUP_CHUNKS;
-        float *const iv = invs + (c & 1) * G * 8;
+        for (int g = 0; g < S::groups; ++g) acc[t][g] = make_float2(0.f, 0.f);
+    int buffer = 0;
+    // A set's operands into the buffer that nobody reads any more: every wave has passed the barrier of the set before, behind its products of the one before that.
+    auto put = [&]() {
+        u32x4 *const op = ops + (size_t)buffer * S::gs * ER_GROUP_CHUNKS;
 #pragma unroll
-        for (int i = 0; i < NI; ++i)
-            if (wave * 64 + i * ER_THREADS < items) op[tid + i * ER_THREADS] = next[i];
-        if (tid < groups * 8) iv[tid] = next_inv;
-        const uint8_t *row[ER_T];
-        uint32_t tail[ER_T];
+        for (int i = 0; i < NI; ++i) op[to[i]] = next[i];
+        if (tid < S::gs * 8) invs[buffer * S::gs * 8 + tid] = next_inv;
+        buffer ^= 1;
+    };
+    for (int c = c0; c < c1; ++c) {
+        f16x8 B[T][NOPS], Bm[T];
+        float d[T], dmin64[T], dblk[R::BLOCK_SCALES ? T : 1][8];
+        const uint8_t *row[T];
+        uint32_t tail[T];
 #pragma unroll
-        for (int t = 0; t < ER_T; ++t) {
+        for (int t = 0; t < T; ++t) {
             row[t] = R::park(raw[t], stage + t * R::STAGE_BYTES, lane);
             tail[t] = raw[t].tail;
         }
-        if (c + 1 < ncol) {
-            fetch(c + 1);
-            ask(c + 1);
-        }
-        f16x8 B[HELD][NOPS], Bm[HELD];
-        float d[HELD], dmin64[HELD], dblk[R::BLOCK_SCALES ? HELD : 1][8];
-        auto decode = [&](int t, int h) {
+        put();  // (in front of the request for the next weights: loads come back in order, and a wait for these would be one for those)
+        if (c + 1 < c1) fetch(c + 1);
+        auto decode = [&](int t) {
             if constexpr (R::BLOCK_SCALES) {
-                R::decode(row[t], tail[t], lane, B[h], Bm[h], dblk[h]);
+                R::decode(row[t], tail[t], lane, B[t], Bm[t], dblk[t]);
                 if (PARTIAL && last_blocks && c == ncol - 1) {  // (their operands are zero, what stands there need not be a number)
 #pragma unroll
                     for (int s = 0; s < 8; ++s) {
-                        dblk[h][s] = s < last_blocks ? dblk[h][s] : 0.f;
-                        Bm[h][s] = s < last_blocks ? Bm[h][s] : (_Float16)0.f;
+                        dblk[t][s] = s < last_blocks ? dblk[t][s] : 0.f;
+                        Bm[t][s] = s < last_blocks ? Bm[t][s] : (_Float16)0.f;
                     }
                 }
             } else {
                 float dm;
-                R::decode(row[t], tail[t], lane, B[h], Bm[h], d[h], dm);
-                dmin64[h] = dm * 64.f;
+                R::decode(row[t], tail[t], lane, B[t], Bm[t], d[t], dm);
+                dmin64[t] = dm * 64.f;
             }
         };
-        // the products of tiles t0 .. t0 + HELD - 1 with every group
-        auto multiply = [&](int t0) {
 #pragma unroll
-            for (int g = 0; g < GM; ++g) {
-                if (g >= groups) break;
+        for (int t = 0; t < T; ++t) decode(t);
+#pragma unroll
+        for (int set = 0; set < S::sets; ++set) {
+            if (set < sets) {
+            if (set > 0) put();
+            const u32x4 *const op = ops + (size_t)(buffer ^ 1) * S::gs * ER_GROUP_CHUNKS;
+            const float *const iv = invs + (buffer ^ 1) * S::gs * 8;
+            const bool more = set + 1 < sets;
+            ask(more ? c : min(c + 1, c1 - 1), more ? set + 1 : 0);  // (behind the last one: that one again)
+            __syncthreads();
+#pragma unroll
+            for (int gi = 0; gi < S::gs; ++gi) {
+                const int g = set * S::gs + gi;
+                if (g < groups) {
                 f16x8 A[9];
 #pragma unroll
-                for (int s = 0; s < 9; ++s) A[s] = __builtin_bit_cast(f16x8, op[(g * 9 + s) * 64 + lane]);
-                const float2 w = *reinterpret_cast<const float2 *>(iv + g * 8 + 2 * kq);
+                for (int s = 0; s < 9; ++s) A[s] = __builtin_bit_cast(f16x8, op[(gi * 9 + s) * 64 + lane]);
+                const float2 w = *reinterpret_cast<const float2 *>(iv + gi * 8 + 2 * kq);
 #pragma unroll
-                for (int h = 0; h < HELD; ++h) {
+                for (int t = 0; t < T; ++t) {
                     float u0, u1;
                     if constexpr (R::BLOCK_SCALES) {
                         u0 = u1 = 0.f;
 #pragma unroll
                         for (int s = 0; s < 8; ++s) {
-                            const f32x4 cs = mfma16(A[s], B[h][s]);
-                            u0 = __builtin_fmaf(dblk[h][s], cs[0] + cs[1], u0);
-                            u1 = __builtin_fmaf(dblk[h][s], cs[2] + cs[3], u1);
+                            const f32x4 cs = mfma16(A[s], B[t][s]);
+                            u0 = __builtin_fmaf(dblk[t][s], cs[0] + cs[1], u0);
+                            u1 = __builtin_fmaf(dblk[t][s], cs[2] + cs[3], u1);
                         }
                         if constexpr (R::MINS) {
-                            const f32x4 cm = mfma16(A[8], Bm[h]);
+                            const f32x4 cm = mfma16(A[8], Bm[t]);
                             u0 = __builtin_fmaf(64.f, cm[0] + cm[1], u0);
                             u1 = __builtin_fmaf(64.f, cm[2] + cm[3], u1);
                         }
                     } else {
                         f32x4 cs = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                        for (int s = 0; s < NOPS; ++s) cs = __builtin_amdgcn_mfma_f32_16x16x32_f16(A[R::aidx(s)], B[h][s], cs, 0, 0, 0);
-                        const f32x4 cm = mfma16(A[8], Bm[h]);
+                        for (int s = 0; s < NOPS; ++s) cs = __builtin_amdgcn_mfma_f32_16x16x32_f16(A[R::aidx(s)], B[t][s], cs, 0, 0, 0);
+                        const f32x4 cm = mfma16(A[8], Bm[t]);
                         const float s0 = cs[0] + cs[1], s1 = cs[2] + cs[3], m0 = cm[0] + cm[1], m1 = cm[2] + cm[3];
-                        u0 = __builtin_fmaf(d[h], s0, -dmin64[h] * m0);
-                        u1 = __builtin_fmaf(d[h], s1, -dmin64[h] * m1);
+                        u0 = __builtin_fmaf(d[t], s0, -dmin64[t] * m0);
+                        u1 = __builtin_fmaf(d[t], s1, -dmin64[t] * m1);
                     }
-                    acc[t0 + h][g].x = __builtin_fmaf(w.x, u0, acc[t0 + h][g].x);
-                    acc[t0 + h][g].y = __builtin_fmaf(w.y, u1, acc[t0 + h][g].y);
+                    acc[t][g].x = __builtin_fmaf(w.x, u0, acc[t][g].x);
+                    acc[t][g].y = __builtin_fmaf(w.y, u1, acc[t][g].y);
                 }
                 // (the operands and products of one group at a time: of more than one there are no registers)
 #pragma unroll
-                for (int h = 0; h < HELD; ++h) asm volatile("" : "+v"(acc[t0 + h][g].x), "+v"(acc[t0 + h][g].y));
+                for (int t = 0; t < T; ++t) asm volatile("" : "+v"(acc[t][g].x), "+v"(acc[t][g].y));
                 __builtin_amdgcn_sched_barrier(0);
+                }
             }
-        };
-        if constexpr (HELD == ER_T) {
-#pragma unroll
-            for (int t = 0; t < ER_T; ++t) decode(t, t);
-            __syncthreads();
-            multiply(0);
-        } else {
-            decode(0, 0);
-            __syncthreads();
-            multiply(0);
-            decode(1, 0);
-            multiply(1);
+            }
         }
     }
+    float *const y0 = a.y + (DUAL ? 0 : (size_t)split * a.split_floats);
+    float2 *const other = reinterpret_cast<float2 *>(ops) + (size_t)(wave >> 1) * S::groups * 64 + lane;
+    if constexpr (DUAL && T == 1) {
+        __syncthreads();
+        if (second) {
 #pragma unroll
-    for (int g = 0; g < GM; ++g) {
-        if (g >= groups) break;
+            for (int g = 0; g < S::groups; ++g) other[g * 64] = acc[0][g];
+        }
+        __syncthreads();
+        if (second) return;
+    }
+#pragma unroll
+    for (int g = 0; g < S::groups; ++g) {
+        if (g >= groups) continue;
+        const float2 up = DUAL ? (T == 1 ? other[g * 64] : acc[T - 1][g]) : acc[T - 1][g];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
             const int b = g * 8 + 2 * kq + r;
             if (b >= ch.z) continue;
-            float *const y = a.y + (size_t)slots[b] * a.n + (lane & 15);
-            const float v0 = r ? acc[0][g].y : acc[0][g].x, v1 = r ? acc[1][g].y : acc[1][g].x;
-            if (DUAL) {
-                if (tile < ntiles) y[tile * 16] = activate(a.act, v0) * v1;
-            } else {
-                if (tile < ntiles) y[tile * 16] = v0;
-                if (tile + 1 < ntiles) y[tile * 16 + 16] = v1;
-            }
+            float *const y = y0 + (size_t)slots[b] * a.n + (lane & 15);
+            const float v0 = r ? acc[0][g].y : acc[0][g].x, v1 = r ? up.y : up.x;
+            if (tile < ntiles) y[tile * 16] = DUAL ? activate(a.act, v0) * v1 : v0;
+            if (!DUAL && T == 2 && tile + 1 < ntiles) y[tile * 16 + 16] = v1;
         }
     }
 }
 
-// groups: the largest that the LDS of a workgroup holds two buffers of, at most 5
-template <int FMT>
-static KernelRef experts_rows_pick(int groups, bool dual) {
-    const void *fn = groups == 1 ? (dual ? (const void *)experts_rows_kernel<FMT, 1, true> : (const void *)experts_rows_kernel<FMT, 1, false>)
-                     : groups == 2 ? (dual ? (const void *)experts_rows_kernel<FMT, 2, true> : (const void *)experts_rows_kernel<FMT, 2, false>)
-                                   : (dual ? (const void *)experts_rows_kernel<FMT, 5, true> : (const void *)experts_rows_kernel<FMT, 5, false>);
-    return {fn, experts_rows_lds<FMT>(groups)};
-}
+// The shapes, by the groups of a chunk: one or two, whose operands LDS holds whole; many, in sets of four.  (32 tokens of which each meets eight of 128 experts, gate and up of
+// 2048 x 768 / down: workgroups of eight waves 64 us in Q4_K and 62 in Q6_K, of four waves 82 and 62; five tokens, six of 64 experts of 2048 x 1408 in Q8_0 82 and 34 against 64 and 32, where
+// eight waves leave a second round nearly empty)
+typedef RowsShape<8, 1, 1, 2> RowsShape1;
+typedef RowsShape<4, 1, 1, 2> RowsShape1Short;
+typedef RowsShape<8, 2, 1, 2> RowsShape2;
+typedef RowsShape<8, 4, 2, 2> RowsShape8;
+typedef RowsShape<8, 4, 3, 2> RowsShape12;
 
+template <int FMT, class S>
+static RowsKernelRef experts_rows_shape(bool dual) {
+    const RowsKernel fn = dual ? experts_rows_kernel<FMT, S, true> : experts_rows_kernel<FMT, S, false>;
+    // (weight rows of a workgroup: its waves' tiles; of a pair of matrices half as many of each)
+    return {fn, experts_rows_lds<FMT, S>(), S::threads, S::waves * er_tiles<FMT, S>() / (dual ? 2 : 1), S::groups};
+}
+// groups: of a chunk, at most 8, of K-quants 12
 template <int FMT>
-static void experts_rows_go(const ExpertRowsArgs &a, unsigned blocks, bool dual, hipStream_t s) {
-    typedef void (*Kernel)(const ExpertRowsArgs);
-    const KernelRef k = experts_rows_pick<FMT>(a.groups, dual);
-    hipLaunchKernelGGL((Kernel)k.fn, dim3(blocks), dim3(ER_THREADS), k.lds, s, a);
+static RowsKernelRef experts_rows_pick(int groups, bool dual) {
+    if (groups <= 1) {
+        if constexpr (RTile<FMT>::BLOCK_SCALES) return experts_rows_shape<FMT, RowsShape1Short>(dual);
+        else return experts_rows_shape<FMT, RowsShape1>(dual);
+    }
+    if (groups <= 2) return experts_rows_shape<FMT, RowsShape2>(dual);
+    if constexpr (!RTile<FMT>::BLOCK_SCALES) {  // (sixteen groups' sums and 32-value blocks' scales do not fit the registers)
+        if (groups > 8) return experts_rows_shape<FMT, RowsShape12>(dual);
+    }
+    return experts_rows_shape<FMT, RowsShape8>(dual);
 }
 
 }  // namespace jitnn

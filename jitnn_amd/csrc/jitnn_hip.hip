@@ -2385,10 +2385,25 @@ int moe_pass_tokens(const jitnn_hip_moe *m) { return std::max(1, MOE_PASS_SLOTS 
 bool experts_on_rows(const jitnn_hip_weight *w) { return gemv_rows_supported(w->fmt); }  // (Q5_0 and Q3_K blocks that were not rewritten have no operands)
 
 // Groups of eight rows in a chunk of an expert's: what most experts have where every one is as likely as any other, so that their weights are read
-// once; at most five, whose operands LDS holds twice.
+// and decoded once; at most what the kernels hold.
 int moe_groups(const jitnn_hip_moe *m, int tokens) {
     const double mean = (double)tokens * m->router->used / m->router->experts;
-    return std::max(1, std::min(5, (int)std::ceil((mean + 2 * std::sqrt(mean)) / 8)));
+    int groups = std::max(1, (int)std::ceil((mean + 2 * std::sqrt(mean)) / 8));
+    for (const jitnn_hip_weight *w : {m->gate, m->up, m->down})
+        if (experts_on_rows(w)) groups = std::min(groups, experts_rows_kernel_ref(w->fmt, groups, false).groups);
+    return groups;
+}
+
+// Shares of the down projection's columns, where its workgroups alone would leave CUs idle: expected chunks x blocks against a workgroup for every CU (two of
+// the small ones).
+int moe_splits(const jitnn_hip_moe *m, int tokens, int groups) {
+    if (!experts_on_rows(m->down)) return 1;
+    const jitnn_hip_router *r = m->router;
+    const RowsKernelRef k = experts_rows_kernel_ref(m->down->fmt, groups, false);
+    const double mean = (double)tokens * r->used / r->experts, met = r->experts * (1 - std::pow(1 - (double)r->used / r->experts, tokens)),
+                 blocks = met * std::max(1.0, mean / (8 * groups)) * ((r->d / 16 + k.tiles - 1) / k.tiles);
+    const int ncol = (m->ffn + 255) / 256, wanted = (int)std::ceil((k.threads > 256 ? 1.0 : 2.0) * g.cus / blocks);
+    return std::max(1, std::min({wanted, 8, ncol / 4}));
 }
 
 // Few tokens: the INT8 products on the raw quants, for weights whose rows are whole chunks of 64 values.
@@ -2403,7 +2418,7 @@ bool moe_few(const jitnn_hip_moe *m, int tokens) {
 struct MoeLayout {
     size_t logits, ids, weights, list, chunks, ops[GR_LAYOUTS], h_ops, g, u, part, total;
     bool layouts[GR_LAYOUTS];  // of x that gate and up ask for
-    int groups, chunks_most;
+    int groups, splits, chunks_most;
     bool few;
 };
 MoeLayout moe_layout(const jitnn_hip_moe *m, int tokens) {
@@ -2418,8 +2433,9 @@ MoeLayout moe_layout(const jitnn_hip_moe *m, int tokens) {
     };
     l.few = moe_few(m, tokens);
     l.groups = moe_groups(m, tokens);
+    l.splits = moe_splits(m, tokens, l.groups);
     l.chunks_most = ExpertLists::chunks_most((int)slots, r->experts, 8 * l.groups);
-    l.logits = take((size_t)tokens * r->experts * sizeof(double));
+    l.logits = take(router_logits_bytes(tokens, r->experts, r->d, false));
     l.ids = take(slots * sizeof(int));
     l.weights = take(slots * sizeof(float));
     l.g = take(slots * m->ffn * sizeof(float));
@@ -2432,7 +2448,7 @@ MoeLayout moe_layout(const jitnn_hip_moe *m, int tokens) {
     for (int i = 0; i < GR_LAYOUTS; ++i) l.ops[i] = l.layouts[i] ? take(experts_ops_bytes(tokens, r->d)) : 0;
     l.h_ops = take(experts_on_rows(m->down) ? experts_ops_bytes(slots, m->ffn) : 0);
     l.u = take(slots * m->ffn * sizeof(float));
-    l.part = take(slots * r->d * sizeof(float));
+    l.part = take(slots * r->d * l.splits * sizeof(float));
     l.total = at;
     return l;
 }
@@ -2479,8 +2495,9 @@ int check_moe_call(const jitnn_hip_moe *m, const float *x, int tokens, const flo
     return check_ready();
 }
 
-// One pass: the experts of `tokens` tokens for given choices, whose lists are made.
-int moe_experts(const jitnn_hip_moe *m, const float *x, int tokens, const int *ids, const float *weights, const float *res, float *y, uint8_t *ws, const MoeLayout &l,
+// One pass: the experts of `tokens` tokens for given choices, whose lists are made.  to_choose (few tokens): the choices are still to be made, of these logits, and go to ids and
+// weights.
+int moe_experts(const jitnn_hip_moe *m, const float *x, int tokens, const int *ids, const float *weights, const RouterArgs *to_choose, const float *res, float *y, uint8_t *ws, const MoeLayout &l,
                 hipStream_t s) {
     const jitnn_hip_router *r = m->router;
     const int slots = tokens * r->used;
@@ -2500,6 +2517,7 @@ int moe_experts(const jitnn_hip_moe *m, const float *x, int tokens, const int *i
         a.used = r->used;
         a.experts = r->experts;
         a.act = m->act;
+        if (to_choose) a.route = *to_choose;
         experts_few_up_launch(m->gate->fmt, a, tokens, g.cus, s);
         e = expert_weights(m->down, r->experts);
         a.w = m->down->dev;
@@ -2514,7 +2532,7 @@ int moe_experts(const jitnn_hip_moe *m, const float *x, int tokens, const int *i
         return JITNN_HIP_OK;
     }
     // out [slots, n] = the products of w (with w2: of both, gated) with rows [rows, k], whose operands stand at ops
-    auto rows = [&](const jitnn_hip_weight *w, const jitnn_hip_weight *w2, const uint8_t *ops, int count, int per_row, float *out) -> int {
+    auto rows = [&](const jitnn_hip_weight *w, const jitnn_hip_weight *w2, const uint8_t *ops, int count, int per_row, int splits, float *out) -> int {
         const ExpertWeights e = expert_weights(w, r->experts);
         ExpertRowsArgs a{};
         a.w = w->dev;
@@ -2530,10 +2548,11 @@ int moe_experts(const jitnn_hip_moe *m, const float *x, int tokens, const int *i
         a.experts = r->experts;
         a.per_row = per_row;
         a.act = m->act;
-        a.groups = l.groups;
-        const KernelRef k = experts_rows_kernel_ref(w->fmt, l.groups, w2 != nullptr);
-        if (int rc = allow_lds(k.fn, k.lds)) return rc;
-        experts_rows_launch(w->fmt, a, l.chunks_most, s);
+        a.splits = splits;
+        a.split_floats = (size_t)slots * e.n;
+        const RowsKernelRef k = experts_rows_kernel_ref(w->fmt, l.groups, w2 != nullptr);
+        if (int rc = allow_lds((const void *)k.fn, k.lds)) return rc;
+        experts_rows_launch(k, a, l.chunks_most, s);
         return JITNN_HIP_OK;
     };
     uint8_t *places[GR_LAYOUTS] = {};
@@ -2541,13 +2560,13 @@ int moe_experts(const jitnn_hip_moe *m, const float *x, int tokens, const int *i
     if (places[0] || places[1] || places[2]) experts_prepare_launch(x, tokens, r->d, places, s);
     const bool pair = experts_on_rows(m->gate) && m->gate->fmt == m->up->fmt;
     if (pair) {
-        if (int rc = rows(m->gate, m->up, places[gemv_rows_layout(m->gate->fmt)], tokens, r->used, gb)) return rc;
+        if (int rc = rows(m->gate, m->up, places[gemv_rows_layout(m->gate->fmt)], tokens, r->used, 1, gb)) return rc;
     } else {
         const jitnn_hip_weight *ws2[2] = {m->gate, m->up};
         float *outs[2] = {gb, ub};
         for (int i = 0; i < 2; ++i) {
             if (!experts_on_rows(ws2[i])) experts_value_launch(expert_weights(ws2[i], r->experts), r->experts, ids, slots, r->used, x, outs[i], s);
-            else if (int rc = rows(ws2[i], nullptr, places[gemv_rows_layout(ws2[i]->fmt)], tokens, r->used, outs[i])) return rc;
+            else if (int rc = rows(ws2[i], nullptr, places[gemv_rows_layout(ws2[i]->fmt)], tokens, r->used, 1, outs[i])) return rc;
         }
         experts_gate_launch(m->act, gb, ub, gb, (size_t)slots * m->ffn, g.cus, s);
     }
@@ -2555,11 +2574,11 @@ int moe_experts(const jitnn_hip_moe *m, const float *x, int tokens, const int *i
         uint8_t *h_places[GR_LAYOUTS] = {};
         h_places[gemv_rows_layout(m->down->fmt)] = ws + l.h_ops;
         experts_prepare_launch(gb, slots, m->ffn, h_places, s);
-        if (int rc = rows(m->down, nullptr, ws + l.h_ops, slots, 1, part)) return rc;
+        if (int rc = rows(m->down, nullptr, ws + l.h_ops, slots, 1, l.splits, part)) return rc;
     } else {
         experts_value_launch(expert_weights(m->down, r->experts), r->experts, ids, slots, 1, gb, part, s);
     }
-    experts_combine_launch(part, ids, weights, res, y, tokens, r->used, r->experts, r->d, g.cus, s);
+    experts_combine_launch(part, l.splits, ids, weights, res, y, tokens, r->used, r->experts, r->d, s);
     HIP_TRY(hipGetLastError());
     return JITNN_HIP_OK;
 }
@@ -2613,7 +2632,7 @@ long long jitnn_hip_router_workspace(const jitnn_hip_router *r, int tokens) {
     if (tokens < 0) return fail(JITNN_HIP_EINVAL, "tokens = %d", tokens);
     long long most = 0;  // (a shorter last pass may need what a longer one does not)
     for (const int t : {std::min(tokens, ROUTER_PASS), tokens % ROUTER_PASS})
-        if (t && router_needs_logits(t, r->experts, r->d, false)) most = std::max(most, (long long)t * r->experts * (long long)sizeof(double));
+        if (t) most = std::max(most, (long long)router_logits_bytes(t, r->experts, r->d, true));
     return most;
 }
 
@@ -2676,9 +2695,11 @@ int jitnn_hip_moe_dev(const jitnn_hip_moe *m, const float *x_dev, int tokens, co
         const MoeLayout l = moe_layout(m, count);
         const float *x = x_dev + (size_t)t * d;
         RouterArgs a = router_args(m->router, x, count, (int *)(ws + l.ids), (float *)(ws + l.weights), ws + l.logits);
+        const bool choose_there = l.few && experts_few_chooses(a.experts);
         if (!l.few) a.lists = moe_lists(ws, l);
-        router_launch(a, (hipStream_t)stream);
-        if (int rc = moe_experts(m, x, count, (const int *)(ws + l.ids), (const float *)(ws + l.weights), residual_dev ? residual_dev + (size_t)t * d : nullptr, y_dev + (size_t)t * d,
+        if (choose_there) router_logits_launch(a, (hipStream_t)stream);
+        else router_launch(a, (hipStream_t)stream);
+        if (int rc = moe_experts(m, x, count, (const int *)(ws + l.ids), (const float *)(ws + l.weights), choose_there ? &a : nullptr, residual_dev ? residual_dev + (size_t)t * d : nullptr, y_dev + (size_t)t * d,
                                  ws, l, (hipStream_t)stream))
             return rc;
     }
@@ -2695,7 +2716,7 @@ int jitnn_hip_moe_experts_dev(const jitnn_hip_moe *m, const float *x_dev, int to
         const MoeLayout l = moe_layout(m, count);
         const int *ids = ids_dev + (size_t)t * used;
         if (!l.few) expert_lists_launch(ids, count * used, m->router->experts, moe_lists((uint8_t *)workspace_dev, l), (hipStream_t)stream);
-        if (int rc = moe_experts(m, x_dev + (size_t)t * d, count, ids, weights_dev + (size_t)t * used, residual_dev ? residual_dev + (size_t)t * d : nullptr,
+        if (int rc = moe_experts(m, x_dev + (size_t)t * d, count, ids, weights_dev + (size_t)t * used, nullptr, residual_dev ? residual_dev + (size_t)t * d : nullptr,
                                  y_dev + (size_t)t * d, (uint8_t *)workspace_dev, l, (hipStream_t)stream))
             return rc;
     }

@@ -1,29 +1,238 @@
-// Launches of the router of a mixture of experts.
+// The router of a mixture of experts: its logits, the choices of a batch and the lists of what each expert gets.
 #include "router.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace jitnn {
 
+typedef double f64x4 __attribute__((ext_vector_type(4)));
+
+// The share of one wave in a logit: quads first, first + step, ... of a row.
+__device__ __forceinline__ double router_dot(const float *__restrict__ x, const float *__restrict__ w, int d, int first, int step) {
+    double acc[4] = {0, 0, 0, 0};
+    int i = 4 * first;
+    step *= 4;
+    for (; i + 3 * step < d; i += 4 * step) {
+        float4 xv[4], wv[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            xv[j] = *reinterpret_cast<const float4 *>(x + i + step * j);
+            wv[j] = *reinterpret_cast<const float4 *>(w + i + step * j);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            acc[j] = fma((double)xv[j].w, (double)wv[j].w, fma((double)xv[j].z, (double)wv[j].z, fma((double)xv[j].y, (double)wv[j].y, fma((double)xv[j].x, (double)wv[j].x, acc[j]))));
+    }
+    for (; i < d; i += step) {
+        const float4 xv = *reinterpret_cast<const float4 *>(x + i), wv = *reinterpret_cast<const float4 *>(w + i);
+        acc[0] = fma((double)xv.w, (double)wv.w, fma((double)xv.z, (double)wv.z, fma((double)xv.y, (double)wv.y, fma((double)xv.x, (double)wv.x, acc[0]))));
+    }
+    return wave_sum64((acc[0] + acc[1]) + (acc[2] + acc[3]));
+}
+
+// Few tokens: a workgroup per logit, whose four waves share out the row.  grid (experts, tokens), 256 threads.
+__global__ void __launch_bounds__(256) router_logits_kernel(const RouterArgs a) {
+    __shared__ double sums[4];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), e = (int)blockIdx.x;
+    const double l = router_dot(a.x + (size_t)blockIdx.y * a.d, a.w + (size_t)e * a.d, a.d, (int)threadIdx.x, 256);
+    if (lane == 0) sums[wave] = l;
+    __syncthreads();
+    if (threadIdx.x == 0) a.logits[(size_t)blockIdx.y * a.experts + e] = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+}
+
+// Many tokens: a workgroup's tile is 16 tokens x 16 experts, its four waves share out the values of its share of a row (a.splits of them along blockIdx.z, each with logits of
+// its own), sixteen at a time: lane r + 16 q holds four consecutive values of row r, and product i of a step takes value i of each - the same four places of x and W, in
+// whatever order.  grid (ceil(tokens / 16), ceil(experts / 16), a.splits), 256 threads.
+__global__ void __launch_bounds__(256) router_tiles_kernel(const RouterArgs a) {
+    __shared__ f64x4 sums[3][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), r = lane & 15, q = lane >> 4;
+    const int t0 = (int)blockIdx.x * 16, e0 = (int)blockIdx.y * 16, steps = (a.d + 15) >> 4;
+    const int from = (int)((long long)steps * blockIdx.z / a.splits) * 16, to = min((int)((long long)steps * (blockIdx.z + 1) / a.splits) * 16, a.d);
+    const float *xp = a.x + (size_t)min(t0 + r, a.tokens - 1) * a.d + 4 * q, *wp = a.w + (size_t)min(e0 + r, a.experts - 1) * a.d + 4 * q;
+    f64x4 acc = {0, 0, 0, 0};
+    auto step = [&](const float4 &xv, const float4 &wv) {
+        acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)xv.x, (double)wv.x, acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)xv.y, (double)wv.y, acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)xv.z, (double)wv.z, acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)xv.w, (double)wv.w, acc, 0, 0, 0);
+    };
+    int at = from + 16 * wave;
+    for (; at + 3 * 64 + 16 <= to; at += 4 * 64) {
+        float4 xv[4], wv[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            xv[j] = *reinterpret_cast<const float4 *>(xp + at + 64 * j);
+            wv[j] = *reinterpret_cast<const float4 *>(wp + at + 64 * j);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) step(xv[j], wv[j]);
+    }
+    for (; at < to; at += 64) {
+        float4 xv = make_float4(0.f, 0.f, 0.f, 0.f), wv = xv;
+        if (at + 4 * q < to) {
+            xv = *reinterpret_cast<const float4 *>(xp + at);
+            wv = *reinterpret_cast<const float4 *>(wp + at);
+        }
+        step(xv, wv);
+    }
+    if (wave) sums[wave - 1][lane] = acc;
+    __syncthreads();
+    if (wave) return;
+    acc = (acc + sums[0][lane]) + (sums[1][lane] + sums[2][lane]);
+    double *const logits = a.logits + (size_t)blockIdx.z * a.tokens * a.experts;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {  // lane r + 16 q: column (expert) r, rows (tokens) q + 4 i
+        const int t = t0 + q + 4 * i, e = e0 + r;
+        if (t < a.tokens && e < a.experts) logits[(size_t)t * a.experts + e] = acc[i];
+    }
+}
+
+// The lists of each expert's slots and their chunks, by one workgroup of 1024 threads: counted, summed up, handed out.  (In what order a list holds its slots
+// is no part of any result: each row of a product is computed by itself.)  hist: [MAX_EXPERTS] in LDS.
+template <class Id>
+__device__ __forceinline__ void make_lists(Id &&id_of, int slots, int experts, const ExpertLists &lists, int *hist) {
+    const int tid = threadIdx.x, lane = tid & 63;
+    for (int e = tid; e < experts; e += 1024) hist[e] = 0;
+    __syncthreads();
+    for (int i = tid; i < slots; i += 1024) {
+        const int e = id_of(i);
+        if ((unsigned)e < (unsigned)experts) atomicAdd(&hist[e], 1);
+    }
+    __syncthreads();
+    if (tid < 64) {
+        int run = 0, made = 0;
+        for (int e0 = 0; e0 < experts; e0 += 64) {
+            const int e = e0 + lane, mine = e < experts ? hist[e] : 0, chunks = (mine + lists.chunk_rows - 1) / lists.chunk_rows;
+            int sum = mine, chunk_sum = chunks;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const int below = __shfl_up(sum, o), chunk_below = __shfl_up(chunk_sum, o);
+                sum += lane >= o ? below : 0;
+                chunk_sum += lane >= o ? chunk_below : 0;
+            }
+            const int first = run + sum - mine;
+            if (e < experts) hist[e] = first;
+            for (int i = 0; i < chunks; ++i) {  // (as even as whole rows allow)
+                const int from = (int)((long long)mine * i / chunks), to = (int)((long long)mine * (i + 1) / chunks);
+                lists.chunks[1 + made + chunk_sum - chunks + i] = int4{e, first + from, to - from, 0};
+            }
+            run += __shfl(sum, 63);
+            made += __shfl(chunk_sum, 63);
+        }
+        if (lane == 0) lists.chunks[0] = int4{made, 0, 0, 0};
+    }
+    __syncthreads();
+    for (int i = tid; i < slots; i += 1024) {
+        const int e = id_of(i);
+        if ((unsigned)e < (unsigned)experts) lists.list[atomicAdd(&hist[e], 1)] = i;
+    }
+}
+
+// A wave per token.  ceil(tokens / 4) workgroups of 256 threads; L: see choose_experts.
+template <int L>
+__global__ void __launch_bounds__(256) choose_kernel(const RouterArgs a) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), t = (int)blockIdx.x * 4 + wave;
+    if (t >= a.tokens) return;
+    double l[L];
+    load_logits(a, t, lane, l);
+    int id;
+    float weight;
+    choose_experts(a, l, lane, id, weight);
+    store_choice(a, t, lane, id, weight);
+}
+
+// Few tokens, one workgroup: the choices of all of them and the experts' lists.
+constexpr int CHOOSE_FEW = 64;
+template <int L>
+__global__ void __launch_bounds__(1024) choose_few_kernel(const RouterArgs a) {
+    __shared__ int ids[CHOOSE_FEW * MAX_USED], hist[MAX_EXPERTS];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    for (int t = wave; t < a.tokens; t += 16) {
+        double l[L];
+        load_logits(a, t, lane, l);
+        int id;
+        float weight;
+        choose_experts(a, l, lane, id, weight);
+        store_choice(a, t, lane, id, weight);
+        if (lane < a.used) ids[t * a.used + lane] = id;
+    }
+    __syncthreads();
+    make_lists([&](int i) { return ids[i]; }, a.tokens * a.used, a.experts, a.lists, hist);
+}
+
+__global__ void __launch_bounds__(1024) expert_lists_kernel(const int *__restrict__ ids, int slots, int experts, const ExpertLists lists) {
+    __shared__ int hist[MAX_EXPERTS];
+    make_lists([&](int i) { return ids[i]; }, slots, experts, lists, hist);
+}
+
+// A router whose weights one workgroup reads in about the time that a second launch would take: logits and choice of a token, 1024 threads.
+template <int L>
+__global__ void __launch_bounds__(1024) router_one_kernel(const RouterArgs a) {
+    __shared__ double logits[MAX_EXPERTS];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), t = (int)blockIdx.x;
+    for (int e = wave; e < a.experts; e += 16) {
+        const double v = router_dot(a.x + (size_t)t * a.d, a.w + (size_t)e * a.d, a.d, lane, 64);
+        if (lane == 0) logits[e] = v;
+    }
+    __syncthreads();
+    if (wave) return;
+    double l[L];
+#pragma unroll
+    for (int i = 0; i < L; ++i) l[i] = logits[min(64 * i + lane, a.experts - 1)];
+    int id;
+    float weight;
+    choose_experts(a, l, lane, id, weight);
+    store_choice(a, t, lane, id, weight);
+}
+
+// f(the experts of a lane, as a type): what a lane does for each is most of a choice's instructions (32 tokens, 8 of 128 experts: 22 us with eight places a lane)
+template <class F>
+static void with_lanes(int experts, F &&f) {
+    if (experts <= 64) f(std::integral_constant<int, 1>{});
+    else if (experts <= 128) f(std::integral_constant<int, 2>{});
+    else if (experts <= 256) f(std::integral_constant<int, 4>{});
+    else f(std::integral_constant<int, 8>{});
+}
+static_assert(MAX_EXPERTS <= 8 * 64, "every expert has a lane");
+
 // One launch for logits and choice: few experts, and few enough tokens for a workgroup each.
-static bool one_launch(int tokens, int experts, int d, bool lists) { return !lists && (long long)experts * d <= 131072 && tokens <= 64; }
+static bool one_launch(int tokens, int experts, int d) { return (long long)experts * d <= 131072 && tokens <= 64; }
 
-bool router_needs_logits(int tokens, int experts, int d, bool lists) { return !one_launch(tokens, experts, d, lists); }
+// A workgroup per logit, up to some 64 MiB of rows through the L2s (32 tokens x 128 experts x 2048 values 6 us, in tiles 14); tiles of 16 x 16 beyond.
+static bool logit_each(int tokens, int experts, int d) { return (long long)tokens * experts * d <= 8 << 20; }
+static int tile_splits(int tokens, int experts, int d) {
+    const int tiles = ((tokens + 15) / 16) * ((experts + 15) / 16);
+    return std::max(1, std::min({1024 / tiles, 8, d / 256}));
+}
 
-void router_launch(const RouterArgs &a, hipStream_t s) {
+size_t router_logits_bytes(int tokens, int experts, int d, bool choice_follows) {
+    if (choice_follows && one_launch(tokens, experts, d)) return 0;
+    return (size_t)tokens * experts * sizeof(double) * (logit_each(tokens, experts, d) ? 1 : tile_splits(tokens, experts, d));
+}
+
+void router_logits_launch(RouterArgs &a, hipStream_t s) {
+    if (logit_each(a.tokens, a.experts, a.d)) {
+        a.splits = 1;
+        hipLaunchKernelGGL(router_logits_kernel, dim3(a.experts, a.tokens), dim3(256), 0, s, a);
+    } else {
+        a.splits = tile_splits(a.tokens, a.experts, a.d);
+        hipLaunchKernelGGL(router_tiles_kernel, dim3((a.tokens + 15) / 16, (a.experts + 15) / 16, a.splits), dim3(256), 0, s, a);
+    }
+}
+
+void router_launch(RouterArgs a, hipStream_t s) {
     const bool lists = a.lists.list != nullptr;
-    if (one_launch(a.tokens, a.experts, a.d, lists)) {
-        hipLaunchKernelGGL(router_one_kernel, dim3(a.tokens), dim3(1024), 0, s, a);
+    if (!lists && one_launch(a.tokens, a.experts, a.d)) {
+        with_lanes(a.experts, [&](auto n) { hipLaunchKernelGGL(router_one_kernel<n()>, dim3(a.tokens), dim3(1024), 0, s, a); });
         return;
     }
-    if (a.tokens <= 8) hipLaunchKernelGGL(router_logits_kernel, dim3((a.experts + 3) / 4, a.tokens), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL(router_tiles_kernel, dim3((a.tokens + 15) / 16, (a.experts + 15) / 16), dim3(256), 0, s, a);
+    router_logits_launch(a, s);
     if (lists && a.tokens <= CHOOSE_FEW) {
-        const int waves = std::max(1, std::min(16, 2048 / a.experts));  // (at most 32 KiB for the logits and their order)
-        hipLaunchKernelGGL(choose_few_kernel, dim3(1), dim3(1024), (size_t)waves * 16 * a.experts, s, a, waves);
+        with_lanes(a.experts, [&](auto n) { hipLaunchKernelGGL(choose_few_kernel<n()>, dim3(1), dim3(1024), 0, s, a); });
         return;
     }
-    hipLaunchKernelGGL(choose_kernel, dim3((a.tokens + 3) / 4), dim3(256), (size_t)64 * a.experts, s, a);
+    with_lanes(a.experts, [&](auto n) { hipLaunchKernelGGL(choose_kernel<n()>, dim3((a.tokens + 3) / 4), dim3(256), 0, s, a); });
     if (lists) expert_lists_launch(a.ids, a.tokens * a.used, a.experts, a.lists, s);
 }
 
