@@ -19,7 +19,7 @@ constexpr int FEW_CHOICE = 128;  // experts of which the first kernel makes the 
 // Turns between two joins of the waves' sums, and a wave's LDS: the digits while they are staged, then two windows of sums.
 constexpr int EF_FLUSH = 24;
 constexpr size_t EF_WAVE_LDS = (size_t)2 * EF_FLUSH * 16 * sizeof(float);
-static_assert(EF_WAVE_LDS >= 3072, "sixteen chunks of three planes");
+static_assert(EF_WAVE_LDS >= 16 * 3 * 64, "sixteen chunks of three planes");
 
 // The digits hold a chunk to 2^-127 at best.  Where a wave's values are all below 2^-63 - products of two small numbers reach that - they are staged times
 // 2^64, and its sums count that much less; beside a larger value the same steps are nothing.
@@ -171,14 +171,16 @@ __global__ void __launch_bounds__(64 * MAXW, MAXW > 8 ? 4 : 2) experts_few_down_
         for (int i = 0; i < 4; ++i) xv[s][i] = reinterpret_cast<const float4 *>(h)[i];
     }
     typename U::Raw buf[NB][S];
-    auto fill = [&](typename U::Raw(&dst)[S], int t) {
+    auto fill = [&](typename U::Raw &dst, int s, int t) {
         const int g = (int)blockIdx.x + t * a.blocks, extent = __builtin_amdgcn_readfirstlane((g - groups) >> 31);
         const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(a.w), 0, extent, 0x00020000);
-#pragma unroll
-        for (int s = 0; s < S; ++s) U::load(dst[s], rs, off[s], (uint32_t)(4 * g & extent) * rowbytes);
+        U::load(dst, rs, off[s], (uint32_t)(4 * g & extent) * rowbytes);
     };
 #pragma unroll
-    for (int i = 0; i < NB; ++i) fill(buf[i], i);
+    for (int i = 0; i < NB; ++i) {
+#pragma unroll
+        for (int s = 0; s < S; ++s) fill(buf[i][s], s, i);
+    }
     __builtin_amdgcn_sched_barrier(0);
     uint32_t xa[S][1][16];
     float sinv[S][1], sums[S][1][U::NSUM], lift[S], odd = 0.f;
@@ -198,17 +200,17 @@ __global__ void __launch_bounds__(64 * MAXW, MAXW > 8 ? 4 : 2) experts_few_down_
 #pragma unroll
             for (int i = 0; i < NB; ++i) {
                 const int t = tb + i;
-                if (t < tend) {
-                    float sum = odd;
+                float sum = odd;
 #pragma unroll
-                    for (int s = 0; s < S; ++s) {
+                for (int s = 0; s < S; ++s) {
+                    if (t < tend) {
                         float acc[1];
                         i8_dot<U, 1>(buf[i][s], cc[s], xa[s], sinv[s], sums[s], acc);
                         sum += live[s] ? acc[0] * lift[s] : 0.f;
                     }
-                    few_emit(sum, part, half * EF_FLUSH + t - t0, lane);
+                    fill(buf[i][s], s, t + NB);
                 }
-                fill(buf[i], t + NB);
+                if (t < tend) few_emit(sum, part, half * EF_FLUSH + t - t0, lane);
             }
         }
         __syncthreads();
@@ -229,7 +231,7 @@ static ExpertFewKernel experts_few_up_pick(int waves) {
 }
 template <class U>
 static ExpertFewKernel experts_few_down_pick(int stretches, int waves) {
-    if (stretches > 1) return experts_few_down_kernel<U, 2, 1, 16>;
+    if (stretches > 1) return experts_few_down_kernel<U, 2, 0, 16>;
     return waves <= 8 ? experts_few_down_kernel<U, 1, 2, 8> : experts_few_down_kernel<U, 1, 1, 16>;
 }
 
