@@ -373,7 +373,7 @@ JITNN_HIP_API int jitnn_hip_router_create(int experts, int d_model, int used, in
                                           const float *selection_bias_host, jitnn_hip_router **out);
 JITNN_HIP_API int jitnn_hip_router_free(jitnn_hip_router *r);
 /* ids and weights [tokens, used] of x [tokens, d_model], in the order of choice.  tokens 0: nothing is done.  x 16-byte aligned.  Workspace as for the attention over pages:
- * device memory of at least jitnn_hip_router_workspace bytes (0 where it returns 0; 16-byte aligned), used until the work has run: calls that may overlap in time,
+ * device memory of jitnn_hip_router_workspace bytes (they do for a call of fewer tokens too; 16-byte aligned), used until the work has run: calls that may overlap in time,
  * recorded graphs among them, need one each. */
 JITNN_HIP_API long long jitnn_hip_router_workspace(const jitnn_hip_router *r, int tokens);
 JITNN_HIP_API int jitnn_hip_router_dev(const jitnn_hip_router *r, const float *x_dev, int tokens, int *ids_dev, float *weights_dev, void *workspace_dev,

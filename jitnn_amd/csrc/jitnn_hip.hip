@@ -2394,24 +2394,33 @@ int moe_groups(const jitnn_hip_moe *m, int tokens) {
     return groups;
 }
 
+// Experts that so many tokens meet, where every one is as likely as any other.
+double moe_met(const jitnn_hip_router *r, int tokens) { return r->experts * (1 - std::pow(1 - (double)r->used / r->experts, tokens)); }
+
 // Shares of the down projection's columns, where its workgroups alone would leave CUs idle: expected chunks x blocks against a workgroup for every CU (two of
 // the small ones).
 int moe_splits(const jitnn_hip_moe *m, int tokens, int groups) {
     if (!experts_on_rows(m->down)) return 1;
     const jitnn_hip_router *r = m->router;
     const RowsKernelRef k = experts_rows_kernel_ref(m->down->fmt, groups, false);
-    const double mean = (double)tokens * r->used / r->experts, met = r->experts * (1 - std::pow(1 - (double)r->used / r->experts, tokens)),
-                 blocks = met * std::max(1.0, mean / (8 * groups)) * ((r->d / 16 + k.tiles - 1) / k.tiles);
+    const double mean = (double)tokens * r->used / r->experts, blocks = moe_met(r, tokens) * std::max(1.0, mean / (8 * groups)) * ((r->d / 16 + k.tiles - 1) / k.tiles);
     const int ncol = (m->ffn + 255) / 256, wanted = (int)std::ceil((k.threads > 256 ? 1.0 : 2.0) * g.cus / blocks);
     return std::max(1, std::min({wanted, 8, ncol / 4}));
 }
 
-// Few tokens: the INT8 products on the raw quants, for weights whose rows are whole chunks of 64 values.
+// Few tokens: the INT8 products on the raw quants, for weights whose rows are whole chunks of 64 values.  They read an expert once for each token that meets it, but as
+// fast as the memory gives, in three launches; the matrix cores' route reads it once, at two thirds of that, between seven launches that cost what 60 MB do.  Both, rows
+// / few, us: two of eight experts of 4096 x 14336, Q4_K and Q6_K, 1 token 93 / 49, 4 228 / 147, 6 256 / 218, 8 264 / 265, 12 278 / 406; four of 16 of 4096 x 2048, Q5_K,
+// 4 87 / 67, 5 88 / 84, 6 89 / 98; eight of 128 of 2048 x 768, 1 49 / 21, 8 84 / 52, 16 102 / 89; six of 64 of 2048 x 1408, Q8_0, 5 97 / 53, 12 135 / 109; eight
+// of 64 of 5120 x 1536 8 215 / 178, 12 264 / 268; two of eight of 4096 x 1024, Q6_K, 1 61 / 16, 8 64 / 33, 16 65 / 48.  Not measured with more tokens.
+constexpr int MOE_FEW_TOKENS = 16;
 bool moe_few(const jitnn_hip_moe *m, int tokens) {
-    if (!g.gemv_i8 || tokens > 1 || m->gate->fmt != m->up->fmt) return false;
+    if (!g.gemv_i8 || tokens > MOE_FEW_TOKENS || m->gate->fmt != m->up->fmt) return false;
     for (const jitnn_hip_weight *w : {m->gate, m->up, m->down})
         if (w->nbytes >= (1ll << 32) || ((uintptr_t)w->dev & 3) != 0) return false;
-    return experts_few_up_supported(m->gate->fmt, m->router->d) && experts_few_down_supported(m->down->fmt, m->ffn, m->router->used);
+    if (!experts_few_up_supported(m->gate->fmt, m->router->d) || !experts_few_down_supported(m->down->fmt, m->ffn, m->router->used)) return false;
+    const double expert = (double)(m->gate->nbytes + m->up->nbytes + m->down->nbytes) / m->router->experts;
+    return tokens == 1 || expert * ((double)tokens * m->router->used - 1.5 * moe_met(m->router, tokens)) <= 60e6;
 }
 
 // What a pass of `tokens` keeps in the workspace, in bytes from its start.
@@ -2489,8 +2498,9 @@ int check_moe_call(const jitnn_hip_moe *m, const float *x, int tokens, const flo
     if (tokens == 0) return JITNN_HIP_OK;
     if (!x || !y) return fail(JITNN_HIP_EINVAL, "input or output is NULL");
     if ((((uintptr_t)x | (uintptr_t)y | (uintptr_t)res) & 15) != 0) return fail(JITNN_HIP_EINVAL, "input, residual and output must be 16-byte aligned");
-    const long long need = jitnn_hip_moe_workspace(m, tokens);
-    if (need < 0) return (int)need;
+    const int pass = moe_pass_tokens(m);
+    long long need = (long long)moe_layout(m, std::min(tokens, pass)).total;
+    if (tokens > pass && tokens % pass) need = std::max(need, (long long)moe_layout(m, tokens % pass).total);
     if (!ws || ((uintptr_t)ws & 15) != 0 || ws_bytes < need) return fail(JITNN_HIP_EINVAL, "workspace of %lld bytes, 16-byte aligned, needed; got %lld", need, ws ? ws_bytes : 0);
     return check_ready();
 }
@@ -2630,9 +2640,8 @@ int jitnn_hip_router_free(jitnn_hip_router *r) {
 long long jitnn_hip_router_workspace(const jitnn_hip_router *r, int tokens) {
     if (!r) return fail(JITNN_HIP_EINVAL, "the router is NULL");
     if (tokens < 0) return fail(JITNN_HIP_EINVAL, "tokens = %d", tokens);
-    long long most = 0;  // (a shorter last pass may need what a longer one does not)
-    for (const int t : {std::min(tokens, ROUTER_PASS), tokens % ROUTER_PASS})
-        if (t) most = std::max(most, (long long)router_logits_bytes(t, r->experts, r->d, true));
+    long long most = 0;  // (fewer tokens may need more: sums in splits)
+    for (int t = std::min(tokens, ROUTER_PASS); t > 0; --t) most = std::max(most, (long long)router_logits_bytes(t, r->experts, r->d, true));
     return most;
 }
 
@@ -2643,7 +2652,9 @@ int jitnn_hip_router_dev(const jitnn_hip_router *r, const float *x_dev, int toke
     if (tokens == 0) return JITNN_HIP_OK;
     if (!x_dev || !ids_dev || !weights_dev) return fail(JITNN_HIP_EINVAL, "input or output is NULL");
     if (((uintptr_t)x_dev & 15) != 0) return fail(JITNN_HIP_EINVAL, "the input must be 16-byte aligned");
-    const long long need = jitnn_hip_router_workspace(r, tokens);
+    long long need = 0;
+    for (const int t : {std::min(tokens, ROUTER_PASS), tokens % ROUTER_PASS})
+        if (t) need = std::max(need, (long long)router_logits_bytes(t, r->experts, r->d, true));
     if (need > 0 && (!workspace_dev || ((uintptr_t)workspace_dev & 15) != 0 || workspace_bytes < need))
         return fail(JITNN_HIP_EINVAL, "workspace of %lld bytes, 16-byte aligned, needed; got %lld", need, workspace_dev ? workspace_bytes : 0);
     if (int rc = check_ready()) return rc;
@@ -2679,10 +2690,8 @@ int jitnn_hip_moe_free(jitnn_hip_moe *m) {
 long long jitnn_hip_moe_workspace(const jitnn_hip_moe *m, int tokens) {
     if (!m) return fail(JITNN_HIP_EINVAL, "the layer is NULL");
     if (tokens < 0) return fail(JITNN_HIP_EINVAL, "tokens = %d", tokens);
-    if (tokens == 0) return 0;
-    const int pass = moe_pass_tokens(m);
-    long long most = (long long)moe_layout(m, std::min(tokens, pass)).total;
-    if (tokens > pass && tokens % pass) most = std::max(most, (long long)moe_layout(m, tokens % pass).total);  // (more, smaller chunks)
+    long long most = 0;  // (fewer tokens may need more: the down projection's splits, smaller chunks)
+    for (int t = std::min(tokens, moe_pass_tokens(m)); t > 0; --t) most = std::max(most, (long long)moe_layout(m, t).total);
     return most;
 }
 

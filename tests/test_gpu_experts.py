@@ -322,3 +322,19 @@ def test_refusals(jn):
         jn.Tensor.wrap_dev(jn.DType.Q4_K, p, 4, 100)
     with pytest.raises(ValueError):
         jn.Tensor.wrap_dev(jn.DType.Q4_K, p + 8, 4, 256)
+
+
+@pytest.mark.parametrize("experts,used,d,ffn,up,down", [(8, 2, 512, 2048, "Q4_K", "Q6_K"), (64, 6, 256, 1408, "Q8_0", "Q8_0"), (100, 1, 64, 64, "Q5_0", "Q4_0")])
+def test_a_workspace_does_for_fewer_tokens(jn, experts, used, d, ffn, up, down):
+    rng = np.random.default_rng(2)
+    layer = ref.Layer(rng, experts, used, d, ffn, up, down)
+    moe = layer.make(jn)
+    most = 150
+    x, y, ws = dev(layer.input(rng, most)), torch.empty(most, d, device="cuda"), space(moe.workspace(most))
+    ids, weights, rs = torch.empty(most, used, dtype=torch.int32, device="cuda"), torch.empty(most, used, device="cuda"), space(moe.router.workspace(most))
+    for tokens in (1, 2, 7, 16, 17, 18, 25, 33, 64, 65, 149):
+        moe.layer_dev(x.data_ptr(), tokens, y.data_ptr(), ws.data_ptr(), moe.workspace(most))
+        moe.router.route_dev(x.data_ptr(), tokens, ids.data_ptr(), weights.data_ptr(), rs.data_ptr(), moe.router.workspace(most))
+        moe.experts_dev(x.data_ptr(), tokens, ids.data_ptr(), weights.data_ptr(), (z := torch.empty(tokens, d, device="cuda")).data_ptr(), ws.data_ptr(), moe.workspace(most))
+        torch.cuda.synchronize()
+        assert torch.equal(y[:tokens], z)
