@@ -26,6 +26,7 @@
 // expression of the dequantiser and multiplied in FP32) so that +-Inf and NaN come out as the reference's FP64 sum
 // gives them (core/ops/Gguf.java:187-205).
 #pragma once
+#include "act.h"
 #include "common.h"
 #include "dequant.h"
 #include "tu.h"
@@ -655,7 +656,7 @@ __host__ __device__ constexpr uint32_t i8_pack(int k, int nblocks, int rows) { r
 // -------------------------------------------------------------------------------------------------- the kernel body
 // rb: the first activation row of this workgroup (launches of more than B rows put the row groups of B along blockIdx.y:
 // their workgroups stream the same weight bytes at the same time, so one of them finds them in the cache)
-template <class U, int B, int PF, bool BIAS, bool NORM, bool DUAL, int MAXW>
+template <class U, int B, int PF, bool BIAS, bool NORM, bool DUAL, int MAXW, bool EPI = false>
 __device__ __forceinline__ void gemv_i8_body(const I8Lead &ld, const I8Args &a, const int bid, const int rb = 0) {
     constexpr int FMT = U::FMT, NB = PF + 1, FL = i8_flush(B);
     static_assert(FL % NB == 0 && FL % 2 == 0, "whole rings (and gate/up pairs) per flush window");
@@ -789,6 +790,7 @@ __device__ __forceinline__ void gemv_i8_body(const I8Lead &ld, const I8Args &a, 
     if constexpr (BIAS) asm volatile("" ::"s"(a.bias[0]));
     if constexpr (NORM) asm volatile("" ::"s"(a.eps));
     if constexpr (SEGMENTS) asm volatile("" ::"s"(a.y[1]), "s"(a.y[2]));
+    if constexpr (EPI) asm volatile("" ::"s"(a.bias[0]), "s"(a.epi.act), "s"(a.epi.res));
     if constexpr (SEGMENTS && BIAS) asm volatile("" ::"s"(a.bias[1]), "s"(a.bias[2]));
     auto group_of = [&](int t) { return bid + (DUAL ? t >> 1 : t) * nblocks; };
     // one output of a window: the partial sums of all waves in wave order
@@ -894,7 +896,13 @@ __device__ __forceinline__ void gemv_i8_body(const I8Lead &ld, const I8Args &a, 
                     float bias = 0.f;
                     if (BIAS) bias = (a.bias[0] + (in1 ? a.bias[1] - a.bias[0] : 0) + (in2 ? a.bias[2] - a.bias[1] : 0))[local];
                     const float sum = NORM ? joined(half, tt, r, jj) * nscale : joined(half, tt, r, jj);
-                    yp[(size_t)(rb + r) * n + local] = BIAS ? sum + bias : sum;
+                    const size_t to = (size_t)(rb + r) * n + local;
+                    if constexpr (EPI) {
+                        const float v = activate(a.epi.act, a.bias[0] ? sum + a.bias[0][local] : sum);
+                        yp[to] = a.epi.res ? v + a.epi.res[to] : v;
+                    } else {
+                        yp[to] = BIAS ? sum + bias : sum;
+                    }
                 }
             }
         }
@@ -913,10 +921,10 @@ __global__ void __launch_bounds__(64 * MAXW, (B > 1 ? 2 : 4)) gemv_i8_kernel(con
     const I8Lead ld{w0, x, wb, nw, wc, (int)(packed & 511u) << 6, (int)((packed >> 9) & 0xfffffu), (int)(packed >> 29) + 1, n, n0, n1};
     gemv_i8_body<U, B, PF, BIAS, NORM, DUAL, MAXW>(ld, a, blockIdx.x, B * (int)blockIdx.y);
 }
-template <class U, int B, int PF, bool BIAS, int MAXW>
+template <class U, int B, int PF, bool BIAS, int MAXW, bool EPI = false>
 __global__ void __launch_bounds__(64 * MAXW, (B > 1 ? 2 : 4)) gemv_i8_plain_kernel(const uint8_t *w0, const float *x, const uint32_t packed, const int n, const I8Args a) {
     const I8Lead ld{w0, x, w0, nullptr, w0, (int)(packed & 511u) << 6, (int)((packed >> 9) & 0xfffffu), (int)(packed >> 29) + 1, n, n, 0};
-    gemv_i8_body<U, B, PF, BIAS, false, false, MAXW>(ld, a, blockIdx.x, B * (int)blockIdx.y);
+    gemv_i8_body<U, B, PF, BIAS, false, false, MAXW, EPI>(ld, a, blockIdx.x, B * (int)blockIdx.y);
 }
 
 // Two sets of matrices in two formats over the same (normalised) activations in one launch - the q / k and the v

@@ -25,6 +25,7 @@ template <class U, int PF, int MAXW>
 static i8_fn pick_mode(int mode) {
     switch (mode) {
     case I8_BIAS: return plain_fn(gemv_i8_plain_kernel<U, 1, PF, true, MAXW>);
+    case I8_EPI: return plain_fn(gemv_i8_plain_kernel<U, 1, PF, false, MAXW, true>);
     case I8_NORM: return fused_fn(gemv_i8_kernel<U, 1, PF, false, true, false, MAXW>);
     case I8_DUAL: return fused_fn(gemv_i8_kernel<U, 1, PF, false, true, true, MAXW>);
     default: return plain_fn(gemv_i8_plain_kernel<U, 1, PF, false, MAXW>);
@@ -42,17 +43,20 @@ static i8_fn pick_pf(int mode, int pf) {
 template <class U, int B>
 static i8_fn pick_batch(int mode, int pf) {
     if (mode == I8_BIAS) return plain_fn(pf <= 1 ? gemv_i8_plain_kernel<U, B, 1, true, 4> : gemv_i8_plain_kernel<U, B, 2, true, 4>);
+    if (mode == I8_EPI) return plain_fn(pf <= 1 ? gemv_i8_plain_kernel<U, B, 1, false, 4, true> : gemv_i8_plain_kernel<U, B, 2, false, 4, true>);
     return plain_fn(pf <= 1 ? gemv_i8_plain_kernel<U, B, 1, false, 4> : gemv_i8_plain_kernel<U, B, 2, false, 4>);
 }
 
-// Q5_1 and Q2_K: formats no fused launch of the decode step is built for - with or without a bias, nothing else
+// Q5_1 and Q2_K: formats no fused launch of the decode step is built for - with or without a bias or an epilogue, nothing else
 template <class U, int MAXW>
 static i8_fn pick_plain(int mode, int pf) {
-    if (mode != I8_BIAS && mode != I8_PLAIN) return i8_fn{};
+    if (mode != I8_BIAS && mode != I8_PLAIN && mode != I8_EPI) return i8_fn{};
     if constexpr (MAXW > 4) {  // (long rows: one turn in flight)
+        if (mode == I8_EPI) return plain_fn(gemv_i8_plain_kernel<U, 1, 1, false, MAXW, true>);
         return plain_fn(mode == I8_BIAS ? gemv_i8_plain_kernel<U, 1, 1, true, MAXW> : gemv_i8_plain_kernel<U, 1, 1, false, MAXW>);
     } else {
         if (mode == I8_BIAS) return plain_fn(pf <= 1 ? gemv_i8_plain_kernel<U, 1, 1, true, MAXW> : gemv_i8_plain_kernel<U, 1, 2, true, MAXW>);
+        if (mode == I8_EPI) return plain_fn(pf <= 1 ? gemv_i8_plain_kernel<U, 1, 1, false, MAXW, true> : gemv_i8_plain_kernel<U, 1, 2, false, MAXW, true>);
         return plain_fn(pf <= 1 ? gemv_i8_plain_kernel<U, 1, 1, false, MAXW> : gemv_i8_plain_kernel<U, 1, 2, false, MAXW>);
     }
 }
@@ -60,14 +64,14 @@ static i8_fn pick_plain(int mode, int pf) {
 template <class U>
 static i8_fn pick_rows(int rows, int waves, int mode, int pf) {
     if (rows == 1) return waves <= 4 ? pick_pf<U, 4>(mode, pf) : pick_plain<U, I8_MAX_WAVES>(mode, 1);  // (long rows: plain or biased, one turn in flight - the fused launches of the decode step have rows of at most 4096 values)
-    if (waves > 4 || rows > 8 || (mode != I8_PLAIN && mode != I8_BIAS)) return i8_fn{};  // (five to eight rows: two groups of four)
+    if (waves > 4 || rows > 8 || (mode != I8_PLAIN && mode != I8_BIAS && mode != I8_EPI)) return i8_fn{};  // (five to eight rows: two groups of four)
     return rows > 2 ? pick_batch<U, 4>(mode, pf) : pick_batch<U, 2>(mode, pf);
 }
 
 template <class U>
 static i8_fn pick_rows_plain(int rows, int waves, int mode, int pf) {
     if (rows == 1) return waves <= 4 ? pick_plain<U, 4>(mode, pf) : pick_plain<U, I8_MAX_WAVES>(mode, 1);
-    if (waves > 4 || rows > 4 || (mode != I8_PLAIN && mode != I8_BIAS)) return i8_fn{};
+    if (waves > 4 || rows > 4 || (mode != I8_PLAIN && mode != I8_BIAS && mode != I8_EPI)) return i8_fn{};
     return rows > 2 ? pick_batch<U, 4>(mode, pf) : pick_batch<U, 2>(mode, pf);
 }
 

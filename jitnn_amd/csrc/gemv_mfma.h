@@ -30,6 +30,7 @@
 // Which eight positions, and in which order, depends on how the format packs its quants (MTile<FMT>::quad_pos and
 // the byte order 0, 2, 1, 3 of the dword decoders); a dot product only needs both operands to agree.
 #pragma once
+#include "act.h"
 #include "common.h"
 
 namespace jitnn {
@@ -403,13 +404,13 @@ __device__ __forceinline__ void mf_build_operands(const float4 (&v)[8], bool hav
     }
 }
 
-// y[b, row] (+)= sum_k W[row, k] x[b, k] (+ bias[row]) for b < rows <= 8; k a multiple of 256, n >= 16.
+// y[b, row] = sum_k W[row, k] x[b, k] (+ bias[row]) for b < rows <= 8, EPI: act of it (+ res[b, row]); k a multiple of 256, n >= 16.  (Long rows: in parts,
+// which a workgroup adds up in y.)
 //   grid: up to one workgroup per group of 16 weight rows (the host caps it at one per CU), MF_THREADS threads,
 //   dynamic LDS gemv_mfma_lds_bytes<FMT>().
-template <int FMT>
-__global__ void __launch_bounds__(MF_THREADS) gemv_mfma_kernel(const uint8_t *__restrict__ W, const float *__restrict__ x,
-                                                                const float *__restrict__ bias, float *__restrict__ y, int n, int k, int rows,
-                                                                int stride) {  // stride: the grid's workgroups (an argument, preloaded with the others: gridDim is fetched from a cold block)
+template <int FMT, bool EPI>
+__device__ __forceinline__ void gemv_mfma_body(const uint8_t *__restrict__ W, const float *__restrict__ x, const float *__restrict__ bias, float *__restrict__ y, int n, int k,
+                                               int rows, int stride, const Epilogue &e) {
     typedef MTile<FMT> T;
     constexpr int CH = T::BYTES / 16;           // whole 16-byte chunks of a tile row
     constexpr int TAIL = T::BYTES % 16;         // 0, or the 2 bytes of Q6_K's d after 13 chunks
@@ -537,13 +538,34 @@ __global__ void __launch_bounds__(MF_THREADS) gemv_mfma_kernel(const uint8_t *__
                 for (int w = 0; w < MF_WAVES; ++w) sum += src[w * MF_GROUPS * 32 * 4];
                 if (grp < ngroups && row >= grp * 16 && br < rows) {
                     float *o = y + (size_t)br * n + row;
-                    if (t0 == 0) *o = bias ? sum + bias[row] : sum;
-                    else *o += sum;
+                    if constexpr (EPI) {
+                        float v = t0 ? *o + sum : bias ? sum + bias[row] : sum;
+                        if (t0 + PASS >= tiles) {
+                            v = activate(e.act, v);
+                            if (e.res) v += e.res[(size_t)br * n + row];
+                        }
+                        *o = v;
+                    } else {
+                        if (t0 == 0) *o = bias ? sum + bias[row] : sum;
+                        else *o += sum;
+                    }
                 }
             }
             __syncthreads();
         }
     }
+}
+
+// stride: the grid's workgroups (an argument, preloaded with the others: gridDim is fetched from a cold block)
+template <int FMT>
+__global__ void __launch_bounds__(MF_THREADS) gemv_mfma_kernel(const uint8_t *__restrict__ W, const float *__restrict__ x, const float *__restrict__ bias, float *__restrict__ y,
+                                                                int n, int k, int rows, int stride) {
+    gemv_mfma_body<FMT, false>(W, x, bias, y, n, k, rows, stride, Epilogue{});
+}
+template <int FMT>
+__global__ void __launch_bounds__(MF_THREADS) gemv_mfma_epilogue_kernel(const uint8_t *__restrict__ W, const float *__restrict__ x, const float *__restrict__ bias,
+                                                                         float *__restrict__ y, int n, int k, int rows, int stride, const Epilogue e) {
+    gemv_mfma_body<FMT, true>(W, x, bias, y, n, k, rows, stride, e);
 }
 
 }  // namespace jitnn

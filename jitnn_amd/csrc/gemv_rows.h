@@ -24,6 +24,7 @@
 // puts several workgroups on a batch, each with a share of the groups (gridDim.y).  Launches that leave this kernel a part of a
 // round, or much to decode per tile, go to gemv_held_kernel (gemv_held.h).
 #pragma once
+#include "act.h"
 #include "common.h"
 #include "gemv_mfma.h"
 
@@ -523,18 +524,16 @@ __host__ __device__ constexpr size_t gemv_rows_stage_bytes(int tiles_per_wave) {
     return (size_t)GR_WAVES * tiles_per_wave * RTile<FMT>::STAGE_BYTES;
 }
 
-// y[b, row] = sum_k W[row, k] x[b, k] (+ bias[row]) (+ res[b, row]) for b < rows <= 8 * groups; k a multiple of 256 (Q4_0, Q4_1, Q8_0: the sum over
+// y[b, row] = sum_k W[row, k] x[b, k] (+ bias[row]), ACT: act of it, (+ res[b, row]) for b < rows <= 8 * groups; k a multiple of 256 (Q4_0, Q4_1, Q8_0: the sum over
 // the whole 256-value columns of a row of any number of blocks), n >= 16.
 //   ops / inv: the output of rows_prepare_kernel<RTile<FMT>::SUMS> for the same x.  grid: up to one workgroup per batch of T tiles of 16
 //   weight rows (the host caps it at one per compute unit) x shares of the groups of activation rows; GR_THREADS threads;
 //   gemv_rows_lds_bytes() + gemv_rows_stage_bytes() of dynamic LDS.
 // T = 2 halves the activation-operand traffic per weight byte; T = 1 is for matrices with too few tiles to give every CU a
 // workgroup otherwise.
-template <int FMT, int T>
-__global__ void __launch_bounds__(GR_THREADS) gemv_rows_kernel(const uint8_t *__restrict__ W, const _Float16 *__restrict__ ops,
-                                                                const float *__restrict__ inv, int n, int k, int rows, int groups,
-                                                                const uint32_t grid,  // gridDim.x | gridDim.y << 16 (an argument, preloaded: gridDim is fetched from a cold block)
-                                                                const float *__restrict__ bias, const float *res, float *y) {  // (res may be y)
+template <int FMT, int T, bool ACT>
+__device__ __forceinline__ void gemv_rows_body(const uint8_t *__restrict__ W, const _Float16 *__restrict__ ops, const float *__restrict__ inv, int n, int k, int rows, int groups,
+                                               const uint32_t grid, const float *__restrict__ bias, const float *res, float *y, int act) {
     // (argument order: the first fourteen dwords arrive in scalar registers with the wave - everything the first loads need; y,
     // which only the last lines use, is asked for here, not between the last product and the first store)
     asm volatile("" ::"s"(y), "s"(res));
@@ -671,13 +670,30 @@ __global__ void __launch_bounds__(GR_THREADS) gemv_rows_kernel(const uint8_t *__
                 if (row >= tile * 16) {  // rows of a ragged last tile that an earlier tile already wrote are skipped
                     const float bv = bias ? bias[row] : 0.f;
                     // (res [rows, n]: a residual that rides along, y = res + x W^T - the layers of a model)
-                    if (b0 < rows) y[(size_t)b0 * n + row] = sum.x + bv + (res ? res[(size_t)b0 * n + row] : 0.f);
-                    if (b0 + 1 < rows) y[(size_t)(b0 + 1) * n + row] = sum.y + bv + (res ? res[(size_t)(b0 + 1) * n + row] : 0.f);
+                    float v0 = sum.x + bv, v1 = sum.y + bv;
+                    if constexpr (ACT) {
+                        v0 = activate(act, v0);
+                        v1 = activate(act, v1);
+                    }
+                    if (b0 < rows) y[(size_t)b0 * n + row] = v0 + (res ? res[(size_t)b0 * n + row] : 0.f);
+                    if (b0 + 1 < rows) y[(size_t)(b0 + 1) * n + row] = v1 + (res ? res[(size_t)(b0 + 1) * n + row] : 0.f);
                 }
             }
         }
         __syncthreads();
     }
+}
+
+// grid: gridDim.x | gridDim.y << 16 (an argument, preloaded: gridDim is fetched from a cold block); res may be y
+template <int FMT, int T>
+__global__ void __launch_bounds__(GR_THREADS) gemv_rows_kernel(const uint8_t *__restrict__ W, const _Float16 *__restrict__ ops, const float *__restrict__ inv, int n, int k, int rows,
+                                                                int groups, const uint32_t grid, const float *__restrict__ bias, const float *res, float *y) {
+    gemv_rows_body<FMT, T, false>(W, ops, inv, n, k, rows, groups, grid, bias, res, y, 0);
+}
+template <int FMT, int T>
+__global__ void __launch_bounds__(GR_THREADS) gemv_rows_act_kernel(const uint8_t *__restrict__ W, const _Float16 *__restrict__ ops, const float *__restrict__ inv, int n, int k, int rows,
+                                                                    int groups, const uint32_t grid, const float *__restrict__ bias, const float *res, float *y, int act) {
+    gemv_rows_body<FMT, T, true>(W, ops, inv, n, k, rows, groups, grid, bias, res, y, act);
 }
 
 }  // namespace jitnn

@@ -1,5 +1,6 @@
 // gemv_rows_kernel: the formats it is built for, and which launches are gemv_held_kernel's instead.
 #include <algorithm>
+#include <type_traits>
 
 #include "gemv_held.h"
 #include "tu.h"
@@ -45,22 +46,23 @@ static RowsGeo rows_geometry(int fmt, int n, int k, int rows, unsigned max_block
 }
 
 template <int FMT>
-static KernelRef kernel_ref(bool two) {
-    return {two ? (const void *)gemv_rows_kernel<FMT, 2> : (const void *)gemv_rows_kernel<FMT, 1>,
+static KernelRef kernel_ref(bool two, bool activated) {
+    return {activated ? (two ? (const void *)gemv_rows_act_kernel<FMT, 2> : (const void *)gemv_rows_act_kernel<FMT, 1>)
+                      : two ? (const void *)gemv_rows_kernel<FMT, 2> : (const void *)gemv_rows_kernel<FMT, 1>,
             gemv_rows_lds_bytes(two ? 2 : 1) + gemv_rows_stage_bytes<FMT>(two ? 2 : 1)};
 }
 
-KernelRef gemv_rows_kernel_ref(int fmt, int n, int k, int rows, unsigned max_blocks) {
+KernelRef gemv_rows_kernel_ref(int fmt, int n, int k, int rows, unsigned max_blocks, bool activated) {
     const bool two = tiles_per_wave(fmt, n, k, rows, max_blocks) == 2;
     switch (fmt) {
-    case F_Q4_K: return kernel_ref<F_Q4_K>(two);
-    case F_Q5_K: return kernel_ref<F_Q5_K>(two);
-    case F_Q6_K: return kernel_ref<F_Q6_K>(two);
-    case F_Q4_0: return kernel_ref<F_Q4_0>(two);
-    case F_Q4_1: return kernel_ref<F_Q4_1>(two);
-    case F_Q8_0: return kernel_ref<F_Q8_0>(two);
-    case F_Q5_1: return kernel_ref<F_Q5_1>(two);
-    case F_Q2_K: return kernel_ref<F_Q2_K>(two);
+    case F_Q4_K: return kernel_ref<F_Q4_K>(two, activated);
+    case F_Q5_K: return kernel_ref<F_Q5_K>(two, activated);
+    case F_Q6_K: return kernel_ref<F_Q6_K>(two, activated);
+    case F_Q4_0: return kernel_ref<F_Q4_0>(two, activated);
+    case F_Q4_1: return kernel_ref<F_Q4_1>(two, activated);
+    case F_Q8_0: return kernel_ref<F_Q8_0>(two, activated);
+    case F_Q5_1: return kernel_ref<F_Q5_1>(two, activated);
+    case F_Q2_K: return kernel_ref<F_Q2_K>(two, activated);
     default: return {nullptr, 0};
     }
 }
@@ -101,7 +103,7 @@ void gemv_rows_prepare_launch(hipStream_t s, const float *x, const float *swiglu
 }
 
 template <int FMT>
-static void launch(unsigned max_blocks, hipStream_t s, const uint8_t *W, const void *scratch, const float *bias, const float *res, float *y, int n, int k,
+static void launch(unsigned max_blocks, hipStream_t s, const uint8_t *W, const void *scratch, const float *bias, const Epilogue &e, float *y, int n, int k,
                    int rows) {
     const int groups = (rows + 7) / 8;
     const _Float16 *ops = reinterpret_cast<const _Float16 *>(scratch);
@@ -109,21 +111,29 @@ static void launch(unsigned max_blocks, hipStream_t s, const uint8_t *W, const v
     const RowsGeo geo = rows_geometry(FMT, n, k, rows, max_blocks);
     const int T = geo.tiles, gy = geo.shares;
     const unsigned blocks = (unsigned)geo.batches < max_blocks ? (unsigned)geo.batches : max_blocks;
-    if (T == 2) hipLaunchKernelGGL((gemv_rows_kernel<FMT, 2>), dim3(blocks, gy), dim3(GR_THREADS), gemv_rows_lds_bytes(2) + gemv_rows_stage_bytes<FMT>(2), s, W, ops, inv, n, k, rows, groups, blocks | ((unsigned)gy << 16), bias, res, y);
-    else hipLaunchKernelGGL((gemv_rows_kernel<FMT, 1>), dim3(blocks, gy), dim3(GR_THREADS), gemv_rows_lds_bytes(1) + gemv_rows_stage_bytes<FMT>(1), s, W, ops, inv, n, k, rows, groups, blocks | ((unsigned)gy << 16), bias, res, y);
+    auto go = [&](auto tiles) {
+        constexpr int TT = decltype(tiles)::value;
+        const dim3 grid(blocks, gy), threads(GR_THREADS);
+        const size_t lds = gemv_rows_lds_bytes(TT) + gemv_rows_stage_bytes<FMT>(TT);
+        const uint32_t packed = blocks | ((unsigned)gy << 16);
+        if (e.act) hipLaunchKernelGGL((gemv_rows_act_kernel<FMT, TT>), grid, threads, lds, s, W, ops, inv, n, k, rows, groups, packed, bias, e.res, y, e.act);
+        else hipLaunchKernelGGL((gemv_rows_kernel<FMT, TT>), grid, threads, lds, s, W, ops, inv, n, k, rows, groups, packed, bias, e.res, y);
+    };
+    if (T == 2) go(std::integral_constant<int, 2>{});
+    else go(std::integral_constant<int, 1>{});
 }
 
-void gemv_rows_main_launch(int fmt, unsigned max_blocks, hipStream_t s, const uint8_t *W, const void *scratch, const float *bias, const float *res, float *y,
+void gemv_rows_main_launch(int fmt, unsigned max_blocks, hipStream_t s, const uint8_t *W, const void *scratch, const float *bias, const Epilogue &e, float *y,
                            int n, int k, int rows) {
     switch (fmt) {
-    case F_Q4_K: launch<F_Q4_K>(max_blocks, s, W, scratch, bias, res, y, n, k, rows); break;
-    case F_Q5_K: launch<F_Q5_K>(max_blocks, s, W, scratch, bias, res, y, n, k, rows); break;
-    case F_Q6_K: launch<F_Q6_K>(max_blocks, s, W, scratch, bias, res, y, n, k, rows); break;
-    case F_Q4_0: launch<F_Q4_0>(max_blocks, s, W, scratch, bias, res, y, n, k, rows); break;
-    case F_Q4_1: launch<F_Q4_1>(max_blocks, s, W, scratch, bias, res, y, n, k, rows); break;
-    case F_Q8_0: launch<F_Q8_0>(max_blocks, s, W, scratch, bias, res, y, n, k, rows); break;
-    case F_Q5_1: launch<F_Q5_1>(max_blocks, s, W, scratch, bias, res, y, n, k, rows); break;
-    case F_Q2_K: launch<F_Q2_K>(max_blocks, s, W, scratch, bias, res, y, n, k, rows); break;
+    case F_Q4_K: launch<F_Q4_K>(max_blocks, s, W, scratch, bias, e, y, n, k, rows); break;
+    case F_Q5_K: launch<F_Q5_K>(max_blocks, s, W, scratch, bias, e, y, n, k, rows); break;
+    case F_Q6_K: launch<F_Q6_K>(max_blocks, s, W, scratch, bias, e, y, n, k, rows); break;
+    case F_Q4_0: launch<F_Q4_0>(max_blocks, s, W, scratch, bias, e, y, n, k, rows); break;
+    case F_Q4_1: launch<F_Q4_1>(max_blocks, s, W, scratch, bias, e, y, n, k, rows); break;
+    case F_Q8_0: launch<F_Q8_0>(max_blocks, s, W, scratch, bias, e, y, n, k, rows); break;
+    case F_Q5_1: launch<F_Q5_1>(max_blocks, s, W, scratch, bias, e, y, n, k, rows); break;
+    case F_Q2_K: launch<F_Q2_K>(max_blocks, s, W, scratch, bias, e, y, n, k, rows); break;
     default: break;
     }
 }
@@ -233,7 +243,7 @@ void gemv_held_slices_launch(const HeldPlan &plan, int fmt, hipStream_t s, const
     held_launch(plan, fmt, s, (unsigned)(plan.slices * plan.per_slice), W, W2, scratch, 0, plan.where, part, n, k, rows);
 }
 
-void gemv_held_launch(const HeldPlan &plan, int fmt, int cus, hipStream_t s, const uint8_t *W, const void *scratch, const float *bias, const float *res,
+void gemv_held_launch(const HeldPlan &plan, int fmt, int cus, hipStream_t s, const uint8_t *W, const void *scratch, const float *bias, const Epilogue &e,
                       float *y, float *part, int n, int k, int rows) {
     if (plan.part && !part) {  // slice after slice into y: the order, and so the bits, of the join
         HeldGeo geo = HeldGeo::unpacked(plan.where);
@@ -243,11 +253,11 @@ void gemv_held_launch(const HeldPlan &plan, int fmt, int cus, hipStream_t s, con
             geo.slices = z == 0;
             held_launch(plan, fmt, s, (unsigned)plan.per_slice, W, nullptr, scratch, z * cols, geo.packed(), y, n, k, rows);
         }
-        rows_join_launch(s, y, y, rows, n, 1, bias, res, (unsigned)cus);
+        rows_join_launch(s, y, y, rows, n, 1, bias, e, (unsigned)cus);
         return;
     }
     gemv_held_slices_launch(plan, fmt, s, W, nullptr, scratch, plan.part ? part : y, n, k, rows);
-    if (plan.part) rows_join_launch(s, part, y, rows, n, plan.slices, bias, res, (unsigned)cus);
+    if (plan.part) rows_join_launch(s, part, y, rows, n, plan.slices, bias, e, (unsigned)cus);
 }
 
 }  // namespace jitnn

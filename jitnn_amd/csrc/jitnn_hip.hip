@@ -237,6 +237,7 @@ struct XregCall {
     const jitnn_hip_weight *w2 = nullptr;
     const float *x = nullptr, *norm_w = nullptr;
     float eps = 0.f;
+    Epilogue epi;  // one matrix, no norm, no w2; launch_i8 only
 };
 
 // kernel arguments of a call; returns the total number of rows
@@ -294,6 +295,7 @@ int i8_args(const XregCall &c, I8Args &a) {
     a.eps = c.eps;
     a.k = c.w[0]->k;
     a.rows = 1;
+    a.epi = c.epi;
     return n;
 }
 
@@ -314,7 +316,7 @@ void i8_shape(int fmt, int groups, int waves, bool dual, int &blocks, int &pf) {
 int launch_i8(const XregCall &c, hipStream_t stream) {
     I8Args a{};
     const int n = i8_args(c, a);
-    const int mode = c.w2 ? I8_DUAL : c.norm_w ? I8_NORM : c.bias ? I8_BIAS : I8_PLAIN;
+    const int mode = c.w2 ? I8_DUAL : c.norm_w ? I8_NORM : c.epi.any() ? I8_EPI : c.bias ? I8_BIAS : I8_PLAIN;
     int blocks, pf;
     i8_shape(c.w[0]->fmt, (n + 3) / 4, (a.k + 1023) / 1024, c.w2 != nullptr, blocks, pf);
     if (c.w[0]->fmt == F_Q5_K && pf > 2) pf = 2;  // (five loads per turn: a fourth buffer does not fit 128 registers)
@@ -336,7 +338,7 @@ bool i8_batch_ok(const jitnn_hip_weight *w, int rows) {
            ((block_values(w->fmt) != 32 && w->fmt != F_Q2_K) || ((uintptr_t)w->dev & 3) == 0);
 }
 
-int launch_i8_batch(const jitnn_hip_weight *w, const float *x, int rows, const float *bias, float *y, hipStream_t stream) {
+int launch_i8_batch(const jitnn_hip_weight *w, const float *x, int rows, const float *bias, const Epilogue &e, float *y, hipStream_t stream) {
     I8Args a{};
     for (int i = 0; i < 3; ++i) {
         a.w[i] = w->dev;
@@ -347,13 +349,14 @@ int launch_i8_batch(const jitnn_hip_weight *w, const float *x, int rows, const f
     a.x = x;
     a.k = w->k;
     a.rows = rows;
+    a.epi = e;
     const int groups = (w->n + 3) / 4;
     // (us per launch by workgroups per CU / turns in flight, two rows - Q4_K 14336 x 4096: 10.4 (1 / 2) 10.3 (2 / 2) 10.6 (2 / 1) 11.6 (1 / 1)
     // 11.9 (3 / 1); Q4_0 11008 x 4096: 7.9 (1 / 2) 8.4 (2 / 1, 2 / 2) 8.6 (1 / 1); Q8_0 4096 x 4096: 6.4 (1 / 1) 6.7 (1 / 2) 6.9 (2 / 1) 7.7 (2 / 2);
     // four rows - Q4_K: 13.1 (1 / 2, 2 / 1) 14.0 (1 / 1); Q4_0: 10.6 (1 / 2) 10.9 (1 / 1) 11.0 (2 / 1); Q8_0: 7.1 (1 / 1) 7.7 (1 / 2) 9.1 (2 / 1))
     const int per_cu = 1, pf = (groups + g.cus - 1) / g.cus >= 8 ? 2 : 1;
     const int blocks = groups < g.cus * per_cu ? groups : g.cus * per_cu;
-    if (!gemv_i8_launch(w->fmt, bias ? I8_BIAS : I8_PLAIN, pf, (unsigned)blocks, stream, a))
+    if (!gemv_i8_launch(w->fmt, e.any() ? I8_EPI : bias ? I8_BIAS : I8_PLAIN, pf, (unsigned)blocks, stream, a))
         return fail(JITNN_HIP_EDEVICE, "no INT8 GEMV kernel for format %d at %d rows of %d values", w->fmt, rows, a.k);
     HIP_TRY(hipGetLastError());
     return JITNN_HIP_OK;
@@ -538,11 +541,11 @@ int launch_gemv_xreg_b2(const jitnn_hip_weight *w, const float *x, const float *
 
 // Batch 2..8, rows a multiple of 256 values long: block sums on the matrix cores, one workgroup of 8 waves per CU
 // (the kernels live in gemv_mfma.hip).
-int launch_gemv_mfma(const KernelRef &v, const jitnn_hip_weight *w, const float *x, int rows, const float *bias, float *y, hipStream_t stream) {
+int launch_gemv_mfma(const KernelRef &v, const jitnn_hip_weight *w, const float *x, int rows, const float *bias, const Epilogue &e, float *y, hipStream_t stream) {
     if (int rc = allow_lds(v.fn, v.lds)) return rc;
     const int groups = (w->n + 15) / 16;
     const int blocks = groups < g.cus ? groups : g.cus;
-    gemv_mfma_launch(w->fmt, (unsigned)blocks, stream, w->dev, x, bias, y, w->n, w->k, rows);
+    gemv_mfma_launch(w->fmt, (unsigned)blocks, stream, w->dev, x, bias, e, y, w->n, w->k, rows);
     HIP_TRY(hipGetLastError());
     return JITNN_HIP_OK;
 }
@@ -560,7 +563,13 @@ int launch_gemv_plain(const jitnn_hip_weight *w, const float *x, int rows, const
     return JITNN_HIP_OK;
 }
 
-int launch_gemv(const jitnn_hip_weight *w, const float *x, int rows, const float *bias, float *y, hipStream_t stream) {
+// The kernels of up to eight rows.  unmet: an epilogue that is asked for; cleared by the kernels that have one.
+int launch_gemv(const jitnn_hip_weight *w, const float *x, int rows, const float *bias, float *y, hipStream_t stream, Epilogue *unmet = nullptr) {
+    const Epilogue e = unmet ? *unmet : Epilogue{};
+    auto met = [&]() {
+        if (unmet) *unmet = Epilogue{};
+        return e;
+    };
     if (is_extra_format(w->fmt)) {
         if (rows == 1) {  // Q5_1 and Q2_K have units of the INT8 matrix-core kernel
             XregCall c;
@@ -568,24 +577,41 @@ int launch_gemv(const jitnn_hip_weight *w, const float *x, int rows, const float
             c.y[0] = y;
             c.bias = bias;
             c.x = x;
-            if (i8_ok(c)) return launch_i8(c, stream);
+            if (i8_ok(c)) {
+                c.epi = met();
+                return launch_i8(c, stream);
+            }
         } else if (i8_batch_ok(w, rows < 4 ? rows : 4)) {
             // up to four rows per launch; more rows - where the one-pass kernel of gemv_rows.h does not take the shape (it has tiles
             // for both formats: 14336 x 4096 at 5..8 rows Q5_1 23 us, Q2_K 19 us against 28, 29 as two launches here) - as a chain of
             // such launches, each streaming the weights again
-            for (int r0 = 0; r0 < rows; r0 += 4)
-                if (int rc = launch_i8_batch(w, x + (size_t)r0 * w->k, rows - r0 < 4 ? rows - r0 : 4, bias, y + (size_t)r0 * w->n, stream)) return rc;
+            met();
+            for (int r0 = 0; r0 < rows; r0 += 4) {
+                const Epilogue part{e.act, e.res ? e.res + (size_t)r0 * w->n : nullptr};
+                if (int rc = launch_i8_batch(w, x + (size_t)r0 * w->k, rows - r0 < 4 ? rows - r0 : 4, bias, part, y + (size_t)r0 * w->n, stream)) return rc;
+            }
             return JITNN_HIP_OK;
         }
         return launch_gemv_plain(w, x, rows, bias, y, stream);
     }
-    if (i8_batch_ok(w, rows)) return launch_i8_batch(w, x, rows, bias, y, stream);
+    if (i8_batch_ok(w, rows)) return launch_i8_batch(w, x, rows, bias, met(), y, stream);
     if (rows == 2 && w->k <= 4096) return launch_gemv_xreg_b2(w, x, bias, y, stream);
     // Q6_K pays the most per weight on the matrix-core path (6-bit quants from two arrays, 16-value scale groups): up to
     // four rows its FP32 kernel is still ahead (measured: 33 vs 43 us at 2 rows, 151 vs 167 us at 4 rows on the output head)
     if (rows >= (w->fmt == F_Q6_K ? 5 : 2) && rows <= 8 && w->k % 256 == 0 && w->n >= 16) {
-        const KernelRef v = gemv_mfma_kernel_ref(w->fmt);
-        if (v.fn && v.lds <= g.max_lds) return launch_gemv_mfma(v, w, x, rows, bias, y, stream);
+        const KernelRef v = gemv_mfma_kernel_ref(w->fmt, e.any());
+        if (v.fn && v.lds <= g.max_lds) return launch_gemv_mfma(v, w, x, rows, bias, met(), y, stream);
+    }
+    if (rows == 1 && e.any()) {
+        XregCall c;
+        c.w[0] = w;
+        c.y[0] = y;
+        c.bias = bias;
+        c.x = x;
+        if (i8_ok(c)) {
+            c.epi = met();
+            return launch_i8(c, stream);
+        }
     }
     if (rows == 1) {
         if (w->k <= 4096) return launch_gemv_xreg(w, x, bias, y, stream);
@@ -1436,12 +1462,14 @@ HeldPlan rows_plan(const jitnn_hip_weight *w, int rows, bool adds, int cus) {
 // swiglu_up: the activations are silu(x) * swiglu_up, formed by the preparation as it reads x.
 // later, defer (one weight, a residual): where the sums come in up to eight slices, they go to later and their join is left to the
 // caller, as *defer.
+// act: of the sum and bias, in front of the residual (one weight, nothing put off).
 // together, room, gdefer (three weights): where one of them comes in slices, all three go to `together` (room floats), one after
 // the other, a weight that has none as its one slice, and the caller joins them, as *gdefer.
 int launch_rows_group(const jitnn_hip_weight *const *ws, float *const *ys, int count, const float *x, int rows, const float *bias, const float *residual,
                       hipStream_t s, ScratchSource src, const float *swiglu_up = nullptr, float *later = nullptr, PfPending *defer = nullptr,
-                      float *together = nullptr, size_t room = 0, PfGroupPending *gdefer = nullptr) {
+                      float *together = nullptr, size_t room = 0, PfGroupPending *gdefer = nullptr, int act = JITNN_HIP_ACT_NONE) {
     const int k = ws[0]->k;
+    const Epilogue epi{act, residual};
     bool need[GR_LAYOUTS] = {};  // the operand layouts the weights ask for
     const size_t one = rows_operand_bytes(rows, k);
     int layouts = 0;
@@ -1476,7 +1504,7 @@ int launch_rows_group(const jitnn_hip_weight *const *ws, float *const *ys, int c
             later_plan = plan[i].slices;
             continue;
         }
-        plan[i] = rows_plan(ws[i], rows, bias || residual, g.cus);
+        plan[i] = rows_plan(ws[i], rows, bias || epi.any(), g.cus);
         part = std::max(part, plan[i].part_bytes(rows, ws[i]->n));
     }
     void *scratch = nullptr;
@@ -1484,7 +1512,7 @@ int launch_rows_group(const jitnn_hip_weight *const *ws, float *const *ys, int c
     if (int rc = workspace(one * layouts + part, s, &scratch, src)) return rc;
     for (int i = 0; i < count; ++i) {
         const KernelRef kr = plan[i].groups_held ? gemv_held_kernel_ref(ws[i]->fmt, plan[i].groups_held)
-                                                 : gemv_rows_kernel_ref(ws[i]->fmt, ws[i]->n, k, rows, (unsigned)g.cus);
+                                                 : gemv_rows_kernel_ref(ws[i]->fmt, ws[i]->n, k, rows, (unsigned)g.cus, act != JITNN_HIP_ACT_NONE);
         if (int rc = allow_lds(kr.fn, kr.lds)) return rc;
     }
     uint8_t *sc[GR_LAYOUTS] = {};
@@ -1496,7 +1524,7 @@ int launch_rows_group(const jitnn_hip_weight *const *ws, float *const *ys, int c
         if (grouped) {
             const int splits = plan[i].groups_held ? plan[i].slices : 1;
             if (plan[i].groups_held) gemv_held_slices_launch(plan[i], ws[i]->fmt, s, ws[i]->dev, nullptr, ops, together, ws[i]->n, k, rows);
-            else gemv_rows_main_launch(ws[i]->fmt, (unsigned)g.cus, s, ws[i]->dev, ops, nullptr, nullptr, together, ws[i]->n, k, rows);
+            else gemv_rows_main_launch(ws[i]->fmt, (unsigned)g.cus, s, ws[i]->dev, ops, nullptr, Epilogue{}, together, ws[i]->n, k, rows);
             if (i == 0) gdefer->part = together;
             gdefer->sg.splits[i] = splits;
             gdefer->sg.n[i] = ws[i]->n;
@@ -1509,8 +1537,8 @@ int launch_rows_group(const jitnn_hip_weight *const *ws, float *const *ys, int c
             defer->splits = later_plan;
             defer->n = ws[i]->n;
         } else if (plan[i].groups_held)
-            gemv_held_launch(plan[i], ws[i]->fmt, g.cus, s, ws[i]->dev, ops, bias, residual, ys[i], part ? (float *)((uint8_t *)scratch + one * layouts) : nullptr, ws[i]->n, k, rows);
-        else gemv_rows_main_launch(ws[i]->fmt, (unsigned)g.cus, s, ws[i]->dev, ops, bias, residual, ys[i], ws[i]->n, k, rows);
+            gemv_held_launch(plan[i], ws[i]->fmt, g.cus, s, ws[i]->dev, ops, bias, epi, ys[i], part ? (float *)((uint8_t *)scratch + one * layouts) : nullptr, ws[i]->n, k, rows);
+        else gemv_rows_main_launch(ws[i]->fmt, (unsigned)g.cus, s, ws[i]->dev, ops, bias, epi, ys[i], ws[i]->n, k, rows);
     }
     HIP_TRY(hipGetLastError());
     return workspace_done(s, src);
@@ -1547,7 +1575,7 @@ int launch_rows_ffn(const RowsFfn &f, const jitnn_hip_weight *wg, const jitnn_hi
     const size_t ops = f.ops, sums = f.sums, ops_down = f.ops_down, total = f.total;
     const bool to_reader = f.to_reader;
     const KernelRef kp = gemv_held_kernel_ref(wg->fmt, pair.groups_held),
-                    kd = down.groups_held ? gemv_held_kernel_ref(wd->fmt, down.groups_held) : gemv_rows_kernel_ref(wd->fmt, wd->n, n, rows, (unsigned)g.cus);
+                    kd = down.groups_held ? gemv_held_kernel_ref(wd->fmt, down.groups_held) : gemv_rows_kernel_ref(wd->fmt, wd->n, n, rows, (unsigned)g.cus, false);
     if (int rc = allow_lds(kp.fn, kp.lds)) return rc;
     if (int rc = allow_lds(kd.fn, kd.lds)) return rc;
     void *scratch = nullptr;
@@ -1570,41 +1598,58 @@ int launch_rows_ffn(const RowsFfn &f, const jitnn_hip_weight *wg, const jitnn_hi
         defer->splits = down.slices;
         defer->n = wd->n;
     } else if (down.groups_held) {
-        gemv_held_launch(down, wd->fmt, g.cus, s, wd->dev, md, nullptr, res, y, (float *)(base + ops + sums + ops_down), wd->n, n, rows);
+        gemv_held_launch(down, wd->fmt, g.cus, s, wd->dev, md, nullptr, Epilogue{0, res}, y, (float *)(base + ops + sums + ops_down), wd->n, n, rows);
     } else {
-        gemv_rows_main_launch(wd->fmt, (unsigned)g.cus, s, wd->dev, md, nullptr, res, y, wd->n, n, rows);
+        gemv_rows_main_launch(wd->fmt, (unsigned)g.cus, s, wd->dev, md, nullptr, Epilogue{0, res}, y, wd->n, n, rows);
     }
     HIP_TRY(hipGetLastError());
     return workspace_done(s);
 }
 
-int launch_gemv_tail(const jitnn_hip_weight *w, const float *x, int rows, float *y, hipStream_t s) {
+template <bool EPI>
+void (*gemv_tail_of(int fmt))(const uint8_t *, const float *, float *, int, int, int, int, const Epilogue) {
+    return fmt == F_Q4_0 ? gemv_tail_kernel<F_Q4_0, EPI> : fmt == F_Q4_1 ? gemv_tail_kernel<F_Q4_1, EPI> : gemv_tail_kernel<F_Q8_0, EPI>;
+}
+int launch_gemv_tail(const jitnn_hip_weight *w, const float *x, int rows, const Epilogue &e, float *y, hipStream_t s) {
     const int blocks = w->k % 256 / 32;
     const size_t lds = gemv_tail_lds_bytes(rows, blocks);
-    auto kernel = w->fmt == F_Q4_0 ? gemv_tail_kernel<F_Q4_0> : w->fmt == F_Q4_1 ? gemv_tail_kernel<F_Q4_1> : gemv_tail_kernel<F_Q8_0>;
+    const auto kernel = e.any() ? gemv_tail_of<true>(w->fmt) : gemv_tail_of<false>(w->fmt);
     if (int rc = allow_lds((const void *)kernel, lds)) return rc;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)((w->n + GT_ROWS - 1) / GT_ROWS)), dim3(GT_THREADS), lds, s, w->dev, x, y, w->n, w->k, rows, blocks);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((w->n + GT_ROWS - 1) / GT_ROWS)), dim3(GT_THREADS), lds, s, w->dev, x, y, w->n, w->k, rows, blocks, e);
     HIP_TRY(hipGetLastError());
     return JITNN_HIP_OK;
 }
 
-int linear_dev(const jitnn_hip_weight *w, const float *x_dev, int rows, const float *bias_dev, float *y_dev, hipStream_t s, ScratchSource src) {
+// y = act(x W^T (+ bias)) (+ res): by the kernel that makes the sums where it has an epilogue, else by a launch behind it (many rows; rows of odd lengths).
+int linear_dev(const jitnn_hip_weight *w, const float *x_dev, int rows, const float *bias_dev, float *y_dev, hipStream_t s, ScratchSource src, const Epilogue &e = Epilogue{}) {
     if (!w || !x_dev || !y_dev) return fail(JITNN_HIP_EINVAL, "weight, input or output is NULL");
     if (rows < 1) return fail(JITNN_HIP_EINVAL, "rows = %d", rows);
     if (int rc = check_ready()) return rc;
+    auto behind = [&](const Epilogue &unmet, float *y, int count) -> int {
+        if (!unmet.any()) return JITNN_HIP_OK;
+        linear_epilogue_launch(unmet.act, unmet.res, y, (size_t)count * w->n, g.cus, s);
+        HIP_TRY(hipGetLastError());
+        return JITNN_HIP_OK;
+    };
     const bool many = rows > g.gemv_max_rows && has_many_row_kernel(w->fmt);
-    count_op(many ? ST_MFMA : ST_GEMV, (long long)w->nbytes + 4ll * rows * ((long long)w->k + w->n) + (bias_dev ? 4ll * w->n : 0));
-    if (many) return launch_prefill(w, x_dev, rows, bias_dev, y_dev, s, src);
+    count_op(many ? ST_MFMA : ST_GEMV, (long long)w->nbytes + 4ll * rows * ((long long)w->k + w->n) + (bias_dev ? 4ll * w->n : 0) + (e.res ? 4ll * rows * w->n : 0));
+    if (many) {
+        if (int rc = launch_prefill(w, x_dev, rows, bias_dev, y_dev, s, src)) return rc;
+        return behind(e, y_dev, rows);
+    }
     // several rows, rows of whole 256-value columns: every row meets the weights in one pass over them (gemv_rows.h)
-    if (rows_path(w, rows)) return launch_rows_group(&w, &y_dev, 1, x_dev, rows, bias_dev, nullptr, s, src);
+    if (rows_path(w, rows)) return launch_rows_group(&w, &y_dev, 1, x_dev, rows, bias_dev, e.res, s, src, nullptr, nullptr, nullptr, nullptr, 0, nullptr, e.act);
     // (no scratch at hand - a stream capture before the first eager call, no memory: the passes of eight, which need none)
     if (rows_ragged_path(w, rows) && workspace_at_hand(rows_operand_bytes(rows, w->k), s, src)) {
         if (int rc = launch_rows_group(&w, &y_dev, 1, x_dev, rows, bias_dev, nullptr, s, src)) return rc;
-        return launch_gemv_tail(w, x_dev, rows, y_dev, s);
+        return launch_gemv_tail(w, x_dev, rows, e, y_dev, s);
     }
     for (int r0 = 0; r0 < rows; r0 += 8) {
         const int nb = rows - r0 < 8 ? rows - r0 : 8;
-        if (int rc = launch_gemv(w, x_dev + (size_t)r0 * w->k, nb, bias_dev, y_dev + (size_t)r0 * w->n, s)) return rc;
+        float *const y = y_dev + (size_t)r0 * w->n;
+        Epilogue unmet{e.act, e.res ? e.res + (size_t)r0 * w->n : nullptr};
+        if (int rc = launch_gemv(w, x_dev + (size_t)r0 * w->k, nb, bias_dev, y, s, &unmet)) return rc;
+        if (int rc = behind(unmet, y, nb)) return rc;
     }
     return JITNN_HIP_OK;
 }
@@ -1629,13 +1674,7 @@ int jitnn_hip_linear_dev(const jitnn_hip_weight *w, const float *x_dev, int rows
 
 int jitnn_hip_linear_act_dev(const jitnn_hip_weight *w, const float *x_dev, int rows, const float *bias_dev, int activation, const float *residual_dev, float *y_dev, void *stream) {
     if (int rc = check_linear_act(w, rows, activation, residual_dev, y_dev)) return rc;
-    hipStream_t s = (hipStream_t)stream;
-    if (int rc = linear_dev(w, x_dev, rows, bias_dev, y_dev, s, SCRATCH_THREAD)) return rc;
-    if (activation != JITNN_HIP_ACT_NONE || residual_dev) {
-        linear_epilogue_launch(activation, residual_dev, y_dev, (size_t)rows * w->n, g.cus, s);
-        HIP_TRY(hipGetLastError());
-    }
-    return JITNN_HIP_OK;
+    return linear_dev(w, x_dev, rows, bias_dev, y_dev, (hipStream_t)stream, SCRATCH_THREAD, Epilogue{activation, residual_dev});
 }
 
 int jitnn_hip_linear_noalloc_dev(const jitnn_hip_weight *w, const float *x_dev, int rows, const float *bias_dev, float *y_dev, void *stream) {

@@ -90,9 +90,16 @@ void prefill_wide_launch(bool dual, int rt, hipStream_t s, const PwArgs &a);
 // rows of W [n, k] as operands to wo; half 0 / 1: the gate / up rows of a dual product, whose row blocks alternate in pairs
 void wide_dequant_launch(int fmt, hipStream_t s, const uint8_t *W, _Float16 *wo, int n, int k, int half);
 
+// What follows the sum and bias of a linear: y = act(...) + res [rows, n] (act.h).  The kernels have a variant of their own with it, so that launches without are as they were.
+struct Epilogue {
+    int act = 0;  // ACT_*
+    const float *res = nullptr;
+    bool any() const { return act != 0 || res; }
+};
+
 // ---- gemv_mfma.hip: gemv_mfma_kernel<fmt>
-KernelRef gemv_mfma_kernel_ref(int fmt);
-void gemv_mfma_launch(int fmt, unsigned blocks, hipStream_t s, const uint8_t *W, const float *x, const float *bias, float *y, int n, int k, int rows);
+KernelRef gemv_mfma_kernel_ref(int fmt, bool epilogue);
+void gemv_mfma_launch(int fmt, unsigned blocks, hipStream_t s, const uint8_t *W, const float *x, const float *bias, const Epilogue &e, float *y, int n, int k, int rows);
 
 // ---- gemv_rows.hip: rows_prepare_kernel + gemv_rows_kernel<fmt>: 2..64 rows in one pass over the weights.  The operands of
 // the activations are prepared once per operand layout a format needs (gemv_rows_layout: block sums per 32 or per 16
@@ -102,13 +109,13 @@ constexpr int GR_LAYOUT_PLAIN = 0, GR_LAYOUT_SUMS16 = 1, GR_LAYOUT_HALVES = 2, G
 bool gemv_rows_supported(int fmt);
 int gemv_rows_layout(int fmt);                     // GR_LAYOUT_* of the format, -1: the kernel is not built for it
 size_t gemv_rows_scratch_bytes(int rows, int k);   // operands + scales of `rows` activation rows of k values
-KernelRef gemv_rows_kernel_ref(int fmt, int n, int k, int rows, unsigned max_blocks);  // the variant gemv_rows_main_launch picks for this shape
+KernelRef gemv_rows_kernel_ref(int fmt, int n, int k, int rows, unsigned max_blocks, bool activated);  // the variant gemv_rows_main_launch picks for this shape
 // every layout with a scratch (scratch[GR_LAYOUTS], nullptr: not wanted) in one launch; swiglu_up != nullptr: the rows are
 // silu(x) * swiglu_up, both [rows, k]
 // (slices > 1, with swiglu_up: both are [slices][rows, k], to be added up)
 void gemv_rows_prepare_launch(hipStream_t s, const float *x, const float *swiglu_up, void *const *scratch, int k, int rows, int slices = 1);
-// y = x W^T (+ bias [n]) (+ res [rows, n])
-void gemv_rows_main_launch(int fmt, unsigned max_blocks, hipStream_t s, const uint8_t *W, const void *scratch, const float *bias, const float *res, float *y,
+// y = act(x W^T (+ bias [n])) (+ res [rows, n])
+void gemv_rows_main_launch(int fmt, unsigned max_blocks, hipStream_t s, const uint8_t *W, const void *scratch, const float *bias, const Epilogue &e, float *y,
                            int n, int k, int rows);
 
 // ---- gemv_held_k.hip, gemv_held_q32.hip: gemv_held_kernel<fmt>, the same products with the activation operands held in
@@ -131,10 +138,10 @@ KernelRef gemv_held_kernel_ref(int fmt, int groups_held);
 // part [slices][rows, n] = the slices of x W^T, behind them those of x W2^T
 void gemv_held_slices_launch(const HeldPlan &plan, int fmt, hipStream_t s, const uint8_t *W, const uint8_t *W2, const void *scratch, float *part, int n, int k,
                              int rows);
-// y = x W^T (+ bias [n]) (+ res [rows, n]); part: plan.part_bytes(rows, n) of scratch, or nullptr: the same bits, a launch per slice
-void gemv_held_launch(const HeldPlan &plan, int fmt, int cus, hipStream_t s, const uint8_t *W, const void *scratch, const float *bias, const float *res,
+// y = act(x W^T (+ bias [n])) (+ res [rows, n]); part: plan.part_bytes(rows, n) of scratch, or nullptr: the same bits, a launch per slice
+void gemv_held_launch(const HeldPlan &plan, int fmt, int cus, hipStream_t s, const uint8_t *W, const void *scratch, const float *bias, const Epilogue &e,
                       float *y, float *part, int n, int k, int rows);
-void rows_join_launch(hipStream_t s, const float *part, float *y, int rows, int n, int slices, const float *bias, const float *res, unsigned cus);
+void rows_join_launch(hipStream_t s, const float *part, float *y, int rows, int n, int slices, const float *bias, const Epilogue &e, unsigned cus);
 
 // ---- gemv_i8.hip: gemv_i8_kernel / gemv_i8_plain_kernel<unit>: GEMV of one to four activation rows with INT8 matrix-core products on the
 // raw quants.  The argument block of the kernels (the launchers put what a wave's first loads need in front of it, as scalar
@@ -151,12 +158,13 @@ struct I8Args {
     float eps;
     int k;
     int rows;  // activation rows (x [rows, k], y [rows, n]); more than one: a single matrix, no norm, no pair
+    Epilogue epi;  // EPI: y[0] = act(w[0] x + bias[0] (or 0)) + res (or 0)
 };
 
-constexpr int I8_PLAIN = 0, I8_BIAS = 1, I8_NORM = 2, I8_DUAL = 3;  // DUAL: norm + the SwiGLU pair
+constexpr int I8_PLAIN = 0, I8_BIAS = 1, I8_NORM = 2, I8_DUAL = 3, I8_EPI = 4;  // DUAL: norm + the SwiGLU pair
 bool gemv_i8_supported(int fmt, int k);
 // One wave per 1024 values of a row (the launchers set the workgroup size); pf = turns of weight bytes in flight per wave beyond the one being multiplied (1..3; 1..2 for
-// two to four activation rows - a.rows in 2..4, rows of at most 4096 values, modes I8_PLAIN and I8_BIAS only)
+// two to four activation rows - a.rows in 2..4, rows of at most 4096 values, modes I8_PLAIN, I8_BIAS and I8_EPI only)
 bool gemv_i8_launch(int fmt, int mode, int pf, unsigned blocks, hipStream_t s, const I8Args &a);  // false: no kernel for this call, nothing launched
 bool gemv_i8_pair_supported(int fmt_a, int fmt_b);
 bool gemv_i8_pair_launch(int fmt_a, int fmt_b, int pf, unsigned blocks_a, unsigned blocks_b, hipStream_t s, const I8Args &a, const I8Args &b);
