@@ -428,6 +428,10 @@ JITNN_HIP_API int jitnn_hip_llama_free(jitnn_hip_llama *m);
 /* Attaches a weight (not owned; shapes are checked: q/o [heads*head_dim, d_model] resp. [d_model, heads*head_dim],
  * k/v [kv_heads*head_dim, d_model], gate/up [ffn, d_model], down [d_model, ffn], output [vocab, d_model]). */
 JITNN_HIP_API int jitnn_hip_llama_set_weight(jitnn_hip_llama *m, int layer, int which, const jitnn_hip_weight *w);
+/* Experts in place of a layer's gate, up and down (which it then need not have): x + moe(RMSNorm(x)).  Not owned; d_model as the model's, any ffn.  NULL: the layer is
+ * dense again.  Their workspace belongs to the model: one token's is allocated here, those of longer passes with the many-token buffers.  Not while work of
+ * this model is under way, nor between a recording and its replays. */
+JITNN_HIP_API int jitnn_hip_llama_set_moe(jitnn_hip_llama *m, int layer, const jitnn_hip_moe *moe);
 /* Copies an RMSNorm weight vector [d_model] from host memory. */
 JITNN_HIP_API int jitnn_hip_llama_set_norm(jitnn_hip_llama *m, int layer, int which, const float *w_host);
 

@@ -129,6 +129,7 @@ def _bind() -> C.CDLL:
         "jitnn_hip_moe_dev": (i, [vp, vp, i, vp, vp, vp, ll, vp]),
         "jitnn_hip_moe_experts_dev": (i, [vp, vp, i, vp, vp, vp, vp, vp, ll, vp]),
         "jitnn_hip_llama_set_rope": (i, [vp, vp]),
+        "jitnn_hip_llama_set_moe": (i, [vp, i, vp]),
         "jitnn_hip_llama_step_dev": (i, [vp, vp, batch, vp, vp, i, vp, vp]),
     }
     for name, (res, args) in sig.items():

@@ -2780,6 +2780,10 @@ struct jitnn_hip_llama {
     float eps, theta;
     const jitnn_hip_weight **w;  // [layers][7] then output
     const jitnn_hip_weight *w_out;
+    const jitnn_hip_moe **moe;   // [layers]: the experts in place of a layer's gate, up and down, nullptr: it has those
+    void *moe_ws[2];             // their workspace: of one token (decode steps), of up to moe_cap (passes of many), allocated with the many-token buffers
+    size_t moe_ws_bytes[2];
+    int moe_cap;
     float *norms;                // [layers][2][d] then output norm [d]
     float *kc, *vc;              // [layers][max_ctx][kv][hd]
     float *cosv, *sinv;          // [max_ctx][hd/2]
@@ -2894,16 +2898,22 @@ int normed_linears(const jitnn_hip_llama *m, const jitnn_hip_weight *const *ws, 
 int check_model(const jitnn_hip_llama *m) {
     if (!m) return fail(JITNN_HIP_EINVAL, "model is NULL");
     for (int l = 0; l < m->layers; ++l)
-        for (int i = 0; i < 7; ++i)
+        for (int i = 0; i < (m->moe[l] ? (int)JITNN_HIP_W_FFN_GATE : 7); ++i)
             if (!m->w[l * 7 + i]) return fail(JITNN_HIP_EINVAL, "layer %d has no weight %d", l, i);
     if (!m->w_out) return fail(JITNN_HIP_EINVAL, "no output weight");
     return JITNN_HIP_OK;
 }
 
-// bytes of every weight a step of the model reads (norm vectors included)
-long long model_weight_bytes(const jitnn_hip_llama *m) {
+// bytes of every weight a step of the model reads (norm vectors included; of experts, as many as so many tokens can meet)
+long long model_weight_bytes(const jitnn_hip_llama *m, int tokens) {
     long long b = m->w_out->nbytes + 4ll * (2 * m->layers + 1) * m->d;
-    for (int i = 0; i < m->layers * 7; ++i) b += m->w[i]->nbytes;
+    for (int l = 0; l < m->layers; ++l) {
+        const jitnn_hip_moe *e = m->moe[l];
+        for (int i = 0; i < (e ? (int)JITNN_HIP_W_FFN_GATE : 7); ++i) b += m->w[l * 7 + i]->nbytes;
+        if (!e) continue;
+        const long long met = std::min<long long>(e->router->experts, (long long)tokens * e->router->used);
+        b += 4ll * e->router->experts * m->d + (long long)(e->gate->nbytes + e->up->nbytes + e->down->nbytes) / e->router->experts * met;
+    }
     return b;
 }
 
@@ -3004,8 +3014,31 @@ void release_or_keep(jitnn_hip_llama *m, void *p) {
     else if (!m->recorded) (void)hipFree(p);  // (no memory to note it: left to the process)
 }
 
+// The workspace of a model's experts for passes of up to `tokens`; which 0: one token's.  The device may still use the old one.
+int moe_reserve(jitnn_hip_llama *m, int which, int tokens) {
+    long long need = 0;
+    for (int l = 0; l < m->layers; ++l)
+        if (m->moe[l]) need = std::max(need, jitnn_hip_moe_workspace(m->moe[l], tokens));
+    if ((size_t)need <= m->moe_ws_bytes[which]) return JITNN_HIP_OK;
+    HIP_TRY(hipDeviceSynchronize());
+    release_or_keep(m, m->moe_ws[which]);
+    m->moe_ws[which] = nullptr;
+    m->moe_ws_bytes[which] = 0;
+    if (hipMalloc(&m->moe_ws[which], (size_t)need) != hipSuccess) {
+        (void)hipGetLastError();
+        m->moe_ws[which] = nullptr;
+        return fail(JITNN_HIP_ENOMEM, "no %lld bytes of device memory for the experts of %d tokens", need, tokens);
+    }
+    m->moe_ws_bytes[which] = (size_t)need;
+    return JITNN_HIP_OK;
+}
+
 // The many-token buffers of a model, for at least `tokens` rows.
 int ensure_prefill(jitnn_hip_llama *m, int tokens) {
+    if (tokens > m->moe_cap) {
+        if (int rc = moe_reserve(m, 1, tokens)) return rc;
+        m->moe_cap = tokens;
+    }
     if (tokens <= m->pf_cap) return JITNN_HIP_OK;
     HIP_TRY(hipDeviceSynchronize());  // earlier calls may still use the old buffers
     m->pf_cap = 0;
@@ -3045,6 +3078,7 @@ void prefill_reserve(const jitnn_hip_llama *m, int tokens, hipStream_t st) {
         };
         want(JITNN_HIP_W_ATTN_Q, 3, false, false);
         want(JITNN_HIP_W_ATTN_O, 1, false, true);
+        if (m->moe[l]) continue;
         want(JITNN_HIP_W_FFN_GATE, 2, prefill_dual_ok(w[JITNN_HIP_W_FFN_GATE], w[JITNN_HIP_W_FFN_UP]), false);
         want(JITNN_HIP_W_FFN_DOWN, 1, false, true);
     }
@@ -3161,7 +3195,10 @@ int run_layers(jitnn_hip_llama *m, const float *x_dev, int T, bool defer, hipStr
         if (int rc = attend(l, q, k, v, att, gp)) return rc;
         // xa = x + Wo att, xb = xa + W2 (silu(W1 n) * (W3 n)), n = RMSNorm(xa)
         if (int rc = residual_linear_rows(w[JITNN_HIP_W_ATTN_O], att, T, x, xn, xa, st, nullptr, nullptr, m->pf[10], &pend)) return rc;
-        if (T > g.gemv_max_rows && prefill_dual_ok(w[JITNN_HIP_W_FFN_GATE], w[JITNN_HIP_W_FFN_UP])) {
+        if (m->moe[l]) {
+            norm_rows(m, xa, T, nw + d, xn, st, &pend);
+            if (int rc = jitnn_hip_moe_dev(m->moe[l], xn, T, xa, xb, m->moe_ws[1], (long long)m->moe_ws_bytes[1], st)) return rc;
+        } else if (T > g.gemv_max_rows && prefill_dual_ok(w[JITNN_HIP_W_FFN_GATE], w[JITNN_HIP_W_FFN_UP])) {
             // gate and up as one product with the SwiGLU in its epilogue: h = silu(W1 n) * (W3 n) directly
             const bool fused = pend.part && pend.out == xa && pend.n == d;
             if (!fused) flush_pending(pend, T, st);
@@ -3240,6 +3277,7 @@ int jitnn_hip_llama_create(int layers, int d_model, int heads, int kv_heads, int
     m->max_ctx = max_ctx; m->eps = rms_eps; m->theta = rope_theta;
     m->attention = -1;
     m->w = new (std::nothrow) const jitnn_hip_weight *[(size_t)layers * 7]();
+    m->moe = new (std::nothrow) const jitnn_hip_moe *[(size_t)layers]();
     m->chunks_max = (max_ctx + 15) / 16;  // the smallest key chunk any head size uses
     const size_t cache = (size_t)layers * max_ctx * kv_heads * head_dim;
     const int qd = heads * head_dim, kd = kv_heads * head_dim, half = head_dim / 2;
@@ -3248,7 +3286,7 @@ int jitnn_hip_llama_create(int layers, int d_model, int heads, int kv_heads, int
         {&m->sinv, (size_t)max_ctx * half}, {&m->xin, (size_t)d_model}, {&m->xa, (size_t)d_model}, {&m->xb, (size_t)d_model}, {&m->xn, (size_t)d_model},
         {&m->q, (size_t)qd + 2 * (size_t)kd}, {&m->att, (size_t)qd}, {&m->gate, (size_t)ffn}, {&m->up, (size_t)ffn},
         {&m->h, (size_t)ffn}, {&m->part, (size_t)heads * m->chunks_max * (head_dim + 2)}, {&m->logits, (size_t)vocab}};
-    bool ok = m->w != nullptr;
+    bool ok = m->w != nullptr && m->moe != nullptr;
     for (auto &b : bufs) {
         if (!ok) break;
         ok = hipMalloc(b.p, b.n * sizeof(float)) == hipSuccess;
@@ -3275,6 +3313,8 @@ int jitnn_hip_llama_free(jitnn_hip_llama *m) {
         if (b) (void)hipFree(b);
     if (m->packed) (void)hipFree(m->packed);
     if (m->paged_ws) (void)hipFree(m->paged_ws);
+    for (void *b : m->moe_ws)
+        if (b) (void)hipFree(b);
     while (m->kept) {
         jitnn_hip_llama::Kept *k = m->kept;
         m->kept = k->next;
@@ -3286,6 +3326,7 @@ int jitnn_hip_llama_free(jitnn_hip_llama *m) {
     if (m->tok_dev) (void)hipFree(m->tok_dev);
     if (m->tok_pin) (void)hipHostFree(m->tok_pin);
     delete[] m->w;
+    delete[] m->moe;
     delete m;
     return JITNN_HIP_OK;
 }
@@ -3304,6 +3345,21 @@ int jitnn_hip_llama_set_weight(jitnn_hip_llama *m, int layer, int which, const j
     }
     if (layer < 0 || layer >= m->layers) return fail(JITNN_HIP_EINVAL, "layer %d of %d", layer, m->layers);
     m->w[layer * 7 + which] = w;
+    return JITNN_HIP_OK;
+}
+
+int jitnn_hip_llama_set_moe(jitnn_hip_llama *m, int layer, const jitnn_hip_moe *e) {
+    if (!m) return fail(JITNN_HIP_EINVAL, "model is NULL");
+    if (layer < 0 || layer >= m->layers) return fail(JITNN_HIP_EINVAL, "layer %d of %d", layer, m->layers);
+    if (e && e->router->d != m->d) return fail(JITNN_HIP_EINVAL, "experts on %d values for a model of %d", e->router->d, m->d);
+    const jitnn_hip_moe *was = m->moe[layer];
+    m->moe[layer] = e;
+    m->moe_cap = 0;  // (the next pass of many tokens looks whether its workspace does)
+    if (!e) return JITNN_HIP_OK;
+    if (int rc = moe_reserve(m, 0, 1)) {
+        m->moe[layer] = was;
+        return rc;
+    }
     return JITNN_HIP_OK;
 }
 
@@ -3348,7 +3404,7 @@ int jitnn_hip_llama_decode_dev(jitnn_hip_llama *m, const float *x_dev, int pos, 
     if (pos < 0 || pos >= m->max_ctx) return fail(JITNN_HIP_EINVAL, "position %d of a cache of %d", pos, m->max_ctx);
     hipStream_t st = (hipStream_t)stream;
     const int d = m->d;
-    count_op(ST_DECODE, model_weight_bytes(m) + 4ll * m->layers * 2 * (pos + 1) * m->kv * m->hd + 4ll * (d + m->vocab));
+    count_op(ST_DECODE, model_weight_bytes(m, 1) + 4ll * m->layers * 2 * (pos + 1) * m->kv * m->hd + 4ll * (d + m->vocab));
     StatNest nest;
     // residual stream: layer input x (the caller's buffer for layer 0, xb afterwards) -> xa after attention -> xb after the FFN
     const float *x = x_dev;
@@ -3369,6 +3425,12 @@ int jitnn_hip_llama_decode_dev(jitnn_hip_llama *m, const float *x_dev, int pos, 
         }
         // xa = x + Wo att, xb = xa + W2 h: the residual rides in the linear's bias slot
         if (int rc = launch_gemv(w[JITNN_HIP_W_ATTN_O], m->att, 1, x, m->xa, st)) return rc;
+        if (m->moe[l]) {
+            norm_rows(m, m->xa, 1, nw + d, m->xn, st, nullptr);
+            if (int rc = jitnn_hip_moe_dev(m->moe[l], m->xn, 1, m->xa, m->xb, m->moe_ws[0], (long long)m->moe_ws_bytes[0], st)) return rc;
+            x = m->xb;
+            continue;
+        }
         // h = silu(W1 n) * (W3 n), n = RMSNorm(xa): one launch when gate and up share a format
         const jitnn_hip_weight *wg = w[JITNN_HIP_W_FFN_GATE], *wu = w[JITNN_HIP_W_FFN_UP];
         if (xreg_ok(wg) && wg->fmt == wu->fmt) {
@@ -3406,7 +3468,7 @@ int jitnn_hip_llama_prefill_dev(jitnn_hip_llama *m, const float *x_dev, int pos0
     if (m->d % 4 != 0) return fail(JITNN_HIP_EUNSUPPORTED, "d_model %d is not a multiple of 4", m->d);
     if (int rc = ensure_prefill(m, tokens)) return rc;
     hipStream_t st = (hipStream_t)stream;
-    count_op(ST_PREFILL, model_weight_bytes(m) + 4ll * m->layers * 2 * (pos0 + tokens) * m->kv * m->hd + 4ll * ((long long)tokens * m->d + (logits_dev ? m->vocab : 0)));
+    count_op(ST_PREFILL, model_weight_bytes(m, tokens) + 4ll * m->layers * 2 * (pos0 + tokens) * m->kv * m->hd + 4ll * ((long long)tokens * m->d + (logits_dev ? m->vocab : 0)));
     StatNest nest;
     const int d = m->d, T = tokens;
     prefill_reserve(m, T, st);
@@ -3488,7 +3550,7 @@ int jitnn_hip_llama_step_dev(jitnn_hip_llama *m, const jitnn_hip_paged_cache *c,
     const int d = m->d, T = b->tokens;
     const long long need = jitnn_hip_paged_attention_workspace(c, b, m->heads);
     if (need < 0) return (int)need;
-    if ((T > m->pf_cap || (size_t)need > m->paged_ws_bytes) && stream_recording(st))
+    if ((T > m->pf_cap || T > m->moe_cap || (size_t)need > m->paged_ws_bytes) && stream_recording(st))
         return fail(JITNN_HIP_EINVAL, "a pass of %d tokens needs larger buffers than the model has, which a recording cannot allocate", T);
     if (stream_recording(st)) m->recorded = true;
     if (int rc = ensure_prefill(m, T)) return rc;
@@ -3504,7 +3566,7 @@ int jitnn_hip_llama_step_dev(jitnn_hip_llama *m, const jitnn_hip_paged_cache *c,
         }
         m->paged_ws_bytes = (size_t)need;
     }
-    count_op(ST_PREFILL, model_weight_bytes(m) + 4ll * ((long long)T * d + (long long)logit_count * m->vocab));
+    count_op(ST_PREFILL, model_weight_bytes(m, T) + 4ll * ((long long)T * d + (long long)logit_count * m->vocab));
     StatNest nest;
     prefill_reserve(m, T, st);
     const long long qd = (long long)m->heads * m->hd, kd = (long long)m->kv * m->hd;

@@ -50,6 +50,11 @@ class LlamaDecoder:
     def set_weight_handle(self, layer: int, which: int, handle) -> None:
         _lib.check(_lib.lib.jitnn_hip_llama_set_weight(self._h, layer, which, handle), "jitnn_hip_llama_set_weight")
 
+    def set_moe(self, layer: int, moe) -> None:
+        """A layer of experts (experts.Moe) in place of the layer's gate, up and down; None: those again."""
+        _lib.check(_lib.lib.jitnn_hip_llama_set_moe(self._h, layer, None if moe is None else moe.handle), "jitnn_hip_llama_set_moe")
+        self._keep.append(moe)
+
     def set_norm(self, layer: int, which: int, w) -> None:
         a = np.ascontiguousarray(w, dtype=np.float32)
         if a.size != self.cfg["d_model"]:

@@ -9,7 +9,7 @@ tokenizer is built from the file's metadata (tokenizer.py).
         result = llm.generate(GenerationRequest("Once upon a time", 200, temperature=0.8, top_p=0.95, seed=1, stop=["\n\n"]))
 
 Llama-style architectures only (RMSNorm, rotary embedding, grouped-query attention, SwiGLU: general.architecture "llama",
-and the same tensor layout under other names where the metadata says so); anything else raises.
+and the same tensor layout under other names where the metadata says so), with a SwiGLU or a mixture of experts in each layer; anything else raises.
 """
 from __future__ import annotations
 
@@ -20,6 +20,7 @@ import warnings
 import numpy as np
 
 from . import _lib
+from .experts import Moe, Router
 from .gguf_file import GgufFile
 from .llama import LlamaDecoder, W_OUTPUT
 from .serving import Rope, SharedPrompt
@@ -27,6 +28,7 @@ from .tokenizer import StreamDecoder, Tokenizer
 
 # GGUF tensor names of a Llama-style layer in the order of the decoder's weight slots
 LAYER_TENSORS = ["attn_q", "attn_k", "attn_v", "attn_output", "ffn_gate", "ffn_up", "ffn_down"]
+ATTENTION_TENSORS = LAYER_TENSORS[:4]
 INTERLEAVED_ROPE_ARCHS = {"llama", "mistral", "granite"}  # llama.cpp's "NORM" rotary embedding: q and k stored permuted for pairs (2i, 2i + 1)
 
 _TOKEN_CB = C.CFUNCTYPE(None, C.c_int, C.c_void_p)
@@ -184,12 +186,13 @@ class Llm:
             d = f.integer(f"{arch}.embedding_length")
             heads = f.integer(f"{arch}.attention.head_count")
             kv = f.integer(f"{arch}.attention.head_count_kv", heads)
-            ffn = f.integer(f"{arch}.feed_forward_length")
+            ffn = f.integer(f"{arch}.feed_forward_length", f.integer(f"{arch}.expert_feed_forward_length", 0)) or f.integer(f"{arch}.expert_feed_forward_length")
             hd = f.integer(f"{arch}.attention.key_length", d // heads)
             eps = f.float_value(f"{arch}.attention.layer_norm_rms_epsilon", 1e-5)
             theta = f.float_value(f"{arch}.rope.freq_base", 10000.0)
             ctx_file = f.integer(f"{arch}.context_length", 2048)
-            for name in ("token_embd.weight", "output_norm.weight", "blk.0.attn_q.weight", "blk.0.ffn_gate.weight"):
+            experts = f.integer(f"{arch}.expert_count", 0)
+            for name in ("token_embd.weight", "output_norm.weight", "blk.0.attn_q.weight") + (() if experts else ("blk.0.ffn_gate.weight",)):
                 if not f.has_tensor(name):
                     raise ValueError(f"{path}: architecture {arch} does not generate text here (no tensor {name}; Llama-style layers are built)")
             emb = f.info("token_embd.weight")
@@ -198,10 +201,15 @@ class Llm:
             dec = LlamaDecoder(layers, d, heads, kv, hd, ffn, vocab, ctx, eps, theta)
             fmts = set()
             for l in range(layers):
-                for slot, tn in enumerate(LAYER_TENSORS):
+                routed = experts > 0 and f.has_tensor(f"blk.{l}.ffn_gate_inp.weight")
+                for slot, tn in enumerate(ATTENTION_TENSORS if routed else LAYER_TENSORS):
                     w = f.tensor(f"blk.{l}.{tn}.weight")
                     fmts.add(w.dtype().name)
                     dec.set_weight(l, slot, w)
+                if routed:
+                    moe, names = Llm._experts(f, arch, l, experts)
+                    dec.set_moe(l, moe)
+                    fmts |= names
                 dec.set_norm(l, 0, f.raw(f"blk.{l}.attn_norm.weight").view(np.float32))
                 dec.set_norm(l, 1, f.raw(f"blk.{l}.ffn_norm.weight").view(np.float32))
             dec.set_norm(0, 2, f.raw("output_norm.weight").view(np.float32))
@@ -221,6 +229,35 @@ class Llm:
         except Exception:
             f.close()
             raise
+
+    @staticmethod
+    def _experts(f: GgufFile, arch: str, l: int, experts: int):
+        """The experts of a layer and their formats: the router's weights (ffn_gate_inp), the experts' own (ffn_gate_exps, ffn_up_exps, ffn_down_exps), a bias of the choice
+        (exp_probs_b).  Weights of the chosen are normalised unless the file says otherwise (expert_weights_norm), times expert_weights_scale; gating by softmax or, expert_gating_func
+        2, sigmoid.  What else a layer may have beside them - experts for every token, groups of experts - is not built and raises."""
+        def plain(name):
+            t = f.info(name)
+            if t.type not in ("F32", "F16"):
+                raise ValueError(f"{f.path()}: {name} is {t.type} (F32 and F16 are built)")
+            return f.raw(name).view(np.float32 if t.type == "F32" else np.float16).reshape(t.shape).astype(np.float32)
+
+        for extra in ("ffn_gate_shexp", "ffn_up_shexp", "ffn_gate_inp_shexp"):
+            if f.has_tensor(f"blk.{l}.{extra}.weight"):
+                raise ValueError(f"{f.path()}: layer {l} has experts for every token ({extra}), which are not built")
+        gating = f.integer(f"{arch}.expert_gating_func", 1)
+        if gating not in (1, 2):
+            raise ValueError(f"{f.path()}: expert gating function {gating} is not built")
+        if f.integer(f"{arch}.expert_group_count", 1) > 1:
+            raise ValueError(f"{f.path()}: experts in groups are not built")
+        bias = next((plain(n) for n in (f"blk.{l}.exp_probs_b.bias", f"blk.{l}.exp_probs_b") if f.has_tensor(n)), None)
+        normalise = f.bool(f"{arch}.expert_weights_norm") if f.has(f"{arch}.expert_weights_norm") else True
+        weights = plain(f"blk.{l}.ffn_gate_inp.weight")
+        if len(weights) != experts:
+            raise ValueError(f"{f.path()}: a router of {len(weights)} experts in layer {l} of a model of {experts}")
+        router = Router(weights, f.integer(f"{arch}.expert_used_count"), "softmax" if gating == 1 else "sigmoid", normalise,
+                        f.float_value(f"{arch}.expert_weights_scale", 1.0) or 1.0, bias)
+        parts = [f.tensor(f"blk.{l}.{n}.weight") for n in ("ffn_gate_exps", "ffn_up_exps", "ffn_down_exps")]
+        return Moe(router, *parts), {p.dtype().name for p in parts}
 
     @staticmethod
     def _rope(f: GgufFile, arch: str, head_dim: int, theta: float):
