@@ -7,6 +7,8 @@
 // the operands cross from L2 to LDS once for the eight of them, while every weight byte is read by one wave only, decoded once and kept in registers for all
 // the groups.  Nothing is added up across waves or workgroups, and a row's result does not depend on the rows beside it.
 #pragma once
+#include <utility>
+
 #include "act.h"
 #include "common.h"
 #include "experts.h"
@@ -16,21 +18,31 @@ namespace jitnn {
 
 constexpr int ER_OP_CHUNKS = 72;                      // 16-byte pieces of a row's operands of one column: [8 blocks and the sums][hi, lo][lane group]
 constexpr int ER_OP_BYTES = ER_OP_CHUNKS * 16;
-constexpr int ER_GROUP_CHUNKS = 9 * 64;               // pieces of the operands of a group of eight rows
 
-// A workgroup's shape: its waves, the groups of eight rows whose operands are in LDS at a time, and how many such sets a chunk has at most.
+// A workgroup's shape: its waves, the groups of eight rows whose operands are in LDS at a time, how many such sets a chunk has at most, and waves per SIMD that the registers
+// are to leave room for.
 template <int WAVES, int GS, int SETS, int PER_SIMD>
 struct RowsShape {
     static constexpr int waves = WAVES, threads = 64 * WAVES, gs = GS, sets = SETS, groups = GS * SETS, per_simd = PER_SIMD;
+    static constexpr int set_rows = 8 * GS, all_rows = 8 * groups, set_chunks = GS * 9 * 64;  // (set_chunks: pieces of a set's operands)
 };
-// Tiles of 16 weight rows that a wave holds: two share the operands that cross LDS, one of Q6_K, which has sixteen operands a tile where the others have eight.
+// Tiles of 16 weight rows that a wave holds: two share the operands that cross LDS; one of Q6_K, which has sixteen operands a tile where the others have eight, and where 128
+// registers have to do.
 template <int FMT, class S>
-__host__ __device__ constexpr int er_tiles() { return RTile<FMT>::NOPS > 8 ? 1 : 2; }
+__host__ __device__ constexpr int er_tiles() { return RTile<FMT>::NOPS > 8 || S::per_simd > 2 ? 1 : 2; }
 template <int FMT, class S>
 __host__ __device__ constexpr size_t experts_rows_lds() {
-    constexpr size_t ops = (size_t)2 * S::gs * (ER_GROUP_CHUNKS * 16 + 8 * sizeof(float)), gated = er_tiles<FMT, S>() == 1 ? (size_t)S::waves / 2 * S::groups * 64 * sizeof(float2) : 0;
-    return (ops > gated ? ops : gated) + (size_t)S::groups * 8 * 2 * sizeof(int) + (size_t)S::waves * er_tiles<FMT, S>() * RTile<FMT>::STAGE_BYTES;
+    constexpr size_t ops = (size_t)2 * (S::set_chunks * 16 + S::set_rows * sizeof(float)), gated = er_tiles<FMT, S>() == 1 ? (size_t)S::waves / 2 * S::groups * 64 * sizeof(float2) : 0;
+    return (ops > gated ? ops : gated) + (size_t)S::all_rows * 2 * sizeof(int) + (size_t)S::waves * er_tiles<FMT, S>() * RTile<FMT>::STAGE_BYTES;
 }
+
+__device__ __forceinline__ f32x4 mfma(const f16x8 &x, const f16x8 &w, const f32x4 &c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(x, w, c, 0, 0, 0); }
+// Sum v of a lane's two: the hi and lo parts' side by side
+__device__ __forceinline__ float joined(const f32x4 &c, int v) { return c[2 * v] + c[2 * v + 1]; }
+template <class F, int... I>
+__device__ __forceinline__ void each_of(std::integer_sequence<int, I...>, F &&f) { (f(std::integral_constant<int, I>{}), ...); }
+template <int N, class F>
+__device__ __forceinline__ void each(F &&f) { each_of(std::make_integer_sequence<int, N>{}, f); }
 
 // Column c of eight rows, as rows_prepare_column, in pieces of a row: operand s (block s of the column; 8: the sums), part and lane group kq at
 // 16-byte piece 8 s + 4 part + kq.  v: the lane's quads (zeros behind the row's last value).
@@ -122,20 +134,22 @@ __device__ __forceinline__ void load_last_column(typename R::Raw &r, const typen
     if constexpr (R::REST > 0) r.c[R::FULL] = ld128_until(q + p.rest, end);
 }
 
-// grid: a.nblocks x a.splits x (at least as many as there are chunks); experts_rows_lds() of dynamic LDS, chunks of at most 8 S::groups rows.
+// grid: a.nblocks x a.splits x (at least as many as there are chunks); experts_rows_lds() of dynamic LDS, chunks of at most S::all_rows rows.
 // DUAL: y = act(gate x) * (up x), a wave having a tile of each, or the one or the other, waves 2 i and 2 i + 1 the same rows of the two.  Otherwise a split takes its share
 // of the columns and has a y of its own.
 template <int FMT, class S, bool DUAL>
 __global__ void __launch_bounds__(S::threads, S::per_simd) experts_rows_kernel(const ExpertRowsArgs a) {
     typedef RTile<FMT> R;
-    constexpr int NOPS = R::NOPS, T = er_tiles<FMT, S>(), NI = S::gs * ER_GROUP_CHUNKS / S::threads + 1;
+    constexpr int NOPS = R::NOPS, T = er_tiles<FMT, S>(), NI = S::set_chunks / S::threads + 1, V = 2;  // (V: sums that a lane has of a tile and a group)
+    constexpr int CHAINS = R::BLOCK_SCALES ? 1 : NOPS / 8;  // sums of a tile and a group that products add to: two in turn where there are as many operands
+    constexpr int AHEAD = S::sets > 1 ? 4 : 8;  // operands that come out of LDS ahead of their products (one set: a group's all at once)
     constexpr bool PARTIAL = R::BLOCK_SCALES;  // (only 32-value blocks have rows that are no whole columns)
     extern __shared__ __attribute__((aligned(16))) uint8_t er_smem[];
     uint8_t *stage = er_smem;                                                                    // per wave: T tiles' bytes of a column
-    uint32_t *const where = reinterpret_cast<uint32_t *>(er_smem + (size_t)S::waves * T * R::STAGE_BYTES);  // [groups * 8] a row's operands, in columns from the first one's
-    int *const slots = reinterpret_cast<int *>(where + S::groups * 8);                           // [groups * 8]
-    u32x4 *const ops = reinterpret_cast<u32x4 *>(slots + S::groups * 8);                         // [2][gs][9][64]
-    float *const invs = reinterpret_cast<float *>(ops + (size_t)2 * S::gs * ER_GROUP_CHUNKS);    // [2][gs * 8]
+    uint32_t *const where = reinterpret_cast<uint32_t *>(er_smem + (size_t)S::waves * T * R::STAGE_BYTES);  // [all_rows] a row's operands, in bytes from the first one's
+    int *const slots = reinterpret_cast<int *>(where + S::all_rows);                             // [all_rows]
+    u32x4 *const ops = reinterpret_cast<u32x4 *>(slots + S::all_rows);                           // [2][gs][9][64]
+    float *const invs = reinterpret_cast<float *>(ops + (size_t)2 * S::set_chunks);              // [2][set_rows]
     const int tid = threadIdx.x, lane = tid & 63, kq = lane >> 4, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     stage += (size_t)wave * T * R::STAGE_BYTES;
     const int per_chunk = a.nblocks * a.splits, u = (int)blockIdx.x / per_chunk, of_chunk = (int)blockIdx.x - u * per_chunk, split = of_chunk / a.nblocks,
@@ -145,8 +159,8 @@ __global__ void __launch_bounds__(S::threads, S::per_simd) experts_rows_kernel(c
     const int ncol = (a.k + 255) >> 8, groups = (ch.z + 7) >> 3, sets = (groups + S::gs - 1) / S::gs;
     const int c0 = (int)((long long)ncol * split / a.splits), c1 = (int)((long long)ncol * (split + 1) / a.splits);
 
-    const int slot = a.list[ch.y + min(min(tid, S::groups * 8 - 1), ch.z - 1)];  // (a place without a row takes the last one again: computed, not stored)
-    static_assert(S::groups * 8 <= S::threads, "a thread for each row");
+    const int slot = a.list[ch.y + min(min(tid, S::all_rows - 1), ch.z - 1)];  // (a place without a row takes the last one again: computed, not stored)
+    static_assert(S::all_rows <= S::threads, "a thread for each row");
     // the weights on their way: the first column of this wave's tiles
     const size_t rowbytes = (size_t)(a.k / block_values(FMT)) * block_bytes(FMT);
     const uint8_t *const w0 = a.w + (size_t)ch.x * a.expert_bytes, *const w1 = DUAL ? a.w2 + (size_t)ch.x * a.expert_bytes : w0;
@@ -169,52 +183,56 @@ __global__ void __launch_bounds__(S::threads, S::per_simd) experts_rows_kernel(c
         for (int t = 0; t < T; ++t) R::load(raw[t], ptr[t], c);
     };
     fetch(c0);
-    if (tid < S::groups * 8) {
+    if (tid < S::all_rows) {
         slots[tid] = slot;
-        where[tid] = (uint32_t)(slot / a.per_row) * (uint32_t)ncol;
+        where[tid] = (uint32_t)(slot / a.per_row) * (uint32_t)ncol * (uint32_t)ER_OP_BYTES;
     }
     __syncthreads();
     // Piece i of this thread: lane l of operand s of group g of a set, whose row is that of l's place.  What the whole rounds leave is shared out over the waves, a few
     // lanes each, the others doing what the last of those does; and a group that the chunk has not is the last row's again: no load stands behind a condition,
     // for at the end of one the compiler waits for what was asked for before it.
-    constexpr int ROUNDS = NI - 1, SHARE = (S::gs * ER_GROUP_CHUNKS - ROUNDS * S::threads) / S::waves;
-    static_assert(SHARE >= 1 && SHARE <= 64 && SHARE * S::waves == S::gs * ER_GROUP_CHUNKS - ROUNDS * S::threads, "whole lanes");
+    constexpr int ROUNDS = NI - 1, SHARE = (S::set_chunks - ROUNDS * S::threads) / S::waves;
+    static_assert(SHARE >= 1 && SHARE <= 64 && SHARE * S::waves == S::set_chunks - ROUNDS * S::threads, "whole lanes");
     uint32_t from[NI];   // one set: where it stands in column 0; several: of the row in its set | where in the row's operands << 16
     int to[NI];
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
         const int idx = i < ROUNDS ? tid + i * S::threads : ROUNDS * S::threads + wave * SHARE + min(lane, SHARE - 1);
-        const int g = idx / ER_GROUP_CHUNKS, rest = idx - g * ER_GROUP_CHUNKS, s = rest >> 6, l = rest & 63;
+        const int g = idx / (9 * 64), rest = idx - g * (9 * 64), s = rest >> 6, l = rest & 63;
         const uint32_t row = (uint32_t)(g * 8 + ((l & 15) >> 1)), piece = (uint32_t)(s * 128 + (l & 1) * 64 + (l >> 4) * 16);
-        from[i] = S::sets == 1 ? where[row] * (uint32_t)ER_OP_BYTES + piece : row | piece << 16;
+        from[i] = S::sets == 1 ? where[row] + piece : row | piece << 16;
         to[i] = idx;
     }
-    const int inv_row = min(tid, S::gs * 8 - 1);
-    const uint32_t inv_from = where[inv_row];
+    const int inv_row = min(tid, S::set_rows - 1);
+    const uint32_t inv_from = where[inv_row] / (uint32_t)(ER_OP_BYTES / 4);
     u32x4 next[NI];
     float next_inv;
     auto ask = [&](int c, int set) {
+        const uint32_t column = (uint32_t)c * ER_OP_BYTES;
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
-            if constexpr (S::sets == 1) next[i] = *reinterpret_cast<const u32x4 *>(a.ops + (size_t)c * ER_OP_BYTES + from[i]);
-            else next[i] = *reinterpret_cast<const u32x4 *>(a.ops + (size_t)(where[set * S::gs * 8 + (from[i] & 0xffffu)] + (uint32_t)c) * ER_OP_BYTES + (from[i] >> 16));
+            const uint32_t at = S::sets == 1 ? from[i] : where[set * S::set_rows + (from[i] & 0xffffu)] + (from[i] >> 16);
+            next[i] = *reinterpret_cast<const u32x4 *>(a.ops + (at + column));
         }
-        next_inv = a.inv[(S::sets == 1 ? inv_from : where[set * S::gs * 8 + inv_row]) + (uint32_t)c];
+        const uint32_t at = S::sets == 1 ? inv_from : where[set * S::set_rows + inv_row] / (uint32_t)(ER_OP_BYTES / 4);
+        next_inv = *reinterpret_cast<const float *>(reinterpret_cast<const uint8_t *>(a.inv) + (at + 4u * (uint32_t)c));
     };
     ask(c0, 0);
 
-    float2 acc[T][S::groups];
+    float acc[T][S::groups][V];
 #pragma unroll
     for (int t = 0; t < T; ++t)
 #pragma unroll
-        for (int g = 0; g < S::groups; ++g) acc[t][g] = make_float2(0.f, 0.f);
+        for (int g = 0; g < S::groups; ++g)
+#pragma unroll
+            for (int v = 0; v < V; ++v) acc[t][g][v] = 0.f;
     int buffer = 0;
     // A set's operands into the buffer that nobody reads any more: every wave has passed the barrier of the set before, behind its products of the one before that.
     auto put = [&]() {
-        u32x4 *const op = ops + (size_t)buffer * S::gs * ER_GROUP_CHUNKS;
+        u32x4 *const op = ops + (size_t)buffer * S::set_chunks;
 #pragma unroll
         for (int i = 0; i < NI; ++i) op[to[i]] = next[i];
-        if (tid < S::gs * 8) invs[buffer * S::gs * 8 + tid] = next_inv;
+        if (tid < S::set_rows) invs[buffer * S::set_rows + tid] = next_inv;
         buffer ^= 1;
     };
     for (int c = c0; c < c1; ++c) {
@@ -247,67 +265,91 @@ __global__ void __launch_bounds__(S::threads, S::per_simd) experts_rows_kernel(c
         };
 #pragma unroll
         for (int t = 0; t < T; ++t) decode(t);
-#pragma unroll
-        for (int set = 0; set < S::sets; ++set) {
-            if (set < sets) {
+        // (sets and groups by their number at compile time: sums that a loop indexes are kept in memory)
+        each<S::sets>([&](auto set_) {
+            constexpr int set = decltype(set_)::value;
+            if (set >= sets) return;
             if (set > 0) put();
-            const u32x4 *const op = ops + (size_t)(buffer ^ 1) * S::gs * ER_GROUP_CHUNKS;
-            const float *const iv = invs + (buffer ^ 1) * S::gs * 8;
+            const u32x4 *const op = ops + (size_t)(buffer ^ 1) * S::set_chunks;
+            const float *const iv = invs + (buffer ^ 1) * S::set_rows;
             const bool more = set + 1 < sets;
             ask(more ? c : min(c + 1, c1 - 1), more ? set + 1 : 0);  // (behind the last one: that one again)
             __syncthreads();
+            constexpr int N = S::gs * 9;
+            f16x8 A[AHEAD + 1];
 #pragma unroll
-            for (int gi = 0; gi < S::gs; ++gi) {
-                const int g = set * S::gs + gi;
-                if (g < groups) {
-                f16x8 A[9];
-#pragma unroll
-                for (int s = 0; s < 9; ++s) A[s] = __builtin_bit_cast(f16x8, op[(gi * 9 + s) * 64 + lane]);
-                const float2 w = *reinterpret_cast<const float2 *>(iv + gi * 8 + 2 * kq);
+            for (int i = 0; i < AHEAD && S::sets > 1; ++i) A[i] = __builtin_bit_cast(f16x8, op[i * 64 + lane]);
+            each<S::gs>([&](auto gi_) {
+                constexpr int gi = decltype(gi_)::value, g = set * S::gs + gi;
+                if (g >= groups) return;
+                const float2 w2 = *reinterpret_cast<const float2 *>(iv + gi * 8 + 2 * kq);
+                const float w[V] = {w2.x, w2.y};
+                f32x4 cs[T][CHAINS], cm[T];
+                float u[T][V];
 #pragma unroll
                 for (int t = 0; t < T; ++t) {
-                    float u0, u1;
-                    if constexpr (R::BLOCK_SCALES) {
-                        u0 = u1 = 0.f;
 #pragma unroll
-                        for (int s = 0; s < 8; ++s) {
-                            const f32x4 cs = mfma16(A[s], B[t][s]);
-                            u0 = __builtin_fmaf(dblk[t][s], cs[0] + cs[1], u0);
-                            u1 = __builtin_fmaf(dblk[t][s], cs[2] + cs[3], u1);
-                        }
-                        if constexpr (R::MINS) {
-                            const f32x4 cm = mfma16(A[8], Bm[t]);
-                            u0 = __builtin_fmaf(64.f, cm[0] + cm[1], u0);
-                            u1 = __builtin_fmaf(64.f, cm[2] + cm[3], u1);
-                        }
-                    } else {
-                        f32x4 cs = {0.f, 0.f, 0.f, 0.f};
+                    for (int i = 0; i < CHAINS; ++i) cs[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                        for (int s = 0; s < NOPS; ++s) cs = __builtin_amdgcn_mfma_f32_16x16x32_f16(A[R::aidx(s)], B[t][s], cs, 0, 0, 0);
-                        const f32x4 cm = mfma16(A[8], Bm[t]);
-                        const float s0 = cs[0] + cs[1], s1 = cs[2] + cs[3], m0 = cm[0] + cm[1], m1 = cm[2] + cm[3];
-                        u0 = __builtin_fmaf(d[t], s0, -dmin64[t] * m0);
-                        u1 = __builtin_fmaf(d[t], s1, -dmin64[t] * m1);
+                    for (int v = 0; v < V; ++v) u[t][v] = 0.f;
+                }
+                if constexpr (S::sets == 1) {
+#pragma unroll
+                    for (int s = 0; s < 9; ++s) A[s] = __builtin_bit_cast(f16x8, op[(gi * 9 + s) * 64 + lane]);
+                }
+                each<9>([&](auto s_) {
+                    constexpr int s = decltype(s_)::value, at = gi * 9 + s;
+                    if constexpr (S::sets > 1 && at + AHEAD < N) A[(at + AHEAD) % (AHEAD + 1)] = __builtin_bit_cast(f16x8, op[(at + AHEAD) * 64 + lane]);
+                    const f16x8 x = A[S::sets > 1 ? at % (AHEAD + 1) : s];
+#pragma unroll
+                    for (int t = 0; t < T; ++t) {
+                        if constexpr (s == 8) {
+                            if constexpr (R::MINS || !R::BLOCK_SCALES) cm[t] = mfma16(x, Bm[t]);
+                        } else if constexpr (R::BLOCK_SCALES) {
+                            const f32x4 block = mfma16(x, B[t][s]);
+#pragma unroll
+                            for (int v = 0; v < V; ++v) u[t][v] = __builtin_fmaf(dblk[t][s], joined(block, v), u[t][v]);
+                        } else {
+                            each<NOPS / 8>([&](auto q) {
+                                constexpr int i = decltype(q)::value, w = s * (NOPS / 8) + i;
+                                static_assert(R::aidx(w) == s, "the weights' operands of one of the activations'");
+                                cs[t][i] = mfma(x, B[t][w], cs[t][i]);
+                            });
+                        }
                     }
-                    acc[t][g].x = __builtin_fmaf(w.x, u0, acc[t][g].x);
-                    acc[t][g].y = __builtin_fmaf(w.y, u1, acc[t][g].y);
+                    if constexpr (S::sets > 1) __builtin_amdgcn_sched_barrier(0);
+                });
+#pragma unroll
+                for (int t = 0; t < T; ++t) {
+#pragma unroll
+                    for (int v = 0; v < V; ++v) {
+                        if constexpr (R::BLOCK_SCALES) {
+                            if constexpr (R::MINS) u[t][v] = __builtin_fmaf(64.f, joined(cm[t], v), u[t][v]);
+                        } else {
+                            const f32x4 all = CHAINS > 1 ? cs[t][0] + cs[t][CHAINS - 1] : cs[t][0];
+                            u[t][v] = __builtin_fmaf(d[t], joined(all, v), -dmin64[t] * joined(cm[t], v));
+                        }
+                        acc[t][g][v] = __builtin_fmaf(w[v], u[t][v], acc[t][g][v]);
+                    }
                 }
                 // (the operands and products of one group at a time: of more than one there are no registers)
 #pragma unroll
-                for (int t = 0; t < T; ++t) asm volatile("" : "+v"(acc[t][g].x), "+v"(acc[t][g].y));
+                for (int t = 0; t < T; ++t)
+#pragma unroll
+                    for (int v = 0; v < V; ++v) asm volatile("" : "+v"(acc[t][g][v]));
                 __builtin_amdgcn_sched_barrier(0);
-                }
-            }
-            }
-        }
+            });
+        });
     }
     float *const y0 = a.y + (DUAL ? 0 : (size_t)split * a.split_floats);
-    float2 *const other = reinterpret_cast<float2 *>(ops) + (size_t)(wave >> 1) * S::groups * 64 + lane;
+    float *const other = reinterpret_cast<float *>(ops) + ((size_t)(wave >> 1) * S::groups * 64 + lane) * V;
     if constexpr (DUAL && T == 1) {
         __syncthreads();
         if (second) {
 #pragma unroll
-            for (int g = 0; g < S::groups; ++g) other[g * 64] = acc[0][g];
+            for (int g = 0; g < S::groups; ++g)
+#pragma unroll
+                for (int v = 0; v < V; ++v) other[g * 64 * V + v] = acc[0][g][v];
         }
         __syncthreads();
         if (second) return;
@@ -315,25 +357,31 @@ __global__ void __launch_bounds__(S::threads, S::per_simd) experts_rows_kernel(c
 #pragma unroll
     for (int g = 0; g < S::groups; ++g) {
         if (g >= groups) continue;
-        const float2 up = DUAL ? (T == 1 ? other[g * 64] : acc[T - 1][g]) : acc[T - 1][g];
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            const int b = g * 8 + 2 * kq + r;
+        for (int v = 0; v < V; ++v) {
+            const int b = g * 8 + V * kq + v;
             if (b >= ch.z) continue;
             float *const y = y0 + (size_t)slots[b] * a.n + (lane & 15);
-            const float v0 = r ? acc[0][g].y : acc[0][g].x, v1 = r ? up.y : up.x;
+            const float v0 = acc[0][g][v], v1 = DUAL && T == 1 ? other[g * 64 * V + v] : acc[T - 1][g][v];
             if (tile < ntiles) y[tile * 16] = DUAL ? activate(a.act, v0) * v1 : v0;
             if (!DUAL && T == 2 && tile + 1 < ntiles) y[tile * 16 + 16] = v1;
         }
     }
 }
 
-// The shapes, by the groups of a chunk: one or two, whose operands LDS holds whole; many, in sets of four.  (32 tokens of which each meets eight of 128 experts, gate and up of
-// 2048 x 768 / down: workgroups of eight waves 64 us in Q4_K and 62 in Q6_K, of four waves 82 and 62; five tokens, six of 64 experts of 2048 x 1408 in Q8_0 82 and 34 against 64 and 32, where
-// eight waves leave a second round nearly empty)
+// The shapes, by the groups of a chunk.
+// One: 32 tokens of which each meets eight of 128 experts, gate and up of 2048 x 768 / down: workgroups of eight waves 64 us in Q4_K and 62 in Q6_K, of four 82 and 62; formats of
+// 32-value blocks, whose scales take registers, the other way round (five tokens, six of 64 experts of 2048 x 1408 in Q8_0 82 and 34 against 64 and 32).
+// Two: with a tile a wave 128 registers do, and a CU has sixteen waves (24 tokens, two of eight experts of 4096 x 14336 in Q5_K 317 -> 266 us); where they do not - Q6_K, 32-value
+// blocks but Q4_0 -, four waves of two tiles (of one of Q6_K) (24 tokens, two of eight of 4096 x 4096: Q8_0 140 us against 152 and 145 of eight waves, Q4_1 84 / 106 / 90, Q6_K
+// 141 / 212 / 148, Q4_0 114 / 107 / 121, Q5_K 98 / - / 101).
+// Three to eight: in sets of four, an eighth faster with the operands read ahead.  512 tokens, two of eight of 4096 x 14336 in Q4_K and Q6_K: 1457 us; groups of sixteen rows, hi
+// and lo parts as operands of their own, 1472; four waves and sets of two 1479; sixteen groups a chunk 2243 (registers); chunks by XCD 1745.  What bounds it there: without its
+// products it takes 1009 us - operands on their way 215, to LDS 70, decoding 125, weights 130 -, without all of those 956; the products alone would be 490.
 typedef RowsShape<8, 1, 1, 2> RowsShape1;
 typedef RowsShape<4, 1, 1, 2> RowsShape1Short;
-typedef RowsShape<8, 2, 1, 2> RowsShape2;
+typedef RowsShape<8, 2, 1, 4> RowsShape2;
+typedef RowsShape<4, 2, 1, 2> RowsShape2Short;
 typedef RowsShape<8, 4, 2, 2> RowsShape8;
 typedef RowsShape<8, 4, 3, 2> RowsShape12;
 
@@ -341,17 +389,20 @@ template <int FMT, class S>
 static RowsKernelRef experts_rows_shape(bool dual) {
     const RowsKernel fn = dual ? experts_rows_kernel<FMT, S, true> : experts_rows_kernel<FMT, S, false>;
     // (weight rows of a workgroup: its waves' tiles; of a pair of matrices half as many of each)
-    return {fn, experts_rows_lds<FMT, S>(), S::threads, S::waves * er_tiles<FMT, S>() / (dual ? 2 : 1), S::groups};
+    return {fn, experts_rows_lds<FMT, S>(), S::threads, S::waves * er_tiles<FMT, S>() / (dual ? 2 : 1), S::all_rows / 8};
 }
-// groups: of a chunk, at most 8, of K-quants 12
+// groups: of a chunk, at most 8
 template <int FMT>
 static RowsKernelRef experts_rows_pick(int groups, bool dual) {
     if (groups <= 1) {
         if constexpr (RTile<FMT>::BLOCK_SCALES) return experts_rows_shape<FMT, RowsShape1Short>(dual);
         else return experts_rows_shape<FMT, RowsShape1>(dual);
     }
-    if (groups <= 2) return experts_rows_shape<FMT, RowsShape2>(dual);
-    if constexpr (!RTile<FMT>::BLOCK_SCALES) {  // (sixteen groups' sums and 32-value blocks' scales do not fit the registers)
+    if (groups <= 2) {
+        if constexpr (FMT == F_Q6_K || (RTile<FMT>::BLOCK_SCALES && FMT != F_Q4_0)) return experts_rows_shape<FMT, RowsShape2Short>(dual);
+        else return experts_rows_shape<FMT, RowsShape2>(dual);
+    }
+    if constexpr (!RTile<FMT>::BLOCK_SCALES) {
         if (groups > 8) return experts_rows_shape<FMT, RowsShape12>(dual);
     }
     return experts_rows_shape<FMT, RowsShape8>(dual);
