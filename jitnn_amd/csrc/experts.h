@@ -23,6 +23,14 @@ struct ExpertLists {
     int chunk_rows = 8;
     static int chunks_most(int slots, int experts, int chunk_rows) { return (slots < experts ? slots : experts) + slots / chunk_rows; }
 };
+// Rows of activations to be prepared as operands (experts_rows.h): x [rows, k], k a multiple of 4, to the layouts that have a place.
+struct ExpertPrepare {
+    const float *x = nullptr;
+    int rows = 0, k = 0;
+    uint8_t *ops[3] = {};  // per layout (GR_LAYOUT_*): nullptr - not wanted
+    float *inv[3] = {};    // [rows, columns]
+    __host__ __device__ int units() const { return ops[0] || ops[1] || ops[2] ? (rows + 7) / 8 * ((k + 255) / 256) : 0; }  // of a wave's work
+};
 struct RouterArgs {
     const float *x, *w;  // [tokens, d], [experts, d]
     const float *bias;   // [experts] or nullptr: added for the choice, not for the weights
@@ -30,6 +38,7 @@ struct RouterArgs {
     int *ids;            // [tokens, used]
     float *weights;      // [tokens, used]
     ExpertLists lists;
+    ExpertPrepare prepare;  // beside the lists, in their launch
     int tokens, experts, d, used;
     bool sigmoid, normalise;
     float scale;
@@ -40,7 +49,7 @@ size_t router_logits_bytes(int tokens, int experts, int d, bool choice_follows);
 void router_logits_launch(RouterArgs &a, hipStream_t s);
 void router_launch(RouterArgs a, hipStream_t s);
 // the lists of choices that somebody else made; an id outside [0, experts) is on none
-void expert_lists_launch(const int *ids, int slots, int experts, const ExpertLists &lists, hipStream_t s);
+void expert_lists_launch(const int *ids, int slots, int experts, const ExpertLists &lists, const ExpertPrepare &prepare, hipStream_t s);
 
 struct ExpertWeights {
     int fmt, n, k;  // of one expert: [n, k]
@@ -66,8 +75,8 @@ struct RowsKernelRef {
     int threads, tiles, groups;  // tiles: of 16 weight rows (of each matrix of a pair) per workgroup; groups: of eight rows per chunk, at most
 };
 size_t experts_ops_bytes(size_t rows, int k);  // the operands of so many rows, and their scales behind them
-// x [rows, k] -> the layouts (GR_LAYOUT_*) that have a place
-void experts_prepare_launch(const float *x, int rows, int k, uint8_t *const *places, hipStream_t s);
+ExpertPrepare experts_prepare(const float *x, int rows, int k, uint8_t *const *places);  // places: per layout (GR_LAYOUT_*), nullptr - not wanted
+void experts_prepare_launch(const ExpertPrepare &p, hipStream_t s);
 // the kernel for chunks of so many groups of eight rows (or of the most it has, where they are more).  pair: y = act(w x) * (w2 x)
 RowsKernelRef experts_rows_kernel_ref(int fmt, int groups, bool pair);
 RowsKernelRef experts_rows_ref_k(int fmt, int groups, bool pair);    // experts_rows_k.hip: Q4_K, Q5_K
@@ -102,7 +111,7 @@ ExpertFewKernel experts_few_down_k(int fmt, bool aligned, int stretches, int wav
 ExpertFewKernel experts_few_down_q32(int fmt, int stretches, int waves);
 
 // ---- experts.hip
-// y [slots, n] = the product of each slot's expert with row slot / per_row of x, in FP32 on the dequantiser's values: any format
+// y [slots, n] = the product of each slot's expert with row slot / per_row of x, in FP32 on the dequantiser's values: Q5_0 and Q3_K blocks as a file has them
 void experts_value_launch(const ExpertWeights &w, int experts, const int *ids, int slots, int per_row, const float *x, float *y, hipStream_t s);
 // h [count] = act(g) * u (h may be g)
 void experts_gate_launch(int act, const float *g, const float *u, float *h, size_t count, int cus, hipStream_t s);

@@ -1,4 +1,4 @@
-// The experts' products for any block format, the gate and the weighted sum of a token's experts.
+// The experts' products for the formats that the matrix cores' kernels have no operands of, the gate, the weighted sum of a token's experts, and what launches those kernels.
 #include "experts.h"
 
 #include <algorithm>
@@ -38,18 +38,8 @@ static void value(const ExpertWeights &w, int experts, const int *ids, int slots
 }
 
 void experts_value_launch(const ExpertWeights &w, int experts, const int *ids, int slots, int per_row, const float *x, float *y, hipStream_t s) {
-    switch (w.fmt) {
-    case F_Q4_0: value<F_Q4_0>(w, experts, ids, slots, per_row, x, y, s); break;
-    case F_Q4_1: value<F_Q4_1>(w, experts, ids, slots, per_row, x, y, s); break;
-    case F_Q8_0: value<F_Q8_0>(w, experts, ids, slots, per_row, x, y, s); break;
-    case F_Q4_K: value<F_Q4_K>(w, experts, ids, slots, per_row, x, y, s); break;
-    case F_Q5_K: value<F_Q5_K>(w, experts, ids, slots, per_row, x, y, s); break;
-    case F_Q6_K: value<F_Q6_K>(w, experts, ids, slots, per_row, x, y, s); break;
-    case F_Q5_0: value<F_Q5_0>(w, experts, ids, slots, per_row, x, y, s); break;
-    case F_Q5_1: value<F_Q5_1>(w, experts, ids, slots, per_row, x, y, s); break;
-    case F_Q2_K: value<F_Q2_K>(w, experts, ids, slots, per_row, x, y, s); break;
-    case F_Q3_K: value<F_Q3_K>(w, experts, ids, slots, per_row, x, y, s); break;
-    }
+    if (w.fmt == F_Q5_0) value<F_Q5_0>(w, experts, ids, slots, per_row, x, y, s);
+    else value<F_Q3_K>(w, experts, ids, slots, per_row, x, y, s);
 }
 
 // ---- few tokens
@@ -96,16 +86,21 @@ size_t experts_ops_bytes(size_t rows, int k) {
     return columns * (ER_OP_BYTES + sizeof(float));
 }
 
-void experts_prepare_launch(const float *x, int rows, int k, uint8_t *const *places, hipStream_t s) {
-    const int ncol = (k + 255) / 256;
-    ExpertPrepareOut o{};
+ExpertPrepare experts_prepare(const float *x, int rows, int k, uint8_t *const *places) {
+    ExpertPrepare p;
+    p.x = x;
+    p.rows = rows;
+    p.k = k;
     for (int l = 0; l < GR_LAYOUTS; ++l) {
-        if (!places[l]) continue;
-        o.ops[l] = places[l];
-        o.inv[l] = reinterpret_cast<float *>(places[l] + (size_t)rows * ncol * ER_OP_BYTES);
+        p.ops[l] = places[l];
+        p.inv[l] = places[l] ? reinterpret_cast<float *>(places[l] + (size_t)rows * ((k + 255) / 256) * ER_OP_BYTES) : nullptr;
     }
-    hipLaunchKernelGGL(experts_prepare_kernel, dim3(ncol, (rows + 7) / 8), dim3(64), 0, s, x, rows, k, o);
+    return p;
 }
+
+__global__ void __launch_bounds__(64) experts_prepare_kernel(const ExpertPrepare p) { experts_prepare_unit(p, (int)blockIdx.x, threadIdx.x); }
+
+void experts_prepare_launch(const ExpertPrepare &p, hipStream_t s) { hipLaunchKernelGGL(experts_prepare_kernel, dim3(p.units()), dim3(64), 0, s, p); }
 
 RowsKernelRef experts_rows_kernel_ref(int fmt, int groups, bool pair) {
     return fmt == F_Q4_K || fmt == F_Q5_K ? experts_rows_ref_k(fmt, groups, pair) : fmt == F_Q6_K || fmt == F_Q2_K ? experts_rows_ref_k6(fmt, groups, pair)

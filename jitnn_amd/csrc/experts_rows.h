@@ -1,7 +1,7 @@
 // The experts' products of many (token, expert) pairs on the matrix cores, at FP32-grade accuracy: gemv_rows_kernel's operands and decoders (gemv_rows.h), for
 // rows that a list gathers.
 //
-// The operands of an activation row are prepared once, row by row (experts_prepare_kernel: FP16 hi and lo parts of the row scaled per 256 values, and the sums of
+// The operands of an activation row are prepared once, row by row (experts_prepare_unit: FP16 hi and lo parts of the row scaled per 256 values, and the sums of
 // its blocks), whoever it will meet: which eight rows stand in one matrix operand, the lists of the experts say when the operand is put together in LDS.
 // A workgroup takes one expert, up to eight times `groups` of its rows and 8 waves x T tiles of 16 weight rows; all its waves are at the same 256 values of K, so that
 // the operands cross from L2 to LDS once for the eight of them, while every weight byte is read by one wave only, decoded once and kept in registers for all
@@ -94,25 +94,21 @@ __device__ __forceinline__ void experts_prepare_column(const float4 (&v)[8], uin
     }
 }
 
-struct ExpertPrepareOut {
-    uint8_t *ops[3];  // per layout (GR_LAYOUT_*): nullptr - not wanted
-    float *inv[3];    // [rows, columns]
-};
-// One wave per (column, eight rows): x [rows, k], k a multiple of 4.  grid (ceil(k / 256), ceil(rows / 8))
-static __global__ void __launch_bounds__(64) experts_prepare_kernel(const float *__restrict__ x, int rows, int k, const ExpertPrepareOut o) {
-    const int lane = threadIdx.x, b = lane >> 3, part = lane & 7, c = (int)blockIdx.x, ncol = (k + 255) >> 8, row = (int)blockIdx.y * 8 + b;
-    const bool have = row < rows;
-    const float *xr = x + (size_t)(have ? row : 0) * k;
+// One wave's unit: a column of eight rows.
+__device__ __forceinline__ void experts_prepare_unit(const ExpertPrepare &p, int unit, int lane) {
+    const int b = lane >> 3, part = lane & 7, ncol = (p.k + 255) >> 8, octet = unit / ncol, c = unit - octet * ncol, row = octet * 8 + b;
+    const bool have = row < p.rows;
+    const float *xr = p.x + (size_t)(have ? row : 0) * p.k;
     float4 v[8];
 #pragma unroll
     for (int t = 0; t < 8; ++t) {
         const int at = c * 256 + 32 * t + 4 * part;
-        v[t] = at < k ? *reinterpret_cast<const float4 *>(xr + at) : make_float4(0.f, 0.f, 0.f, 0.f);
+        v[t] = at < p.k ? *reinterpret_cast<const float4 *>(xr + at) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
     const size_t at = (size_t)row * ncol + c;
-    if (o.ops[0]) experts_prepare_column<32, false>(v, o.ops[0] + at * ER_OP_BYTES, o.inv[0] + at, have, part);
-    if (o.ops[1]) experts_prepare_column<16, false>(v, o.ops[1] + at * ER_OP_BYTES, o.inv[1] + at, have, part);
-    if (o.ops[2]) experts_prepare_column<32, true>(v, o.ops[2] + at * ER_OP_BYTES, o.inv[2] + at, have, part);
+    if (p.ops[0]) experts_prepare_column<32, false>(v, p.ops[0] + at * ER_OP_BYTES, p.inv[0] + at, have, part);
+    if (p.ops[1]) experts_prepare_column<16, false>(v, p.ops[1] + at * ER_OP_BYTES, p.inv[1] + at, have, part);
+    if (p.ops[2]) experts_prepare_column<32, true>(v, p.ops[2] + at * ER_OP_BYTES, p.inv[2] + at, have, part);
 }
 
 // Sixteen bytes of which those from `end` on are zero and not read: the sixteen in front of `end`, moved down (there are as many: a matrix is no smaller).

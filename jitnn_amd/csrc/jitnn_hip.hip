@@ -2527,6 +2527,13 @@ ExpertLists moe_lists(uint8_t *ws, const MoeLayout &l) {
     return lists;
 }
 
+// The tokens' rows as operands, in the layouts that gate and up ask for.
+ExpertPrepare moe_prepare(const jitnn_hip_moe *m, const float *x, int tokens, uint8_t *ws, const MoeLayout &l) {
+    uint8_t *places[GR_LAYOUTS];
+    for (int i = 0; i < GR_LAYOUTS; ++i) places[i] = l.layouts[i] ? ws + l.ops[i] : nullptr;
+    return experts_prepare(x, tokens, m->router->d, places);
+}
+
 ExpertWeights expert_weights(const jitnn_hip_weight *w, int experts) {
     return {w->fmt, w->n / experts, w->k, w->dev, (size_t)(w->n / experts) * (size_t)(w->k / block_values(w->fmt)) * block_bytes(w->fmt)};
 }
@@ -2544,7 +2551,7 @@ int check_moe_call(const jitnn_hip_moe *m, const float *x, int tokens, const flo
     return check_ready();
 }
 
-// One pass: the experts of `tokens` tokens for given choices, whose lists are made.  to_choose (few tokens): the choices are still to be made, of these logits, and go to ids and
+// One pass: the experts of `tokens` tokens for given choices, whose lists and operands (moe_prepare) are made.  to_choose (few tokens): the choices are still to be made, of these logits, and go to ids and
 // weights.
 int moe_experts(const jitnn_hip_moe *m, const float *x, int tokens, const int *ids, const float *weights, const RouterArgs *to_choose, const float *res, float *y, uint8_t *ws, const MoeLayout &l,
                 hipStream_t s) {
@@ -2606,7 +2613,6 @@ int moe_experts(const jitnn_hip_moe *m, const float *x, int tokens, const int *i
     };
     uint8_t *places[GR_LAYOUTS] = {};
     for (int i = 0; i < GR_LAYOUTS; ++i) places[i] = l.layouts[i] ? ws + l.ops[i] : nullptr;
-    if (places[0] || places[1] || places[2]) experts_prepare_launch(x, tokens, r->d, places, s);
     const bool pair = experts_on_rows(m->gate) && m->gate->fmt == m->up->fmt;
     if (pair) {
         if (int rc = rows(m->gate, m->up, places[gemv_rows_layout(m->gate->fmt)], tokens, r->used, 1, gb)) return rc;
@@ -2622,7 +2628,7 @@ int moe_experts(const jitnn_hip_moe *m, const float *x, int tokens, const int *i
     if (experts_on_rows(m->down)) {
         uint8_t *h_places[GR_LAYOUTS] = {};
         h_places[gemv_rows_layout(m->down->fmt)] = ws + l.h_ops;
-        experts_prepare_launch(gb, slots, m->ffn, h_places, s);
+        experts_prepare_launch(experts_prepare(gb, slots, m->ffn, h_places), s);
         if (int rc = rows(m->down, nullptr, ws + l.h_ops, slots, 1, l.splits, part)) return rc;
     } else {
         experts_value_launch(expert_weights(m->down, r->experts), r->experts, ids, slots, 1, gb, part, s);
@@ -2744,7 +2750,10 @@ int jitnn_hip_moe_dev(const jitnn_hip_moe *m, const float *x_dev, int tokens, co
         const float *x = x_dev + (size_t)t * d;
         RouterArgs a = router_args(m->router, x, count, (int *)(ws + l.ids), (float *)(ws + l.weights), ws + l.logits);
         const bool choose_there = l.few && experts_few_chooses(a.experts);
-        if (!l.few) a.lists = moe_lists(ws, l);
+        if (!l.few) {
+            a.lists = moe_lists(ws, l);
+            a.prepare = moe_prepare(m, x, count, ws, l);
+        }
         if (choose_there) router_logits_launch(a, (hipStream_t)stream);
         else router_launch(a, (hipStream_t)stream);
         if (int rc = moe_experts(m, x, count, (const int *)(ws + l.ids), (const float *)(ws + l.weights), choose_there ? &a : nullptr, residual_dev ? residual_dev + (size_t)t * d : nullptr, y_dev + (size_t)t * d,
@@ -2763,9 +2772,11 @@ int jitnn_hip_moe_experts_dev(const jitnn_hip_moe *m, const float *x_dev, int to
         const int count = std::min(pass, tokens - t), d = m->router->d, used = m->router->used;
         const MoeLayout l = moe_layout(m, count);
         const int *ids = ids_dev + (size_t)t * used;
-        if (!l.few) expert_lists_launch(ids, count * used, m->router->experts, moe_lists((uint8_t *)workspace_dev, l), (hipStream_t)stream);
-        if (int rc = moe_experts(m, x_dev + (size_t)t * d, count, ids, weights_dev + (size_t)t * used, nullptr, residual_dev ? residual_dev + (size_t)t * d : nullptr,
-                                 y_dev + (size_t)t * d, (uint8_t *)workspace_dev, l, (hipStream_t)stream))
+        uint8_t *const ws = (uint8_t *)workspace_dev;
+        const float *const x = x_dev + (size_t)t * d;
+        if (!l.few) expert_lists_launch(ids, count * used, m->router->experts, moe_lists(ws, l), moe_prepare(m, x, count, ws, l), (hipStream_t)stream);
+        if (int rc = moe_experts(m, x, count, ids, weights_dev + (size_t)t * used, nullptr, residual_dev ? residual_dev + (size_t)t * d : nullptr,
+                                 y_dev + (size_t)t * d, ws, l, (hipStream_t)stream))
             return rc;
     }
     return JITNN_HIP_OK;

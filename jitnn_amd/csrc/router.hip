@@ -1,4 +1,5 @@
 // The router of a mixture of experts: its logits, the choices of a batch and the lists of what each expert gets.
+#include "experts_rows.h"
 #include "router.h"
 
 #include <algorithm>
@@ -113,10 +114,8 @@ __device__ __forceinline__ void make_lists(Id &&id_of, int slots, int experts, c
             }
             const int first = run + sum - mine;
             if (e < experts) hist[e] = first;
-            for (int i = 0; i < chunks; ++i) {  // (as even as whole rows allow)
-                const int from = (int)((long long)mine * i / chunks), to = (int)((long long)mine * (i + 1) / chunks);
-                lists.chunks[1 + made + chunk_sum - chunks + i] = int4{e, first + from, to - from, 0};
-            }
+            const int each = chunks > 1 ? mine / chunks : mine, more = mine - each * chunks;  // (as even as whole rows allow)
+            for (int i = 0; i < chunks; ++i) lists.chunks[1 + made + chunk_sum - chunks + i] = int4{e, first + i * each + min(i, more), each + (i < more), 0};
             run += __shfl(sum, 63);
             made += __shfl(chunk_sum, 63);
         }
@@ -142,12 +141,20 @@ __global__ void __launch_bounds__(256) choose_kernel(const RouterArgs a) {
     store_choice(a, t, lane, id, weight);
 }
 
+// The workgroups behind the one that makes the lists: sixteen units each, which wait for nothing.
+__device__ __forceinline__ void prepare_beside(const ExpertPrepare &p, int wave, int lane) {
+    const int unit = ((int)blockIdx.x - 1) * 16 + wave;
+    if (unit < p.units()) experts_prepare_unit(p, unit, lane);
+}
+static unsigned beside(const ExpertPrepare &p) { return (unsigned)((p.units() + 15) / 16); }
+
 // Few tokens, one workgroup: the choices of all of them and the experts' lists.
 constexpr int CHOOSE_FEW = 64;
 template <int L>
 __global__ void __launch_bounds__(1024) choose_few_kernel(const RouterArgs a) {
     __shared__ int ids[CHOOSE_FEW * MAX_USED], hist[MAX_EXPERTS];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    if (blockIdx.x > 0) return prepare_beside(a.prepare, wave, lane);
     for (int t = wave; t < a.tokens; t += 16) {
         double l[L];
         load_logits(a, t, lane, l);
@@ -161,8 +168,9 @@ __global__ void __launch_bounds__(1024) choose_few_kernel(const RouterArgs a) {
     make_lists([&](int i) { return ids[i]; }, a.tokens * a.used, a.experts, a.lists, hist);
 }
 
-__global__ void __launch_bounds__(1024) expert_lists_kernel(const int *__restrict__ ids, int slots, int experts, const ExpertLists lists) {
+__global__ void __launch_bounds__(1024) expert_lists_kernel(const int *__restrict__ ids, int slots, int experts, const ExpertLists lists, const ExpertPrepare prepare) {
     __shared__ int hist[MAX_EXPERTS];
+    if (blockIdx.x > 0) return prepare_beside(prepare, __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), threadIdx.x & 63);
     make_lists([&](int i) { return ids[i]; }, slots, experts, lists, hist);
 }
 
@@ -229,15 +237,15 @@ void router_launch(RouterArgs a, hipStream_t s) {
     }
     router_logits_launch(a, s);
     if (lists && a.tokens <= CHOOSE_FEW) {
-        with_lanes(a.experts, [&](auto n) { hipLaunchKernelGGL(choose_few_kernel<n()>, dim3(1), dim3(1024), 0, s, a); });
+        with_lanes(a.experts, [&](auto n) { hipLaunchKernelGGL(choose_few_kernel<n()>, dim3(1 + beside(a.prepare)), dim3(1024), 0, s, a); });
         return;
     }
     with_lanes(a.experts, [&](auto n) { hipLaunchKernelGGL(choose_kernel<n()>, dim3((a.tokens + 3) / 4), dim3(256), 0, s, a); });
-    if (lists) expert_lists_launch(a.ids, a.tokens * a.used, a.experts, a.lists, s);
+    if (lists) expert_lists_launch(a.ids, a.tokens * a.used, a.experts, a.lists, a.prepare, s);
 }
 
-void expert_lists_launch(const int *ids, int slots, int experts, const ExpertLists &lists, hipStream_t s) {
-    hipLaunchKernelGGL(expert_lists_kernel, dim3(1), dim3(1024), 0, s, ids, slots, experts, lists);
+void expert_lists_launch(const int *ids, int slots, int experts, const ExpertLists &lists, const ExpertPrepare &prepare, hipStream_t s) {
+    hipLaunchKernelGGL(expert_lists_kernel, dim3(1 + beside(prepare)), dim3(1024), 0, s, ids, slots, experts, lists, prepare);
 }
 
 }  // namespace jitnn
