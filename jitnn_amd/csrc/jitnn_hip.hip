@@ -2501,6 +2501,19 @@ MoeLayout moe_layout(const jitnn_hip_moe *m, int tokens) {
     return l;
 }
 
+// The most that a pass of `from` to `to` tokens keeps there: fewer tokens may need more, for the down projection's splits and smaller chunks.
+long long moe_most(const jitnn_hip_moe *m, int from, int to) {
+    long long most = 0;
+    for (int t = std::min(to, moe_pass_tokens(m)); t >= from; --t) most = std::max(most, (long long)moe_layout(m, t).total);
+    return most;
+}
+// Layers of one kind have one workspace's size.
+bool moe_alike(const jitnn_hip_moe *a, const jitnn_hip_moe *b) {
+    auto same = [](const jitnn_hip_weight *v, const jitnn_hip_weight *w) { return v->fmt == w->fmt && v->nbytes == w->nbytes && ((uintptr_t)v->dev & 3) == ((uintptr_t)w->dev & 3); };
+    return a->ffn == b->ffn && a->router->experts == b->router->experts && a->router->used == b->router->used && a->router->d == b->router->d && same(a->gate, b->gate) &&
+           same(a->up, b->up) && same(a->down, b->down);
+}
+
 RouterArgs router_args(const jitnn_hip_router *r, const float *x, int tokens, int *ids, float *weights, void *logits) {
     RouterArgs a{};
     a.x = x;
@@ -2735,9 +2748,7 @@ int jitnn_hip_moe_free(jitnn_hip_moe *m) {
 long long jitnn_hip_moe_workspace(const jitnn_hip_moe *m, int tokens) {
     if (!m) return fail(JITNN_HIP_EINVAL, "the layer is NULL");
     if (tokens < 0) return fail(JITNN_HIP_EINVAL, "tokens = %d", tokens);
-    long long most = 0;  // (fewer tokens may need more: the down projection's splits, smaller chunks)
-    for (int t = std::min(tokens, moe_pass_tokens(m)); t > 0; --t) most = std::max(most, (long long)moe_layout(m, t).total);
-    return most;
+    return moe_most(m, 1, tokens);
 }
 
 int jitnn_hip_moe_dev(const jitnn_hip_moe *m, const float *x_dev, int tokens, const float *residual_dev, float *y_dev, void *workspace_dev, long long workspace_bytes, void *stream) {
@@ -3025,11 +3036,16 @@ void release_or_keep(jitnn_hip_llama *m, void *p) {
     else if (!m->recorded) (void)hipFree(p);  // (no memory to note it: left to the process)
 }
 
-// The workspace of a model's experts for passes of up to `tokens`; which 0: one token's.  The device may still use the old one.
+// The workspace of a model's experts for passes of up to `tokens`, which are more than it has been made for; which 0: one token's.  The device may still use the old one.
 int moe_reserve(jitnn_hip_llama *m, int which, int tokens) {
     long long need = 0;
-    for (int l = 0; l < m->layers; ++l)
-        if (m->moe[l]) need = std::max(need, jitnn_hip_moe_workspace(m->moe[l], tokens));
+    const jitnn_hip_moe *last = nullptr;
+    for (int l = 0; l < m->layers; ++l) {
+        const jitnn_hip_moe *e = m->moe[l];
+        if (!e || (last && moe_alike(e, last))) continue;
+        need = std::max(need, moe_most(e, which ? m->moe_cap + 1 : 1, tokens));
+        last = e;
+    }
     if ((size_t)need <= m->moe_ws_bytes[which]) return JITNN_HIP_OK;
     HIP_TRY(hipDeviceSynchronize());
     release_or_keep(m, m->moe_ws[which]);

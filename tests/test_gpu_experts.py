@@ -338,3 +338,59 @@ def test_a_workspace_does_for_fewer_tokens(jn, experts, used, d, ffn, up, down):
         moe.experts_dev(x.data_ptr(), tokens, ids.data_ptr(), weights.data_ptr(), (z := torch.empty(tokens, d, device="cuda")).data_ptr(), ws.data_ptr(), moe.workspace(most))
         torch.cuda.synchronize()
         assert torch.equal(y[:tokens], z)
+
+
+@pytest.mark.parametrize("up,down", [("Q4_K", "Q2_K"), ("Q5_K", "Q6_K"), ("Q6_K", "Q4_K"), ("Q2_K", "Q5_K"), ("Q8_0", "Q4_0"), ("Q4_1", "Q5_1")])
+@pytest.mark.parametrize("tokens", [65, 171, 300])
+def test_many_rows_of_an_expert(jn, up, down, tokens):
+    """More rows than a chunk holds, chunks of every number of groups; an expert of one row beside them, one of none."""
+    rng = np.random.default_rng(tokens)
+    layer = ref.Layer(rng, 4, 1, 256, 768, up, down)
+    moe = layer.make(jn)
+    x = layer.input(rng, tokens)
+    ids = (rng.random((tokens, 1)) < 0.35).astype(np.int32) * 2
+    ids[tokens // 3] = 1
+    weights = rng.standard_normal((tokens, 1)).astype(np.float32)
+    ref.close(Call(moe, x, None, ids, weights).result(), layer.experts_of(x, ids, weights), layer.tolerance)
+
+
+@pytest.mark.parametrize("experts", [129, 200, 512])
+@pytest.mark.parametrize("tokens", [1, 3, 16, 40, 70])
+def test_many_experts(jn, experts, tokens):
+    rng = np.random.default_rng(experts + tokens)
+    layer = ref.Layer(rng, experts, 5, 256, 64, "Q4_0", "Q8_0", bias=(0.1 * rng.standard_normal(experts)).astype(np.float32))
+    x = layer.input(rng, tokens)
+    ref.close(Call(layer.make(jn), x).result(), layer.experts_of(x, *layer.route(x)), layer.tolerance)
+
+
+def test_weights_beyond_31_bits(jn):
+    """Experts that stand more than 2 GiB into their matrices: the results of a layer that has them alone, at one token bit for bit."""
+    experts, d, ffn = 63, 4096, 8192
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    scales = torch.tensor([0.01], dtype=torch.float16).view(torch.uint8).cuda()
+
+    def blocks(count):
+        raw = torch.empty(count, 34, dtype=torch.uint8, device="cuda").random_(0, 256, generator=gen)
+        raw[:, :2] = scales
+        return raw
+
+    big = [blocks(experts * d * ffn // 32) for _ in range(3)]
+    assert big[0].numel() > 1 << 31
+    last = [61, 62]
+    small = [b.reshape(experts, -1)[last].contiguous() for b in big]
+    shapes = ((ffn, d), (ffn, d), (d, ffn))
+    layers = []
+    for count, parts in ((experts, big), (2, small)):
+        router = jn.Router(np.zeros((count, d), dtype=np.float32), 2)
+        layers.append(jn.Moe(router, *(jn.Tensor.wrap_dev(jn.DType.Q8_0, p.data_ptr(), count, *s) for p, s in zip(parts, shapes))))
+    rng = np.random.default_rng(1)
+    for tokens in (1, 5, 20):
+        x = (0.001 * rng.standard_normal((tokens, d))).astype(np.float32)
+        ids = rng.integers(0, 2, (tokens, 2))
+        weights = rng.standard_normal((tokens, 2)).astype(np.float32)
+        got, want = Call(layers[0], x, None, ids + 61, weights).result(), Call(layers[1], x, None, ids, weights).result()
+        assert np.isfinite(want).all() and want.any()
+        if tokens == 1:
+            assert np.array_equal(got, want)
+        else:  # (two experts and 63 may go another way, or come in another number of parts: either is off by one tolerance at most)
+            ref.close(got, want, 2 * ref.tolerance(["Q8_0"] * 3))
