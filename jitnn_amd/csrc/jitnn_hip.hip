@@ -2448,18 +2448,19 @@ int moe_splits(const jitnn_hip_moe *m, int tokens, int groups) {
 }
 
 // Few tokens: the INT8 products on the raw quants, for weights whose rows are whole chunks of 64 values.  They read an expert once for each token that meets it, but as
-// fast as the memory gives, in three launches; the matrix cores' route reads it once, at two thirds of that, between seven launches that cost what 60 MB do.  Both, rows
+// fast as the memory gives, in three launches; the matrix cores' route reads it once, at two thirds of that, between six launches that cost what 120 MB do.  Both, rows
 // / few, us: two of eight experts of 4096 x 14336, Q4_K and Q6_K, 1 token 93 / 49, 4 228 / 147, 6 256 / 218, 8 264 / 265, 12 278 / 406; four of 16 of 4096 x 2048, Q5_K,
-// 4 87 / 67, 5 88 / 84, 6 89 / 98; eight of 128 of 2048 x 768, 1 49 / 21, 8 84 / 52, 16 102 / 89; six of 64 of 2048 x 1408, Q8_0, 5 97 / 53, 12 135 / 109; eight
-// of 64 of 5120 x 1536 8 215 / 178, 12 264 / 268; two of eight of 4096 x 1024, Q6_K, 1 61 / 16, 8 64 / 33, 16 65 / 48.  Not measured with more tokens.
-constexpr int MOE_FEW_TOKENS = 16;
+// 4 87 / 67, 5 88 / 84, 6 89 / 98, 16 99 / 222; eight of 128 of 2048 x 768, 1 49 / 21, 8 84 / 52, 16 103 / 89, 24 127 / 136, 32 137 / 169; six of 64 of 2048 x 1408, Q8_0,
+// 5 97 / 53, 16 152 / 127, 24 168 / 194; eight of 64 of 5120 x 1536 8 215 / 178, 12 264 / 268; two of eight of 4096 x 1024, Q6_K, 1 61 / 16, 12 63 / 44, 16 63 / 48, 24 55 / 77;
+// eight of 256 of 2048 x 512, Q4_0, 16 109 / 49, 32 157 / 78, 64 208 / 130; two of 32 of 1024 x 2048, 32 50 / 38, 48 52 / 60.  Not measured with more tokens.
+constexpr int MOE_FEW_TOKENS = 64;
 bool moe_few(const jitnn_hip_moe *m, int tokens) {
     if (!g.gemv_i8 || tokens > MOE_FEW_TOKENS || m->gate->fmt != m->up->fmt) return false;
     for (const jitnn_hip_weight *w : {m->gate, m->up, m->down})
         if (w->nbytes >= (1ll << 32) || ((uintptr_t)w->dev & 3) != 0) return false;
     if (!experts_few_up_supported(m->gate->fmt, m->router->d) || !experts_few_down_supported(m->down->fmt, m->ffn, m->router->used)) return false;
     const double expert = (double)(m->gate->nbytes + m->up->nbytes + m->down->nbytes) / m->router->experts;
-    return tokens == 1 || expert * ((double)tokens * m->router->used - 1.5 * moe_met(m->router, tokens)) <= 60e6;
+    return tokens == 1 || expert * ((double)tokens * m->router->used - 1.5 * moe_met(m->router, tokens)) <= 120e6;
 }
 
 // What a pass of `tokens` keeps in the workspace, in bytes from its start.

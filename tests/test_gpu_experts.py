@@ -394,3 +394,13 @@ def test_weights_beyond_31_bits(jn):
             assert np.array_equal(got, want)
         else:  # (two experts and 63 may go another way, or come in another number of parts: either is off by one tolerance at most)
             ref.close(got, want, 2 * ref.tolerance(["Q8_0"] * 3))
+
+
+@pytest.mark.parametrize("up,down", [f for f in FORMATS if "Q5_0" not in f])
+@pytest.mark.parametrize("experts,used", [(200, 1), (20, 2)])
+def test_few_rows_of_an_expert(jn, experts, used, up, down):
+    """More tokens than the INT8 products are for, over so many experts that each has a row or a few: chunks of one group and of two."""
+    rng = np.random.default_rng(experts)
+    layer = ref.Layer(rng, experts, used, 256, 256, up, down)
+    x = layer.input(rng, 67)
+    ref.close(Call(layer.make(jn), x).result(), layer.experts_of(x, *layer.route(x)), layer.tolerance)
