@@ -371,9 +371,10 @@ __global__ void __launch_bounds__(S::threads, S::per_simd) experts_rows_kernel(c
 // Two: with a tile a wave 128 registers do, and a CU has sixteen waves (24 tokens, two of eight experts of 4096 x 14336 in Q5_K 317 -> 266 us); where they do not - Q6_K, 32-value
 // blocks but Q4_0 -, four waves of two tiles (of one of Q6_K) (24 tokens, two of eight of 4096 x 4096: Q8_0 140 us against 152 and 145 of eight waves, Q4_1 84 / 106 / 90, Q6_K
 // 141 / 212 / 148, Q4_0 114 / 107 / 121, Q5_K 98 / - / 101).
-// Three to eight: in sets of four, an eighth faster with the operands read ahead.  512 tokens, two of eight of 4096 x 14336 in Q4_K and Q6_K: 1457 us; groups of sixteen rows, hi
-// and lo parts as operands of their own, 1472; four waves and sets of two 1479; sixteen groups a chunk 2243 (registers); chunks by XCD 1745.  What bounds it there: without its
-// products it takes 1009 us - operands on their way 215, to LDS 70, decoding 125, weights 130 -, without all of those 956; the products alone would be 490.
+// Three to twelve (to eight of 32-value blocks: registers): in sets of four, whose operands come out of LDS ahead of their products.  512 tokens, two of eight of 4096 x 14336 in Q4_K
+// and Q6_K: 1380 us, with eight at most - more chunks where an expert has more rows than most - 1457; groups of sixteen rows, hi and lo parts as operands of their own, 1472; four
+// waves and sets of two 1479; sixteen groups a chunk 1600 to 2243 (registers).  What bounds it there, of 1490: without its products it took 1009 us - operands on their way 215,
+// to LDS 70, decoding 125, weights 130 -, without all of those 956; the products alone would be 490.
 typedef RowsShape<8, 1, 1, 2> RowsShape1;
 typedef RowsShape<4, 1, 1, 2> RowsShape1Short;
 typedef RowsShape<8, 2, 1, 4> RowsShape2;
@@ -387,7 +388,7 @@ static RowsKernelRef experts_rows_shape(bool dual) {
     // (weight rows of a workgroup: its waves' tiles; of a pair of matrices half as many of each)
     return {fn, experts_rows_lds<FMT, S>(), S::threads, S::waves * er_tiles<FMT, S>() / (dual ? 2 : 1), S::all_rows / 8};
 }
-// groups: of a chunk, at most 8
+// groups: of a chunk, at most 12, of 32-value blocks 8
 template <int FMT>
 static RowsKernelRef experts_rows_pick(int groups, bool dual) {
     if (groups <= 1) {
