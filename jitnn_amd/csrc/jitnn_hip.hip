@@ -3052,6 +3052,7 @@ int moe_reserve(jitnn_hip_llama *m, int which, int tokens) {
     release_or_keep(m, m->moe_ws[which]);
     m->moe_ws[which] = nullptr;
     m->moe_ws_bytes[which] = 0;
+    if (which) m->moe_cap = 0;
     if (hipMalloc(&m->moe_ws[which], (size_t)need) != hipSuccess) {
         (void)hipGetLastError();
         m->moe_ws[which] = nullptr;

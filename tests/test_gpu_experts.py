@@ -404,3 +404,17 @@ def test_few_rows_of_an_expert(jn, experts, used, up, down):
     layer = ref.Layer(rng, experts, used, 256, 256, up, down)
     x = layer.input(rng, 67)
     ref.close(Call(layer.make(jn), x).result(), layer.experts_of(x, *layer.route(x)), layer.tolerance)
+
+
+@pytest.mark.parametrize("gate,up,down", [("Q5_0", "Q5_0", "Q3_K"), ("Q3_K", "Q8_0", "Q5_0"), ("Q4_K", "Q3_K", "Q6_K"), ("Q4_K", "Q4_K", "Q5_0")])
+@pytest.mark.parametrize("tokens", [1, 9, 70])
+def test_blocks_that_are_left_as_they_are(jn, gate, up, down, tokens):
+    """Q5_0 and Q3_K blocks in the caller's device memory, which nobody rewrites, beside formats that the matrix cores' kernels take."""
+    rng = np.random.default_rng(tokens)
+    layer = ref.Layer(rng, 5, 2, 256, 512, up=up, down=down, gate=gate)
+    raw = [dev(r) for r in layer.raw]
+    router = jn.Router(layer.router / layer.size, 2)
+    moe = jn.Moe(router, *(jn.Tensor.wrap_dev(jn.DType[f], r.data_ptr(), *s) for f, r, s in zip(layer.formats, raw, layer.shapes)))
+    x = layer.input(rng, tokens)
+    res = rng.standard_normal(x.shape).astype(np.float32)
+    ref.close(Call(moe, x, res).result(), layer.experts_of(x, *layer.route(x), res), layer.tolerance)
