@@ -93,15 +93,16 @@ struct ExpertFewArgs {
     const int *ids;         // [tokens, used]
     const float *weights;   // down: [tokens, used]
     const float *res;       // down: [tokens, n] or nullptr
-    float *y;               // up: [tokens, used, n]; down: [tokens, n] (may be res)
+    float *y;               // up: [tokens, used, n]; down: [parts][tokens, n] (may be res)
     int n, k, used, experts, act, blocks;
     unsigned by_rows;       // up: reciprocal of n / 4
     RouterArgs route;       // up: logits that are there, of which every wave makes the choice for itself (and the first one leaves it at ids and weights); logits nullptr: ids are there
 };
-// whether rows of k values (up) and `used` of ffn values behind one another (down) have a kernel
+// whether rows of k values (up) and `used` of ffn values behind one another (down) have a kernel; in how many parts (one at least), each with a y to be added up, the latter
 bool experts_few_chooses(int experts);  // whether the first launch can make the choices
 bool experts_few_up_supported(int fmt, int k);
 bool experts_few_down_supported(int fmt, int ffn, int used);
+int experts_few_down_parts(int ffn, int used);
 void experts_few_up_launch(int fmt, ExpertFewArgs a, int tokens, int cus, hipStream_t s);
 void experts_few_down_launch(int fmt, ExpertFewArgs a, int tokens, int cus, hipStream_t s);
 typedef void (*ExpertFewKernel)(const ExpertFewArgs);

@@ -52,8 +52,11 @@ bool experts_few_up_supported(int fmt, int k) {
     return (quants32(fmt) ? fmt != F_Q5_0 && k % 64 == 0 : fmt != F_Q3_K) && k <= 1024 * I8_MAX_WAVES;  // (rows of whole chunks of 64 values)
 }
 
+static int few_stretches(int ffn, int used) { return (int)(((long long)used * ffn + 1023) / 1024); }
+int experts_few_down_parts(int ffn, int used) { return (few_stretches(ffn, used) + 2 * I8_MAX_WAVES - 1) / (2 * I8_MAX_WAVES); }
+
 bool experts_few_down_supported(int fmt, int ffn, int used) {
-    return (quants32(fmt) ? fmt != F_Q5_0 && ffn % 64 == 0 : fmt != F_Q3_K) && (long long)used * ffn <= 2 * 1024 * I8_MAX_WAVES;
+    return (quants32(fmt) ? fmt != F_Q5_0 && ffn % 64 == 0 : fmt != F_Q3_K) && experts_few_down_parts(ffn, used) <= 8;
 }
 
 // Workgroups for `groups` row groups of each of `tokens`, so many waves a CU in all and every workgroup as many turns as the others.
@@ -72,11 +75,12 @@ void experts_few_up_launch(int fmt, ExpertFewArgs a, int tokens, int cus, hipStr
 }
 
 void experts_few_down_launch(int fmt, ExpertFewArgs a, int tokens, int cus, hipStream_t s) {
-    const int all = (int)(((long long)a.used * a.k + 1023) / 1024), stretches = all > I8_MAX_WAVES ? 2 : 1, waves = (all + stretches - 1) / stretches;
+    const int all = few_stretches(a.k, a.used), parts = experts_few_down_parts(a.k, a.used), each = (all + parts - 1) / parts, stretches = each > I8_MAX_WAVES ? 2 : 1,
+              waves = (each + stretches - 1) / stretches;
     const bool aligned = a.k % 512 == 0 && ((uintptr_t)a.w & 3) == 0;
-    a.blocks = few_blocks(a.n / 4, tokens, waves, cus, 16);
+    a.blocks = few_blocks(a.n / 4, tokens * parts, waves, cus, 16);
     const ExpertFewKernel fn = quants32(fmt) ? experts_few_down_q32(fmt, stretches, waves) : experts_few_down_k(fmt, aligned, stretches, waves);
-    hipLaunchKernelGGL(fn, dim3(a.blocks, tokens), dim3(64 * waves), (size_t)waves * EF_WAVE_LDS, s, a);
+    hipLaunchKernelGGL(fn, dim3(a.blocks, tokens, parts), dim3(64 * waves), (size_t)waves * EF_WAVE_LDS, s, a);
 }
 
 // ---- on the matrix cores

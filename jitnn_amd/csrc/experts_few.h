@@ -160,8 +160,8 @@ __global__ void __launch_bounds__(64 * MAXW, 4) experts_few_up_kernel(const Expe
     }
 }
 
-// y [token, n] = res + the sum over the token's places of share * (down h).  grid (a.blocks, tokens); wave w takes stretches w, w + waves, ... (S at most) of 1024 values of the
-// long row.
+// y [token, n] = res + the sum over the token's places of share * (down h).  grid (a.blocks, tokens, parts); wave w takes stretches w, w + waves, ... (S at most) of 1024 values of its
+// part of the long row, which has a y of its own.
 template <class U, int S, int PF, int MAXW>
 __global__ void __launch_bounds__(64 * MAXW, MAXW > 8 ? 4 : 2) experts_few_down_kernel(const ExpertFewArgs a) {
     constexpr int NB = PF + 1;
@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(64 * MAXW, MAXW > 8 ? 4 : 2) experts_few_down_
     extern __shared__ __align__(16) uint8_t ef_smem[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), waves = (int)(blockDim.x >> 6);
     float *const part = reinterpret_cast<float *>(ef_smem + (size_t)wave * EF_WAVE_LDS);
-    const int b = lane >> 2, j = lane & 3, per = a.k >> 6, chunks = a.used * per, token = (int)blockIdx.y;
+    const int b = lane >> 2, j = lane & 3, per = a.k >> 6, chunks = a.used * per, token = (int)blockIdx.y, first = (int)blockIdx.z * S * waves * 16;
     const uint32_t rowbytes = (uint32_t)(a.k / block_values(U::FMT)) * block_bytes(U::FMT);
     const int groups = a.n >> 2, turns = (groups + a.blocks - 1) / a.blocks;
     typename U::Off off[S];
@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(64 * MAXW, MAXW > 8 ? 4 : 2) experts_few_down_
     float share[S];
 #pragma unroll
     for (int s = 0; s < S; ++s) {
-        const int at = (wave + s * waves) * 16 + b;
+        const int at = first + (wave + s * waves) * 16 + b;
         const int c = min(at, chunks - 1), place = c / per;
         cc[s] = c - place * per;
         const int e = a.ids[(size_t)token * a.used + place];
@@ -238,7 +238,7 @@ __global__ void __launch_bounds__(64 * MAXW, MAXW > 8 ? 4 : 2) experts_few_down_
         for (int o = tid; o < 4 * (tend - t0); o += 64 * waves) {
             const int tt = o >> 2, jj = o & 3, g = (int)blockIdx.x + (t0 + tt) * a.blocks;
             if (g < groups) {
-                const size_t to = (size_t)token * a.n + 4 * g + jj;
+                const size_t to = ((size_t)blockIdx.z * gridDim.y + token) * a.n + 4 * g + jj;
                 const float sum = few_joined<MAXW>(ef_smem, waves, half * EF_FLUSH + tt, jj);
                 a.y[to] = a.res ? sum + a.res[to] : sum;
             }

@@ -2423,18 +2423,32 @@ int moe_pass_tokens(const jitnn_hip_moe *m) { return std::max(1, MOE_PASS_SLOTS 
 
 bool experts_on_rows(const jitnn_hip_weight *w) { return gemv_rows_supported(w->fmt); }  // (Q5_0 and Q3_K blocks that were not rewritten have no operands)
 
+// Experts that so many tokens meet, where every one is as likely as any other.
+double moe_met(const jitnn_hip_router *r, int tokens) { return r->experts * (1 - std::pow(1 - (double)r->used / r->experts, tokens)); }
+
+// Chunks of so many groups that so many tokens make, about.
+double moe_chunks(const jitnn_hip_router *r, int tokens, int groups) {
+    return moe_met(r, tokens) * std::max(1.0, (double)tokens * r->used / r->experts / (8 * groups));
+}
+
 // Groups of eight rows in a chunk of an expert's: what most experts have where every one is as likely as any other, so that their weights are read
-// and decoded once; at most what the kernels hold.
+// and decoded once; at most what the kernels hold; fewer where gate and up, which have no shares of K, would have no workgroup for three quarters of the CUs.  us with
+// none asked for / half / three quarters / all: 229 tokens, four of nine experts of 2560 x 512, Q4_K and Q5_K 112 / 78 / 71 / 72; 256, two of eight of 2048 x 2048 108 / 105 / 99 / 121;
+// 512, two of eight of 1024 x 1024, Q4_K 76 / 64 / 66 / 66, Q8_0 96 / 95 / 101 / 101; 200, two of eight of 2048 x 1024, Q4_0 107 / 68 / 67 / 66.
 int moe_groups(const jitnn_hip_moe *m, int tokens) {
-    const double mean = (double)tokens * m->router->used / m->router->experts;
+    const jitnn_hip_router *r = m->router;
+    const double mean = (double)tokens * r->used / r->experts;
     int groups = std::max(1, (int)std::ceil((mean + 2 * std::sqrt(mean)) / 8));
     for (const jitnn_hip_weight *w : {m->gate, m->up, m->down})
         if (experts_on_rows(w)) groups = std::min(groups, experts_rows_kernel_ref(w->fmt, groups, false).groups);
+    if (!experts_on_rows(m->gate) || m->gate->fmt != m->up->fmt) return groups;
+    auto workgroups = [&](int with) {
+        const RowsKernelRef k = experts_rows_kernel_ref(m->gate->fmt, with, true);
+        return moe_chunks(r, tokens, with) * ((m->ffn / 16 + k.tiles - 1) / k.tiles);
+    };
+    while (groups > 1 && 4 * workgroups(groups) < 3 * g.cus) groups = (groups + 1) / 2;
     return groups;
 }
-
-// Experts that so many tokens meet, where every one is as likely as any other.
-double moe_met(const jitnn_hip_router *r, int tokens) { return r->experts * (1 - std::pow(1 - (double)r->used / r->experts, tokens)); }
 
 // Shares of the down projection's columns, where its workgroups alone would leave CUs idle: expected chunks x blocks against a workgroup for every CU (two of
 // the small ones).
@@ -2442,12 +2456,13 @@ int moe_splits(const jitnn_hip_moe *m, int tokens, int groups) {
     if (!experts_on_rows(m->down)) return 1;
     const jitnn_hip_router *r = m->router;
     const RowsKernelRef k = experts_rows_kernel_ref(m->down->fmt, groups, false);
-    const double mean = (double)tokens * r->used / r->experts, blocks = moe_met(r, tokens) * std::max(1.0, mean / (8 * groups)) * ((r->d / 16 + k.tiles - 1) / k.tiles);
+    const double blocks = moe_chunks(r, tokens, groups) * ((r->d / 16 + k.tiles - 1) / k.tiles);
     const int ncol = (m->ffn + 255) / 256, wanted = (int)std::ceil((k.threads > 256 ? 1.0 : 2.0) * g.cus / blocks);
     return std::max(1, std::min({wanted, 8, ncol / 4}));
 }
 
-// Few tokens: the INT8 products on the raw quants, for weights whose rows are whole chunks of 64 values.  They read an expert once for each token that meets it, but as
+// Few tokens: the INT8 products on the raw quants, for weights whose rows are whole chunks of 64 values.  (One token, seven of 36 experts of 512 x 13568, whose down projection
+// comes in three parts that a launch more joins: 45 us, by the other route 71.)  They read an expert once for each token that meets it, but as
 // fast as the memory gives, in three launches; the matrix cores' route reads it once, at two thirds of that, between six launches that cost what 120 MB do.  Both, rows
 // / few, us: two of eight experts of 4096 x 14336, Q4_K and Q6_K, 1 token 93 / 49, 4 228 / 147, 6 256 / 218, 8 264 / 265, 12 278 / 406; four of 16 of 4096 x 2048, Q5_K,
 // 4 87 / 67, 5 88 / 84, 6 89 / 98, 16 99 / 222; eight of 128 of 2048 x 768, 1 49 / 21, 8 84 / 52, 16 103 / 89, 24 127 / 136, 32 137 / 169; six of 64 of 2048 x 1408, Q8_0,
@@ -2459,8 +2474,10 @@ bool moe_few(const jitnn_hip_moe *m, int tokens) {
     for (const jitnn_hip_weight *w : {m->gate, m->up, m->down})
         if (w->nbytes >= (1ll << 32) || ((uintptr_t)w->dev & 3) != 0) return false;
     if (!experts_few_up_supported(m->gate->fmt, m->router->d) || !experts_few_down_supported(m->down->fmt, m->ffn, m->router->used)) return false;
-    const double expert = (double)(m->gate->nbytes + m->up->nbytes + m->down->nbytes) / m->router->experts;
-    return tokens == 1 || expert * ((double)tokens * m->router->used - 1.5 * moe_met(m->router, tokens)) <= 120e6;
+    // (a wave takes 1024 values of a row of gate and up, whatever there are: 512 cost as much)
+    const double pair = (double)(m->gate->nbytes + m->up->nbytes), down = (double)m->down->nbytes, whole = (m->router->d + 1023) / 1024 * 1024.0 / m->router->d;
+    const double each = (double)tokens * m->router->used, met = 1.5 * moe_met(m->router, tokens);
+    return tokens == 1 || (each * (pair * whole + down) - met * (pair + down)) / m->router->experts <= 120e6;
 }
 
 // What a pass of `tokens` keeps in the workspace, in bytes from its start.
@@ -2488,8 +2505,12 @@ MoeLayout moe_layout(const jitnn_hip_moe *m, int tokens) {
     l.ids = take(slots * sizeof(int));
     l.weights = take(slots * sizeof(float));
     l.g = take(slots * m->ffn * sizeof(float));
-    l.total = at;
-    if (l.few) return l;
+    if (l.few) {
+        const int parts = experts_few_down_parts(m->ffn, r->used);
+        l.part = parts > 1 ? take((size_t)parts * tokens * r->d * sizeof(float)) : 0;
+        l.total = at;
+        return l;
+    }
     l.list = take(slots * sizeof(int));
     l.chunks = take(((size_t)l.chunks_most + 1) * sizeof(int4));
     for (const jitnn_hip_weight *w : {m->gate, m->up})
@@ -2592,12 +2613,14 @@ int moe_experts(const jitnn_hip_moe *m, const float *x, int tokens, const int *i
         e = expert_weights(m->down, r->experts);
         a.w = m->down->dev;
         a.expert_bytes = e.expert_bytes;
+        const int parts = experts_few_down_parts(m->ffn, r->used);
         a.x = gb;
-        a.res = res;
-        a.y = y;
+        a.res = parts > 1 ? nullptr : res;
+        a.y = parts > 1 ? part : y;
         a.n = e.n;
         a.k = e.k;
         experts_few_down_launch(m->down->fmt, a, tokens, g.cus, s);
+        if (parts > 1) rows_join_launch(s, part, y, tokens, r->d, parts, nullptr, Epilogue{0, res}, (unsigned)g.cus);
         HIP_TRY(hipGetLastError());
         return JITNN_HIP_OK;
     }

@@ -418,3 +418,24 @@ def test_blocks_that_are_left_as_they_are(jn, gate, up, down, tokens):
     x = layer.input(rng, tokens)
     res = rng.standard_normal(x.shape).astype(np.float32)
     ref.close(Call(moe, x, res).result(), layer.experts_of(x, *layer.route(x), res), layer.tolerance)
+
+
+@pytest.mark.parametrize("experts,used,d,ffn,up,down", [(9, 8, 256, 4352, "Q4_K", "Q6_K"), (5, 4, 64, 10752, "Q8_0", "Q4_0"), (6, 5, 512, 13312, "Q5_K", "Q2_K"), (40, 33, 128, 6400, "Q4_1", "Q8_0")])
+@pytest.mark.parametrize("tokens", [1, 3])
+def test_long_rows_in_parts(jn, experts, used, d, ffn, up, down, tokens):
+    """Down projections of one token that are longer than a workgroup takes: parts, the last of them ragged, that a launch more adds up with the residual."""
+    rng = np.random.default_rng(ffn)
+    layer = ref.Layer(rng, experts, used, d, ffn, up, down)
+    moe = layer.make(jn)
+    x = layer.input(rng, tokens)
+    res = rng.standard_normal(x.shape).astype(np.float32)
+    ids, weights = layer.route(x)
+    want = layer.experts_of(x, ids, weights, res)
+    call = Call(moe, x, res)
+    ref.close(call.result(), want, layer.tolerance)
+    call.y.copy_(call.residual)
+    call.residual = call.y  # y is the residual
+    ref.close(call.result(), want, layer.tolerance)
+    bad = ids.copy()
+    bad[0] = -1
+    assert np.array_equal(Call(moe, x, res, bad, weights).result()[0], res[0])
