@@ -439,3 +439,18 @@ def test_long_rows_in_parts(jn, experts, used, d, ffn, up, down, tokens):
     bad = ids.copy()
     bad[0] = -1
     assert np.array_equal(Call(moe, x, res, bad, weights).result()[0], res[0])
+
+
+@pytest.mark.parametrize("up,down", [f for f in FORMATS if "Q5_0" not in f])
+@pytest.mark.parametrize("tokens", [20, 45, 70, 201])
+def test_large_chunks(jn, up, down, tokens):
+    """So many rows of weights that chunks are as large as a kernel holds: groups in one set, in two and three, the last one ragged, and experts of several chunks."""
+    rng = np.random.default_rng(tokens)
+    layer = ref.Layer(rng, 2, 2, 256, 12288, up, down)
+    x = layer.input(rng, tokens)
+    ids, weights = np.tile([1, 0], (tokens, 1)), rng.standard_normal((tokens, 2)).astype(np.float32)
+    want = np.zeros(x.shape)
+    for j, e in enumerate((1, 0)):
+        gate, up_, down_ = (v[e] for v in layer.values)
+        want += weights[:, j:j + 1] * ((ref.activate("silu", x.astype(np.float64) @ gate.T) * (x.astype(np.float64) @ up_.T)) @ down_.T)
+    ref.close(Call(layer.make(jn), x, None, ids, weights).result(), want, layer.tolerance)
