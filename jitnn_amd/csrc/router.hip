@@ -233,8 +233,9 @@ static void with_lanes(int experts, F &&f) {
 }
 static_assert(MAX_EXPERTS <= 8 * 64, "every expert has a lane");
 
-// One launch for logits and choice: few experts, and few enough tokens for a workgroup each.
-static bool one_launch(int tokens, int experts, int d) { return (long long)experts * d <= 131072 && tokens <= 64; }
+// One launch for logits and choice: so few weights that a token's one workgroup has read them when a second launch would start.  One / two launches, us: 8 experts of 4096 values, 1
+// token 4.2 / 5.9, 64 tokens 4.7 / 6.2; 16 of 4096 6.1 / 5.9; 128 of 512 8.9 / 6.2; 64 of 2048 10.1 / 5.9.
+static bool one_launch(int tokens, int experts, int d) { return (long long)experts * d <= 49152 && tokens <= 64; }
 
 // A workgroup per logit, up to some 64 MiB of rows through the L2s (32 tokens x 128 experts x 2048 values 6 us, in tiles 14); tiles of 16 x 16 beyond.
 static bool logit_each(int tokens, int experts, int d) { return (long long)tokens * experts * d <= 8 << 20; }
