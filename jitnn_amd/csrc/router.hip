@@ -237,8 +237,8 @@ static_assert(MAX_EXPERTS <= 8 * 64, "every expert has a lane");
 // token 4.2 / 5.9, 64 tokens 4.7 / 6.2; 16 of 4096 6.1 / 5.9; 128 of 512 8.9 / 6.2; 64 of 2048 10.1 / 5.9.
 static bool one_launch(int tokens, int experts, int d) { return (long long)experts * d <= 49152 && tokens <= 64; }
 
-// A workgroup per logit, while all of them together read no more than 64 MiB of rows through the L2s, 136 for up to 128 tokens, where tiles are few; tiles beyond.  Logits and
-// choice, tiles / a workgroup per logit, us: 64 tokens x 64 experts x 4096 values 13.4 / 9.3, 26 x 194 x 3040 13.6 / 10.5, 64 x 128 x 2048 11.6 / 10.4, 40 x 256 x 2048 12.0 / 12.1;
+// A workgroup per logit, while all of them together read no more than 64 MiB of rows through the L2s, 136 for up to 128 tokens, where tiles are few; tiles beyond.  At 128 tokens the
+// two are about level (64 experts of 2048 values 9.7 a workgroup per logit, 129 tokens in tiles 10.9; 128 of 1024 12.2, 129 tokens 10.3).  Logits and choice, tiles / a workgroup per logit, us: 64 tokens x 64 experts x 4096 values 13.4 / 9.3, 26 x 194 x 3040 13.6 / 10.5, 64 x 128 x 2048 11.6 / 10.4, 40 x 256 x 2048 12.0 / 12.1;
 // 344 x 63 x 832 10.4 / 14.8, 512 x 8 x 4096 9.3 / 14.4.
 static bool logit_each(int tokens, int experts, int d) { return (long long)tokens * experts * d <= (tokens <= 128 ? 17 : 8) << 20; }
 static int tile_side(int tokens, int experts) { return tokens > 16 && experts > 16 ? 32 : 16; }
