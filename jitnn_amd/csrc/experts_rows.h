@@ -16,6 +16,7 @@
 #include "common.h"
 #include "experts.h"
 #include "gemv_rows.h"
+#include "row_end.h"
 
 namespace jitnn {
 
@@ -116,12 +117,10 @@ __device__ __forceinline__ void experts_prepare_unit(const ExpertPrepare &p, int
 
 // Sixteen bytes of which those from `end` on are zero and not read: the sixteen in front of `end`, moved down (there are as many: a matrix is no smaller).
 __device__ __forceinline__ u32x4 ld128_until(const uint8_t *p, const uint8_t *end) {
-    const int behind = max((int)(p + 16 - end), 0), by = 8 * min(behind, 16);  // (of a wave's columns, so never far behind)
+    const int behind = bytes_behind((long long)(p - end) + 16);
     const u32x4 v = ld128<2>(p - behind);
-    const unsigned long long lo = (unsigned long long)v.y << 32 | v.x, hi = (unsigned long long)v.w << 32 | v.z;
-    const unsigned long long down = by == 0 ? lo : by < 64 ? lo >> by | hi << (64 - by) : by < 128 ? hi >> (by - 64) : 0;
-    const unsigned long long up = by < 64 ? hi >> by : 0;
-    return u32x4{(uint32_t)down, (uint32_t)(down >> 32), (uint32_t)up, (uint32_t)(up >> 32)};
+    const Halves h = moved_down({(unsigned long long)v.y << 32 | v.x, (unsigned long long)v.w << 32 | v.z}, behind);
+    return u32x4{(uint32_t)h.lo, (uint32_t)(h.lo >> 32), (uint32_t)h.hi, (uint32_t)(h.hi >> 32)};
 }
 
 // The last column of rows that are no whole columns (32-value blocks): what lies behind a row's last block is the next row, behind the last row nobody's.
