@@ -48,7 +48,17 @@ __device__ __forceinline__ void few_round(float4 (&xv)[4]) {
                  max(__float_as_uint(xv[i].z) & 0x7fffffffu, __float_as_uint(xv[i].w) & 0x7fffffffu));
     am = max(am, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)am, 0xB1, 0xF, 0xF, true));  // quad_perm [1,0,3,2]
     am = max(am, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)am, 0x4E, 0xF, 0xF, true));  // quad_perm [2,3,0,1]
-    const uint32_t eb = min(max(am >> 23, 22u), 254u);  // (the scale that i8_stage takes: it finds these values whole)
+    if (__builtin_amdgcn_ballot_w64(am - 0x7f7ffffeu < 2u) != 0) {  // (the two largest finite values would become infinite: the next one below, which does not)
+        auto finite = [](float v) {
+            const uint32_t u = __float_as_uint(v), m = u & 0x7fffffffu;
+            return m - 0x7f7ffffeu < 2u ? __uint_as_float(u - (m - 0x7f7ffffdu)) : v;
+        };
+#pragma unroll
+        for (int i = 0; i < 4; ++i) xv[i] = make_float4(finite(xv[i].x), finite(xv[i].y), finite(xv[i].z), finite(xv[i].w));
+        am = am - 0x7f7ffffeu < 2u ? 0x7f7ffffdu : am;
+    }
+    // (the scale that i8_stage takes, which finds these values whole: the exponent behind the rounding, which the two largest mantissas of 24 bits raise)
+    const uint32_t eb = min(max((am + 2u) >> 23, 22u), 254u);
     const float up = __uint_as_float((275u - eb) << 23), down = __uint_as_float((eb - 21u) << 23);
     auto rounded = [&](float v) { return (__builtin_fmaf(v, up, 12582912.f) - 12582912.f) * down; };
 #pragma unroll

@@ -1,4 +1,4 @@
-"""Layers of experts at their borders: matrices beyond 2 GiB whose rows are no whole columns, inputs next to a power of two and to the largest FP32 value, overlapping buffers."""
+"""Layers of experts at their borders: matrices beyond 2 GiB whose rows are no whole columns, inputs next to a power of two and to the largest FP32 value."""
 import numpy as np
 import pytest
 import torch
@@ -41,3 +41,58 @@ def test_ragged_rows_of_weights_beyond_31_bits(jn):
         share = np.where(ids == e, weights, 0).sum(1, keepdims=True, dtype=np.float64)
         want += share * ((ref.activate("silu", x.astype(np.float64) @ gate.T) * (x.astype(np.float64) @ up.T)) @ down.T)
     ref.close(Call(moe, x, None, ids, weights).result(), want, ref.tolerance(["Q8_0"] * 3))
+
+
+def q6_k(quants):
+    """Q6_K blocks of whole numbers -32..31, [rows, a multiple of 256]: every scale 1."""
+    q = (np.asarray(quants, dtype=np.int32) + 32).astype(np.uint8).reshape(-1, 2, 4, 32)  # [block, half, quarter, place]
+    low = np.stack([q[:, :, 0] & 15 | (q[:, :, 2] & 15) << 4, q[:, :, 1] & 15 | (q[:, :, 3] & 15) << 4], axis=2)
+    high = q[:, :, 0] >> 4 | (q[:, :, 1] >> 4) << 2 | (q[:, :, 2] >> 4) << 4 | (q[:, :, 3] >> 4) << 6
+    n = len(q)
+    return np.concatenate([low.reshape(n, 128), high.reshape(n, 64), np.ones((n, 16), dtype=np.uint8), np.full((n, 1), np.float16(1)).view(np.uint8)], axis=1).astype(np.uint8)
+
+
+def q8_0(quants, scale):
+    q = np.asarray(quants, dtype=np.int8).reshape(-1, 32)
+    return np.concatenate([np.full((len(q), 1), np.float16(scale)).view(np.uint8), q.view(np.uint8)], axis=1)
+
+
+def one_expert(jn, d, fmt, gate, up, down):
+    router = jn.Router(np.zeros((1, d), dtype=np.float32), 1)
+    return jn.Moe(router, *(jn.Tensor.quantized(jn.DType[fmt], w.reshape(-1), 1, d, d) for w in (gate, up, down)), activation=None)
+
+
+@pytest.mark.parametrize("tokens", [1, 3])
+def test_inputs_next_to_a_power_of_two(jn, tokens):
+    """A value that rounds up to the next power of two beside values of half a step: what is rounded counts with the quant less its offset of 32, so sixteen values of half a step, 2^-22 of
+    the largest each, that meet a weight of 1 may go missing, and no more."""
+    d = 256
+    quants = np.zeros((3, d, d), dtype=np.int32)
+    quants[0, :, 32:48] = 1  # gate: the sixteen small values
+    quants[1, :, 0] = 1      # up: the largest one
+    np.fill_diagonal(quants[2], 1)
+    raw = [q6_k(q) for q in quants]
+    assert all(np.array_equal(ref.dequantised("Q6_K", r.reshape(-1), d, d), q) for r, q in zip(raw, quants))
+    x = np.zeros((tokens, d), dtype=np.float32)
+    x[:, 0] = np.nextafter(np.float32(2), np.float32(0))
+    x[:, 32:48] = 2.0 ** -21
+    got = Call(one_expert(jn, d, "Q6_K", *raw), x, None, np.zeros((tokens, 1)), np.ones((tokens, 1))).result()
+    want = x[:, :1].astype(np.float64) * 16 * 2.0 ** -21
+    assert (np.abs(got - want) <= 2 * 16 * (2 * 2.0 ** -22) * (1 + 2.0 ** -18)).all(), got[0, 0]
+
+
+@pytest.mark.parametrize("bits", [0x7f7fffff, 0x7f7ffffe, 0x7f7ffffd, 0xff7fffff])
+def test_inputs_next_to_the_largest_value(jn, bits):
+    """The largest FP32 values are finite, and so are the products that they make."""
+    d = 128
+    quants = np.zeros((3, d, d), dtype=np.int32)
+    quants[0, :, 0] = 1   # gate: the large value
+    quants[1, :, 70] = 1  # up: a small one
+    np.fill_diagonal(quants[2], 1)
+    scales = (2.0 ** -24, 1.0, 1.0)
+    raw = [q8_0(q, s) for q, s in zip(quants, scales)]
+    x = np.zeros((1, d), dtype=np.float32)
+    x[0, 0] = np.array([bits], dtype=np.uint32).view(np.float32)[0]
+    x[0, 70] = 2.0 ** -60
+    got = Call(one_expert(jn, d, "Q8_0", *raw), x, None, np.zeros((1, 1)), np.ones((1, 1))).result()
+    ref.close(got, np.full((1, d), x[0, 0].astype(np.float64) * 2.0 ** -84), ref.tolerance(["Q8_0"] * 3))
