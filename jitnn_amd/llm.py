@@ -186,12 +186,14 @@ class Llm:
             d = f.integer(f"{arch}.embedding_length")
             heads = f.integer(f"{arch}.attention.head_count")
             kv = f.integer(f"{arch}.attention.head_count_kv", heads)
-            ffn = f.integer(f"{arch}.feed_forward_length", f.integer(f"{arch}.expert_feed_forward_length", 0)) or f.integer(f"{arch}.expert_feed_forward_length")
+            experts = f.integer(f"{arch}.expert_count", 0)
+            ffn = f.integer(f"{arch}.feed_forward_length", 0 if experts else None)
+            if experts and not ffn:  # (no dense layers)
+                ffn = f.integer(f"{arch}.expert_feed_forward_length")
             hd = f.integer(f"{arch}.attention.key_length", d // heads)
             eps = f.float_value(f"{arch}.attention.layer_norm_rms_epsilon", 1e-5)
             theta = f.float_value(f"{arch}.rope.freq_base", 10000.0)
             ctx_file = f.integer(f"{arch}.context_length", 2048)
-            experts = f.integer(f"{arch}.expert_count", 0)
             for name in ("token_embd.weight", "output_norm.weight", "blk.0.attn_q.weight") + (() if experts else ("blk.0.ffn_gate.weight",)):
                 if not f.has_tensor(name):
                     raise ValueError(f"{path}: architecture {arch} does not generate text here (no tensor {name}; Llama-style layers are built)")
