@@ -9,12 +9,14 @@ tokenizer is built from the file's metadata (tokenizer.py).
         result = llm.generate(GenerationRequest("Once upon a time", 200, temperature=0.8, top_p=0.95, seed=1, stop=["\n\n"]))
 
 Llama-style architectures only (RMSNorm, rotary embedding, grouped-query attention, SwiGLU: general.architecture "llama",
-and the same tensor layout under other names where the metadata says so), with a SwiGLU or a mixture of experts in each layer; anything else raises.
+and the same tensor layout under other names where the metadata says so), with a SwiGLU or a mixture of experts in each layer; anything else raises
+(a file without experts that has more tensors than those loads with a warning).
 """
 from __future__ import annotations
 
 import ctypes as C
 import math
+import re
 import warnings
 
 import numpy as np
@@ -29,6 +31,9 @@ from .tokenizer import StreamDecoder, Tokenizer
 # GGUF tensor names of a Llama-style layer in the order of the decoder's weight slots
 LAYER_TENSORS = ["attn_q", "attn_k", "attn_v", "attn_output", "ffn_gate", "ffn_up", "ffn_down"]
 ATTENTION_TENSORS = LAYER_TENSORS[:4]
+EXPERT_TENSORS = ["ffn_gate_inp", "ffn_gate_exps", "ffn_up_exps", "ffn_down_exps"]
+NORM_TENSORS = ["attn_norm", "ffn_norm"]
+LAYER_TENSOR = re.compile(r"blk\.(0|[1-9][0-9]{0,8})\.(.+)")
 INTERLEAVED_ROPE_ARCHS = {"llama", "mistral", "granite"}  # llama.cpp's "NORM" rotary embedding: q and k stored permuted for pairs (2i, 2i + 1)
 
 _TOKEN_CB = C.CFUNCTYPE(None, C.c_int, C.c_void_p)
@@ -197,18 +202,24 @@ class Llm:
             for name in ("token_embd.weight", "output_norm.weight", "blk.0.attn_q.weight") + (() if experts else ("blk.0.ffn_gate.weight",)):
                 if not f.has_tensor(name):
                     raise ValueError(f"{path}: architecture {arch} does not generate text here (no tensor {name}; Llama-style layers are built)")
+            routed = {int(m[1]) for m in map(LAYER_TENSOR.fullmatch, f.tensor_infos()) if experts > 0 and m and m[2] == "ffn_gate_inp.weight"}
+            unread = Llm._unread(f, layers, routed)
+            if unread:
+                what = ", ".join(unread[:4]) + (f" and {len(unread) - 4} more" if len(unread) > 4 else "")
+                if routed:
+                    raise ValueError(f"{path}: what {what} are for is not built")
+                warnings.warn(f"{path}: nothing here reads {what}; the text is that of a model without them")
             emb = f.info("token_embd.weight")
             vocab = emb.shape[0]
             ctx = min(ctx_file, max_context) if max_context else min(ctx_file, 4096)
             dec = LlamaDecoder(layers, d, heads, kv, hd, ffn, vocab, ctx, eps, theta)
             fmts = set()
             for l in range(layers):
-                routed = experts > 0 and f.has_tensor(f"blk.{l}.ffn_gate_inp.weight")
-                for slot, tn in enumerate(ATTENTION_TENSORS if routed else LAYER_TENSORS):
+                for slot, tn in enumerate(ATTENTION_TENSORS if l in routed else LAYER_TENSORS):
                     w = f.tensor(f"blk.{l}.{tn}.weight")
                     fmts.add(w.dtype().name)
                     dec.set_weight(l, slot, w)
-                if routed:
+                if l in routed:
                     moe, names = Llm._experts(f, arch, l, experts)
                     dec.set_moe(l, moe)
                     fmts |= names
@@ -233,19 +244,31 @@ class Llm:
             raise
 
     @staticmethod
+    def _unread(f: GgufFile, layers: int, routed) -> list:
+        """The tensors that nothing here reads - norms of the heads' queries and keys, biases, experts for every token, layers beyond the model's: it would be another model without
+        them.  (Those of the rotary positions are _rope's.)"""
+        dense = {f"{n}.weight" for n in LAYER_TENSORS + NORM_TENSORS}
+        sparse = {f"{n}.weight" for n in ATTENTION_TENSORS + EXPERT_TENSORS + NORM_TENSORS} | {"exp_probs_b.bias", "exp_probs_b"}
+
+        def is_read(name):
+            m = LAYER_TENSOR.fullmatch(name)
+            if m:
+                return int(m[1]) < layers and m[2] in (sparse if int(m[1]) in routed else dense)
+            return name in ("token_embd.weight", "output_norm.weight", "output.weight") or name.startswith("rope_")
+
+        return [n for n in f.tensor_infos() if not is_read(n)]
+
+    @staticmethod
     def _experts(f: GgufFile, arch: str, l: int, experts: int):
         """The experts of a layer and their formats: the router's weights (ffn_gate_inp), the experts' own (ffn_gate_exps, ffn_up_exps, ffn_down_exps), a bias of the choice
         (exp_probs_b).  Weights of the chosen are normalised unless the file says otherwise (expert_weights_norm), times expert_weights_scale; gating by softmax or, expert_gating_func
-        2, sigmoid.  What else a layer may have beside them - experts for every token, groups of experts - is not built and raises."""
+        2, sigmoid.  Other gating functions and groups of experts are not built and raise, as do files with experts that have tensors nobody reads (_unread)."""
         def plain(name):
             t = f.info(name)
             if t.type not in ("F32", "F16"):
                 raise ValueError(f"{f.path()}: {name} is {t.type} (F32 and F16 are built)")
             return f.raw(name).view(np.float32 if t.type == "F32" else np.float16).reshape(t.shape).astype(np.float32)
 
-        for extra in ("ffn_gate_shexp", "ffn_up_shexp", "ffn_gate_inp_shexp"):
-            if f.has_tensor(f"blk.{l}.{extra}.weight"):
-                raise ValueError(f"{f.path()}: layer {l} has experts for every token ({extra}), which are not built")
         gating = f.integer(f"{arch}.expert_gating_func", 1)
         if gating not in (1, 2):
             raise ValueError(f"{f.path()}: expert gating function {gating} is not built")
@@ -258,7 +281,7 @@ class Llm:
             raise ValueError(f"{f.path()}: a router of {len(weights)} experts in layer {l} of a model of {experts}")
         router = Router(weights, f.integer(f"{arch}.expert_used_count"), "softmax" if gating == 1 else "sigmoid", normalise,
                         f.float_value(f"{arch}.expert_weights_scale", 1.0) or 1.0, bias)
-        parts = [f.tensor(f"blk.{l}.{n}.weight") for n in ("ffn_gate_exps", "ffn_up_exps", "ffn_down_exps")]
+        parts = [f.tensor(f"blk.{l}.{n}.weight") for n in EXPERT_TENSORS[1:]]
         return Moe(router, *parts), {p.dtype().name for p in parts}
 
     @staticmethod
