@@ -34,6 +34,7 @@ ATTENTION_TENSORS = LAYER_TENSORS[:4]
 EXPERT_TENSORS = ["ffn_gate_inp", "ffn_gate_exps", "ffn_up_exps", "ffn_down_exps"]
 NORM_TENSORS = ["attn_norm", "ffn_norm"]
 LAYER_TENSOR = re.compile(r"blk\.(0|[1-9][0-9]{0,8})\.(.+)")
+NORMALISING_ARCHS = {"llama"}  # whose chosen experts' weights sum to one where the file does not say (expert_weights_norm)
 INTERLEAVED_ROPE_ARCHS = {"llama", "mistral", "granite"}  # llama.cpp's "NORM" rotary embedding: q and k stored permuted for pairs (2i, 2i + 1)
 
 _TOKEN_CB = C.CFUNCTYPE(None, C.c_int, C.c_void_p)
@@ -209,6 +210,7 @@ class Llm:
                 if routed:
                     raise ValueError(f"{path}: what {what} are for is not built")
                 warnings.warn(f"{path}: nothing here reads {what}; the text is that of a model without them")
+            routing = Llm._routing(f, arch) if routed else None
             emb = f.info("token_embd.weight")
             vocab = emb.shape[0]
             ctx = min(ctx_file, max_context) if max_context else min(ctx_file, 4096)
@@ -220,7 +222,7 @@ class Llm:
                     fmts.add(w.dtype().name)
                     dec.set_weight(l, slot, w)
                 if l in routed:
-                    moe, names = Llm._experts(f, arch, l, experts)
+                    moe, names = Llm._experts(f, l, experts, routing)
                     dec.set_moe(l, moe)
                     fmts |= names
                 dec.set_norm(l, 0, f.raw(f"blk.{l}.attn_norm.weight").view(np.float32))
@@ -259,28 +261,35 @@ class Llm:
         return [n for n in f.tensor_infos() if not is_read(n)]
 
     @staticmethod
-    def _experts(f: GgufFile, arch: str, l: int, experts: int):
+    def _routing(f: GgufFile, arch: str) -> dict:
+        """How a file's routers choose: weights of the chosen are normalised or not as the file says (expert_weights_norm; one that does not has to be of NORMALISING_ARCHS), times
+        expert_weights_scale; gating by softmax or, expert_gating_func 2, sigmoid.  Other gating functions and groups of experts are not built and raise."""
+        gating = f.integer(f"{arch}.expert_gating_func", 1)
+        if gating not in (1, 2):
+            raise ValueError(f"{f.path()}: expert gating function {gating} is not built")
+        if f.integer(f"{arch}.expert_group_count", 1) > 1:
+            raise ValueError(f"{f.path()}: experts in groups are not built")
+        norm = f"{arch}.expert_weights_norm"
+        if not f.has(norm) and arch not in NORMALISING_ARCHS:
+            raise ValueError(f"{f.path()}: no {norm}: whether the weights of the chosen experts sum to one is not known for {arch}")
+        return dict(used=f.integer(f"{arch}.expert_used_count"), gating="softmax" if gating == 1 else "sigmoid", normalise=f.bool(norm) if f.has(norm) else True,
+                    scale=f.float_value(f"{arch}.expert_weights_scale", 1.0) or 1.0)
+
+    @staticmethod
+    def _experts(f: GgufFile, l: int, experts: int, routing: dict):
         """The experts of a layer and their formats: the router's weights (ffn_gate_inp), the experts' own (ffn_gate_exps, ffn_up_exps, ffn_down_exps), a bias of the choice
-        (exp_probs_b).  Weights of the chosen are normalised unless the file says otherwise (expert_weights_norm), times expert_weights_scale; gating by softmax or, expert_gating_func
-        2, sigmoid.  Other gating functions and groups of experts are not built and raise, as do files with experts that have tensors nobody reads (_unread)."""
+        (exp_probs_b).  routing: _routing's.  What else a layer may have raises before (_unread)."""
         def plain(name):
             t = f.info(name)
             if t.type not in ("F32", "F16"):
                 raise ValueError(f"{f.path()}: {name} is {t.type} (F32 and F16 are built)")
             return f.raw(name).view(np.float32 if t.type == "F32" else np.float16).reshape(t.shape).astype(np.float32)
 
-        gating = f.integer(f"{arch}.expert_gating_func", 1)
-        if gating not in (1, 2):
-            raise ValueError(f"{f.path()}: expert gating function {gating} is not built")
-        if f.integer(f"{arch}.expert_group_count", 1) > 1:
-            raise ValueError(f"{f.path()}: experts in groups are not built")
         bias = next((plain(n) for n in (f"blk.{l}.exp_probs_b.bias", f"blk.{l}.exp_probs_b") if f.has_tensor(n)), None)
-        normalise = f.bool(f"{arch}.expert_weights_norm") if f.has(f"{arch}.expert_weights_norm") else True
         weights = plain(f"blk.{l}.ffn_gate_inp.weight")
         if len(weights) != experts:
             raise ValueError(f"{f.path()}: a router of {len(weights)} experts in layer {l} of a model of {experts}")
-        router = Router(weights, f.integer(f"{arch}.expert_used_count"), "softmax" if gating == 1 else "sigmoid", normalise,
-                        f.float_value(f"{arch}.expert_weights_scale", 1.0) or 1.0, bias)
+        router = Router(weights, selection_bias=bias, **routing)
         parts = [f.tensor(f"blk.{l}.{n}.weight") for n in EXPERT_TENSORS[1:]]
         return Moe(router, *parts), {p.dtype().name for p in parts}
 

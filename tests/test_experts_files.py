@@ -66,3 +66,28 @@ def test_what_a_file_may_have(tmp_path, monkeypatch):
             jitnn_amd.Llm.load(tmp_path / "dense.gguf").close()
         except Exception as e:  # (no device here)
             assert not isinstance(e, ValueError), e
+
+
+def test_whether_weights_sum_to_one(tmp_path, monkeypatch):
+    """Without the key only where the architecture says so; with it whatever the file says."""
+    from jitnn_amd.gguf_file import GgufFile
+    from jitnn_amd.llm import Llm
+
+    def routing(name):
+        f = GgufFile.open(tmp_path / name)
+        try:
+            return Llm._routing(f, f.architecture())
+        finally:
+            f.close()
+
+    write_experts(tmp_path / "a.gguf", monkeypatch)
+    assert routing("a.gguf") == dict(used=2, gating="softmax", normalise=True, scale=1.0)
+    write_experts(tmp_path / "b.gguf", monkeypatch, meta={"llama.expert_weights_norm": False, "llama.expert_weights_scale": 2.5, "llama.expert_gating_func": 2}.items())
+    assert routing("b.gguf") == dict(used=2, gating="sigmoid", normalise=False, scale=2.5)
+    monkeypatch.setattr(model_files, "write_gguf", lambda p, m, tensors, write=model_files.write_gguf: write(
+        p, {k.replace("llama.", "testarch.", 1): "testarch" if k == "general.architecture" else v for k, v in m.items()}, tensors))
+    write_experts(tmp_path / "c.gguf", monkeypatch)
+    refused(tmp_path / "c.gguf", "no testarch.expert_weights_norm")
+    for norm in (True, False):
+        write_experts(tmp_path / "d.gguf", monkeypatch, meta={"llama.expert_weights_norm": norm}.items())
+        assert routing("d.gguf")["normalise"] is norm
