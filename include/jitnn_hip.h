@@ -384,7 +384,7 @@ JITNN_HIP_API int jitnn_hip_router_dev(const jitnn_hip_router *r, const float *x
  *   y = residual (or 0) + the sum over a token's experts e of weight_e * down_e (act(gate_e x) * (up_e x))
  * jitnn_hip_moe_dev routes x [tokens, d_model] itself; jitnn_hip_moe_experts_dev takes ids and weights [tokens, used] that exist: an id outside [0, experts)
  * counts for nothing, one that stands twice counts twice.  FP32-grade at any number of tokens (error ~1e-6).  x must be finite where it meets an expert: a
- * token with values that are not gives a row that is not.  y may be x or the residual; tokens 0: nothing is done.  x, residual and y 16-byte aligned.  Workspace as
+ * token with values that are not gives a row that is not.  y may be x or the residual, but not overlap either in part; tokens 0: nothing is done.  x, residual and y 16-byte aligned.  Workspace as
  * above (long calls go through the experts in passes of 4096 / used tokens: it does not grow beyond those).  Allocates nothing; may be recorded. */
 typedef struct jitnn_hip_moe jitnn_hip_moe;
 JITNN_HIP_API int jitnn_hip_moe_create(const jitnn_hip_router *router, const jitnn_hip_weight *gate, const jitnn_hip_weight *up, const jitnn_hip_weight *down,

@@ -1654,12 +1654,14 @@ int linear_dev(const jitnn_hip_weight *w, const float *x_dev, int rows, const fl
     return JITNN_HIP_OK;
 }
 
+// two arrays of so many bytes
+bool overlaps(const void *a, const void *b, size_t bytes) { return (uintptr_t)a < (uintptr_t)b + bytes && (uintptr_t)b < (uintptr_t)a + bytes; }
+
 // What an epilogue adds to the checks of a linear (which come after these): y apart from the residual, which a launch may read after another has written y.
 int check_linear_act(const jitnn_hip_weight *w, int rows, int activation, const float *residual, const float *y) {
     if (activation < 0 || activation >= ACT_COUNT) return fail(JITNN_HIP_EINVAL, "activation %d", activation);
     if (w && rows > 0 && residual && y) {
-        const size_t bytes = (size_t)rows * w->n * sizeof(float);
-        if ((uintptr_t)residual < (uintptr_t)y + bytes && (uintptr_t)y < (uintptr_t)residual + bytes) return fail(JITNN_HIP_EINVAL, "the output overlaps the residual");
+        if (overlaps(residual, y, (size_t)rows * w->n * sizeof(float))) return fail(JITNN_HIP_EINVAL, "the output overlaps the residual");
     }
     return JITNN_HIP_OK;
 }
@@ -2579,6 +2581,9 @@ int check_moe_call(const jitnn_hip_moe *m, const float *x, int tokens, const flo
     if (tokens == 0) return JITNN_HIP_OK;
     if (!x || !y) return fail(JITNN_HIP_EINVAL, "input or output is NULL");
     if ((((uintptr_t)x | (uintptr_t)y | (uintptr_t)res) & 15) != 0) return fail(JITNN_HIP_EINVAL, "input, residual and output must be 16-byte aligned");
+    const size_t bytes = (size_t)tokens * m->router->d * sizeof(float);
+    for (const float *in : {x, res})  // (the same array is read before it is written, row by row; a shifted one is not)
+        if (in && in != y && overlaps(in, y, bytes)) return fail(JITNN_HIP_EINVAL, "the output overlaps the input or the residual");
     const int pass = moe_pass_tokens(m);
     long long need = (long long)moe_layout(m, std::min(tokens, pass)).total;
     if (tokens > pass && tokens % pass) need = std::max(need, (long long)moe_layout(m, tokens % pass).total);

@@ -1,4 +1,4 @@
-"""Layers of experts at their borders: matrices beyond 2 GiB whose rows are no whole columns, inputs next to a power of two and to the largest FP32 value."""
+"""Layers of experts at their borders: matrices beyond 2 GiB whose rows are no whole columns, inputs next to a power of two and to the largest FP32 value, outputs that overlap."""
 import numpy as np
 import pytest
 import torch
@@ -96,3 +96,31 @@ def test_inputs_next_to_the_largest_value(jn, bits):
     x[0, 70] = 2.0 ** -60
     got = Call(one_expert(jn, d, "Q8_0", *raw), x, None, np.zeros((1, 1)), np.ones((1, 1))).result()
     ref.close(got, np.full((1, d), x[0, 0].astype(np.float64) * 2.0 ** -84), ref.tolerance(["Q8_0"] * 3))
+
+
+@pytest.mark.parametrize("tokens", [4, 70])
+def test_outputs_that_overlap_in_part(jn, tokens):
+    """An output shifted against the input or the residual would be written where rows are still to be read; beside them it is an output like any other."""
+    d = 256
+    layer = ref.Layer(np.random.default_rng(1), 4, 2, d, 512)
+    moe = layer.make(jn)
+    n = moe.workspace(tokens)
+    buffer, ws = torch.full((3 * tokens, d), 3.0, device="cuda"), torch.empty(n, dtype=torch.uint8, device="cuda")
+    other, ids, weights = torch.zeros(tokens, d, device="cuda"), torch.zeros(tokens, 2, dtype=torch.int32, device="cuda"), torch.ones(tokens, 2, device="cuda")
+
+    def both(x, y, res=0):
+        moe.layer_dev(x, tokens, y, ws.data_ptr(), n, res)
+        moe.experts_dev(x, tokens, ids.data_ptr(), weights.data_ptr(), y, ws.data_ptr(), n, res)
+
+    at = lambda row, values=0: buffer.data_ptr() + 4 * (row * d + values)
+    for shifted in (at(tokens, 4), at(tokens, -4), at(tokens + 1), at(2 * tokens - 1), at(1), at(2 * tokens, -4)):
+        for args in ((at(tokens), shifted), (other.data_ptr(), shifted, at(tokens)), (shifted, shifted, at(tokens))):
+            with pytest.raises(ValueError, match="overlaps"):
+                both(*args)
+    torch.cuda.synchronize()
+    assert (buffer == 3).all()
+    both(at(tokens), at(2 * tokens), at(0))
+    both(at(tokens), at(0), at(2 * tokens))
+    both(at(0), at(tokens))
+    torch.cuda.synchronize()
+    assert torch.isfinite(buffer).all()
