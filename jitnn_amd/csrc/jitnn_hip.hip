@@ -2425,6 +2425,9 @@ int moe_pass_tokens(const jitnn_hip_moe *m) { return std::max(1, MOE_PASS_SLOTS 
 
 bool experts_on_rows(const jitnn_hip_weight *w) { return gemv_rows_supported(w->fmt); }  // (Q5_0 and Q3_K blocks that were not rewritten have no operands)
 
+// Gate and up in one launch of the matrix cores' kernels.
+bool experts_pair(const jitnn_hip_moe *m) { return experts_on_rows(m->gate) && m->gate->fmt == m->up->fmt; }
+
 // Experts that so many tokens meet, where every one is as likely as any other.
 double moe_met(const jitnn_hip_router *r, int tokens) { return r->experts * (1 - std::pow(1 - (double)r->used / r->experts, tokens)); }
 
@@ -2443,7 +2446,7 @@ int moe_groups(const jitnn_hip_moe *m, int tokens) {
     int groups = std::max(1, (int)std::ceil((mean + 2 * std::sqrt(mean)) / 8));
     for (const jitnn_hip_weight *w : {m->gate, m->up, m->down})
         if (experts_on_rows(w)) groups = std::min(groups, experts_rows_kernel_ref(w->fmt, groups, false).groups);
-    if (!experts_on_rows(m->gate) || m->gate->fmt != m->up->fmt) return groups;
+    if (!experts_pair(m)) return groups;
     auto workgroups = [&](int with) {
         const RowsKernelRef k = experts_rows_kernel_ref(m->gate->fmt, with, true);
         return moe_chunks(r, tokens, with) * ((m->ffn / 16 + k.tiles - 1) / k.tiles);
@@ -2519,7 +2522,7 @@ MoeLayout moe_layout(const jitnn_hip_moe *m, int tokens) {
         if (experts_on_rows(w)) l.layouts[gemv_rows_layout(w->fmt)] = true;
     for (int i = 0; i < GR_LAYOUTS; ++i) l.ops[i] = l.layouts[i] ? take(experts_ops_bytes(tokens, r->d)) : 0;
     l.h_ops = take(experts_on_rows(m->down) ? experts_ops_bytes(slots, m->ffn) : 0);
-    l.u = take(slots * m->ffn * sizeof(float));
+    l.u = take(experts_pair(m) ? 0 : slots * m->ffn * sizeof(float));  // (a pair's products meet in registers)
     l.part = take(slots * r->d * l.splits * sizeof(float));
     l.total = at;
     return l;
@@ -2655,8 +2658,7 @@ int moe_experts(const jitnn_hip_moe *m, const float *x, int tokens, const int *i
     };
     uint8_t *places[GR_LAYOUTS] = {};
     for (int i = 0; i < GR_LAYOUTS; ++i) places[i] = l.layouts[i] ? ws + l.ops[i] : nullptr;
-    const bool pair = experts_on_rows(m->gate) && m->gate->fmt == m->up->fmt;
-    if (pair) {
+    if (experts_pair(m)) {
         if (int rc = rows(m->gate, m->up, places[gemv_rows_layout(m->gate->fmt)], tokens, r->used, 1, gb)) return rc;
     } else {
         const jitnn_hip_weight *ws2[2] = {m->gate, m->up};

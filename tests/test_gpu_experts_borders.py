@@ -124,3 +124,17 @@ def test_outputs_that_overlap_in_part(jn, tokens):
     both(at(0), at(tokens))
     torch.cuda.synchronize()
     assert torch.isfinite(buffer).all()
+
+
+def test_the_workspace_of_a_pair(jn):
+    """Gate and up of one format run as a pair and never leave registers; of two formats each has an array of its own in the workspace."""
+    experts, used, d, ffn, tokens = 4, 2, 256, 1024, 2048
+    rng = np.random.default_rng(1)
+    pair, apart = ref.Layer(rng, experts, used, d, ffn, up="Q4_K").make(jn), ref.Layer(rng, experts, used, d, ffn, up="Q5_K", gate="Q4_K").make(jn)
+    array = tokens * used * ffn * 4
+    # (the same operands, lists and sums in both; chunks are no smaller in the second)
+    assert apart.workspace(tokens) - pair.workspace(tokens) >= array - 65536
+    # of one pass beside the array itself: operands of x and of the gated values (1152 bytes and a scale per 256 values), the products (rows of four columns are not shared out), choices
+    # and logits
+    most = array + (tokens * d + tokens * used * ffn) // 256 * 1156 + tokens * used * d * 4 + tokens * (experts * 8 * 8 + used * 16) + 65536
+    assert pair.workspace(tokens) <= most
