@@ -3067,7 +3067,8 @@ void release_or_keep(jitnn_hip_llama *m, void *p) {
     else if (!m->recorded) (void)hipFree(p);  // (no memory to note it: left to the process)
 }
 
-// The workspace of a model's experts for passes of up to `tokens`, which are more than it has been made for; which 0: one token's.  The device may still use the old one.
+// The workspace of a model's experts for passes of up to `tokens`, which are more than it has been made for; which 0: one token's.  The device may still use the old one.  A decode step's stays where
+// there is no room for a larger one: the experts that are there go on.
 int moe_reserve(jitnn_hip_llama *m, int which, int tokens) {
     long long need = 0;
     const jitnn_hip_moe *last = nullptr;
@@ -3079,17 +3080,15 @@ int moe_reserve(jitnn_hip_llama *m, int which, int tokens) {
     }
     if ((size_t)need <= m->moe_ws_bytes[which]) return JITNN_HIP_OK;
     HIP_TRY(hipDeviceSynchronize());
-    release_or_keep(m, m->moe_ws[which]);
-    m->moe_ws[which] = nullptr;
-    m->moe_ws_bytes[which] = 0;
-    if (which) m->moe_cap = 0;
-    if (hipMalloc(&m->moe_ws[which], (size_t)need) != hipSuccess) {
+    auto alloc = [](size_t bytes) -> void * {
+        void *p = nullptr;
+        if (hipMalloc(&p, bytes) == hipSuccess) return p;
         (void)hipGetLastError();
-        m->moe_ws[which] = nullptr;
-        return fail(JITNN_HIP_ENOMEM, "no %lld bytes of device memory for the experts of %d tokens", need, tokens);
-    }
-    m->moe_ws_bytes[which] = (size_t)need;
-    return JITNN_HIP_OK;
+        return nullptr;
+    };
+    const bool ok = replace_buffer(m->moe_ws[which], m->moe_ws_bytes[which], (size_t)need, which != 0, alloc, [&](void *p) { release_or_keep(m, p); });
+    if (which && !m->moe_ws[which]) m->moe_cap = 0;  // (the next pass asks for all it needs)
+    return ok ? JITNN_HIP_OK : fail(JITNN_HIP_ENOMEM, "no %lld bytes of device memory for the experts of %d tokens", need, tokens);
 }
 
 // The many-token buffers of a model, for at least `tokens` rows.

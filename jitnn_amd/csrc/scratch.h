@@ -1,4 +1,4 @@
-// A thread's grow-only block of device memory, as a policy over an allocator: host code without any HIP, so that it can be
+// A thread's grow-only block of device memory, as a policy over an allocator, and a buffer that a larger one replaces: host code without any HIP, so that it can be
 // driven on a machine that has no GPU (tests/scratch_block_test.cpp).
 #pragma once
 #include <algorithm>
@@ -103,6 +103,24 @@ public:
         *this = ScratchBlock{};
     }
 };
+
+// A buffer of `need` bytes in place of the one of `bytes` that is held; where there is no room for it the one held stays, unless give_up: then that goes first (what it held is of no use to this
+// call), and is gone where that does not help.
+template <class Alloc, class Release>
+bool replace_buffer(void *&held, size_t &bytes, size_t need, bool give_up, Alloc &&alloc, Release &&release) {
+    void *p = alloc(need);
+    if (!p && held && give_up) {
+        release(held);
+        held = nullptr;
+        bytes = 0;
+        p = alloc(need);
+    }
+    if (!p) return false;
+    if (held) release(held);
+    held = p;
+    bytes = need;
+    return true;
+}
 
 // The start of a prompt pass: sizes that were refused are asked for again by whoever needs them, and where the pass knows its largest
 // launches (0: it does not) both blocks move to their sizes at once, not step by step.
