@@ -3067,9 +3067,8 @@ void release_or_keep(jitnn_hip_llama *m, void *p) {
     else if (!m->recorded) (void)hipFree(p);  // (no memory to note it: left to the process)
 }
 
-// The workspace of a model's experts for passes of up to `tokens`, which are more than it has been made for; which 0: one token's.  The device may still use the old one.  A decode step's stays where
-// there is no room for a larger one: the experts that are there go on.
-int moe_reserve(jitnn_hip_llama *m, int which, int tokens) {
+// What the workspace of a model's experts has to be for passes of up to `tokens`, which 0: of one token's; less than there is where it has been made for as many.
+size_t moe_need(const jitnn_hip_llama *m, int which, int tokens) {
     long long need = 0;
     const jitnn_hip_moe *last = nullptr;
     for (int l = 0; l < m->layers; ++l) {
@@ -3078,7 +3077,13 @@ int moe_reserve(jitnn_hip_llama *m, int which, int tokens) {
         need = std::max(need, moe_most(e, which ? m->moe_cap + 1 : 1, tokens));
         last = e;
     }
-    if ((size_t)need <= m->moe_ws_bytes[which]) return JITNN_HIP_OK;
+    return (size_t)need;
+}
+
+// That workspace.  The device may still use the old one.  A decode step's stays where there is no room for a larger one: the experts that are there go on.
+int moe_reserve(jitnn_hip_llama *m, int which, int tokens) {
+    const size_t need = moe_need(m, which, tokens);
+    if (need <= m->moe_ws_bytes[which]) return JITNN_HIP_OK;
     HIP_TRY(hipDeviceSynchronize());
     auto alloc = [](size_t bytes) -> void * {
         void *p = nullptr;
@@ -3086,9 +3091,9 @@ int moe_reserve(jitnn_hip_llama *m, int which, int tokens) {
         (void)hipGetLastError();
         return nullptr;
     };
-    const bool ok = replace_buffer(m->moe_ws[which], m->moe_ws_bytes[which], (size_t)need, which != 0, alloc, [&](void *p) { release_or_keep(m, p); });
+    const bool ok = replace_buffer(m->moe_ws[which], m->moe_ws_bytes[which], need, which != 0, alloc, [&](void *p) { release_or_keep(m, p); });
     if (which && !m->moe_ws[which]) m->moe_cap = 0;  // (the next pass asks for all it needs)
-    return ok ? JITNN_HIP_OK : fail(JITNN_HIP_ENOMEM, "no %lld bytes of device memory for the experts of %d tokens", need, tokens);
+    return ok ? JITNN_HIP_OK : fail(JITNN_HIP_ENOMEM, "no %zu bytes of device memory for the experts of %d tokens", need, tokens);
 }
 
 // The many-token buffers of a model, for at least `tokens` rows.
@@ -3608,9 +3613,10 @@ int jitnn_hip_llama_step_dev(jitnn_hip_llama *m, const jitnn_hip_paged_cache *c,
     const int d = m->d, T = b->tokens;
     const long long need = jitnn_hip_paged_attention_workspace(c, b, m->heads);
     if (need < 0) return (int)need;
-    if ((T > m->pf_cap || T > m->moe_cap || (size_t)need > m->paged_ws_bytes) && stream_recording(st))
+    const bool recording = stream_recording(st);
+    if (recording && (T > m->pf_cap || (T > m->moe_cap && moe_need(m, 1, T) > m->moe_ws_bytes[1]) || (size_t)need > m->paged_ws_bytes))
         return fail(JITNN_HIP_EINVAL, "a pass of %d tokens needs larger buffers than the model has, which a recording cannot allocate", T);
-    if (stream_recording(st)) m->recorded = true;
+    if (recording) m->recorded = true;
     if (int rc = ensure_prefill(m, T)) return rc;
     if ((size_t)need > m->paged_ws_bytes) {
         HIP_TRY(hipDeviceSynchronize());  // earlier passes may still use the old one

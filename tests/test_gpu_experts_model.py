@@ -170,6 +170,50 @@ def test_recorded_passes(jn, tokens):
     dec.close()
 
 
+def test_a_pass_is_recorded_after_experts_change(jn):
+    """Experts that need no more than the workspace there is, and a layer that is dense again: a pass of a size that has run may be recorded as before."""
+    dec, layers, _, _ = build(jn, CFG, 15)
+    tokens = 20
+    table, starts, lens = (torch.tensor(a, dtype=torch.int32, device="cuda") for a in ([[0, 1]], [0, tokens], [tokens]))
+    cache = jn.PagedCache(CFG["layers"], CFG["kv_heads"], CFG["head_dim"], 2, 64, 0)
+    batch = jn.Batch(1, tokens, tokens, 64, table.data_ptr(), 2, starts.data_ptr(), lens.data_ptr())
+    x, rows = torch.randn(tokens, CFG["d_model"], device="cuda"), torch.arange(tokens, dtype=torch.int32, device="cuda")
+    logits = torch.empty(tokens, CFG["vocab"], device="cuda")
+
+    def run():
+        dec.step_dev(cache, batch, x.data_ptr(), rows.data_ptr(), tokens, logits.data_ptr(), torch.cuda.current_stream().cuda_stream)
+        return logits
+
+    moes = [ref.Layer(np.random.default_rng(s), 6, 2, CFG["d_model"], 512).make(jn) for s in (1, 2)]
+    dec.set_moe(1, moes[0])
+    run()
+    torch.cuda.synchronize()
+    for moe in (moes[1], None, moes[0]):
+        dec.set_moe(1, moe)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            run()
+        logits.fill_(0)
+        for _ in range(3):
+            graph.replay()
+            torch.cuda.synchronize()
+            replayed = logits.cpu().numpy()
+            assert np.array_equal(run().cpu().numpy(), replayed) and replayed.any()
+        del graph
+    # more than there is room for: refused, and nothing is recorded
+    dec.set_moe(1, ref.Layer(np.random.default_rng(3), 6, 6, CFG["d_model"], 2048).make(jn))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(ValueError, match="recording"):
+            run()
+        logits.fill_(1)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert (logits == 1).all()
+    assert np.isfinite(run().cpu().numpy()).all()
+    dec.close()
+
+
 # ---------------------------------------------------------------------------------------------- files
 
 def write_experts(path, monkeypatch, experts=6, used=2, ffn=256, meta=(), extra=(), drop=(), router_type="F32", bias=False, layers=(0, 1)):
