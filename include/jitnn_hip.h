@@ -363,7 +363,7 @@ JITNN_HIP_API int jitnn_hip_verify_drafts_dev(const float *logits_dev, long long
 
 /* The router of a layer of experts (Shazeer et al., "Outrageously Large Neural Networks: The Sparsely-Gated Mixture-of-Experts Layer", 2017), which the
  * reference does not have: l = x W^T, p = softmax(l) over all experts or sigmoid(l), the `used` experts with the largest l - with a selection bias, the
- * largest p + bias - and their weights scale * p, normalise: divided by the sum of those chosen.  Sums and p in FP64, the same choice whatever the order of
+ * largest p + bias - and their weights scale * p, normalise: divided by the sum of those chosen.  Sums and p in FP64, the same choice of the same row whatever the order of
  * a sum; ties go to the lowest index, logits that are not numbers come last.  Weights [experts, d_model] and bias [experts] are copied from host memory;
  * immutable afterwards and usable by any number of threads.  experts at most 512, used at most 64, d_model a multiple of 4. */
 typedef struct jitnn_hip_router jitnn_hip_router;
@@ -429,7 +429,8 @@ JITNN_HIP_API int jitnn_hip_llama_free(jitnn_hip_llama *m);
  * k/v [kv_heads*head_dim, d_model], gate/up [ffn, d_model], down [d_model, ffn], output [vocab, d_model]). */
 JITNN_HIP_API int jitnn_hip_llama_set_weight(jitnn_hip_llama *m, int layer, int which, const jitnn_hip_weight *w);
 /* Experts in place of a layer's gate, up and down (which it then need not have): x + moe(RMSNorm(x)).  Not owned; d_model as the model's, any ffn.  NULL: the layer is
- * dense again.  Their workspace belongs to the model: one token's is allocated here, those of longer passes with the many-token buffers.  Not while work of
+ * dense again.  The same rows choose the same experts at any number of tokens; but in a pass of more than 64 the attention's linears have FP16 operands (jitnn_hip_linear), so that a token's row
+ * comes to the router about 2e-3 off what it is by itself, and experts that lie closer together than that may change places.  Their workspace belongs to the model: one token's is allocated here, those of longer passes with the many-token buffers.  Not while work of
  * this model is under way, nor between a recording and its replays. */
 JITNN_HIP_API int jitnn_hip_llama_set_moe(jitnn_hip_llama *m, int layer, const jitnn_hip_moe *moe);
 /* Copies an RMSNorm weight vector [d_model] from host memory. */

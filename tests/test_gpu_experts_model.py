@@ -101,6 +101,46 @@ def test_long_prompt(jn, tokens):
     dec.close()
 
 
+def leading(rng, dec, layers, at, tokens, experts=6, used=2):
+    """Experts that a token's own value leads to, past what the layers in between add -> the tokens' rows, each along two of the routers' directions."""
+    d = dec.cfg["d_model"]
+    rows, largest = rng.standard_normal((experts, d)) / np.sqrt(d), 0.0
+    for l in at:
+        moe = ref.Layer(rng, experts, used, d, 512)
+        moe.router = (rows / 4).astype(np.float32)
+        largest = max(largest, np.sqrt((moe.values[2] ** 2).mean() * moe.ffn))
+        layers[l]["moe"] = moe
+        layers[l]["ffn_norm"] = (layers[l]["ffn_norm"] * moe.size).astype(np.float32)
+        dec.set_norm(l, 1, layers[l]["ffn_norm"])
+    pairs = np.array([rng.permutation(experts)[:2] for _ in range(tokens)])
+    return (largest * (np.sqrt(d / 2) * rows[pairs].sum(1) + 0.3 * rng.standard_normal((tokens, d)))).astype(np.float32)
+
+
+# The linears of the attention have FP16 operands here, so that what reaches the router differs between a token by itself and a prompt: logits that lie closer together than that may be chosen
+# either way.  These lie apart: logits of about 4 whose input is off by three linears' 2e-3 at most are off by 0.024 against a gap of about a standard deviation, one, and the choice of every token
+# is the plain one.  The weights of two experts change by a quarter of what their logits do, 0.6 % a layer beside test_long_prompt's 1.5 % of FP16 linears: 3 % in all.  (Another second expert
+# changes a token's logits by 5.8 % at least.)
+@pytest.mark.parametrize("tokens", [70, 130])
+def test_choices_of_a_long_prompt(jn, tokens):
+    dec, layers, out_norm, out_w = build(jn, CFG, 16)
+    rng = np.random.default_rng(tokens)
+    x = leading(rng, dec, layers, (0, 2), tokens)
+    for l in (0, 2):
+        dec.set_moe(l, layers[l]["moe"].make(jn))
+    want, gap = forward(CFG, layers, out_norm, out_w, *caches(CFG), x, 0)
+    assert gap > 0.9
+    table, starts, lens = (torch.tensor(a, dtype=torch.int32, device="cuda") for a in ([[0, 1, 2]], [0, tokens], [tokens]))
+    cache = jn.PagedCache(CFG["layers"], CFG["kv_heads"], CFG["head_dim"], 3, 64, 0)
+    batch = jn.Batch(1, tokens, tokens, 192, table.data_ptr(), 3, starts.data_ptr(), lens.data_ptr())
+    xd, rows, logits = torch.from_numpy(x).cuda(), torch.arange(tokens, dtype=torch.int32, device="cuda"), torch.empty(tokens, CFG["vocab"], device="cuda")
+    dec.step_dev(cache, batch, xd.data_ptr(), rows.data_ptr(), tokens, logits.data_ptr(), torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    got = logits.cpu().numpy()
+    assert all(norm_err(g, w) <= 3e-2 for g, w in zip(got, want))
+    assert norm_err(dec.prefill(x, 0), want[-1]) <= 3e-2
+    dec.close()
+
+
 def test_layers_change_places(jn):
     """Experts in, experts out: the dense layer's results come back bit for bit, and a model without dense weights where experts stand runs."""
     dec, layers, out_norm, out_w = build(jn, CFG, 13)
