@@ -5,8 +5,8 @@
 // stretch meets another expert's weights and has been multiplied by that expert's share, so that y is one dot product per row of d_model: no joining launch, and
 // the order of the sums does not depend on the launch's shape.
 // A row with a value that is not finite gives a row of NaN.
-// Bound by memory: one token, two of eight experts of 4096 x 14336, gate and up in Q4_K 132 MB in 26.4 us (5.0 TB/s), down in Q6_K 96 MB in 22.3 (4.3), 50.6 us for the layer; eight of
-// 128 of 2048 x 768 14 MB in 9.7 and 10 MB in 8.7: starts and dependent reads - logits, choice, weights.
+// Bound by memory: one token, two of eight experts of 4096 x 14336, gate and up in Q4_K 132 MB in 27.2 us (4.9 TB/s), down in Q6_K 96 MB in 23.2 (4.1), 51.1 us for the layer; eight of
+// 128 of 2048 x 768 14 MB in 9.8 and 10 MB in 8.6: starts and dependent reads - logits, choice, weights.
 #pragma once
 #include "act.h"
 #include "common.h"

@@ -8,7 +8,7 @@
 // the groups.  Nothing is added up across waves or workgroups but shares of K (a.splits), which whoever reads
 // them adds up in order, and a row's result does not depend on the rows beside it.
 // Bound by what turns quants into operands - vector units 53 (Q4_K) to 66 % (Q5_K, Q6_K) busy for chunks of up to sixteen rows: with every expert's weights in the caches
-// 32 tokens over 128 experts took 122 us instead of 139, 24 over eight 227 instead of 274 -, by operands and products in turn for more (see the shapes).
+// 32 tokens over 128 experts took 122 us instead of 139, 24 over eight 227 instead of 274 (260 since) -, by operands and products in turn for more (see the shapes).
 #pragma once
 #include <utility>
 
@@ -374,7 +374,7 @@ __global__ void __launch_bounds__(S::threads, S::per_simd) experts_rows_kernel(c
 // blocks but Q4_0 -, four waves of two tiles (of one of Q6_K) (24 tokens, two of eight of 4096 x 4096: Q8_0 140 us against 152 and 145 of eight waves, Q4_1 84 / 106 / 90, Q6_K
 // 141 / 212 / 148, Q4_0 114 / 107 / 121, Q5_K 98 / - / 101).
 // Three to twelve (to eight of 32-value blocks: registers): in sets of four, whose operands come out of LDS ahead of their products.  512 tokens, two of eight of 4096 x 14336 in Q4_K
-// and Q6_K: 1380 us, with eight at most - more chunks where an expert has more rows than most - 1457; groups of sixteen rows, hi and lo parts as operands of their own, 1472; four
+// and Q6_K: 1380 us (1340 since the lists and the tokens' operands are made in one launch), with eight at most - more chunks where an expert has more rows than most - 1457; groups of sixteen rows, hi and lo parts as operands of their own, 1472; four
 // waves and sets of two 1479; sixteen groups a chunk 1600 to 2243 (registers).  What bounds it there, of 1490: without its products it took 1009 us - operands on their way 215,
 // to LDS 70, decoding 125, weights 130 -, without all of those 956; the products alone would be 490.
 typedef RowsShape<8, 1, 1, 2> RowsShape1;
