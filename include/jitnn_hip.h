@@ -198,7 +198,8 @@ JITNN_HIP_API int jitnn_hip_quantize_q8_0_dev(const float *x_dev, long long nume
  * output tensor once, block-quantised tensors at numel / blockValues * blockBytes - the same "algorithmic bytes" the
  * benchmark divides by time.  Operators: "linear_gemv" (up to 64 rows), "linear_mfma" (more rows), "dequantize",
  * "quantize_q8_0", "llama_decode", "llama_prefill" (the two model steps count their own linears and experts under themselves, not
- * under the linear operators).  Routers, experts, attention over pages and verification are counted where a model's step runs them, not where they are called by themselves.  Writes up to cap entries and returns the number of operators; thread-safe. */
+ * under the linear operators).  Routers, experts, attention over pages and verification are counted where a model's step runs them,
+ * not where they are called by themselves.  Writes up to cap entries and returns the number of operators; thread-safe. */
 typedef struct jitnn_hip_stat {
     char name[32];
     long long calls;
